@@ -52,12 +52,15 @@ if which in ("all", "cuda"):
             sources=[
                 "csrc/ops/bindings.cpp",
                 "csrc/ops/attn_api.cpp",
+                "csrc/ops/layer_api.cpp",
                 "csrc/kernels/umma_probe.cu",
                 "csrc/kernels/flash_fwd_sm100.cu",
                 "csrc/kernels/attn_fwd_persistent.cu",
                 "csrc/kernels/flash_bwd_sm100.cu",
                 "csrc/kernels/attn_bwd_noalloc.cu",
                 "csrc/kernels/legacy_fp32.cu",
+                "csrc/kernels/rms_norm.cu",
+                "csrc/kernels/rotary.cu",
                 "csrc/comm/symmetric.cpp",
                 "csrc/comm/ring_engine.cpp",
                 "csrc/comm/ring_engine_p.cpp",

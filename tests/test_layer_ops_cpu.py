@@ -1,0 +1,57 @@
+"""Host-side parts of the decoder-layer operators: refusals of host tensors, and the
+frequencies of rotary positions."""
+import math
+
+import pytest
+import torch
+
+
+def test_host_tensors_are_refused():
+    from multi_gpu_flashattention_b200 import apply_rotary, rms_norm, rms_norm_fp8
+    x, w = torch.randn(4, 64), torch.ones(64)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        rms_norm(x, w)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        rms_norm_fp8(x, w)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        apply_rotary(torch.randn(4, 2, 64), None, torch.arange(4), torch.ones(32, dtype=torch.float64))
+
+
+def test_gradient_of_the_8_bit_output_is_refused():
+    from multi_gpu_flashattention_b200 import rms_norm_fp8
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rms_norm_fp8(torch.randn(4, 64, requires_grad=True), torch.ones(64))
+
+
+@pytest.mark.parametrize("rd", [2, 64, 128])
+def test_frequencies(rd):
+    from multi_gpu_flashattention_b200 import rotary_frequencies
+    inv, mag = rotary_frequencies(rd)
+    assert inv.dtype == torch.float64 and mag == 1.0
+    for i in range(rd // 2):
+        assert inv[i].item() == pytest.approx(10000.0 ** (-2 * i / rd), rel=1e-14)
+    lin, _ = rotary_frequencies(rd, scaling="linear", factor=4.0)
+    torch.testing.assert_close(lin * 4, inv)
+
+
+def test_frequencies_by_base_and_by_frequency():
+    from multi_gpu_flashattention_b200 import rotary_frequencies
+    inv, _ = rotary_frequencies(128)
+    wide, _ = rotary_frequencies(128, scaling="base", factor=8.0)
+    assert wide[0] == 1.0 and wide[-1].item() == pytest.approx(inv[-1].item() / 8.0, rel=1e-12)
+    ramp, mag = rotary_frequencies(128, scaling="ramp", factor=4.0, original_length=4096)
+    turns = 4096 * inv / (2 * math.pi)
+    assert mag == pytest.approx(1 + 0.1 * math.log(4.0))
+    assert torch.equal(ramp[turns > 40], inv[turns > 40])
+    torch.testing.assert_close(ramp[turns < 0.9], inv[turns < 0.9] / 4)
+    share = ((inv - ramp) / (inv - inv / 4))[(turns < 30) & (turns > 1.2)]
+    assert (share.diff() > 0).all() and share.min() > 0 and share.max() < 1
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=63), dict(rotary_dim=0), dict(rotary_dim=64, base=1.0),
+                                dict(rotary_dim=64, factor=0.5), dict(rotary_dim=64, scaling="other"),
+                                dict(rotary_dim=64, scaling="ramp"), dict(rotary_dim=2, scaling="base")])
+def test_frequencies_refused(kw):
+    from multi_gpu_flashattention_b200 import rotary_frequencies
+    with pytest.raises(ValueError):
+        rotary_frequencies(**kw)
