@@ -1,0 +1,222 @@
+// Attention of new tokens over a paged cache: parameters, the division of the work
+// that the kernels share, and their launch functions.
+//
+// Sequence b has n_b new tokens (rows [cu_q[b], cu_q[b + 1]) of q), which are the last
+// of its kv_b tokens; token i sees keys [0, kv_b - n_b + i] (causal) or all of them.
+// The `group` query heads of a key head share its keys, so a unit of work packs them:
+// row r of (b, key head) is token r / group, head r % group.
+//
+// Division of the work. A unit (b, key head, block of tokens) reads a run of key
+// tiles; all units' runs, laid end to end, are cut into equal shares, one per CTA,
+// whatever the sequences' lengths. A share covers whole units, which the CTA finishes,
+// and at most two parts (its first and last), which it leaves, unnormalised in fp32, in
+// a workspace for paged_merge_kernel. The shares follow from the lengths alone, which
+// the kernels read on the device: the host knows none of them, nothing waits for it,
+// and the result does not depend on timing.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#ifdef __CUDACC__
+#include "sm100_ptx.cuh"
+#endif
+
+namespace mgfa {
+
+constexpr int kPagedMaxSeqs = 4096;
+constexpr int kPagedMaxGroup = 128;
+
+struct PagedParams {
+  // problem
+  const void* q = nullptr;      // [tokens, heads, head_dim], strides in elements
+  int64_t q_stride_t = 0, q_stride_h = 0;
+  void* out = nullptr;          // q's type
+  int64_t o_stride_t = 0, o_stride_h = 0;
+  float* lse = nullptr;         // [heads, tokens] natural log, or null
+  const int* page_table = nullptr;  // [rows, width]
+  int64_t table_stride = 0;
+  const int* kv_lens = nullptr;     // [rows]
+  const int* slots = nullptr;       // [seqs]: row of the table and of kv_lens (null: b)
+  const int* cu_q = nullptr;        // [seqs + 1]
+  int seqs = 0, rows = 0, width = 0, page = 0, pages = 0;
+  int tokens = 0, heads = 0, kv_heads = 0, group = 0, head_dim = 0;
+  int max_new = 0;
+  int causal = 1, fp16 = 0;
+  float scale_log2 = 0.f;
+  // division of the work
+  int block_tokens = 0;  // new tokens of a unit
+  int tile = 0;          // keys of a tile
+  int min_share = 1;     // tiles
+  int grid = 0;          // CTAs
+  int unit_rows = 0;     // rows of a part in the workspace
+  // workspace: parts [2 * grid][unit_rows][head_dim] and their (max, sum), log2 units
+  float* part_o = nullptr;
+  float2* part_ml = nullptr;
+  uint32_t* status = nullptr;
+  uint64_t wait_limit_ns = 0;
+};
+
+#ifdef __CUDACC__
+namespace dev {
+
+// Sequence b as the kernels use it, whatever the arrays say: n new tokens from row q0,
+// all inside [0, tokens) and at most max_new; kv within the table's row. `bad` says that
+// something had to be cut.
+struct PagedSeq {
+  int q0, n, kv, row;
+  bool bad;
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+  PagedSeq s;
+  s.q0 = __ldg(p.cu_q + b);
+  int end = __ldg(p.cu_q + b + 1);
+  s.row = p.slots ? __ldg(p.slots + b) : b;
+  s.bad = s.q0 < 0 || end < s.q0 || end > p.tokens || end - s.q0 > p.max_new || s.row < 0 ||
+          s.row >= p.rows;
+  if (s.bad) {
+    s.n = s.kv = s.q0 = s.row = 0;
+    return s;
+  }
+  s.n = end - s.q0;
+  s.kv = __ldg(p.kv_lens + s.row);
+  const int64_t most = int64_t(p.width) * p.page;
+  if (s.kv < 0 || s.kv > most) {
+    s.bad = true;
+    s.kv = s.kv < 0 ? 0 : int(most);
+  }
+  return s;
+}
+
+// Keys that the last of tokens [t, t + block) sees; tiles of that run, at least one (a
+// unit without a visible key still writes its rows).
+__device__ __forceinline__ int paged_unit_tiles(const PagedParams& p, const PagedSeq& s, int unit) {
+  int last = (unit + 1) * p.block_tokens;
+  last = last < s.n ? last : s.n;
+  int seen = p.causal ? s.kv - s.n + last : s.kv;
+  seen = seen < s.kv ? seen : s.kv;
+  return seen > 0 ? (seen + p.tile - 1) / p.tile : 1;
+}
+
+__device__ __forceinline__ int paged_units(const PagedParams& p, const PagedSeq& s) {
+  return (s.n + p.block_tokens - 1) / p.block_tokens;
+}
+
+// prefix[b] = tiles of one key head's units of the sequences before b; prefix[seqs] the
+// total. Called by all kThreads threads of the CTA; `sums` holds kThreads / 32 values.
+template <int kThreads>
+__device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* prefix,
+                                             uint32_t* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t before = 0;
+  bool bad = false;
+  for (int base = 0; base < p.seqs; base += kThreads) {
+    const int b = base + int(threadIdx.x);
+    uint32_t mine = 0;
+    if (b < p.seqs) {
+      const PagedSeq s = paged_seq(p, b);
+      bad |= s.bad;
+      const int units = paged_units(p, s);
+      for (int u = 0; u < units; ++u) mine += uint32_t(paged_unit_tiles(p, s, u));
+    }
+    uint32_t scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) sums[warp] = scan;
+    __syncthreads();
+    uint32_t here = before, all = before;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const uint32_t v = sums[w];
+      if (w < warp) here += v;
+      all += v;
+    }
+    if (b < p.seqs) prefix[b] = here + scan - mine;
+    before = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[p.seqs] = before;
+  if (bad && blockIdx.x == 0 && p.status) record_error(p.status, kErrBadArgument, 60, 0);
+  __syncthreads();
+}
+
+struct PagedShare {
+  uint64_t total, per;
+  __device__ __forceinline__ PagedShare(const PagedParams& p, const uint32_t* prefix) {
+    total = uint64_t(prefix[p.seqs]) * uint32_t(p.kv_heads);
+    per = (total + uint32_t(p.grid) - 1) / uint32_t(p.grid);
+    if (per < uint32_t(p.min_share)) per = uint32_t(p.min_share);
+  }
+  __device__ __forceinline__ uint64_t begin(int cta) const {
+    const uint64_t w = per * uint32_t(cta);
+    return w < total ? w : total;
+  }
+};
+
+// The unit that contains tile w of the whole run, and the tiles [first, first + tiles)
+// that are the unit's.
+struct PagedUnit {
+  PagedSeq s;
+  int b, hk, unit, tiles;
+  uint64_t first;
+};
+
+__device__ __forceinline__ PagedUnit paged_find(const PagedParams& p, const uint32_t* prefix,
+                                                uint64_t w) {
+  PagedUnit u;
+  int lo = 0, hi = p.seqs;  // the last b with prefix[b] * kv_heads <= w
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (uint64_t(prefix[mid]) * uint32_t(p.kv_heads) <= w) lo = mid;
+    else hi = mid;
+  }
+  u.b = lo;
+  u.s = paged_seq(p, lo);
+  const uint32_t per_head = prefix[lo + 1] - prefix[lo];
+  const uint64_t base = uint64_t(prefix[lo]) * uint32_t(p.kv_heads);
+  u.hk = int((w - base) / per_head);
+  u.first = base + uint64_t(u.hk) * per_head;
+  u.unit = 0;
+  u.tiles = paged_unit_tiles(p, u.s, 0);
+  while (u.first + uint32_t(u.tiles) <= w) {
+    u.first += uint32_t(u.tiles);
+    u.tiles = paged_unit_tiles(p, u.s, ++u.unit);
+  }
+  return u;
+}
+
+// The unit behind `u`, which is not the last.
+__device__ __forceinline__ void paged_next(const PagedParams& p, const uint32_t* prefix,
+                                           PagedUnit& u) {
+  u.first += uint32_t(u.tiles);
+  if (++u.unit >= paged_units(p, u.s)) {
+    u.unit = 0;
+    if (++u.hk >= p.kv_heads) {
+      u.hk = 0;
+      do ++u.b;
+      while (u.b + 1 < p.seqs && prefix[u.b + 1] == prefix[u.b]);
+      u.s = paged_seq(p, u.b);
+    }
+  }
+  u.tiles = paged_unit_tiles(p, u.s, u.unit);
+}
+
+}  // namespace dev
+#endif
+
+// Few rows a key head (max_new * group <= 32).
+void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
+                         cudaStream_t stream);
+// More rows: tcgen05 tiles.
+void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                        const PagedParams& p, cudaStream_t stream);
+// Joins the parts; launched behind either.
+void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
+
+}  // namespace mgfa

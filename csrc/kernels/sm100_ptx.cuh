@@ -30,6 +30,7 @@ enum : uint32_t {
   kErrTagMismatch = 3,   // a received slot carried the wrong (step, owner) tag
   kErrBadArgument = 4,
   kErrBounds = 5,        // (debug builds) an access outside its buffer was skipped
+  kErrNoPages = 6,       // a cache has too few free pages
 };
 
 // Status word layout: code in bits [0,8), role/site in [8,16), step in [16,32).

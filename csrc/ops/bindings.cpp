@@ -49,6 +49,26 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rms_norm_bwd(
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_apply(
     torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
     torch::Tensor inv_freq, bool interleaved, double magnitude, double sign);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
+    torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new,
+    c10::optional<torch::Tensor> slots, bool causal, double scale,
+    c10::optional<torch::Tensor> out, bool want_lse, torch::Tensor status, int64_t wait_limit_ns);
+void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                 torch::Tensor refs, torch::Tensor grown);
+torch::Tensor cache_reserve(torch::Tensor k, torch::Tensor table, torch::Tensor lens,
+                            torch::Tensor refs, torch::Tensor grown, torch::Tensor status,
+                            torch::Tensor slots, torch::Tensor cu, int64_t tokens);
+void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                 torch::Tensor refs, torch::Tensor grown, torch::Tensor status, int64_t layer,
+                 torch::Tensor new_k, torch::Tensor new_v, torch::Tensor slots, torch::Tensor cu);
+void cache_free(torch::Tensor k, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
+                torch::Tensor grown, torch::Tensor status, torch::Tensor slots);
+void cache_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                torch::Tensor refs, torch::Tensor grown, torch::Tensor status, torch::Tensor src,
+                torch::Tensor dst, bool share);
+void cache_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                   torch::Tensor refs, torch::Tensor grown, torch::Tensor status);
 }  // namespace mgfa
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -93,6 +113,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_fp8", &mgfa::rms_norm_fp8);
   m.def("rms_norm_bwd", &mgfa::rms_norm_bwd);
   m.def("rotary_apply", &mgfa::rotary_apply);
+  m.def("paged_attention", &mgfa::paged_attention);
+  m.def("cache_check", &mgfa::cache_check);
+  m.def("cache_reserve", &mgfa::cache_reserve);
+  m.def("cache_write", &mgfa::cache_write);
+  m.def("cache_free", &mgfa::cache_free);
+  m.def("cache_fork", &mgfa::cache_fork);
+  m.def("cache_compact", &mgfa::cache_compact);
   mgfa::register_ring_engine(m);
   mgfa::register_ring_engine_p(m);
   mgfa::register_ring_exchange(m);

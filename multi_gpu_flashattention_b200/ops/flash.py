@@ -32,7 +32,8 @@ class KernelStatusError(RuntimeError):
 
 _CODES = {1: "mbarrier wait timed out", 2: "peer flag wait timed out",
           3: "received slot carried the wrong tag", 4: "bad argument",
-          5: "out-of-bounds store skipped (debug build)"}
+          5: "out-of-bounds store skipped (debug build)",
+          6: "the cache has too few free pages"}
 
 
 def _status_error(v: int, what: str) -> KernelStatusError:
@@ -140,11 +141,48 @@ def status_monitor(device) -> StatusMonitor:
     return m
 
 
+class HostStatus:
+    """The status word of the paged-cache calls that pass none, for one device, in
+    pinned host memory: kernels write it across the bus, only where they have an error
+    to report, and the host reads it like any variable. A call costs no read-back, and a
+    replayed CUDA graph reports as an eager call does. The next such call on the device
+    (and check_errors()) raises KernelStatusError for a non-zero word and re-arms it."""
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        self.word = torch.zeros(1, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        self._value = self.word.numpy()
+
+    def poll(self, wait: bool = False) -> None:
+        """Raise KernelStatusError if a kernel has reported an error so far; wait=True
+        waits for the device's work first."""
+        if wait and self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        v = int(self._value[0]) & 0xFFFFFFFF
+        if v:
+            self._value[0] = 0
+            raise _status_error(v, "paged cache")
+
+
+_HOST_STATUS: dict = {}
+
+
+def host_status(device) -> HostStatus:
+    """The HostStatus of `device` (created on first use)."""
+    h = _HOST_STATUS.get(device)
+    if h is None:
+        h = _HOST_STATUS[device] = HostStatus(device)
+    return h
+
+
 def check_errors(device=None, wait: bool = True) -> None:
     """Raise KernelStatusError if a kernel launched by a public call (one that
     was given no explicit status word) on `device` (default: every device used
     so far) reported an error. wait=True first waits for those calls to finish;
     wait=False only looks at the ones already finished."""
+    for d, h in list(_HOST_STATUS.items()):
+        if device is None or d == torch.device(device):
+            h.poll(wait=wait)
     mons = [status_monitor(device)] if device is not None else list(_MONITORS.values())
     for m in mons:
         m.poll(wait=wait)

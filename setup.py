@@ -53,6 +53,7 @@ if which in ("all", "cuda"):
                 "csrc/ops/bindings.cpp",
                 "csrc/ops/attn_api.cpp",
                 "csrc/ops/layer_api.cpp",
+                "csrc/ops/paged_api.cpp",
                 "csrc/kernels/umma_probe.cu",
                 "csrc/kernels/flash_fwd_sm100.cu",
                 "csrc/kernels/attn_fwd_persistent.cu",
@@ -61,6 +62,9 @@ if which in ("all", "cuda"):
                 "csrc/kernels/legacy_fp32.cu",
                 "csrc/kernels/rms_norm.cu",
                 "csrc/kernels/rotary.cu",
+                "csrc/kernels/paged_decode.cu",
+                "csrc/kernels/paged_chunk.cu",
+                "csrc/kernels/paged_cache.cu",
                 "csrc/comm/symmetric.cpp",
                 "csrc/comm/ring_engine.cpp",
                 "csrc/comm/ring_engine_p.cpp",
