@@ -9,10 +9,13 @@
 // h is rounded before the norm reads it, so that y, and the backward pass that has
 // only the stored h, belong to the same stream. All sums are in fp32.
 //
-// Bound by memory: every tensor is read or written once. A row stays in the
-// registers of the T threads that own it (N vectors of 16 bytes each, or single
-// elements where a row is not 16-byte aligned), so the statistics and the output
-// need one pass; T grows with the row so that a thread holds at most 8 vectors.
+// Bound by memory: every tensor is read or written once. At 16384 x 4096 bf16 with a
+// residual the forward takes 85 us (6.3 TB/s) and the backward 112 us (4.8 TB/s, with
+// 9 us for dw's parts). A row stays in the
+// registers of the T threads that own it (N vectors each), so the statistics and the
+// output need one pass. A vector is 16 bytes, or 2 elements or one where the rows'
+// width or alignment asks for it; T grows with the row, which leaves a thread 8 to 16
+// elements up to a width of 4096, and 32 beyond.
 #include "rms_norm.cuh"
 
 #include <cuda_bf16.h>
@@ -20,38 +23,148 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
+
+#include "pairs.cuh"
 
 namespace mgfa {
 namespace {
 
-constexpr int kMaxThreads = 512;
+using namespace mgfa::dev;
 
-template <class E>
-__device__ __forceinline__ float to_f(E v);
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f(float v) { return v; }
-template <class E>
-__device__ __forceinline__ E from_f(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ float from_f(float v) { return v; }
+// Threads of a block whose threads hold `elements` (shape_of).
+constexpr int max_threads(int elements) { return elements <= 16 ? 256 : 512; }
 
-template <class E, int V>
-struct alignas(sizeof(E) * V) Pack {
-  E e[V];
+// How a thread's share of a row lies in memory.
+enum : int {
+  kAligned = 0,  // rows start on 16-byte boundaries and dim is a multiple of a vector
+  kShifted = 1,  // row r starts r * dim elements behind one: the vectors are the aligned ones
+                 // that cover the row, and its first and last are taken by elements
+  kSingle = 2,   // single elements, for any strides
 };
+
+// A thread's share of a row: N vectors of V elements, vector j at column
+// (j * blockDim.x + threadIdx.x) * V - shift. N * V is even; columns outside the row are
+// zero.
+template <class E, int V, int N, int kLay>
+struct Share {
+  using P = PairOf<E>;
+  using Raw = typename P::Raw;
+  using Vec = typename Bytes<V * sizeof(E)>::T;
+  static constexpr int kPairs = N * V / 2;
+  union {
+    Raw raw[kPairs];
+    Vec vec[N];
+  };
+  static __device__ __forceinline__ int shift(int64_t row, int dim) {
+    return kLay == kShifted ? int(uint32_t(row) * uint32_t(dim) % V) : 0;
+  }
+  static __device__ __forceinline__ int col(int j, int shift) {
+    return (j * int(blockDim.x) + int(threadIdx.x)) * V - shift;
+  }
+  static __device__ __forceinline__ bool whole(int c, int dim) {
+    return kLay == kShifted ? c >= 0 && c + V <= dim : c < dim;
+  }
+  // `last`: no row follows. Elsewhere a shifted row's first and last vector reach into its
+  // neighbours, whose elements are cut.
+  __device__ __forceinline__ void load(const void* row_at, int dim, int shift, bool live, bool last) {
+    const E* row = static_cast<const E*>(row_at);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = col(j, shift);
+      Vec v = {};
+      if (live && c < dim && (kLay != kShifted || !last || c + V <= dim))
+        v = __ldg(reinterpret_cast<const Vec*>(row + c));
+      vec[j] = v;
+    }
+    if constexpr (kLay == kShifted) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = col(j, shift);
+        if (!live || c >= dim || whole(c, dim)) continue;
+        uint16_t* half = reinterpret_cast<uint16_t*>(&vec[j]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const bool in = c + i >= 0 && c + i < dim;
+          if constexpr (sizeof(E) == 2) {
+            uint16_t x = half[i];
+            if (last && c + V > dim && in) x = reinterpret_cast<const uint16_t*>(row)[c + i];
+            half[i] = in ? x : uint16_t(0);
+          } else {
+            float x = reinterpret_cast<float*>(&vec[j])[i];
+            if (last && c + V > dim && in) x = reinterpret_cast<const float*>(row)[c + i];
+            reinterpret_cast<float*>(&vec[j])[i] = in ? x : 0.f;
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(void* row_at, int dim, int shift) const {
+    E* row = static_cast<E*>(row_at);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = col(j, shift);
+      if (whole(c, dim)) *reinterpret_cast<Vec*>(row + c) = vec[j];
+      if constexpr (kLay == kShifted) {
+        if (c < dim && !whole(c, dim)) {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            float e[2];
+            f2_unpack(at(j * V / 2 + i), e[0], e[1]);  // exact: they are E's already
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (c + 2 * i + k >= 0 && c + 2 * i + k < dim) row[c + 2 * i + k] = from_f<E>(e[k]);
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ uint64_t at(int k) const { return P::wide(raw[k]); }
+  __device__ __forceinline__ void put(int k, uint64_t v) { raw[k] = P::narrow(v); }
+  // Says that the pairs may have changed, so that the compiler widens them again instead
+  // of keeping both forms in registers.
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+      if constexpr (sizeof(Raw) == 4) asm volatile("" : "+r"(raw[k]));
+      else asm volatile("" : "+l"(raw[k]));
+    }
+  }
+};
+
+// The weights of a thread's columns as fp32 pairs, from E or fp32.
+template <class E, int V, int N, int kLay>
+__device__ __forceinline__ void load_w(const void* w, int weight_f32, int dim, int shift,
+                                       uint64_t (&f)[N * V / 2]) {
+  using S = Share<E, V, N, kLay>;
+  if (kLay != kShifted && !weight_f32) {
+    S s;
+    s.load(w, dim, 0, true, true);
+#pragma unroll
+    for (int k = 0; k < N * V / 2; ++k) f[k] = s.at(k);
+  } else {
+    float e[N * V];
+#pragma unroll
+    for (int i = 0; i < N * V; ++i) {
+      const int c = S::col(i / V, shift) + i % V;
+      e[i] = c < 0 || c >= dim ? 0.f
+             : weight_f32     ? __ldg(static_cast<const float*>(w) + c)
+                              : to_f(static_cast<const E*>(w)[c]);
+    }
+#pragma unroll
+    for (int k = 0; k < N * V / 2; ++k) f[k] = f2_pack(e[2 * k], e[2 * k + 1]);
+  }
+}
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+__device__ __forceinline__ float f2_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
 }
 
 struct Sum {
@@ -73,236 +186,213 @@ __device__ __forceinline__ float row_reduce(float v, float* buf) {
   __syncthreads();  // the previous reduction's readers are done
   if ((threadIdx.x & 31) == 0) row[threadIdx.x >> 5] = v;
   __syncthreads();
-  float t = row[0];
-  for (int i = 1; i < warps; ++i) t = Op::of(t, row[i]);
-  return t;
+  // at most 16 warps, in an order that is every thread's
+  const int lane = threadIdx.x & 31;
+  v = lane < warps ? row[lane] : 0.f;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = Op::of(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
-template <class E, int V, int N>
-__device__ __forceinline__ void load_w(const void* w, int weight_f32, int dim, float (&f)[N][V]) {
+// The rows that a CTA of block (T, R) takes, R at a time (T threads a row): every
+// gridDim.x-th set. kShifted: those whose columns are the same threads', rows V * k apart;
+// gridDim.x is a multiple of V.
+template <int V, int kLay>
+struct Rows {
+  static constexpr int kApart = kLay == kShifted ? V : 1;
+  int64_t lead, step;  // the first row, and from set to set
+  __device__ __forceinline__ Rows()
+      : lead(int64_t(blockIdx.x / kApart) * blockDim.y * kApart + blockIdx.x % kApart),
+        step(int64_t(gridDim.x) * blockDim.y) {}
+  static __device__ __forceinline__ int64_t mine(int64_t base) { return base + threadIdx.y * kApart; }
+};
+
+// The thread's weights in E, held in registers where no vector load reaches them.
+template <class E, int V, int N, int kLay>
+struct Weights {
+  Share<E, V, N, kLay> held;
+  const void* w;
+  int weight_f32, dim, shift;
+  __device__ __forceinline__ Weights(const void* weight, int f32, int d, int s)
+      : w(weight), weight_f32(f32), dim(d), shift(s) {
+    if constexpr (kLay == kShifted) {
+      if (sizeof(E) == 4 || !f32) {
+        uint64_t f[N * V / 2];
+        load_w<E, V, N, kLay>(w, f32, dim, shift, f);
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * V;
-    if (c < dim) {
-      if (weight_f32) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[j][i] = __ldg(static_cast<const float*>(w) + c + i);
-      } else {
-        const Pack<E, V> p = *reinterpret_cast<const Pack<E, V>*>(static_cast<const E*>(w) + c);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[j][i] = to_f(p.e[i]);
+        for (int k = 0; k < N * V / 2; ++k) held.put(k, f[k]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[j][i] = 0.f;
     }
   }
-}
+  __device__ __forceinline__ void get(uint64_t (&f)[N * V / 2]) {
+    if (kLay == kShifted && (sizeof(E) == 4 || !weight_f32)) {
+      held.renew();
+#pragma unroll
+      for (int k = 0; k < N * V / 2; ++k) f[k] = held.at(k);
+    } else {
+      asm volatile("" : "+l"(w));  // read them again
+      load_w<E, V, N, kLay>(w, weight_f32, dim, shift, f);
+    }
+  }
+};
 
-// V elements per vector, N vectors per thread; block (T, R): R rows of T threads.
-template <class E, int V, int N, bool kRes, bool k8>
-__global__ void __launch_bounds__(kMaxThreads) rms_norm_fwd_kernel(const NormFwdParams p) {
+template <class E, int V, int N, int kLay, bool kRes, bool k8>
+__global__ void __launch_bounds__(max_threads(N * V)) rms_norm_fwd_kernel(const NormFwdParams p) {
+  using S = Share<E, V, N, kLay>;
   __shared__ float buf[8 * 32];
-  const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  const bool live = row < p.rows;  // rows past the end take part in the barriers only
-  const E* x = static_cast<const E*>(p.x) + (live ? row : 0) * p.x_stride;
-  const E* r = kRes ? static_cast<const E*>(p.residual) + (live ? row : 0) * p.r_stride : nullptr;
-  Pack<E, V> h[N];
+  constexpr int kPairs = N * V / 2;
+  const Rows<V, kLay> rows;
+  const int shift = S::shift(rows.mine(rows.lead), p.dim);
+  Weights<E, V, N, kLay> weights(p.weight, p.weight_f32, p.dim, shift);
+  for (int64_t base = rows.lead; base < p.rows; base += rows.step) {
+    const int64_t row = rows.mine(base);
+    const bool live = row < p.rows;  // rows past the end take part in the barriers only
+    S h;
+    h.load(static_cast<const E*>(p.x) + row * p.x_stride, p.dim, shift, live, row + 1 >= p.rows);
+    if constexpr (kRes) {
+      S r;
+      r.load(static_cast<const E*>(p.residual) + row * p.r_stride, p.dim, shift, live, row + 1 >= p.rows);
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * V;
-    if (c < p.dim) h[j] = *reinterpret_cast<const Pack<E, V>*>(x + c);
-  }
-  if constexpr (kRes) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      if (c < p.dim) {
-        const Pack<E, V> q = *reinterpret_cast<const Pack<E, V>*>(r + c);
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[j].e[i] = from_f<E>(to_f(h[j].e[i]) + to_f(q.e[i]));
-      }
+      for (int k = 0; k < kPairs; ++k) h.put(k, f2_add(h.at(k), r.at(k)));
+      if (live) h.store(static_cast<E*>(p.h) + row * p.dim, p.dim, shift);
     }
-  }
-  float w[N][V];
-  load_w<E, V, N>(p.weight, p.weight_f32, p.dim, w);
-  float sum = 0.f;
+    uint64_t w[kPairs];
+    weights.get(w);
+    uint64_t acc[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * V;
-    if (c < p.dim) {
+    for (int k = 0; k < kPairs; ++k) acc[k & 1] = f2_fma(h.at(k), h.at(k), acc[k & 1]);
+    const float sum = row_reduce<Sum>(f2_sum(f2_add(acc[0], acc[1])), buf);
+    const float rstd = 1.f / sqrtf(sum / float(p.dim) + p.eps);
+    const uint64_t rstd2 = f2_pack(rstd, rstd);
+    if (p.rstd && live && threadIdx.x == 0) p.rstd[row] = rstd;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float f = to_f(h[j].e[i]);
-        sum = fmaf(f, f, sum);
-      }
-      if (kRes && live)
-        *reinterpret_cast<Pack<E, V>*>(static_cast<E*>(p.h) + row * p.dim + c) = h[j];
-    }
-  }
-  sum = row_reduce<Sum>(sum, buf);
-  const float rstd = 1.f / sqrtf(sum / float(p.dim) + p.eps);
-  if (p.rstd && live && threadIdx.x == 0) p.rstd[row] = rstd;
-  if constexpr (!k8) {
-    if (!live) return;
+    for (int k = 0; k < kPairs; ++k) w[k] = f2_mul(f2_mul(h.at(k), rstd2), w[k]);  // the output
+    if constexpr (!k8) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      if (c < p.dim) {
-        Pack<E, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o.e[i] = from_f<E>(to_f(h[j].e[i]) * rstd * w[j][i]);
-        *reinterpret_cast<Pack<E, V>*>(static_cast<E*>(p.y) + row * p.dim + c) = o;
-      }
-    }
-  } else {
-    float top[N], row_top = 0.f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      top[j] = 0.f;
-      if (c < p.dim) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          w[j][i] *= to_f(h[j].e[i]) * rstd;  // from here on the output
-          top[j] = max_nan(top[j], fabsf(w[j][i]));
-        }
-      }
-      row_top = max_nan(row_top, top[j]);
-    }
-    // A group is a power of two of columns, V * (at most 32) aligned lanes of a warp.
-    if (p.group == 0) {
-      row_top = row_reduce<MaxNan>(row_top, buf);
-#pragma unroll
-      for (int j = 0; j < N; ++j) top[j] = row_top;
+      for (int k = 0; k < kPairs; ++k) h.put(k, w[k]);
+      if (live) h.store(static_cast<E*>(p.y) + row * p.dim, p.dim, shift);
     } else {
-      const int lanes = p.group / V;
+      float y[N * V];
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        for (int o = lanes >> 1; o > 0; o >>= 1)
-          top[j] = max_nan(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-    }
-    if (!live) return;
-    const int groups = p.group ? p.dim / p.group : 1;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      if (c >= p.dim) continue;
-      float scale = top[j] / 448.f;      // 448: the largest e4m3 value
-      if (!(scale > 0.f)) scale = 1.f;   // nothing but zeros, or a NaN
-      if (p.group ? c % p.group == 0 : c == 0)
-        p.scale[row * groups + (p.group ? c / p.group : 0)] = scale;
-      Pack<uint8_t, V> o;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        o.e[i] = __nv_cvt_float_to_fp8(w[j][i] / scale, __NV_SATFINITE, __NV_E4M3);
-      *reinterpret_cast<Pack<uint8_t, V>*>(static_cast<uint8_t*>(p.y) + row * p.dim + c) = o;
-    }
-  }
-}
-
-// Each CTA takes every gridDim.x-th set of R rows and keeps its columns' part of dw
-// in registers. While a row is reduced, the next one's loads are under way (N <= 2;
-// wider rows have the loads of 4 vectors and more a tensor in flight as it is, and
-// no registers to hold two rows). The parts are added by norm_dw_kernel, in the CTAs'
-// order, so dw does not depend on timing.
-template <class E, int V, int N>
-__global__ void __launch_bounds__(kMaxThreads) rms_norm_bwd_kernel(const NormBwdParams p) {
-  constexpr bool kAhead = N * V * sizeof(E) <= 32;
-  extern __shared__ float sh[];  // row_reduce: blockDim.y * 32; then dw: blockDim.y * dim
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t step = int64_t(gridDim.x) * blockDim.y;
-  float w[N][V], dw[N][V];
-  if constexpr (kAhead) load_w<E, V, N>(p.weight, p.weight_f32, p.dim, w);
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) dw[j][i] = 0.f;
-  Pack<E, V> h[N], dy[N], dh[N];
-  float rstd = 0.f;
-  auto load = [&](int64_t row) {
-    const bool live = row < p.rows;
-    const int64_t at = live ? row : 0;
-    rstd = live ? __ldg(p.rstd + at) : 0.f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[j].e[i] = dy[j].e[i] = dh[j].e[i] = from_f<E>(0.f);
-      if (live && c < p.dim) {
-        if (p.dy) {
-          h[j] = *reinterpret_cast<const Pack<E, V>*>(static_cast<const E*>(p.h) + at * p.h_stride + c);
-          dy[j] = *reinterpret_cast<const Pack<E, V>*>(static_cast<const E*>(p.dy) + at * p.dy_stride + c);
-        }
-        if (p.dh)
-          dh[j] = *reinterpret_cast<const Pack<E, V>*>(static_cast<const E*>(p.dh) + at * p.dh_stride + c);
-      }
-    }
-  };
-  // A CTA's first row exists, so every thread of the CTA makes the same number of steps.
-  const int64_t first = int64_t(blockIdx.x) * blockDim.y;
-  if (kAhead && first < p.rows) load(first + threadIdx.y);
-  for (int64_t base = first; base < p.rows; base += step) {
-    const int64_t row = base + threadIdx.y;
-    if constexpr (!kAhead) {
-      load(row);
-      load_w<E, V, N>(p.weight, p.weight_f32, p.dim, w);
-    }
-    Pack<E, V> h1[N], dy1[N], dh1[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      h1[j] = h[j];
-      dy1[j] = dy[j];
-      dh1[j] = dh[j];
-    }
-    const float rs = rstd;
-    if (kAhead && base + step < p.rows) load(row + step);
-    float dot = 0.f;  // sum of w dy n
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float dn = to_f(dy1[j].e[i]) * (to_f(h1[j].e[i]) * rs);
-        dw[j][i] += dn;
-        dot = fmaf(dn, w[j][i], dot);
-      }
-    dot = row_reduce<Sum>(dot, sh) / float(p.dim);
-    if (row < p.rows) {
+      for (int k = 0; k < kPairs; ++k) f2_unpack(w[k], y[2 * k], y[2 * k + 1]);
+      float top[N], row_top = 0.f;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int c = (j * blockDim.x + threadIdx.x) * V;
-        if (c < p.dim) {
-          Pack<E, V> o;
+        top[j] = 0.f;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float g = to_f(dy1[j].e[i]) * w[j][i] - to_f(h1[j].e[i]) * rs * dot;
-            o.e[i] = from_f<E>(fmaf(rs, g, to_f(dh1[j].e[i])));
-          }
-          *reinterpret_cast<Pack<E, V>*>(static_cast<E*>(p.dx) + row * p.dim + c) = o;
+        for (int i = 0; i < V; ++i)  // a NaN statistic makes 0 * NaN of columns outside the row
+          if (S::col(j, shift) + i >= 0 && S::col(j, shift) + i < p.dim)
+            top[j] = max_nan(top[j], fabsf(y[j * V + i]));
+        row_top = max_nan(row_top, top[j]);
+      }
+      // A group is a power of two of columns, V * (at most 32) aligned lanes of a warp.
+      if (p.group == 0) {
+        row_top = row_reduce<MaxNan>(row_top, buf);
+#pragma unroll
+        for (int j = 0; j < N; ++j) top[j] = row_top;
+      } else {
+        const int lanes = p.group / V;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          for (int o = lanes >> 1; o > 0; o >>= 1)
+            top[j] = max_nan(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+      }
+      const int groups = p.group ? p.dim / p.group : 1;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = S::col(j, shift);
+        if (!live || c >= p.dim) continue;
+        float scale = top[j] / 448.f;      // 448: the largest e4m3 value
+        if (!(scale > 0.f)) scale = 1.f;   // nothing but zeros, or a NaN
+        if (p.group ? c % p.group == 0 : c <= 0)
+          p.scale[row * groups + (p.group ? c / p.group : 0)] = scale;
+        uint8_t* dst = static_cast<uint8_t*>(p.y) + row * p.dim + c;
+        if (V == 1 || !S::whole(c, p.dim)) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (c + i >= 0 && c + i < p.dim)
+              dst[i] = __nv_cvt_float_to_fp8(y[j * V + i] / scale, __NV_SATFINITE, __NV_E4M3);
+        } else if constexpr (V > 1) {
+          uint16_t o[V / 2];
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i)
+            o[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[j * V + 2 * i] / scale, y[j * V + 2 * i + 1] / scale),
+                                            __NV_SATFINITE, __NV_E4M3);
+          *reinterpret_cast<typename Bytes<V>::T*>(dst) = *reinterpret_cast<typename Bytes<V>::T*>(o);
         }
       }
     }
+  }
+}
+
+// A CTA keeps its columns' part of dw in registers over all its rows; several CTAs of an
+// SM cover one another's reductions. Aligned weights are read again for every row (they
+// stay in L1) to leave the registers to the rows. The parts are added by norm_dw_kernel,
+// in the CTAs' order, so dw does not depend on timing.
+template <class E, int V, int N, int kLay>
+__global__ void __launch_bounds__(max_threads(N * V), N * V > 16 ? 1 : sizeof(E) == 4 ? 2 : 3)
+    rms_norm_bwd_kernel(const NormBwdParams p) {
+  using S = Share<E, V, N, kLay>;
+  constexpr int kPairs = N * V / 2;
+  extern __shared__ float sh[];  // row_reduce: blockDim.y * 32; then dw: blockDim.y * dim
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint64_t dw[kPairs];
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k) dw[k] = f2_pack(0.f, 0.f);
+  const float inv_dim = 1.f / float(p.dim);
+  const Rows<V, kLay> rows;
+  const int shift = S::shift(rows.mine(rows.lead), p.dim);
+  Weights<E, V, N, kLay> weights(p.weight, p.weight_f32, p.dim, shift);
+  for (int64_t base = rows.lead; base < p.rows; base += rows.step) {
+    const int64_t row = rows.mine(base);
+    const bool live = row < p.rows;
+    const bool last = row + 1 >= p.rows;
+    S h, dy, dh;
+    h.load(static_cast<const E*>(p.h) + row * p.h_stride, p.dim, shift, live && p.dy, last);
+    dy.load(static_cast<const E*>(p.dy) + row * p.dy_stride, p.dim, shift, live && p.dy, last);
+    dh.load(static_cast<const E*>(p.dh) + row * p.dh_stride, p.dim, shift, live && p.dh, last);
+    const float rstd = live ? __ldg(p.rstd + row) : 0.f;
+    const uint64_t rstd2 = f2_pack(rstd, rstd);
+    uint64_t acc = f2_pack(0.f, 0.f);  // sum of w dy n
+    {
+      uint64_t w[kPairs];
+      weights.get(w);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const uint64_t t = f2_mul(dy.at(k), f2_mul(h.at(k), rstd2));
+        dw[k] = f2_add(dw[k], t);
+        acc = f2_fma(t, w[k], acc);
+      }
+    }
+    const float dot = row_reduce<Sum>(f2_sum(acc), sh) * inv_dim;  // mean of w dy n
+    const float c = -dot * rstd;                                    // dx = rstd (w dy + c h) + dh
+    const uint64_t c2 = f2_pack(c, c);
+    h.renew();
+    dy.renew();
+    {
+      uint64_t w[kPairs];
+      weights.get(w);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k)
+        dh.put(k, f2_fma(rstd2, f2_fma(dy.at(k), w[k], f2_mul(c2, h.at(k))), dh.at(k)));
+    }
+    if (live) dh.store(static_cast<E*>(p.dx) + row * p.dim, p.dim, shift);
   }
   if (!p.dw_part) return;
   float* part = p.dw_part + int64_t(blockIdx.x) * p.dim;
-  if (blockDim.y == 1) {
+  float* to = blockDim.y == 1 ? part : sh + threadIdx.y * p.dim;
+  if (blockDim.y > 1) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      if (c < p.dim)
+  for (int k = 0; k < kPairs; ++k) {
+    float e[2];
+    f2_unpack(dw[k], e[0], e[1]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) part[c + i] = dw[j][i];
+    for (int i = 0; i < 2; ++i) {
+      const int at = 2 * k + i, col = S::col(at / V, shift) + at % V;
+      if (col >= 0 && col < p.dim) to[col] = e[i];
     }
-    return;
   }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * V;
-    if (c < p.dim)
-#pragma unroll
-      for (int i = 0; i < V; ++i) sh[threadIdx.y * p.dim + c + i] = dw[j][i];
-  }
+  if (blockDim.y == 1) return;
   __syncthreads();
   for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < p.dim; c += blockDim.x * blockDim.y) {
     float t = 0.f;
@@ -333,80 +423,92 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int pa
 }
 
 struct Shape {
-  int n;      // vectors per thread
+  int n;      // vectors of a thread
   dim3 block;
 };
 
-// T threads (a multiple of 32) per row with n vectors each, and rows packed until a
-// block has 256 threads. dim <= 16384, so n <= 4 (16-bit vectors), 8 (fp32 vectors) or
-// 32 (single elements).
-Shape shape_of(int dim, int v) {
-  const int vecs = (dim + v - 1) / v;
-  int n = vecs > 256 ? 2 : 1;
-  while (vecs > n * kMaxThreads) n *= 2;
-  const int t = ((vecs + n - 1) / n + 31) / 32 * 32;
-  return {n, dim3(t, std::max(1, std::min(8, 256 / t)))};
-}
-
-template <class E, int V, int N>
-void fwd_n(const NormFwdParams& p, dim3 block, cudaStream_t s) {
-  const dim3 grid(unsigned((p.rows + block.y - 1) / block.y));
-  if (p.scale) {
-    if (p.residual) rms_norm_fwd_kernel<E, V, N, true, true><<<grid, block, 0, s>>>(p);
-    else rms_norm_fwd_kernel<E, V, N, false, true><<<grid, block, 0, s>>>(p);
-  } else {
-    if (p.residual) rms_norm_fwd_kernel<E, V, N, true, false><<<grid, block, 0, s>>>(p);
-    else rms_norm_fwd_kernel<E, V, N, false, false><<<grid, block, 0, s>>>(p);
-  }
+// Elements of a thread, then T threads (a multiple of 32) for a row, and rows packed
+// until a block has 256 threads. At 16384 x 4096 and 32768 x 2048 bf16, 16 elements take
+// 84 and 84 us forward and 107 and 108 us back; 32 take 83 us and 131 us at 4096, and 8
+// take 91 us and 126 us at 2048.
+Shape shape_of(int dim, int v, int lay) {
+  const int covered = lay == kShifted ? dim + v - 1 : dim;
+  int e = covered <= 512 ? 8 : covered <= 4096 ? 16 : 32;
+  if (e < v) e = v;
+  const int t = ((covered + e - 1) / e + 31) / 32 * 32;
+  return {e / v, dim3(t, std::max(1, std::min(8, 256 / t)))};
 }
 
 template <class E>
-void fwd_e(const NormFwdParams& p, cudaStream_t s) {
-  constexpr int kV = 16 / sizeof(E);
-  const Shape sh = shape_of(p.dim, p.vec ? kV : 1);
-  if (p.vec) {
-    switch (sh.n) {
-      case 1: return fwd_n<E, kV, 1>(p, sh.block, s);
-      case 2: return fwd_n<E, kV, 2>(p, sh.block, s);
-      case 4: return fwd_n<E, kV, 4>(p, sh.block, s);
-      default:
-        if constexpr (sizeof(E) == 4) fwd_n<E, kV, 8>(p, sh.block, s);
-        return;
+int vec_elements(int lay) { return lay == kSingle ? 1 : 16 / int(sizeof(E)); }
+
+// f(vector's elements, number, layout) as compile-time constants, for what shape_of gives.
+template <class E, class F>
+void with_shape(int lay, int n, F f) {
+  auto pick = [&](auto vc, auto lc) {
+    constexpr int V = decltype(vc)::value;
+    switch (n * V) {
+      case 8: return f(vc, std::integral_constant<int, 8 / V>(), lc);
+      case 16: return f(vc, std::integral_constant<int, 16 / V>(), lc);
+      default: return f(vc, std::integral_constant<int, 32 / V>(), lc);
     }
-  }
-  switch (sh.n) {
-    case 1: case 2: return fwd_n<E, 1, 2>(p, sh.block, s);
-    case 4: case 8: return fwd_n<E, 1, 8>(p, sh.block, s);
-    default: return fwd_n<E, 1, 32>(p, sh.block, s);
-  }
+  };
+  using Full = std::integral_constant<int, 16 / sizeof(E)>;
+  if (lay == kAligned) pick(Full(), std::integral_constant<int, kAligned>());
+  else if (lay == kShifted) pick(Full(), std::integral_constant<int, kShifted>());
+  else pick(std::integral_constant<int, 1>(), std::integral_constant<int, kSingle>());
 }
 
-template <class E, int V, int N>
-void bwd_n(const NormBwdParams& p, dim3 block, int parts, cudaStream_t s) {
-  size_t smem = block.y * 32 * sizeof(float);
-  if (block.y > 1) smem = std::max(smem, size_t(block.y) * p.dim * sizeof(float));
-  rms_norm_bwd_kernel<E, V, N><<<parts, block, smem, s>>>(p);
+// CTAs for all rows, `most` a SM at a time; kShifted: a multiple of the vectors' elements.
+int64_t ctas_of(const Shape& sh, int layout, int v, int64_t rows, int64_t most) {
+  const int64_t sets = (rows + sh.block.y - 1) / sh.block.y, apart = layout == kShifted ? v : 1;
+  return (std::min(sets, most) + apart - 1) / apart * apart;
+}
+
+template <class E>
+void fwd_e(const NormFwdParams& p, int sm_count, cudaStream_t s) {
+  const int v = vec_elements<E>(p.layout);
+  const Shape sh = shape_of(p.dim, v, p.layout);
+  with_shape<E>(p.layout, sh.n, [&](auto vc, auto n, auto lay) {
+    constexpr int V = decltype(vc)::value, N = decltype(n)::value, L = decltype(lay)::value;
+    auto fn = p.scale ? (p.residual ? rms_norm_fwd_kernel<E, V, N, L, true, true>
+                                    : rms_norm_fwd_kernel<E, V, N, L, false, true>)
+                      : (p.residual ? rms_norm_fwd_kernel<E, V, N, L, true, false>
+                                    : rms_norm_fwd_kernel<E, V, N, L, false, false>);
+    // A CTA a set of rows; kShifted, whose weights are slow to load, as many as run at once.
+    int64_t most = p.rows;
+    if (L == kShifted) {
+      int n_sm = 1;
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n_sm, fn, int(sh.block.x * sh.block.y), 0);
+      most = int64_t(sm_count) * std::max(1, n_sm);
+    }
+    fn<<<unsigned(ctas_of(sh, L, v, p.rows, most)), sh.block, 0, s>>>(p);
+  });
+}
+
+size_t bwd_smem(int dim, const Shape& sh) {
+  const size_t sums = sh.block.y * 32 * sizeof(float);
+  return sh.block.y > 1 ? std::max(sums, size_t(sh.block.y) * dim * sizeof(float)) : sums;
+}
+
+template <class E>
+int bwd_resident(const NormBwdParams& p, const Shape& sh) {
+  int n = 1;
+  with_shape<E>(p.layout, sh.n, [&](auto v, auto k, auto lay) {
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+        &n, rms_norm_bwd_kernel<E, decltype(v)::value, decltype(k)::value, decltype(lay)::value>,
+        int(sh.block.x * sh.block.y), bwd_smem(p.dim, sh));
+  });
+  return std::max(1, n);
 }
 
 template <class E>
 void bwd_e(const NormBwdParams& p, int parts, cudaStream_t s) {
-  constexpr int kV = 16 / sizeof(E);
-  const Shape sh = shape_of(p.dim, p.vec ? kV : 1);
-  if (p.vec) {
-    switch (sh.n) {
-      case 1: bwd_n<E, kV, 1>(p, sh.block, parts, s); break;
-      case 2: bwd_n<E, kV, 2>(p, sh.block, parts, s); break;
-      case 4: bwd_n<E, kV, 4>(p, sh.block, parts, s); break;
-      default:
-        if constexpr (sizeof(E) == 4) bwd_n<E, kV, 8>(p, sh.block, parts, s);
-    }
-  } else {
-    switch (sh.n) {
-      case 1: case 2: bwd_n<E, 1, 2>(p, sh.block, parts, s); break;
-      case 4: case 8: bwd_n<E, 1, 8>(p, sh.block, parts, s); break;
-      default: bwd_n<E, 1, 32>(p, sh.block, parts, s);
-    }
-  }
+  const Shape sh = shape_of(p.dim, vec_elements<E>(p.layout), p.layout);
+  with_shape<E>(p.layout, sh.n, [&](auto v, auto n, auto lay) {
+    rms_norm_bwd_kernel<E, decltype(v)::value, decltype(n)::value, decltype(lay)::value>
+        <<<parts, sh.block, bwd_smem(p.dim, sh), s>>>(p);
+  });
   if (!p.dw_part) return;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.dim + 31) / 32);
@@ -422,23 +524,29 @@ void bwd_e(const NormBwdParams& p, int parts, cudaStream_t s) {
   else cudaLaunchKernelEx(&cfg, norm_dw_kernel<E>, part, parts, p.dim, static_cast<E*>(p.dw));
 }
 
-int vec_of(NormType t, int vec) { return vec ? (t == NormType::kF32 ? 4 : 8) : 1; }
-
 }  // namespace
 
-void rms_norm_fwd_launch(NormType t, const NormFwdParams& p, cudaStream_t stream) {
+void rms_norm_fwd_launch(NormType t, const NormFwdParams& p, int sm_count, cudaStream_t stream) {
   switch (t) {
-    case NormType::kBf16: return fwd_e<__nv_bfloat16>(p, stream);
-    case NormType::kF16: return fwd_e<__half>(p, stream);
-    default: return fwd_e<float>(p, stream);
+    case NormType::kBf16: return fwd_e<__nv_bfloat16>(p, sm_count, stream);
+    case NormType::kF16: return fwd_e<__half>(p, sm_count, stream);
+    default: return fwd_e<float>(p, sm_count, stream);
   }
 }
 
-int rms_norm_bwd_parts(NormType t, int64_t rows, int dim, int vec, int sm_count) {
-  const Shape sh = shape_of(dim, vec_of(t, vec));
-  const int threads = int(sh.block.x * sh.block.y);
-  const int64_t sets = (rows + sh.block.y - 1) / sh.block.y;
-  return int(std::min<int64_t>(sets, int64_t(sm_count) * std::max(1, 768 / threads)));
+template <class E>
+static int bwd_parts(const NormBwdParams& p, int sm_count) {
+  const int v = vec_elements<E>(p.layout);
+  const Shape sh = shape_of(p.dim, v, p.layout);
+  return int(ctas_of(sh, p.layout, v, p.rows, int64_t(sm_count) * bwd_resident<E>(p, sh)));
+}
+
+int rms_norm_bwd_parts(NormType t, const NormBwdParams& p, int sm_count) {
+  switch (t) {
+    case NormType::kBf16: return bwd_parts<__nv_bfloat16>(p, sm_count);
+    case NormType::kF16: return bwd_parts<__half>(p, sm_count);
+    default: return bwd_parts<float>(p, sm_count);
+  }
 }
 
 void rms_norm_bwd_launch(NormType t, const NormBwdParams& p, int parts, cudaStream_t stream) {

@@ -23,7 +23,8 @@ struct NormFwdParams {
   int dim = 0;
   int group = 0;
   int weight_f32 = 0;
-  int vec = 0;  // 1: every row is 16-byte aligned and dim a multiple of a 16-byte vector
+  int layout = 2;  // 0: rows on 16-byte boundaries, dim a multiple of 16 bytes; 1: row r is
+                   // r * dim elements behind such a boundary; 2: any
   float eps = 0.f;
 };
 
@@ -40,14 +41,14 @@ struct NormBwdParams {
   int64_t dy_stride = 0, dh_stride = 0, h_stride = 0;
   int dim = 0;
   int weight_f32 = 0;
-  int vec = 0;
+  int layout = 2;
 };
 
 constexpr int kNormMaxDim = 16384;
 
-void rms_norm_fwd_launch(NormType t, const NormFwdParams& p, cudaStream_t stream);
+void rms_norm_fwd_launch(NormType t, const NormFwdParams& p, int sm_count, cudaStream_t stream);
 // Rows of dw_part: one per CTA of the backward kernel.
-int rms_norm_bwd_parts(NormType t, int64_t rows, int dim, int vec, int sm_count);
+int rms_norm_bwd_parts(NormType t, const NormBwdParams& p, int sm_count);
 void rms_norm_bwd_launch(NormType t, const NormBwdParams& p, int parts, cudaStream_t stream);
 
 }  // namespace mgfa

@@ -27,7 +27,7 @@ struct RotaryParams {
   int head_dim = 0, rotary_dim = 0;
   int positions64 = 0;   // int64 positions (else int32)
   int interleaved = 0;   // pairs (2i, 2i + 1); else (i, i + rotary_dim / 2)
-  int vec = 0;           // 1: 16-byte accesses throughout
+  int vec = 0;           // 1: every head starts and ends on a 16-byte boundary
   float magnitude = 1.f; // factor on the rotated values
   float sign = 1.f;      // -1: the transpose, for gradients
 };

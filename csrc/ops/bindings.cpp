@@ -37,18 +37,14 @@ void flash_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tens
                c10::optional<torch::Tensor> delta_in, torch::Tensor status, int64_t wait_limit_ns);
 std::vector<torch::Tensor> flash_bwd_preprocess(torch::Tensor dout, torch::Tensor out,
                                                 torch::Tensor lse);
-std::tuple<torch::Tensor, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> rms_norm_fwd(
-    torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps,
-    bool need_rstd);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rms_norm(
+    torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps);
 std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> rms_norm_fp8(
     torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps,
     int64_t group);
-std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rms_norm_bwd(
-    c10::optional<torch::Tensor> dy, c10::optional<torch::Tensor> dh, torch::Tensor h,
-    torch::Tensor weight, torch::Tensor rstd, bool need_dw);
-std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_apply(
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> apply_rotary(
     torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
-    torch::Tensor inv_freq, bool interleaved, double magnitude, double sign);
+    torch::Tensor inv_freq, bool interleaved, double magnitude);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new,
@@ -109,10 +105,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "forward launch whose arrival flag is never set (bounded-wait failure path)",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("wait_limit_ns"),
         py::arg("status") = py::none());
-  m.def("rms_norm_fwd", &mgfa::rms_norm_fwd);
+  m.def("rms_norm", &mgfa::rms_norm);
   m.def("rms_norm_fp8", &mgfa::rms_norm_fp8);
-  m.def("rms_norm_bwd", &mgfa::rms_norm_bwd);
-  m.def("rotary_apply", &mgfa::rotary_apply);
+  m.def("apply_rotary", &mgfa::apply_rotary);
   m.def("paged_attention", &mgfa::paged_attention);
   m.def("cache_check", &mgfa::cache_check);
   m.def("cache_reserve", &mgfa::cache_reserve);

@@ -1,5 +1,7 @@
 // Torch-facing entry points of the per-token operators of a decoder layer:
 // root-mean-square norm (rms_norm.cu) and rotary positions (rotary.cu).
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/types.h>
 #include "../common/check.hpp"
 #include <ATen/cuda/CUDAContext.h>
@@ -18,11 +20,9 @@ int device_sm_count(int device);
 
 namespace {
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 using OptTensor = c10::optional<torch::Tensor>;
-
-bool aligned16(const torch::Tensor& t) {
-  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-}
 
 NormType norm_type(const torch::Tensor& t, const char* name) {
   MGFA_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
@@ -44,8 +44,26 @@ torch::Tensor as_rows(const torch::Tensor& t) {
   return r;
 }
 
-bool rows_vec(const torch::Tensor& r, int v) {
-  return aligned16(r) && (r.size(0) <= 1 || r.stride(0) % v == 0);
+// Whether row i of r starts i * dim elements behind a 16-byte boundary, up to whole
+// vectors of v elements.
+bool rows_vec(const torch::Tensor& r, int64_t dim, int v) {
+  return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 &&
+         (r.size(0) <= 1 || (r.stride(0) - dim) % v == 0);
+}
+
+// NormFwdParams::layout of rows (of undefined tensors: none); the outputs are packed. A
+// weight of x's type is read in vectors where the rows are aligned.
+int norm_layout(int64_t dim, std::initializer_list<const torch::Tensor*> rows,
+                const torch::Tensor& weight) {
+  const torch::Tensor& x = **rows.begin();
+  const int v = 16 / int(x.element_size());
+  for (const torch::Tensor* r : rows)
+    if (r->defined() && !rows_vec(*r, dim, v)) return 2;
+  // a shifted row covers up to v - 1 columns more
+  if (dim % v) return dim + v - 1 <= kNormMaxDim ? 1 : 2;
+  return weight.scalar_type() != x.scalar_type() ||
+                 reinterpret_cast<uintptr_t>(weight.data_ptr()) % 16 == 0
+             ? 0 : 1;
 }
 
 void check_norm_inputs(const torch::Tensor& x, const torch::Tensor& weight,
@@ -85,14 +103,12 @@ NormFwd norm_fwd(const torch::Tensor& x, const torch::Tensor& weight_in, const O
   const int v = t == NormType::kF32 ? 4 : 8;
   torch::Tensor xr = as_rows(x), rr, weight = weight_in.contiguous();
   if (residual.has_value()) rr = as_rows(*residual);
-  auto vec = [&] {
-    return dim % v == 0 && rows_vec(xr, v) && (!rr.defined() || rows_vec(rr, v)) &&
-           aligned16(weight);
-  };
-  if (group && !vec()) {  // the scales of column groups need vector loads
-    if (!rows_vec(xr, v)) xr = xr.clone(at::MemoryFormat::Contiguous);
-    if (rr.defined() && !rows_vec(rr, v)) rr = rr.clone(at::MemoryFormat::Contiguous);
-    if (!aligned16(weight)) weight = weight.clone();
+  int layout = norm_layout(dim, {&xr, &rr}, weight);
+  if (group && layout != 0) {  // the scales of column groups need aligned vectors
+    if (!rows_vec(xr, dim, v)) xr = xr.clone(at::MemoryFormat::Contiguous);
+    if (rr.defined() && !rows_vec(rr, dim, v)) rr = rr.clone(at::MemoryFormat::Contiguous);
+    weight = weight.clone();
+    layout = 0;
   }
   NormFwd out;
   out.y = torch::empty(x.sizes(), x.options().dtype(eight ? at::kFloat8_e4m3fn : x.scalar_type()));
@@ -120,11 +136,11 @@ NormFwd norm_fwd(const torch::Tensor& x, const torch::Tensor& weight_in, const O
   p.scale = eight ? out.scale.data_ptr<float>() : nullptr;
   p.dim = dim;
   p.group = int(group);
-  p.vec = vec();
+  p.layout = layout;
   p.eps = float(eps);
   MGFA_CHECK(p.rows < (int64_t(1) << 31), "too many rows");
   if (p.rows > 0) {
-    rms_norm_fwd_launch(t, p, at::cuda::getCurrentCUDAStream());
+    rms_norm_fwd_launch(t, p, device_sm_count(x.get_device()), at::cuda::getCurrentCUDAStream());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   return out;
@@ -133,14 +149,6 @@ NormFwd norm_fwd(const torch::Tensor& x, const torch::Tensor& weight_in, const O
 OptTensor opt(const torch::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 }  // namespace
-
-// y, h (with a residual) and rstd [rows] (when asked for).
-std::tuple<torch::Tensor, OptTensor, OptTensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight,
-                                                             OptTensor residual, double eps,
-                                                             bool need_rstd) {
-  NormFwd o = norm_fwd(x, weight, residual, eps, need_rstd, false, 0);
-  return {o.y, opt(o.h), opt(o.rstd)};
-}
 
 // y (e4m3), scale [..., dim / group] (group 0: [..., 1]) and h (with a residual).
 std::tuple<torch::Tensor, torch::Tensor, OptTensor> rms_norm_fp8(torch::Tensor x,
@@ -151,26 +159,25 @@ std::tuple<torch::Tensor, torch::Tensor, OptTensor> rms_norm_fp8(torch::Tensor x
   return {o.y, o.scale, opt(o.h)};
 }
 
+namespace {
+
 // dx (which is the residual's gradient too) and the weight's gradient (when asked for)
-// from the gradients of y and h, either of which may be absent.
-std::tuple<torch::Tensor, OptTensor> rms_norm_bwd(OptTensor dy, OptTensor dh, torch::Tensor h,
-                                                  torch::Tensor weight_in, torch::Tensor rstd,
-                                                  bool need_dw) {
-  check_norm_inputs(h, weight_in, dh);
-  if (dy.has_value())
-    MGFA_CHECK(dy->scalar_type() == h.scalar_type() && dy->sizes() == h.sizes() &&
-                   dy->device() == h.device(),
+// from the gradients of y and h, either of which may be undefined.
+std::tuple<torch::Tensor, torch::Tensor> norm_bwd(const torch::Tensor& dy, const torch::Tensor& dh,
+                                                  const torch::Tensor& h,
+                                                  const torch::Tensor& weight_in,
+                                                  const torch::Tensor& rstd, bool need_dw) {
+  check_norm_inputs(h, weight_in, opt(dh));
+  if (dy.defined())
+    MGFA_CHECK(dy.scalar_type() == h.scalar_type() && dy.sizes() == h.sizes() &&
+                   dy.device() == h.device(),
                "dy must match the stream's dtype, shape and device");
   const int dim = int(h.size(-1));
   c10::cuda::CUDAGuard guard(h.device());
   const NormType t = norm_type(h, "h");
-  const int v = t == NormType::kF32 ? 4 : 8;
   torch::Tensor hr = as_rows(h), dyr, dhr, weight = weight_in.contiguous();
-  if (dy.has_value()) dyr = as_rows(*dy);
-  if (dh.has_value()) dhr = as_rows(*dh);
-  MGFA_CHECK(rstd.is_cuda() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() &&
-                 rstd.numel() == hr.size(0),
-             "rstd must be a contiguous float32 [rows] tensor");
+  if (dy.defined()) dyr = as_rows(dy);
+  if (dh.defined()) dhr = as_rows(dh);
   torch::Tensor dx = torch::empty(h.sizes(), h.options()), dw, part;
   NormBwdParams p;
   p.h = hr.data_ptr();
@@ -189,14 +196,12 @@ std::tuple<torch::Tensor, OptTensor> rms_norm_bwd(OptTensor dy, OptTensor dh, to
   p.dx = dx.data_ptr();
   p.rows = hr.size(0);
   p.dim = dim;
-  p.vec = dim % v == 0 && rows_vec(hr, v) && (!dyr.defined() || rows_vec(dyr, v)) &&
-          (!dhr.defined() || rows_vec(dhr, v)) && aligned16(weight);
+  p.layout = norm_layout(dim, {&hr, &dyr, &dhr}, weight);
   if (p.rows == 0) {
     if (need_dw) dw = torch::zeros({dim}, weight.options());
-    return {dx, opt(dw)};
+    return {dx, dw};
   }
-  const int parts =
-      rms_norm_bwd_parts(t, p.rows, dim, p.vec, device_sm_count(h.get_device()));
+  const int parts = rms_norm_bwd_parts(t, p, device_sm_count(h.get_device()));
   if (need_dw) {
     dw = torch::empty({dim}, weight.options());
     part = torch::empty({parts, dim}, h.options().dtype(at::kFloat));
@@ -205,7 +210,54 @@ std::tuple<torch::Tensor, OptTensor> rms_norm_bwd(OptTensor dy, OptTensor dh, to
   }
   rms_norm_bwd_launch(t, p, parts, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {dx, opt(dw)};
+  return {dx, dw};
+}
+
+// Gradients that cannot be differentiated again: an error where that is tried.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "this operator's gradient has no gradient of its own", int(grads.size()));
+  return (*node)(std::move(grads));
+}
+
+struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& x,
+                               const torch::Tensor& weight, const OptTensor& residual, double eps) {
+    NormFwd o = norm_fwd(x, weight, residual, eps, true, false, 0);
+    ctx->save_for_backward({o.h.defined() ? o.h : x, weight, o.rstd});
+    ctx->set_materialize_grads(false);
+    if (!o.h.defined()) return {o.y};
+    return {o.y, o.h};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool res = grads.size() > 1;
+    const torch::Tensor dy = grads[0], dh = res ? grads[1] : torch::Tensor();
+    if (!dy.defined() && !dh.defined()) return {{}, {}, {}, {}};
+    const variable_list saved = ctx->get_saved_variables();
+    auto [dx, dw] = norm_bwd(dy, dh, saved[0], saved[1], saved[2], ctx->needs_input_grad(1));
+    return once({ctx->needs_input_grad(0) ? dx : torch::Tensor(), dw,
+                 res && ctx->needs_input_grad(2) ? dx : torch::Tensor(), {}});
+  }
+};
+
+bool wants_grad(const torch::Tensor& a, const OptTensor& b) {
+  return at::GradMode::is_enabled() && (a.requires_grad() || (b.has_value() && b->requires_grad()));
+}
+
+}  // namespace
+
+// y and h (with a residual); differentiable.
+std::tuple<torch::Tensor, OptTensor> rms_norm(torch::Tensor x, torch::Tensor weight,
+                                              OptTensor residual, double eps) {
+  if (wants_grad(x, residual) || wants_grad(weight, {})) {
+    variable_list o = RmsNormFn::apply(x, weight, residual, eps);
+    return {o[0], o.size() > 1 ? OptTensor(o[1]) : OptTensor()};
+  }
+  NormFwd o = norm_fwd(x, weight, residual, eps, false, false, 0);
+  return {o.y, opt(o.h)};
 }
 
 // ------------------------------------------------------------------ rotary positions
@@ -227,10 +279,13 @@ RotaryTensor rotary_tensor(const torch::Tensor& t, torch::Tensor& out, const cha
 
 }  // namespace
 
+namespace {
+
 // q (and k) with rotary positions; sign -1 rotates back (the gradient).
-std::tuple<torch::Tensor, OptTensor> rotary_apply(torch::Tensor q, OptTensor k_in,
-                                                  torch::Tensor positions, torch::Tensor inv_freq,
-                                                  bool interleaved, double magnitude, double sign) {
+std::tuple<torch::Tensor, torch::Tensor> rotary(torch::Tensor q, const OptTensor& k_in,
+                                                const torch::Tensor& positions,
+                                                const torch::Tensor& inv_freq, bool interleaved,
+                                                double magnitude, double sign) {
   const NormType t = norm_type(q, "q");
   MGFA_CHECK(q.dim() == 3 || q.dim() == 4,
              "q must be [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]");
@@ -279,14 +334,52 @@ std::tuple<torch::Tensor, OptTensor> rotary_apply(torch::Tensor q, OptTensor k_i
     return reinterpret_cast<uintptr_t>(r.in) % 16 == 0 && r.stride_b % v == 0 &&
            r.stride_t % v == 0 && r.stride_h % v == 0;
   };
-  p.vec = (p.rotary_dim / 2) % v == 0 && (D - p.rotary_dim) % v == 0 && vec_tensor(p.x[0]) &&
-          (!k.defined() || vec_tensor(p.x[1]));
+  p.vec = D % v == 0 && vec_tensor(p.x[0]) && (!k.defined() || vec_tensor(p.x[1]));
+  MGFA_CHECK(p.x[0].heads + int64_t(p.x[1].heads) <= 4096, "at most 4096 heads");
   MGFA_CHECK(B * L < (int64_t(1) << 31), "too many tokens");
   if (B * L > 0 && p.x[0].heads + p.x[1].heads > 0) {
     rotary_launch(RotaryType(int(t)), p, device_sm_count(q.get_device()),
                   at::cuda::getCurrentCUDAStream());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
+  return {qo, ko};
+}
+
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& q, const OptTensor& k,
+                               const torch::Tensor& positions, const torch::Tensor& inv_freq,
+                               bool interleaved, double magnitude) {
+    auto [qo, ko] = rotary(q, k, positions, inv_freq, interleaved, magnitude, 1.0);
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->set_materialize_grads(false);
+    if (!ko.defined()) return {qo};
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const torch::Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : torch::Tensor();
+    if (!dq.defined() && !dk.defined()) return {{}, {}, {}, {}, {}, {}};
+    const variable_list saved = ctx->get_saved_variables();
+    const bool il = ctx->saved_data["interleaved"].toBool();
+    const double mag = ctx->saved_data["magnitude"].toDouble();
+    if (!dq.defined())
+      return once({{}, std::get<0>(rotary(dk, {}, saved[0], saved[1], il, mag, -1.0)), {}, {}, {}, {}});
+    auto [gq, gk] = rotary(dq, opt(dk), saved[0], saved[1], il, mag, -1.0);
+    return once({gq, gk, {}, {}, {}, {}});
+  }
+};
+
+}  // namespace
+
+std::tuple<torch::Tensor, OptTensor> apply_rotary(torch::Tensor q, OptTensor k,
+                                                  torch::Tensor positions, torch::Tensor inv_freq,
+                                                  bool interleaved, double magnitude) {
+  if (wants_grad(q, k)) {
+    variable_list o = RotaryFn::apply(q, k, positions, inv_freq, interleaved, magnitude);
+    return {o[0], o.size() > 1 ? OptTensor(o[1]) : OptTensor()};
+  }
+  auto [qo, ko] = rotary(q, k, positions, inv_freq, interleaved, magnitude, 1.0);
   return {qo, opt(ko)};
 }
 

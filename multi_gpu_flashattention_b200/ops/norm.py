@@ -18,32 +18,10 @@ import torch
 from .._ext import C
 
 
-class _RMSNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, h, rstd = C().rms_norm_fwd(x, weight, residual, eps, True)
-        ctx.save_for_backward(x if h is None else h, weight, rstd)
-        ctx.set_materialize_grads(False)
-        return y if h is None else (y, h)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        if dy is None and dh is None:
-            return None, None, None, None
-        need_x, need_w, need_r, _ = ctx.needs_input_grad
-        dx, dw = C().rms_norm_bwd(dy, dh, h, weight, rstd, need_w)
-        return dx if need_x else None, dw, dx if need_r else None, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6):
-    """y, or (y, h) with a residual; differentiable in x, weight and residual."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                    (residual is not None and residual.requires_grad)):
-        return _RMSNormFn.apply(x, weight, residual, eps)
-    y, h, _ = C().rms_norm_fwd(x, weight, residual, eps, False)
+    """y, or (y, h) with a residual; differentiable (once) in x, weight and residual."""
+    y, h = C().rms_norm(x, weight, residual, eps)
     return y if h is None else (y, h)
 
 

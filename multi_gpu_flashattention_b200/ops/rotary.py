@@ -59,36 +59,13 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
     return inv.to(device) if device is not None else inv, magnitude
 
 
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved, magnitude):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.cfg = (interleaved, magnitude)
-        ctx.set_materialize_grads(False)
-        qo, ko = C().rotary_apply(q, k, positions, inv_freq, interleaved, magnitude, 1.0)
-        return qo if ko is None else (qo, ko)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk=None):
-        positions, inv_freq = ctx.saved_tensors
-        if dq is None and dk is None:
-            return (None,) * 6
-        a, b = (dk, None) if dq is None else (dq, dk)
-        ga, gb = C().rotary_apply(a, b, positions, inv_freq, *ctx.cfg, -1.0)
-        gq, gk = (None, ga) if dq is None else (ga, gb)
-        return gq, gk, None, None, None, None
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                  inv_freq: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0):
-    """q and k (k may be None) with rotary positions; differentiable in q and k.
+    """q and k (k may be None) with rotary positions; differentiable (once) in q and k.
 
     q, k: [tokens, heads, head_dim] or [batch, tokens, heads, head_dim], bfloat16, float16
     or float32, head_dim up to 256, of one dtype; they may be strided, the results are
     contiguous. positions: int32 or int64 [tokens], or [batch, tokens]. inv_freq:
     float64 [rotary_dim / 2] (rotary_frequencies). Returns (q', k'), or q' alone."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFn.apply(q, k, positions, inv_freq, interleaved, magnitude)
-    qo, ko = C().rotary_apply(q, k, positions, inv_freq, interleaved, magnitude, 1.0)
+    qo, ko = C().apply_rotary(q, k, positions, inv_freq, interleaved, magnitude)
     return qo if ko is None else (qo, ko)

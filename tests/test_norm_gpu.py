@@ -77,7 +77,8 @@ def _check(x, w, r, dy, dh):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,dim", [(1, 1), (3, 7), (5, 64), (1, 100), (257, 128), (33, 1000),
                                       (7, 1024), (700, 2056), (2, 4096), (1300, 4096), (3, 5001),
-                                      (2, 8192), (3, 12345), (5, 16384)])
+                                      (2, 8192), (3, 12345), (5, 16384), (9, 6806),
+                                      (300, 30), (4, 10002)])
 def test_forward_and_gradients(rows, dim, dtype, residual):
     _check(*_make(rows, dim, dtype, residual, seed=rows + dim))
 
@@ -193,6 +194,36 @@ def test_infinities_and_nan_stay_in_their_rows():
         assert torch.equal(y[row], clean[row]) and torch.isfinite(y8[row].float()).all()
     assert y[1].isnan().all() and y8[1].float().isnan().all() and scale[1] == 1
     assert y[3, 7].isnan() and not y[3, :7].any()
+
+
+def test_second_derivative_is_refused():
+    from multi_gpu_flashattention_b200 import rms_norm
+    x, w, _, dy, _ = _make(4, 64, torch.float32, False)
+    xs = x.requires_grad_()
+    (g,) = torch.autograd.grad([rms_norm(xs, w)], [xs], [dy], create_graph=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        g.sum().backward()
+
+
+def test_training_step_in_a_graph():
+    """Forward and gradients captured together, replayed on other values."""
+    from multi_gpu_flashattention_b200 import rms_norm
+    x, w, r, dy, dh = _make(70, 512, torch.bfloat16, True)
+    xs, ws, rs = (t.requires_grad_() for t in (x, w, r))
+    step = lambda: torch.autograd.grad(rms_norm(xs, ws, residual=rs), [xs, ws, rs], [dy, dh])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    with torch.no_grad():
+        xs.mul_(2).add_(1)
+    g.replay()
+    for a, b in zip(out, step()):
+        assert torch.equal(a, b)
 
 
 def test_empty():
