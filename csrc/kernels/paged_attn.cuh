@@ -10,9 +10,11 @@
 // tiles; all units' runs, laid end to end, are cut into equal shares, one per CTA,
 // whatever the sequences' lengths. A share covers whole units, which the CTA finishes,
 // and at most two parts (its first and last), which it leaves, unnormalised in fp32, in
-// a workspace for paged_merge_kernel. The shares follow from the lengths alone, which
-// the kernels read on the device: the host knows none of them, nothing waits for it,
-// and the result does not depend on timing.
+// a workspace for paged_merge_kernel. A cut that would leave `snap` tiles or fewer of a
+// unit on one side moves to the unit's border: a part's way through the workspace costs
+// more than that (`snap` is at most half a share). The shares follow from the lengths alone, which the kernel reads on
+// the device: the host knows none of them, nothing waits for it, and the result does not
+// depend on timing.
 #pragma once
 
 #include <cuda.h>
@@ -50,11 +52,15 @@ struct PagedParams {
   int block_tokens = 0;  // new tokens of a unit
   int tile = 0;          // keys of a tile
   int min_share = 1;     // tiles
+  int snap = 0;          // tiles
   int grid = 0;          // CTAs
   int unit_rows = 0;     // rows of a part in the workspace
-  // workspace: parts [2 * grid][unit_rows][head_dim] and their (max, sum), log2 units
+  // workspace: parts [2 * grid][unit_rows][head_dim] and their (max, sum), log2 units; the
+  // parts of share c are 2 c (a unit that an earlier share began) and 2 c + 1
   float* part_o = nullptr;
   float2* part_ml = nullptr;
+  int4* join = nullptr;  // [grid] of the unit that share c began and others go on with:
+                         // its first row of q, first head, rows (0: none), last share
   uint32_t* status = nullptr;
   uint64_t wait_limit_ns = 0;
 };
@@ -146,19 +152,6 @@ __device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* pre
   __syncthreads();
 }
 
-struct PagedShare {
-  uint64_t total, per;
-  __device__ __forceinline__ PagedShare(const PagedParams& p, const uint32_t* prefix) {
-    total = uint64_t(prefix[p.seqs]) * uint32_t(p.kv_heads);
-    per = (total + uint32_t(p.grid) - 1) / uint32_t(p.grid);
-    if (per < uint32_t(p.min_share)) per = uint32_t(p.min_share);
-  }
-  __device__ __forceinline__ uint64_t begin(int cta) const {
-    const uint64_t w = per * uint32_t(cta);
-    return w < total ? w : total;
-  }
-};
-
 // The unit that contains tile w of the whole run, and the tiles [first, first + tiles)
 // that are the unit's.
 struct PagedUnit {
@@ -205,6 +198,56 @@ __device__ __forceinline__ void paged_next(const PagedParams& p, const uint32_t*
     }
   }
   u.tiles = paged_unit_tiles(p, u.s, u.unit);
+}
+
+struct PagedShare {
+  const PagedParams& p;
+  const uint32_t* prefix;
+  uint64_t total, per;
+  uint32_t snap;
+  __device__ __forceinline__ PagedShare(const PagedParams& params, const uint32_t* pre)
+      : p(params), prefix(pre) {
+    total = uint64_t(prefix[p.seqs]) * uint32_t(p.kv_heads);
+    per = (total + uint32_t(p.grid) - 1) / uint32_t(p.grid);
+    if (per < uint32_t(p.min_share)) per = uint32_t(p.min_share);
+    snap = per / 2 < uint32_t(p.snap) ? uint32_t(per / 2) : uint32_t(p.snap);
+  }
+  // The first tile of share c; `u`, the unit that it lies in, where there is one.
+  __device__ __forceinline__ uint64_t begin(int c, PagedUnit& u) const {
+    uint64_t w = per * uint32_t(c);
+    if (w >= total) return total;
+    u = paged_find(p, prefix, w);
+    const uint64_t end = u.first + uint32_t(u.tiles);
+    if (w - u.first <= snap) return u.first;
+    if (end - w <= snap) {
+      w = end;
+      if (w < total) paged_next(p, prefix, u);
+    }
+    return w;
+  }
+  // The share of a unit's last tile.
+  __device__ __forceinline__ int last(const PagedUnit& u) const {
+    const uint64_t end = u.first + uint32_t(u.tiles);
+    int c = int((end - 1) / per);
+    PagedUnit v;
+    while (begin(c, v) >= end) --c;  // a cut that has moved to this unit's end
+    return c;
+  }
+};
+
+// What share c, of tiles [begin, end), leaves for others to go on with. `u` is its last
+// unit.
+__device__ __forceinline__ void paged_join(const PagedShare& share, const PagedUnit& u, bool any,
+                                           uint64_t begin, uint64_t end) {
+  const PagedParams& p = share.p;
+  if (!p.join) return;
+  int4 j = make_int4(0, 0, 0, 0);
+  if (any && u.first >= begin && u.first + uint32_t(u.tiles) > end) {
+    int n = u.s.n - u.unit * p.block_tokens;
+    n = n < p.block_tokens ? n : p.block_tokens;
+    j = make_int4(u.s.q0 + u.unit * p.block_tokens, u.hk * p.group, n * p.group, share.last(u));
+  }
+  p.join[blockIdx.x] = j;
 }
 
 }  // namespace dev

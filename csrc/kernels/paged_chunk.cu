@@ -48,6 +48,7 @@ struct __align__(1024) ChunkSmem {
   uint32_t tmem_base;
   uint32_t abort_flag;
   uint32_t sums[kWarps];
+  PagedUnit unit[8];  // of the softmax warps, whose registers hold scores
 };
 
 template <int kD, bool kF16>
@@ -84,15 +85,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   paged_prefix<kThreads>(p, prefix, s.sums);
   const PagedShare share(p, prefix);
-  const uint64_t begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
-  if (begin >= end) return;  // the whole CTA
+  PagedUnit u, behind;
+  const uint64_t begin = share.begin(blockIdx.x, u), end = share.begin(blockIdx.x + 1, behind);
+  if (begin >= end) {  // the whole CTA
+    if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
+    return;
+  }
   if (warp == 0) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   const int tile_tokens = p.block_tokens / 2;
-  PagedUnit u = paged_find(p, prefix, begin);
 
   if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
@@ -166,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       w = u.first + uint32_t(t1);
       if (w < end) paged_next(p, prefix, u);
     }
+    if (lane == 0) paged_join(share, u, true, begin, end);
     // Never leave with a copy outstanding.
     volatile uint32_t never = 0;
     AbortState drain{&never, nullptr, p.wait_limit_ns};
@@ -287,22 +292,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_off + t * 128;
     const uint32_t o_addr = tmem + lane_off + kOCol + t * kD;
-    const int r_tok = t * tile_tokens + r / p.group, r_head = r % p.group;
-    const bool r_used = r < tile_tokens * p.group;
+    PagedUnit& su = s.unit[warp];
+    if (lane == 0) su = u;
+    __syncwarp();
     uint32_t sc = 0, oc = 0;  // phases used so far
     bool ok = true;
     for (uint64_t w = begin; ok && w < end;) {
-      const int t0 = int(w - u.first);
-      const int t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
-      const int tok0 = u.unit * p.block_tokens;
-      if (u.s.n - tok0 > t * tile_tokens) {  // this tile has a token
-        const int tok = tok0 + r_tok;
-        const bool valid = r_used && tok < u.s.n;
+      const int t0 = int(w - su.first);
+      const int t1 = end - su.first < uint64_t(su.tiles) ? int(end - su.first) : su.tiles;
+      const int tok0 = su.unit * p.block_tokens + t * tile_tokens;  // this tile's first token
+      if (su.s.n > tok0) {
         // keys that this row sees, and those that the tile's first row, hence each, does
-        int lim = p.causal ? u.s.kv - u.s.n + tok + 1 : u.s.kv;
-        lim = !valid ? 0 : lim < u.s.kv ? lim : u.s.kv;
-        int full = p.causal ? u.s.kv - u.s.n + tok0 + t * tile_tokens + 1 : u.s.kv;
-        full = full < u.s.kv ? full : u.s.kv;
+        const int n = su.s.n, kv = su.s.kv;
+        const int tok = tok0 + r / p.group;
+        int lim = p.causal ? kv - n + tok + 1 : kv;
+        lim = r >= tile_tokens * p.group || tok >= n ? 0 : lim < kv ? lim : kv;
+        int full = p.causal ? kv - n + tok0 + 1 : kv;
+        full = full < kv ? full : kv;
         float m = -INFINITY, l = 0.f;
         for (int j = t0; j < t1; ++j) {
           ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[t], sc & 1, ab, 90 + t));
@@ -333,8 +339,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t pk[2][32];
           float lacc[4] = {0.f, 0.f, 0.f, 0.f};
           exp_half<kF16, 0, true>(sr, 0, p.scale_log2, neg_m, pk[0], lacc);
+          tmem_st32(s_addr, pk[0]);
           exp_half<kF16, 0, true>(sr, 1, p.scale_log2, neg_m, pk[1], lacc);
-          tmem_st32x2_sync(s_addr, pk[0], pk[1]);
+          tmem_st32(s_addr + 32, pk[1]);
           l += (lacc[0] + lacc[1]) + (lacc[2] + lacc[3]);
           // S(j) was issued behind PV(j - 1), and its barrier has completed: O is at rest
           if (__any_sync(0xffffffffu, rescale)) {
@@ -348,6 +355,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32_sync(o_addr + ch * 32, orow);
             }
           }
+          tmem_wait_st();
+          regs_live32(pk[0]);
+          regs_live32(pk[1]);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.p_full[t]);
@@ -356,11 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         ++oc;
         tc_fence_after();
-        const bool done = t0 == 0 && t1 == u.tiles;
-        const float scale = !done ? 1.f : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const int64_t row_tok = u.s.q0 + tok, head = int64_t(u.hk) * p.group + r_head;
+        const bool done = t0 == 0 && t1 == su.tiles;
+        const bool valid = r < tile_tokens * p.group && tok < su.s.n;
+        const float scale = !done ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const int r_head = r % p.group;
+        const int64_t row_tok = su.s.q0 + tok, head = int64_t(su.hk) * p.group + r_head;
         const int64_t slot = 2 * int64_t(blockIdx.x) + (t0 > 0 ? 0 : 1);
-        const int64_t part = slot * p.unit_rows + r_tok * p.group + r_head;
+        const int64_t part = slot * p.unit_rows + (tok - su.unit * p.block_tokens) * p.group + r_head;
 #pragma unroll
         for (int ch = 0; ch < kOChunks; ++ch) {
           uint32_t orow[32];
@@ -389,8 +401,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.lse[head * p.tokens + row_tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         }
       }
-      w = u.first + uint32_t(t1);
-      if (w < end) paged_next(p, prefix, u);
+      w = su.first + uint32_t(t1);
+      __syncwarp();
+      if (w < end && lane == 0) paged_next(p, prefix, su);
+      __syncwarp();
     }
   }
   // ---- teardown

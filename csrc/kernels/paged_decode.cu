@@ -95,9 +95,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   paged_prefix<kThreads>(p, prefix, s.sums);  // its barriers cover the initialisation
   const PagedShare share(p, prefix);
-  const uint64_t begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
-  if (begin >= end) return;  // the whole CTA
-  PagedUnit u = paged_find(p, prefix, begin);
+  PagedUnit u, behind;
+  const uint64_t begin = share.begin(blockIdx.x, u), end = share.begin(blockIdx.x + 1, behind);
+  if (begin >= end) {  // the whole CTA
+    if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
+    return;
+  }
   uint32_t it = 0;
 
   if (warp == kConsumers) {
@@ -145,6 +148,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       w = u.first + uint32_t(t1);
       if (w < end) paged_next(p, prefix, u);
     }
+    if (lane == 0) paged_join(share, u, true, begin, end);
     // Never leave with a copy outstanding: the last kStages tiles' barriers.
     volatile uint32_t never = 0;
     AbortState drain{&never, nullptr, p.wait_limit_ns};
@@ -390,83 +394,85 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ---------------------------------------------------------------------- joining the parts
-// CTA (c, y): the unit across the border between shares c and c + 1, if c + 1 is the
-// first border inside it; rows [y * 8, y * 8 + 8). One warp per row: the row's weights
-// 2^(m_i - max) first (lane i holds part i), then the weighted sum of the parts' rows.
-constexpr int kMergeThreads = 256;
+// CTA (c, y): rows [y * kRows, y * kRows + kRows) of the unit that share c began and
+// others went on with (join[c]), if there is one. kSplit warps share a row: each first
+// finds the row's maximum over all parts (lane i holds part i), then adds every kSplit-th
+// part's row, weighted by 2^(m_i - max); the warps' sums are added in order.
+constexpr int kMergeWarps = 16;
 
-template <int kD, bool kF16>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedParams p) {
-  extern __shared__ uint32_t prefix_m[];
-  __shared__ uint32_t sums[kMergeThreads / 32];
-  paged_prefix<kMergeThreads>(p, prefix_m, sums);  // the lengths are inputs: no need to wait
-  const PagedShare share(p, prefix_m);
-  const int c = blockIdx.x;
-  const uint64_t border = share.begin(c + 1);
-  PagedUnit u = {};
-  bool mine = border < share.total;
-  if (mine) {
-    u = paged_find(p, prefix_m, border);
-    mine = u.first != border && u.first >= share.begin(c);
-  }
-  // every CTA waits for the parts' kernel, so this one never completes before it
+template <int kD, bool kF16, int kSplit, int kRows>
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const PagedParams p) {
+  constexpr int kE = kD / 32, kAtOnce = kMergeWarps / kSplit;
+  __shared__ float sh[kSplit > 1 ? kMergeWarps : 1][kD];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!mine) return;
-  const int rows = (p.block_tokens < u.s.n - u.unit * p.block_tokens
-                        ? p.block_tokens
-                        : u.s.n - u.unit * p.block_tokens) * p.group;
-  const int r = blockIdx.y * (kMergeThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  const int last = int((u.first + uint32_t(u.tiles) - 1) / share.per);  // the last share's CTA
-  auto slot = [&](int i) { return 2 * int64_t(i) + (i == c ? 1 : 0); };
-  float top = -INFINITY;
-  for (int i = c + lane; i <= last; i += 32)
-    top = fmaxf(top, p.part_ml[slot(i) * p.unit_rows + r].x);
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 j = p.join[c];
+  const int part = warp % kSplit;
+  for (int r0 = blockIdx.y * kRows; r0 < j.z && r0 < int(blockIdx.y + 1) * kRows; r0 += kAtOnce) {
+    const int r = r0 + warp / kSplit;
+    const bool live = r < j.z;
+    auto slot = [&](int i) { return (2 * int64_t(i) + (i == c ? 1 : 0)) * p.unit_rows + r; };
+    float top = -INFINITY, total = 0.f, acc[kE];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
-  constexpr int kE = kD / 32;
-  float acc[kE];
+    for (int e = 0; e < kE; ++e) acc[e] = 0.f;
+    if (live) {
+      for (int i = c + lane; i <= j.w; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
 #pragma unroll
-  for (int e = 0; e < kE; ++e) acc[e] = 0.f;
-  for (int i0 = c; i0 <= last; i0 += 32) {
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (i0 + lane <= last) ml = p.part_ml[slot(i0 + lane) * p.unit_rows + r];
-    const float wt = ex2_approx(ml.x - base);
-    total += ml.y * wt;
-    const int m = last - i0 + 1 < 32 ? last - i0 + 1 : 32;
-#pragma unroll 4
-    for (int j = 0; j < m; ++j) {
-      const float f = __shfl_sync(0xffffffffu, wt, j);
-      const float* src = p.part_o + (slot(i0 + j) * p.unit_rows + r) * kD + lane * kE;
-      if constexpr (kE == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        acc[0] = fmaf(f, v.x, acc[0]);
-        acc[1] = fmaf(f, v.y, acc[1]);
-        acc[2] = fmaf(f, v.z, acc[2]);
-        acc[3] = fmaf(f, v.w, acc[3]);
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(f, v.x, acc[0]);
-        acc[1] = fmaf(f, v.y, acc[1]);
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float base = top == -INFINITY ? 0.f : top;
+      for (int i0 = c; i0 <= j.w; i0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (i0 + lane <= j.w) ml = p.part_ml[slot(i0 + lane)];
+        const float wt = ex2_approx(ml.x - base);
+        total += ml.y * wt;
+        const int n = j.w - i0 + 1 < 32 ? j.w - i0 + 1 : 32;
+#pragma unroll 8
+        for (int i = part; i < n; i += kSplit) {
+          const float f = __shfl_sync(0xffffffffu, wt, i);
+          const float* src = p.part_o + slot(i0 + i) * kD + lane * kE;
+          if constexpr (kE == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            acc[0] = fmaf(f, v.x, acc[0]);
+            acc[1] = fmaf(f, v.y, acc[1]);
+            acc[2] = fmaf(f, v.z, acc[2]);
+            acc[3] = fmaf(f, v.w, acc[3]);
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            acc[0] = fmaf(f, v.x, acc[0]);
+            acc[1] = fmaf(f, v.y, acc[1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if constexpr (kSplit > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kE; ++e) sh[warp][lane * kE + e] = acc[e];
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int k = 1; k < kSplit; ++k)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) acc[e] += sh[warp + k][lane * kE + e];
       }
     }
+    if (!live || part) continue;
+    const float base = top == -INFINITY ? 0.f : top;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int tok = j.x + r / p.group, head = j.y + r % p.group;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.o_stride_t +
+                    int64_t(head) * p.o_stride_h + lane * kE;
+    if constexpr (kE == 4)
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack16<kF16>(acc[0] * inv, acc[1] * inv), pack16<kF16>(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out) = pack16<kF16>(acc[0] * inv, acc[1] * inv);
+    if (p.lse && lane == 0)
+      p.lse[int64_t(head) * p.tokens + tok] =
+          total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const int tok = u.s.q0 + u.unit * p.block_tokens + r / p.group, head = u.hk * p.group + r % p.group;
-  uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.o_stride_t +
-                  int64_t(head) * p.o_stride_h + lane * kE;
-  if constexpr (kE == 4)
-    *reinterpret_cast<uint2*>(out) =
-        make_uint2(pack16<kF16>(acc[0] * inv, acc[1] * inv), pack16<kF16>(acc[2] * inv, acc[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(out) = pack16<kF16>(acc[0] * inv, acc[1] * inv);
-  if (p.lse && lane == 0)
-    p.lse[int64_t(head) * p.tokens + tok] =
-        total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
 }
 
 void cuda_ok(cudaError_t e) {
@@ -497,21 +503,28 @@ void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const Pag
   else p.fp16 ? decode_rows<128, true>(mk, mv, p, s) : decode_rows<128, false>(mk, mv, p, s);
 }
 
-void paged_merge_launch(const PagedParams& p, cudaStream_t s) {
-  if (p.grid < 2) return;
+template <int kD, bool kF16>
+void merge_launch(const PagedParams& p, cudaStream_t s) {
+  // A few rows and up to a part of every share, or many rows and mostly two or three
+  // parts.
+  const bool few = p.unit_rows <= 32;
+  const int rows = few ? 4 : 32;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.grid - 1, (p.unit_rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32));
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.dynamicSmemBytes = 4 * (p.seqs + 1);
+  cfg.gridDim = dim3(p.grid - 1, (p.unit_rows + rows - 1) / rows);
+  cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto fn = p.head_dim == 64 ? (p.fp16 ? paged_merge_kernel<64, true> : paged_merge_kernel<64, false>)
-                             : (p.fp16 ? paged_merge_kernel<128, true> : paged_merge_kernel<128, false>);
-  cuda_ok(cudaLaunchKernelEx(&cfg, fn, p));
+  cuda_ok(cudaLaunchKernelEx(&cfg, few ? paged_merge_kernel<kD, kF16, 4, 4> : paged_merge_kernel<kD, kF16, 1, 32>, p));
+}
+
+void paged_merge_launch(const PagedParams& p, cudaStream_t s) {
+  if (p.grid < 2) return;
+  if (p.head_dim == 64) p.fp16 ? merge_launch<64, true>(p, s) : merge_launch<64, false>(p, s);
+  else p.fp16 ? merge_launch<128, true>(p, s) : merge_launch<128, false>(p, s);
 }
 
 }  // namespace mgfa

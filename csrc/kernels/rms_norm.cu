@@ -11,11 +11,11 @@
 //
 // Bound by memory: every tensor is read or written once. At 16384 x 4096 bf16 with a
 // residual the forward takes 85 us (6.3 TB/s) and the backward 112 us (4.8 TB/s, with
-// 9 us for dw's parts). A row stays in the
-// registers of the T threads that own it (N vectors each), so the statistics and the
-// output need one pass. A vector is 16 bytes, or 2 elements or one where the rows'
-// width or alignment asks for it; T grows with the row, which leaves a thread 8 to 16
-// elements up to a width of 4096, and 32 beyond.
+// 9 us for dw's parts). A row stays in the registers of the T threads that own it (N
+// vectors each), so the statistics and the output need one pass. A vector is 16 bytes,
+// also where the width is no multiple of that (kShifted: 16384 x 4095 takes 219 + 359
+// us, by single elements 255 + 374), and one element for other strides; T grows with the
+// row, which leaves a thread 8 to 16 elements up to a width of 4096, and 32 beyond.
 #include "rms_norm.cuh"
 
 #include <cuda_bf16.h>

@@ -165,6 +165,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
     p.unit_rows = p.block_tokens * p.group;
     p.tile = 128;
     p.min_share = 2;
+    p.snap = 4;
     units = (T / p.block_tokens + seqs) * Hk;
     p.grid = sms;
   }
@@ -173,9 +174,10 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   torch::Tensor work;
   if (p.grid > 1) {
     const int64_t rows = 2 * int64_t(p.grid) * p.unit_rows;
-    work = torch::empty({rows * (D + 2)}, q.options().dtype(at::kFloat));
+    work = torch::empty({rows * (D + 2) + 4 * int64_t(p.grid)}, q.options().dtype(at::kFloat));
     p.part_o = work.data_ptr<float>();
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * D);
+    p.join = reinterpret_cast<int4*>(p.part_o + rows * D);
+    p.part_ml = reinterpret_cast<float2*>(p.join + p.grid);
   }
   const uint32_t chunk = uint32_t(std::min<int64_t>(page, p.tile));
   const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, 1, 1});
