@@ -14,12 +14,14 @@
 // unit on one side moves to the unit's border: a part's way through the workspace costs
 // more than that (`snap` is at most half a share). The shares follow from the lengths alone, which the kernel reads on
 // the device: the host knows none of them, nothing waits for it, and the result does not
-// depend on timing.
+// depend on timing. Where the host can see that every unit is short, they are dealt out
+// whole instead, which needs neither the lengths' sum nor a join.
 #pragma once
 
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #ifdef __CUDACC__
@@ -53,6 +55,9 @@ struct PagedParams {
   int tile = 0;          // keys of a tile
   int min_share = 1;     // tiles
   int snap = 0;          // tiles
+  int max_units = 0;     // of a sequence and key head
+  int units = 0;         // seqs * kv_heads * max_units
+  int whole = 0;         // 1: the units are dealt out whole: no shares, no parts
   int grid = 0;          // CTAs
   int unit_rows = 0;     // rows of a part in the workspace
   // workspace: parts [2 * grid][unit_rows][head_dim] and their (max, sum), log2 units; the
@@ -225,22 +230,43 @@ struct PagedShare {
     }
     return w;
   }
+  // The first tile behind share c.
+  __device__ __forceinline__ uint64_t end(int c) const {
+    PagedUnit u;
+    const uint64_t w = per * uint32_t(c + 1);
+    return snap ? begin(c + 1, u) : w < total ? w : total;
+  }
   // The share of a unit's last tile.
   __device__ __forceinline__ int last(const PagedUnit& u) const {
     const uint64_t end = u.first + uint32_t(u.tiles);
     int c = int((end - 1) / per);
+    if (!snap) return c;
     PagedUnit v;
     while (begin(c, v) >= end) --c;  // a cut that has moved to this unit's end
     return c;
   }
 };
 
+// Unit number `id` where p.whole: they count key heads, then units from the last (in a
+// causal chunk the longest) to the first, then sequences. False where there is none.
+__device__ __forceinline__ bool paged_whole(const PagedParams& p, int id, PagedUnit& u) {
+  const int rest = id / p.kv_heads, k = rest % p.max_units;
+  u.b = rest / p.max_units;
+  u.hk = id - rest * p.kv_heads;
+  u.unit = p.max_units - 1 - k;
+  u.s = paged_seq(p, u.b);
+  if (u.s.bad && k == 0 && u.hk == 0) record_error(p.status, kErrBadArgument, 60, 0);
+  if (u.unit >= paged_units(p, u.s)) return false;
+  u.first = 0;
+  u.tiles = paged_unit_tiles(p, u.s, u.unit);
+  return true;
+}
+
 // What share c, of tiles [begin, end), leaves for others to go on with. `u` is its last
 // unit.
 __device__ __forceinline__ void paged_join(const PagedShare& share, const PagedUnit& u, bool any,
                                            uint64_t begin, uint64_t end) {
   const PagedParams& p = share.p;
-  if (!p.join) return;
   int4 j = make_int4(0, 0, 0, 0);
   if (any && u.first >= begin && u.first + uint32_t(u.tiles) > end) {
     int n = u.s.n - u.unit * p.block_tokens;
@@ -250,8 +276,77 @@ __device__ __forceinline__ void paged_join(const PagedShare& share, const PagedU
   p.join[blockIdx.x] = j;
 }
 
+// A CTA's way through its work, run by run: tiles [t0, t1) of unit u. Its threads walk
+// alike, each warp's or each its own copy.
+struct PagedWalk {
+  PagedUnit u;
+  int t0, t1;
+  uint64_t begin, end;  // shares: of tiles
+  int id;               // p.whole: the unit's number
+
+  // The first run; false where there is none. Called by all kThreads threads, whose
+  // earlier writes to shared memory all see after it.
+  template <int kThreads>
+  __device__ __forceinline__ bool start(const PagedParams& p, uint32_t* prefix, uint32_t* sums) {
+    if (p.whole) {
+      id = int(blockIdx.x) - int(gridDim.x);
+      const bool any = next(p, prefix);
+      __syncthreads();
+      return any;
+    }
+    paged_prefix<kThreads>(p, prefix, sums);
+    const PagedShare share(p, prefix);
+    begin = share.begin(blockIdx.x, u);
+    end = share.end(blockIdx.x);
+    if (begin >= end) {
+      if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
+      return false;
+    }
+    run(begin);
+    return true;
+  }
+  __device__ __forceinline__ void run(uint64_t w) {
+    t0 = int(w - u.first);
+    t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
+  }
+  __device__ __forceinline__ bool next(const PagedParams& p, const uint32_t* prefix) {
+    if (p.whole) {
+      do {
+        id += int(gridDim.x);
+        if (id >= p.units) return false;
+      } while (!paged_whole(p, id, u));
+      t0 = 0;
+      t1 = u.tiles;
+      return true;
+    }
+    const uint64_t w = u.first + uint32_t(t1);
+    if (w >= end) return false;
+    paged_next(p, prefix, u);
+    run(w);
+    return true;
+  }
+  __device__ __forceinline__ bool complete() const { return t0 == 0 && t1 == u.tiles; }
+  // The workspace's part that takes an incomplete run.
+  __device__ __forceinline__ int64_t part() const { return 2 * int64_t(blockIdx.x) + (t0 > 0 ? 0 : 1); }
+  // After the last run, by one thread.
+  __device__ __forceinline__ void leave(const PagedParams& p, const uint32_t* prefix) const {
+    if (!p.whole) paged_join(PagedShare(p, prefix), u, true, begin, end);
+  }
+};
+
 }  // namespace dev
 #endif
+
+// Lets `fn` use all of an SM's shared memory; once for each device that it runs on.
+template <class Fn>
+cudaError_t paged_allow_smem(Fn fn, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev);
+  return e;
+}
 
 // Few rows a key head (max_new * group <= 32).
 void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,

@@ -11,6 +11,7 @@
 // A sequence is served whole or not at all: where its pages do not suffice, its slot is
 // named twice or out of range, or its row is too short, it stays as it was (its `grown`
 // is 0, so that write() leaves it alone) and the status word says so.
+#include "paged_attn.cuh"
 #include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
 
@@ -439,11 +440,6 @@ void cuda_ok(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("cache pages: ") + cudaGetErrorString(e));
 }
 
-template <class Fn>
-void allow_smem(Fn fn) {
-  cuda_ok(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PlanSmem))));
-}
-
 void move_launch(const CacheState& c, const CachePool& pool, const int* count, const PageMove* moves,
                  const int* place, int64_t most, int sm_count, cudaStream_t s) {
   const int64_t pieces = (int64_t(c.page) * pool.heads * pool.head_dim / 8 + kPiece - 1) / kPiece;
@@ -465,7 +461,8 @@ void move_launch(const CacheState& c, const CachePool& pool, const int* count, c
 
 void cache_reserve_launch(const CacheState& c, const int* slots, const int* cu, int seqs,
                           int* positions, int tokens, cudaStream_t s) {
-  allow_smem(cache_reserve_kernel);
+  static std::atomic<uint64_t> allowed{0};
+  cuda_ok(paged_allow_smem(cache_reserve_kernel, allowed));
   cache_reserve_kernel<<<1, kPlanThreads, sizeof(PlanSmem), s>>>(c, slots, cu, seqs, positions, tokens);
   if (tokens > kPositionsInPlan)
     cache_positions_kernel<<<(tokens + 255) / 256, 256, 0, s>>>(c, slots, cu, seqs, positions, tokens);
@@ -487,7 +484,8 @@ void cache_free_launch(const CacheState& c, const int* slots, int n, cudaStream_
 
 void cache_fork_launch(const CacheState& c, const CachePool& pool, const int* src, const int* dst,
                        int n, bool share, int* count, PageMove* moves, int sm_count, cudaStream_t s) {
-  allow_smem(cache_fork_kernel);
+  static std::atomic<uint64_t> allowed{0};
+  cuda_ok(paged_allow_smem(cache_fork_kernel, allowed));
   cache_fork_kernel<<<1, kPlanThreads, sizeof(PlanSmem), s>>>(c, src, dst, n, share ? 1 : 0, count, moves);
   cuda_ok(cudaGetLastError());
   move_launch(c, pool, count, moves, nullptr, share ? n : int64_t(n) * c.width, sm_count, s);

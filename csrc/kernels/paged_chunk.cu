@@ -10,9 +10,11 @@
 //   warp 9          MMA: S_t = Q_t K^T (both operands in shared memory), O_t += P_t V
 //                   (P read from TMEM, where it overwrote S)
 // TMEM (512 columns): S0/P0 [0, 128), S1/P1 [128, 256), O0 and O1 from 256.
-// While one tile's softmax runs, the tensor cores work for the other; a CTA runs its
-// whole share of the work (paged_attn.cuh) through the same barriers, so the next
-// unit's Q, K and first scores are under way during a unit's epilogue.
+// While one tile's softmax runs, the tensor cores work for the other. A unit of one tile
+// (up to 128 rows) gives both halves work all the same: they take its even and odd key
+// tiles, each with a maximum, sum and O of its own, which the first joins from TMEM. A
+// CTA runs its whole share of the work (paged_attn.cuh) through the same barriers, so
+// the next unit's Q, K and first scores are under way during a unit's epilogue.
 // Bound by the tensor cores and the exponentials for long chunks, and by memory when a
 // unit has few rows.
 // O is rescaled only when the running maximum grows by more than 2^8: with the stale
@@ -41,15 +43,50 @@ struct __align__(1024) ChunkSmem {
   uint16_t q[2][kHalves][kTile * 64];  // [tile][64 columns]
   uint16_t k[2][kHalves][kTile * 64];  // [stage][64 columns]
   uint16_t v[2][kHalves][kTile * 64];
+  // Of each softmax warp: 64 bytes of its 32 rows. When the halves join, a warp of the
+  // second writes no rows, and leaves their (maximum, sum) here.
+  uint4 out[8][32][4];
   uint64_t q_full, q_empty;
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2], o_full[2], x_full, x_empty;
   uint64_t drain;
   uint32_t tmem_base;
   uint32_t abort_flag;
   uint32_t sums[kWarps];
-  PagedUnit unit[8];  // of the softmax warps, whose registers hold scores
+  // The runs, which the producer finds a few ahead: run number i in slot i & 3.
+  struct Run {
+    PagedSeq s;
+    int hk, unit, t0, t1, complete, part;  // t1 < 0: there is none
+  } runs[4];
+  uint64_t run_full[4], run_empty[4];
 };
+
+// A warp's 32 rows of 64 bytes, one per lane, to the rows' places: through shared memory,
+// so that four lanes write 64 bytes in a row at once (a lane writing its own row touches
+// 32 lines with each store, which took longer than the softmax of two key tiles).
+__device__ __forceinline__ void store_rows(uint4 (&stage)[32][4], const uint4 (&v)[4], uint32_t lane,
+                                           uint8_t* row_at, bool valid) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) stage[lane][i ^ ((lane >> 1) & 3)] = v[i];
+  __syncwarp();
+  const uint64_t at = valid ? reinterpret_cast<uint64_t>(row_at) : 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t row = i * 8 + (lane >> 2), piece = lane & 3;
+    const uint64_t to = __shfl_sync(0xffffffffu, at, row);
+    if (to) *reinterpret_cast<uint4*>(to + piece * 16) = stage[row][piece ^ ((row >> 1) & 3)];
+  }
+  __syncwarp();
+}
+
+// Scores [n, 64) to -inf; n is 64 or more in most tiles.
+__device__ __forceinline__ void hide(uint32_t (&sr)[64], int n) {
+  if (__any_sync(0xffffffffu, n < 64)) {
+#pragma unroll
+    for (int c = 0; c < 64; ++c)
+      if (c >= n) sr[c] = 0xff800000u;
+  }
+}
 
 template <int kD, bool kF16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -80,17 +117,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s.p_full[i], 4);  // one arrival per softmax warp
       mbar_init(&s.o_full[i], 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s.run_full[i], 1);
+      mbar_init(&s.run_empty[i], 9);  // the MMA's and the softmax's warps
+    }
+    mbar_init(&s.x_full, 4);
+    mbar_init(&s.x_empty, 4);
     mbar_init(&s.drain, 1);
     fence_mbar_init();
   }
-  paged_prefix<kThreads>(p, prefix, s.sums);
-  const PagedShare share(p, prefix);
-  PagedUnit u, behind;
-  const uint64_t begin = share.begin(blockIdx.x, u), end = share.begin(blockIdx.x + 1, behind);
-  if (begin >= end) {  // the whole CTA
-    if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
-    return;
-  }
+  PagedWalk at;
+  if (!at.start<kThreads>(p, prefix, s.sums)) return;  // the whole CTA
   if (warp == 0) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
@@ -107,15 +144,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int chunk = p.page < kTile ? p.page : kTile;  // keys of one box
     const uint32_t q_bytes = uint32_t(tile_tokens * p.group * kD * 2);
-    uint32_t it = 0, seg = 0;
+    uint32_t it = 0, seg = 0, run = 0;
+    auto publish = [&](int t1) {
+      const bool free = __all_sync(0xffffffffu, mbar_wait(&s.run_empty[run & 3], ((run >> 2) & 1) ^ 1, ab, 73));
+      if (free && lane == 0) {
+        auto& r = s.runs[run & 3];
+        r.s = at.u.s;
+        r.hk = at.u.hk;
+        r.unit = at.u.unit;
+        r.t0 = at.t0;
+        r.t1 = t1;
+        r.complete = at.complete();
+        r.part = int(at.part());
+        mbar_arrive(&s.run_full[run & 3]);
+      }
+      ++run;
+      return free;
+    };
     bool ok = true;
-    for (uint64_t w = begin; ok && w < end; ++seg) {
-      const int t0 = int(w - u.first);
-      const int t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
+    do {
+      const PagedUnit& u = at.u;
       const int tok0 = u.unit * p.block_tokens;
       const int tiles = u.s.n - tok0 > tile_tokens ? 2 : 1;
+      if (!(ok = publish(at.t1))) break;
       ok = __all_sync(0xffffffffu, mbar_wait(&s.q_empty, (seg & 1) ^ 1, ab, 70));
       if (!ok) break;
+      ++seg;
       if (lane == 0) {
         mbar_arrive_expect_tx(&s.q_full, tiles * q_bytes);
         for (int t = 0; t < tiles; ++t)
@@ -124,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         u.s.q0 + tok0 + t * tile_tokens, 0);
       }
       const int* row = p.page_table + int64_t(u.s.row) * p.table_stride;
-      for (int j = t0; j < t1; ++j, ++it) {
+      for (int j = at.t0; j < at.t1; ++j, ++it) {
         const int st = it & 1;
         const uint32_t ph = ((it >> 1) & 1) ^ 1;
         // boxes that hold a key below kv; the others' keys are masked, their values cut
@@ -163,14 +217,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         key % p.page, u.hk, page);
         __syncwarp();
       }
-      if (!ok) {
-        ++seg;  // this unit's Q is on its way
-        break;
-      }
-      w = u.first + uint32_t(t1);
-      if (w < end) paged_next(p, prefix, u);
-    }
-    if (lane == 0) paged_join(share, u, true, begin, end);
+    } while (ok && at.next(p, prefix));
+    if (ok) publish(-1);
+    if (lane == 0) at.leave(p, prefix);
     // Never leave with a copy outstanding.
     volatile uint32_t never = 0;
     AbortState drain{&never, nullptr, p.wait_limit_ns};
@@ -180,103 +229,106 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(&s.v_full[i & 1], (i >> 1) & 1, drain, 0);
     }
   } else if (warp == 9) {
+    uint32_t run = 0;
     // ------------------------------------------------------------ MMA issuer
     const uint32_t idesc_s = make_idesc_16(128, 128, 0, 0, kF16);
     const uint32_t idesc_o = make_idesc_16(128, kD, 0, 1, kF16);
-    auto issue_s = [&](int t, int st) {
-      const uint32_t qb = smem_u32(s.q[t][0]), kb = smem_u32(s.k[st][0]);
+    // S_t = Q_qt K(stage)^T, then its barriers
+    auto issue_s = [&](int t, int qt, int st, bool k_done, bool q_done) {
+      if (lane == 0) {
+        const uint32_t qb = smem_u32(s.q[qt][0]), kb = smem_u32(s.k[st][0]);
 #pragma unroll
-      for (int kk = 0; kk < kKSteps; ++kk) {
-        const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-        mma_ss(tmem + t * 128, make_sdesc_sw128(qb + off, 16, 1024),
-               make_sdesc_sw128(kb + off, 16, 1024), idesc_s, kk > 0);
+        for (int kk = 0; kk < kKSteps; ++kk) {
+          const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+          mma_ss(tmem + t * 128, make_sdesc_sw128(qb + off, 16, 1024),
+                 make_sdesc_sw128(kb + off, 16, 1024), idesc_s, kk > 0);
+        }
+        mma_commit(&s.s_full[t]);
+        if (k_done) mma_commit(&s.k_empty[st]);
+        if (q_done) mma_commit(&s.q_empty);
       }
     };
-    auto issue_o = [&](int t, int st, uint32_t acc) {
-      const uint32_t vb = smem_u32(s.v[st][0]);
+    auto issue_o = [&](int t, int st, bool acc, bool v_done, bool o_done) {
+      if (lane == 0) {
+        const uint32_t vb = smem_u32(s.v[st][0]);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)  // 128 keys, 16 a step
-        mma_ts(tmem + kOCol + t * kD, tmem + t * 128 + kk * 8,
-               make_sdesc_sw128(vb + kk * 2048, kHalfBytes, 1024), idesc_o,
-               (acc || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < 8; ++kk)  // 128 keys, 16 a step
+          mma_ts(tmem + kOCol + t * kD, tmem + t * 128 + kk * 8,
+                 make_sdesc_sw128(vb + kk * 2048, kHalfBytes, 1024), idesc_o,
+                 (acc || kk > 0) ? 1u : 0u);
+        if (v_done) mma_commit(&s.v_empty[st]);
+        if (o_done) mma_commit(&s.o_full[t]);
+      }
     };
     auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
-      return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity, ab, site)));
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, site));
+      tc_fence_after();
+      return ok;
     };
     uint32_t it = 0, seg = 0, pc[2] = {0, 0};  // phases used so far
     bool ok = true;
-    for (uint64_t w = begin; ok && w < end; ++seg) {
-      const int t0 = int(w - u.first);
-      const int t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
-      const bool two = u.s.n - u.unit * p.block_tokens > tile_tokens;
-      if (!(ok = wait(&s.q_full, seg & 1, 80))) break;
-      if (!(ok = wait(&s.k_full[it & 1], (it >> 1) & 1, 81))) break;
-      tc_fence_after();
-      if (lane == 0) {
-        issue_s(0, it & 1);
-        mma_commit(&s.s_full[0]);
-        if (two) {
-          issue_s(1, it & 1);
-          mma_commit(&s.s_full[1]);
-        }
-        mma_commit(&s.k_empty[it & 1]);
-        if (t0 + 1 == t1) mma_commit(&s.q_empty);
-      }
-      for (int j = t0; j < t1; ++j, ++it) {
-        const int st = it & 1, st1 = st ^ 1;
-        const uint32_t ph = (it >> 1) & 1, ph1 = ((it + 1) >> 1) & 1;
-        const bool more = j + 1 < t1;
-        if (!(ok = wait(&s.v_full[st], ph, 82))) break;
-        const int left = u.s.kv - j * kTile;
-        if (left < kTile) {
-          // Values behind the sequence's end may be anything, and 0 * NaN is NaN. Swizzling
-          // stays within a 128-byte row, so rows [left, 128) are one run of each half.
-          const int from = (left < 0 ? 0 : left) * 8;  // 16-byte pieces
-          for (int hf = 0; hf < kHalves; ++hf)
-            for (int i = from + int(lane); i < kTile * 8; i += 32)
-              reinterpret_cast<uint4*>(s.v[st][hf])[i] = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        // A unit's first P_t also says that all four warps have read the last unit's O_t.
-        if (!(ok = wait(&s.p_full[0], pc[0] & 1, 85))) break;
-        ++pc[0];
-        tc_fence_after();
-        if (lane == 0) issue_o(0, st, j > t0);
-        if (more) {
-          if (!(ok = wait(&s.k_full[st1], ph1, 86))) break;
-          tc_fence_after();
-          if (lane == 0) {
-            issue_s(0, st1);
-            mma_commit(&s.s_full[0]);
-          }
-        } else if (lane == 0) {
-          mma_commit(&s.o_full[0]);
-        }
-        if (two) {
-          if (!(ok = wait(&s.p_full[1], pc[1] & 1, 87))) break;
-          ++pc[1];
-          tc_fence_after();
-          if (lane == 0) issue_o(1, st, j > t0);
-        }
-        if (lane == 0) {
-          mma_commit(&s.v_empty[st]);
-          if (more) {
-            if (two) {
-              issue_s(1, st1);
-              mma_commit(&s.s_full[1]);
-            }
-            mma_commit(&s.k_empty[st1]);
-            if (j + 2 == t1) mma_commit(&s.q_empty);
-          } else if (two) {
-            mma_commit(&s.o_full[1]);
-          }
-        }
+    // K tile number i has arrived; V tile number i has, and is cut behind the sequence's end
+    auto wait_k = [&](uint32_t i) { return wait(&s.k_full[i & 1], (i >> 1) & 1, 81); };
+    auto wait_v = [&](uint32_t i, int left) {
+      if (!wait(&s.v_full[i & 1], (i >> 1) & 1, 82)) return false;
+      if (left < kTile) {
+        // Values behind the end may be anything, and 0 * NaN is NaN. Swizzling stays
+        // within a 128-byte row, so rows [left, 128) are one run of each half.
+        const int from = (left < 0 ? 0 : left) * 8;  // 16-byte pieces
+        for (int hf = 0; hf < kHalves; ++hf)
+          for (int x = from + int(lane); x < kTile * 8; x += 32)
+            reinterpret_cast<uint4*>(s.v[i & 1][hf])[x] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
         __syncwarp();
       }
+      return true;
+    };
+    // A unit's first P_t also says that the warps have read the last unit's O_t.
+    auto wait_p = [&](int t) { return wait(&s.p_full[t], pc[t]++ & 1, 85 + t); };
+    for (;; ++run) {
+      if (!(ok = wait(&s.run_full[run & 3], (run >> 2) & 1, 88))) break;
+      const auto& u = s.runs[run & 3];
+      const int t0 = u.t0, t1 = u.t1, kv = u.s.kv;
+      const bool two = u.s.n - u.unit * p.block_tokens > tile_tokens;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.run_empty[run & 3]);
+      if (t1 < 0) break;
+      if (!(ok = wait(&s.q_full, seg++ & 1, 80) && wait_k(it))) break;
+      if (two) {
+        issue_s(0, 0, it & 1, false, false);
+        issue_s(1, 1, it & 1, true, t0 + 1 == t1);
+        for (int j = t0; j < t1; ++j, ++it) {
+          const int st = it & 1;
+          const bool more = j + 1 < t1;
+          if (!(ok = wait_v(it, kv - j * kTile) && wait_p(0))) break;
+          issue_o(0, st, j > t0, false, !more);
+          if (more) {
+            if (!(ok = wait_k(it + 1))) break;
+            issue_s(0, 0, st ^ 1, false, false);
+          }
+          if (!(ok = wait_p(1))) break;
+          issue_o(1, st, j > t0, true, !more);
+          if (more) issue_s(1, 1, st ^ 1, true, j + 2 == t1);
+        }
+      } else {
+        // Tile j goes to half (j - t0) & 1.
+        issue_s(0, 0, it & 1, true, t0 + 1 == t1);
+        if (t0 + 1 < t1) {
+          if (!(ok = wait_k(it + 1))) break;
+          issue_s(1, 0, (it + 1) & 1, true, t0 + 2 == t1);
+        }
+        for (int j = t0; j < t1; ++j, ++it) {
+          const int t = (j - t0) & 1, st = it & 1;
+          const bool more = j + 2 < t1;
+          if (!(ok = wait_v(it, kv - j * kTile) && wait_p(t))) break;
+          issue_o(t, st, j - t0 >= 2, true, !more);
+          if (more) {
+            if (!(ok = wait_k(it + 2))) break;
+            issue_s(t, 0, st, true, j + 3 == t1);
+          }
+        }
+      }
       if (!ok) break;
-      w = u.first + uint32_t(t1);
-      if (w < end) paged_next(p, prefix, u);
     }
     // Every issued MMA has finished before TMEM is released.
     if (lane == 0) {
@@ -292,42 +344,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_off + t * 128;
     const uint32_t o_addr = tmem + lane_off + kOCol + t * kD;
-    PagedUnit& su = s.unit[warp];
-    if (lane == 0) su = u;
-    __syncwarp();
-    uint32_t sc = 0, oc = 0;  // phases used so far
+    float2* const other = reinterpret_cast<float2*>(s.out[4 + (warp & 3)]);  // by lane
+    uint32_t sc = 0, oc = 0, xc = 0, run = 0;  // phases used so far
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, site));
+      tc_fence_after();
+      return ok;
+    };
     bool ok = true;
-    for (uint64_t w = begin; ok && w < end;) {
-      const int t0 = int(w - su.first);
-      const int t1 = end - su.first < uint64_t(su.tiles) ? int(end - su.first) : su.tiles;
-      const int tok0 = su.unit * p.block_tokens + t * tile_tokens;  // this tile's first token
-      if (su.s.n > tok0) {
+    for (;; ++run) {
+      if (!(ok = wait(&s.run_full[run & 3], (run >> 2) & 1, 96))) break;
+      const auto& u = s.runs[run & 3];
+      const int n = u.s.n, kv = u.s.kv, t0 = u.t0, t1 = u.t1;
+      if (t1 < 0) break;
+      const bool two = n - u.unit * p.block_tokens > tile_tokens;
+      const int tok0 = u.unit * p.block_tokens + (two ? t * tile_tokens : 0);
+      const int j0 = two ? t0 : t0 + t, step = two ? 1 : 2;  // this half's key tiles
+      float m = -INFINITY, l = 0.f;
+      {
         // keys that this row sees, and those that the tile's first row, hence each, does
-        const int n = su.s.n, kv = su.s.kv;
         const int tok = tok0 + r / p.group;
         int lim = p.causal ? kv - n + tok + 1 : kv;
         lim = r >= tile_tokens * p.group || tok >= n ? 0 : lim < kv ? lim : kv;
         int full = p.causal ? kv - n + tok0 + 1 : kv;
         full = full < kv ? full : kv;
-        float m = -INFINITY, l = 0.f;
-        for (int j = t0; j < t1; ++j) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[t], sc & 1, ab, 90 + t));
-          if (!ok) break;
+        for (int j = j0; j < t1; j += step) {
+          if (!(ok = wait(&s.s_full[t], sc & 1, 90 + t))) break;
           ++sc;
-          tc_fence_after();
-          uint32_t sr[128];
-          tmem_ld64_sync(s_addr, &sr[0]);
-          tmem_ld64_sync(s_addr + 64, &sr[64]);
-          if ((j + 1) * kTile > full) {
-            const int n_vis = lim - j * kTile;
-#pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (c >= n_vis) sr[c] = 0xff800000u;  // -inf
-          }
-          const float m_new = fmaxf(m, row_max<128>(sr) * p.scale_log2);
+          // Keys [64, 128) are read twice, for the maximum and for the exponentials: a row's
+          // 128 scores at once, next to the probabilities, do not fit a thread's registers.
+          // (The probabilities of keys [64, 128) go where scores of [32, 64) lie, so they are
+          // stored last.)
+          const int n_vis = (j + 1) * kTile > full ? lim - j * kTile : kTile;
+          uint32_t sr[64], pk[2][32];
+          tmem_ld64_sync(s_addr + 64, sr);
+          hide(sr, n_vis - 64);
+          float m_new = row_max<64>(sr);
+          tmem_ld64_sync(s_addr, sr);
+          hide(sr, n_vis);
+          m_new = fmaxf(m, fmaxf(m_new, row_max<64>(sr)) * p.scale_log2);
           float alpha = 1.f;
           bool rescale = false;
-          if (j == t0) {
+          if (j == j0) {
             m = m_new;
           } else if (m_new > m + kRescaleThreshold) {
             alpha = ex2_approx(m - m_new);
@@ -335,17 +393,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             rescale = true;
           }
           const float neg_m = m == -INFINITY ? 0.f : -m;
-          l *= alpha;
-          uint32_t pk[2][32];
-          float lacc[4] = {0.f, 0.f, 0.f, 0.f};
-          exp_half<kF16, 0, true>(sr, 0, p.scale_log2, neg_m, pk[0], lacc);
-          tmem_st32(s_addr, pk[0]);
-          exp_half<kF16, 0, true>(sr, 1, p.scale_log2, neg_m, pk[1], lacc);
-          tmem_st32(s_addr + 32, pk[1]);
-          l += (lacc[0] + lacc[1]) + (lacc[2] + lacc[3]);
-          // S(j) was issued behind PV(j - 1), and its barrier has completed: O is at rest
+          float lacc[4] = {0.f, 0.f, 0.f, 0.f}, unused[4];
+          exp_pairs<kF16, 0, true, 32>(sr, 0, p.scale_log2, neg_m, pk[0], lacc, unused);
+          tmem_ld64_sync(s_addr + 64, sr);
+          hide(sr, n_vis - 64);
+          exp_pairs<kF16, 0, true, 32>(sr, 0, p.scale_log2, neg_m, pk[1], lacc, unused);
+          tmem_st32x2_sync(s_addr, pk[0], pk[1]);
+          l = l * alpha + ((lacc[0] + lacc[1]) + (lacc[2] + lacc[3]));
+          // S_t was issued behind the last PV_t, and its barrier has completed: O_t is at rest
           if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
+#pragma unroll 1
             for (int ch = 0; ch < kOChunks; ++ch) {
               uint32_t orow[32];
               tmem_ld32_sync(o_addr + ch * 32, orow);
@@ -355,56 +412,97 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32_sync(o_addr + ch * 32, orow);
             }
           }
-          tmem_wait_st();
-          regs_live32(pk[0]);
-          regs_live32(pk[1]);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.p_full[t]);
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s.o_full[t], oc & 1, ab, 92 + t));
-        if (!ok) break;
+      }
+      if (!ok) break;
+      if (j0 < t1) {
+        if (!(ok = wait(&s.o_full[t], oc & 1, 92 + t))) break;
         ++oc;
-        tc_fence_after();
-        const bool done = t0 == 0 && t1 == su.tiles;
-        const bool valid = r < tile_tokens * p.group && tok < su.s.n;
-        const float scale = !done ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        const int r_head = r % p.group;
-        const int64_t row_tok = su.s.q0 + tok, head = int64_t(su.hk) * p.group + r_head;
-        const int64_t slot = 2 * int64_t(blockIdx.x) + (t0 > 0 ? 0 : 1);
-        const int64_t part = slot * p.unit_rows + (tok - su.unit * p.block_tokens) * p.group + r_head;
-#pragma unroll
-        for (int ch = 0; ch < kOChunks; ++ch) {
-          uint32_t orow[32];
-          tmem_ld32_sync(o_addr + ch * 32, orow);
-          if (!valid) continue;
+        const bool joined = !two && t0 + 1 < t1;  // both halves have a part of these rows
+        if (joined && t == 1) {
+          other[lane] = make_float2(m, l);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.x_full);
+          if (!(ok = wait(&s.x_empty, xc & 1, 95))) break;
+          ++xc;
+        } else {
+          float w0 = 1.f, w1 = 0.f;
+          if (joined) {
+            if (!(ok = wait(&s.x_full, xc & 1, 94))) break;
+            ++xc;
+            const float2 o = other[lane];
+            const float top = fmaxf(m, o.x), base = top == -INFINITY ? 0.f : top;
+            w0 = ex2_approx(m - base);
+            w1 = ex2_approx(o.x - base);
+            l = l * w0 + o.y * w1;
+            m = top;
+          }
+          const bool done = u.complete;
+          const int tok = tok0 + r / p.group, r_head = r % p.group;
+          const bool valid = r < tile_tokens * p.group && tok < u.s.n;
+          const int64_t row_tok = u.s.q0 + tok, head = int64_t(u.hk) * p.group + r_head;
+          const int64_t part = int64_t(u.part) * p.unit_rows +
+                               (tok - u.unit * p.block_tokens) * p.group + r_head;
           if (done) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
-                                                  row_tok * p.o_stride_t + head * p.o_stride_h + ch * 32);
-            float v[32];
+            const float scale = l == 0.f ? 0.f : 1.f / l;
+            w0 *= scale;
+            w1 *= scale;
+          }
+          uint8_t* to = done ? reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) +
+                                                          row_tok * p.o_stride_t + head * p.o_stride_h)
+                             : reinterpret_cast<uint8_t*>(p.part_o + part * kD);
+          // one copy of the code for all columns: fetching it takes longer than running it
+#pragma unroll 1
+          for (int ch = 0; ch < kOChunks; ++ch) {
+            uint32_t orow[32];
+            tmem_ld32_sync(o_addr + ch * 32, orow);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(orow[c]) * scale;
+            for (int c = 0; c < 32; ++c) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * w0);
+            if (joined) {
+              uint32_t more_o[32];
+              tmem_ld32_sync(o_addr + kD + ch * 32, more_o);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              dst[c] = make_uint4(pack16<kF16>(v[8 * c], v[8 * c + 1]), pack16<kF16>(v[8 * c + 2], v[8 * c + 3]),
-                                  pack16<kF16>(v[8 * c + 4], v[8 * c + 5]), pack16<kF16>(v[8 * c + 6], v[8 * c + 7]));
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * kD + ch * 32);
+              for (int c = 0; c < 32; ++c)
+                orow[c] = __float_as_uint(fmaf(__uint_as_float(more_o[c]), w1, __uint_as_float(orow[c])));
+              if (ch == kOChunks - 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.x_empty);
+              }
+            }
+            auto f = [&](int c) { return __uint_as_float(orow[c]); };
+            if (done) {
+              uint4 v[4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              dst[c] = make_uint4(orow[4 * c], orow[4 * c + 1], orow[4 * c + 2], orow[4 * c + 3]);
+              for (int c = 0; c < 4; ++c)
+                v[c] = make_uint4(pack16<kF16>(f(8 * c), f(8 * c + 1)), pack16<kF16>(f(8 * c + 2), f(8 * c + 3)),
+                                  pack16<kF16>(f(8 * c + 4), f(8 * c + 5)), pack16<kF16>(f(8 * c + 6), f(8 * c + 7)));
+              store_rows(s.out[warp], v, lane, to + ch * 64, valid);
+            } else {
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                uint4 v[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  v[c] = make_uint4(orow[16 * hf + 4 * c], orow[16 * hf + 4 * c + 1],
+                                    orow[16 * hf + 4 * c + 2], orow[16 * hf + 4 * c + 3]);
+                store_rows(s.out[warp], v, lane, to + ch * 128 + hf * 64, valid);
+              }
+            }
+          }
+          if (valid) {
+            if (!done) p.part_ml[part] = make_float2(m, l);
+            else if (p.lse)
+              p.lse[head * p.tokens + row_tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
         }
-        if (valid) {
-          if (!done) p.part_ml[part] = make_float2(m, l);
-          else if (p.lse)
-            p.lse[head * p.tokens + row_tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-        }
       }
-      w = su.first + uint32_t(t1);
       __syncwarp();
-      if (w < end && lane == 0) paged_next(p, prefix, su);
-      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.run_empty[run & 3]);
     }
   }
   // ---- teardown
@@ -419,7 +517,8 @@ void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
                   const PagedParams& p, cudaStream_t s) {
   const int smem = int(sizeof(ChunkSmem<kD>)) + 1024 + 4 * (p.seqs + 1);
   auto fn = paged_chunk_kernel<kD, kF16>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = paged_allow_smem(fn, allowed);
   if (e == cudaSuccess) {
     fn<<<p.grid, kThreads, smem, s>>>(mq, mk, mv, p);
     e = cudaGetLastError();

@@ -93,14 +93,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     fence_mbar_init();
   }
-  paged_prefix<kThreads>(p, prefix, s.sums);  // its barriers cover the initialisation
-  const PagedShare share(p, prefix);
-  PagedUnit u, behind;
-  const uint64_t begin = share.begin(blockIdx.x, u), end = share.begin(blockIdx.x + 1, behind);
-  if (begin >= end) {  // the whole CTA
-    if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
-    return;
-  }
+  PagedWalk at;
+  if (!at.start<kThreads>(p, prefix, s.sums)) return;  // the whole CTA
   uint32_t it = 0;
 
   if (warp == kConsumers) {
@@ -111,11 +105,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     const int chunk = p.page < kKeys ? p.page : kKeys;  // keys of one box
     bool ok = true;
-    for (uint64_t w = begin; ok && w < end;) {
-      const int t0 = int(w - u.first);
-      const int t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
+    do {
+      const PagedUnit& u = at.u;
       const int* row = p.page_table + int64_t(u.s.row) * p.table_stride;
-      for (int t = t0; t < t1; ++t, ++it) {
+      for (int t = at.t0; t < at.t1; ++t, ++it) {
         const int st = it % kStages;
         if (!__all_sync(0xffffffffu, mbar_wait(&s.empty[st], ((it / kStages) & 1) ^ 1, ab, 61))) {
           ok = false;
@@ -144,11 +137,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         __syncwarp();
       }
-      if (!ok) break;
-      w = u.first + uint32_t(t1);
-      if (w < end) paged_next(p, prefix, u);
-    }
-    if (lane == 0) paged_join(share, u, true, begin, end);
+    } while (ok && at.next(p, prefix));
+    if (lane == 0) at.leave(p, prefix);
     // Never leave with a copy outstanding: the last kStages tiles' barriers.
     volatile uint32_t never = 0;
     AbortState drain{&never, nullptr, p.wait_limit_ns};
@@ -168,9 +158,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   // A wait that ran out must not leave the other warps in a barrier: such a warp goes on
   // to the unit's end without its tiles, and there all four stop.
   bool ok = true;
-  for (uint64_t w = begin; w < end;) {
-    const int t0 = int(w - u.first);
-    const int t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
+  do {
+    const PagedUnit& u = at.u;
     const int rows = u.s.n * p.group;
     // queries: row r = token r / group, head r % group
     for (int i = threadIdx.x; i < kR * (kD / 8); i += kConsumers * 32) {
@@ -209,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int n = 0; n < kD / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
     }
-    for (int t = t0; t < t1; ++t, ++it) {
+    for (int t = at.t0; t < at.t1; ++t, ++it) {
       const int st = it % kStages;
       ok = __all_sync(0xffffffffu, mbar_wait(&s.full[st], (it / kStages) & 1, ab, 63));
       if (!ok) break;
@@ -356,8 +345,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       consumers_sync();
     }
-    const bool done = t0 == 0 && t1 == u.tiles;
-    const int64_t slot = 2 * int64_t(blockIdx.x) + (t0 > 0 ? 0 : 1);
+    const bool done = at.complete();
+    const int64_t slot = at.part();
     for (int i = threadIdx.x; i < kR * (kD / 8); i += kConsumers * 32) {
       const int r = i / (kD / 8), c = (i % (kD / 8)) * 8;
       if (r >= rows || *ab.flag) continue;
@@ -387,10 +376,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     if (threadIdx.x == 0) s.stop = *ab.flag;
     consumers_sync();  // q, acc and ml are free again
-    if (s.stop) break;
-    w = u.first + uint32_t(t1);
-    if (w < end) paged_next(p, prefix, u);
-  }
+  } while (!s.stop && at.next(p, prefix));
 }
 
 // ---------------------------------------------------------------------- joining the parts
@@ -483,8 +469,8 @@ template <int kD, bool kF16, int kMT>
 void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s) {
   const int smem = int(sizeof(DecodeSmem<kD, kMT>)) + 1024 + 4 * (p.seqs + 1);
   auto fn = paged_decode_kernel<kD, kF16, kMT>;
-  // per device and cheap: set at each launch, for the size that this one needs
-  cuda_ok(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> allowed{0};
+  cuda_ok(paged_allow_smem(fn, allowed));
   fn<<<p.grid, kThreads, smem, s>>>(mk, mv, p);
   cuda_ok(cudaGetLastError());
 }
@@ -522,7 +508,6 @@ void merge_launch(const PagedParams& p, cudaStream_t s) {
 }
 
 void paged_merge_launch(const PagedParams& p, cudaStream_t s) {
-  if (p.grid < 2) return;
   if (p.head_dim == 64) p.fp16 ? merge_launch<64, true>(p, s) : merge_launch<64, false>(p, s);
   else p.fp16 ? merge_launch<128, true>(p, s) : merge_launch<128, false>(p, s);
 }

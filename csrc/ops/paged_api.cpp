@@ -6,7 +6,9 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstring>
 #include <tuple>
 
 #include "../kernels/paged_attn.cuh"
@@ -27,10 +29,25 @@ void check_ints(const torch::Tensor& t, const torch::Tensor& like, int64_t dims,
              name, " must be a contiguous int32 CUDA tensor of ", dims, " dimension(s) on the cache's device");
 }
 
+// The words of host_status_word(), which are never freed.
+constexpr int kHostWords = 1024;
+int* host_words() {
+  static int* words = [] {
+    void* p = nullptr;
+    C10_CUDA_CHECK(cudaHostAlloc(&p, kHostWords * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+    return static_cast<int*>(std::memset(p, 0, kHostWords * sizeof(int)));
+  }();
+  return words;
+}
+std::atomic<int> host_words_used{0};
+
 uint32_t* status_ptr(const torch::Tensor& t) {
-  MGFA_CHECK(t.scalar_type() == at::kInt && t.numel() >= 1 && (t.is_cuda() || t.is_pinned()),
-             "status must be an int32 tensor in CUDA or pinned host memory");
-  return reinterpret_cast<uint32_t*>(t.data_ptr<int>());
+  MGFA_CHECK(t.scalar_type() == at::kInt && t.numel() >= 1, "status must be an int32 tensor");
+  int* p = t.data_ptr<int>();
+  // asking the driver about a pointer costs as much as a launch
+  if (!t.is_cuda() && !(host_words_used.load() && p >= host_words() && p < host_words() + kHostWords))
+    MGFA_CHECK(t.is_pinned(), "status must be in CUDA or pinned host memory");
+  return reinterpret_cast<uint32_t*>(p);
 }
 
 // 16-bit values, head_dim 64 or 128 (the last dimension, contiguous), every row on a
@@ -70,6 +87,13 @@ CUtensorMap map16(const torch::Tensor& t, std::initializer_list<int64_t> order,
 }
 
 }  // namespace
+
+// A status word in pinned host memory, for the life of the process.
+torch::Tensor host_status_word() {
+  const int i = host_words_used.fetch_add(1);
+  MGFA_CHECK(i < kHostWords, "too many status words");
+  return torch::from_blob(host_words() + i, {1}, torch::TensorOptions().dtype(at::kInt));
+}
 
 std::tuple<torch::Tensor, OptTensor> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
@@ -170,9 +194,16 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
     p.grid = sms;
   }
   const int64_t tiles = std::max<int64_t>(1, (int64_t(p.width) * page + p.tile - 1) / p.tile);
-  p.grid = int(std::min<int64_t>(p.grid, (units * tiles + p.min_share - 1) / p.min_share));
+  // Sequences of at most 8 tiles stay whole: one CTA's way through them takes less than
+  // the joining kernel would (PLACE).
+  p.whole = tiles <= 8;
+  p.max_units = (p.max_new + p.block_tokens - 1) / p.block_tokens;
+  MGFA_CHECK(seqs * Hk * p.max_units < (int64_t(1) << 30), "too many sequences, heads and tokens");
+  p.units = int(seqs * Hk * p.max_units);
+  p.grid = int(std::min<int64_t>(p.grid, p.whole ? p.units : (units * tiles + p.min_share - 1) / p.min_share));
   torch::Tensor work;
-  if (p.grid > 1) {
+  const bool parts = p.grid > 1 && !p.whole;
+  if (parts) {
     const int64_t rows = 2 * int64_t(p.grid) * p.unit_rows;
     work = torch::empty({rows * (D + 2) + 4 * int64_t(p.grid)}, q.options().dtype(at::kFloat));
     p.part_o = work.data_ptr<float>();
@@ -189,7 +220,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
     const CUtensorMap mq = map16(q, {2, 1, 0, -1}, {64, uint32_t(group), uint32_t(p.block_tokens / 2), 1});
     paged_chunk_launch(mq, mk, mv, p, stream);
   }
-  paged_merge_launch(p, stream);
+  if (parts) paged_merge_launch(p, stream);
   return {out, want_lse ? OptTensor(lse) : OptTensor()};
 }
 

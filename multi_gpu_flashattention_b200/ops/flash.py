@@ -150,7 +150,8 @@ class HostStatus:
 
     def __init__(self, device):
         self.device = torch.device(device)
-        self.word = torch.zeros(1, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        self.word = C().host_status_word() if self.device.type == "cuda" else \
+            torch.zeros(1, dtype=torch.int32)
         self._value = self.word.numpy()
 
     def poll(self, wait: bool = False) -> None:

@@ -149,6 +149,21 @@ def test_many_units_per_cta():
     _both(Problem([90] * 40, [95 + i for i in range(40)], 8, 8, 64, 16))
 
 
+@pytest.mark.parametrize("new,kv", [([128] * 40, [128] * 40), ([64] * 200, [64] * 199 + [1100]),
+                                    ([256] * 2, [8000] * 2), ([24] * 3, [5000, 300, 24]),
+                                    ([1, 40, 128, 129, 200, 333], [1, 40, 300, 129, 1500, 340])])
+def test_again_between_other_kernels(new, kv):
+    """The same call on SMs whose registers and memories other kernels have used since."""
+    p = Problem(new, kv, 32, 8, 128, 64)
+    want, want_lse = p.run()
+    p.check(want, want_lse)
+    for _ in range(4):
+        x = torch.randn(1500, 1500, device="cuda", dtype=torch.float64)
+        int(((x @ x).abs().amax(-1) > 1e9).sum())
+        out, lse = p.run()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 # ------------------------------------------------------------------ rows and masks
 @pytest.mark.parametrize("new,heads", [([4, 3], 4), ([60, 50], 4)])
 def test_tokens_without_a_visible_key(new, heads):
