@@ -5,7 +5,7 @@ gradients are summed over the ranks.
 
     torchrun --nproc-per-node N --master-addr 127.0.0.1 examples/train_ring_lm.py \
         [--seq 65536] [--layers 4] [--d-model 1024] [--heads 8] [--kv-heads 2] \
-        [--head-dim 128] [--steps 50] [--layout zigzag] [--backend fused]
+        [--head-dim 128] [--steps 50] [--layout zigzag] [--backend fused] [--fused-ops]
 
 On GPUs (NCCL) the model runs in bf16 with the sm_100a kernels; without a GPU
 the ranks use gloo and the fp32 `torch` backend (use small sizes). The data is
@@ -53,6 +53,8 @@ def parse(argv=None):
     ap.add_argument("--layout", default="zigzag", choices=["contiguous", "zigzag", "striped"])
     ap.add_argument("--backend", default=None,
                     help="ring backend (default: fused on GPUs, torch without)")
+    ap.add_argument("--fused-ops", action="store_true",
+                    help="norms and rotary embeddings on the sm_100a kernels (GPUs)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--save", default=None, help="checkpoint written at the end")
     ap.add_argument("--resume", default=None, help="checkpoint to start from")
@@ -84,7 +86,7 @@ def main(argv=None):
 
     torch.manual_seed(a.seed)  # identical initial parameters on every rank
     model = RingTransformerLM(a.vocab, a.d_model, a.layers, a.heads, a.kv_heads,
-                              a.head_dim).to(dev, dtype)
+                              a.head_dim, fused_ops=a.fused_ops).to(dev, dtype)
     opt = torch.optim.AdamW(model.parameters(), lr=a.lr, weight_decay=0.0)
     lay = RingLayout(a.layout, a.seq, world, mask="causal")
     ids = synthetic_batch(a.batch, a.seq, a.vocab, a.seed)

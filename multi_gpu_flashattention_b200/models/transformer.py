@@ -15,6 +15,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.norm import rms_norm
+from ..ops.paged import PagedKVCache
+from ..ops.rotary import apply_rotary, rotary_frequencies
 from ..parallel.api import ring_attention
 from ..parallel.layouts import RingLayout
 
@@ -41,15 +44,33 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, base: float = 10000.0) -> t
     return torch.cat([x1 * cos - x2 * sin, x1 * sin + x2 * cos], dim=-1).to(x.dtype)
 
 
+_INV_FREQ: dict = {}
+
+
+def _frequencies(head_dim: int, device: torch.device) -> torch.Tensor:
+    """rotary()'s frequencies on a device, float64 (made once, with a synchronous copy; a
+    module's buffer would follow it to 16 bits)."""
+    key = (head_dim, device)
+    if key not in _INV_FREQ:
+        _INV_FREQ[key] = rotary_frequencies(head_dim, device=device)[0]
+    return _INV_FREQ[key]
+
+
 class RingAttentionBlock(nn.Module):
-    """Pre-norm block: x + Attn(RMSNorm(x)); then + SwiGLU(RMSNorm(.))."""
+    """Pre-norm block: x + Attn(RMSNorm(x)); then + SwiGLU(RMSNorm(.)).
+
+    fused_ops: the norms (the second with the attention's residual) and the rotary
+    embeddings run on the kernels, for CUDA tensors; each rounds its result once, where
+    the plain ops round between."""
 
     def __init__(self, d_model: int, n_heads: int, n_kv_heads: Optional[int] = None,
-                 head_dim: int = 128, mlp_mult: int = 4, causal: bool = True):
+                 head_dim: int = 128, mlp_mult: int = 4, causal: bool = True,
+                 fused_ops: bool = False):
         super().__init__()
         self.h, self.hkv = n_heads, n_kv_heads or n_heads
         self.d = head_dim
         self.causal = causal
+        self.fused_ops = fused_ops
         self.norm1, self.norm2 = RMSNorm(d_model), RMSNorm(d_model)
         self.wq = nn.Linear(d_model, self.h * head_dim, bias=False)
         self.wk = nn.Linear(d_model, self.hkv * head_dim, bias=False)
@@ -65,15 +86,27 @@ class RingAttentionBlock(nn.Module):
         B, L, _ = x.shape
         pos = layout.positions(rank)
         pos = torch.cat([pos, pos.new_zeros(L - pos.numel())]) if pos.numel() < L else pos
-        h = self.norm1(x)
-        q = rotary(self.wq(h).view(B, L, self.h, self.d), pos)
-        k = rotary(self.wk(h).view(B, L, self.hkv, self.d), pos)
+        fused = self.fused_ops and x.is_cuda
+        h = rms_norm(x, self.norm1.weight, eps=self.norm1.eps) if fused else self.norm1(x)
+        q = self.wq(h).view(B, L, self.h, self.d)
+        k = self.wk(h).view(B, L, self.hkv, self.d)
         v = self.wv(h).view(B, L, self.hkv, self.d)
+        if fused:
+            q, k = apply_rotary(q, k, pos.to(x.device), _frequencies(self.d, x.device))
+        else:
+            q, k = rotary(q, pos), rotary(k, pos)
         a = ring_attention(q.contiguous(), k.contiguous(), v.contiguous(), causal=self.causal,
                            group=group, layout=layout, backend=backend)
-        x = x + self.wo(a.reshape(B, L, self.h * self.d).to(x.dtype))
-        h = self.norm2(x)
-        return x + self.w2(F.silu(self.w1(h)) * self.w3(h))
+        a = self.wo(a.reshape(B, L, self.h * self.d).to(x.dtype))
+        if fused:
+            h, x = rms_norm(a, self.norm2.weight, residual=x, eps=self.norm2.eps)
+        else:
+            x = x + a
+            h = self.norm2(x)
+        return x + self.mlp(h)
+
+    def mlp(self, h: torch.Tensor) -> torch.Tensor:
+        return self.w2(F.silu(self.w1(h)) * self.w3(h))
 
 
 IGNORE_INDEX = -100
@@ -107,11 +140,13 @@ class RingTransformerLM(nn.Module):
 
     def __init__(self, vocab: int, d_model: int, n_layers: int, n_heads: int,
                  n_kv_heads: Optional[int] = None, head_dim: int = 128, mlp_mult: int = 4,
-                 tie_embeddings: bool = True):
+                 tie_embeddings: bool = True, fused_ops: bool = False):
         super().__init__()
         self.embed = nn.Embedding(vocab, d_model)
+        self.fused_ops = fused_ops
         self.blocks = nn.ModuleList(
-            RingAttentionBlock(d_model, n_heads, n_kv_heads, head_dim, mlp_mult, causal=True)
+            RingAttentionBlock(d_model, n_heads, n_kv_heads, head_dim, mlp_mult, causal=True,
+                               fused_ops=fused_ops)
             for _ in range(n_layers))
         self.norm = RMSNorm(d_model)
         self.head = nn.Linear(d_model, vocab, bias=False)
@@ -128,7 +163,38 @@ class RingTransformerLM(nn.Module):
         x = self.embed(ids)
         for blk in self.blocks:
             x = blk(x, layout, rank, group=group, backend=backend)
-        return self.head(self.norm(x))
+        h = rms_norm(x, self.norm.weight, eps=self.norm.eps) if self.fused_ops and x.is_cuda else self.norm(x)
+        return self.head(h)
+
+    def make_cache(self, pages: int, page_size: int, slots: int, max_tokens: int) -> PagedKVCache:
+        """An empty paged cache for serve(), of the model's type and device."""
+        w = self.embed.weight
+        return PagedKVCache.allocate(len(self.blocks), pages, page_size, self.blocks[0].hkv,
+                                     self.blocks[0].d, slots, max_tokens, dtype=w.dtype, device=w.device)
+
+    @torch.no_grad()
+    def serve(self, ids: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
+              cu_seqlens: torch.Tensor, max_seqlen: int) -> torch.Tensor:
+        """Logits [tokens, vocab] of the sequences' next tokens, on one GPU.
+
+        ids [tokens] packs the new tokens of the sequences in `slots`: sequence b's are
+        ids[cu_seqlens[b]:cu_seqlens[b + 1]], at most max_seqlen, the first of a prompt,
+        a chunk of one, or single tokens. They join the cache and see all that it holds of
+        their sequence (slots, cu_seqlens: int32 CUDA tensors). Rows outside every sequence
+        hold nothing. bfloat16 or float16 parameters, head_dim 64 or 128."""
+        pos = cache.reserve(slots, cu_seqlens, ids.numel())
+        inv_freq = _frequencies(self.blocks[0].d, ids.device)
+        x = self.embed(ids)
+        h = rms_norm(x, self.blocks[0].norm1.weight, eps=self.blocks[0].norm1.eps)
+        for i, blk in enumerate(self.blocks):
+            q, k, v = (w(h).view(ids.numel(), -1, blk.d) for w in (blk.wq, blk.wk, blk.wv))
+            q, k = apply_rotary(q, k, pos, inv_freq)
+            cache.write(i, k, v, slots, cu_seqlens)
+            a = cache.attend(i, q, slots, cu_seqlens, max_seqlen)
+            h, x = rms_norm(blk.wo(a.flatten(1)), blk.norm2.weight, residual=x, eps=blk.norm2.eps)
+            after = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm
+            h, x = rms_norm(blk.mlp(h), after.weight, residual=x, eps=after.eps)
+        return self.head(h)
 
     def loss(self, ids: torch.Tensor, targets: torch.Tensor, layout: RingLayout, rank: int = 0,
              group=None, backend: Optional[str] = None) -> torch.Tensor:

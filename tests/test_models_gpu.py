@@ -1,0 +1,151 @@
+"""The decoder's operators together, as a model uses them: served over a paged cache and
+trained with the fused norms and rotary positions, against the same model in 64 bits.
+
+The bound: the kernels round no more often than the model's plain 16-bit operators do (a
+norm rounds once and not twice, a rotation once, attention as flash_attn does), so the
+distance from the 64-bit model is at most that of the plain 16-bit model, up to the
+chance of the individual roundings, for which half as much again is allowed.
+"""
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+VOCAB, DIM, LAYERS, HEADS, KV, D = 97, 256, 3, 4, 2, 64
+
+
+def _model(dtype, fused=False, seed=0):
+    from multi_gpu_flashattention_b200 import RingTransformerLM
+    torch.manual_seed(seed)
+    m = RingTransformerLM(VOCAB, DIM, LAYERS, HEADS, KV, head_dim=D, mlp_mult=2, fused_ops=fused)
+    torch.nn.init.normal_(m.embed.weight, std=0.5)
+    for blk in m.blocks:
+        for n in (blk.norm1, blk.norm2):
+            torch.nn.init.normal_(n.weight, 1.0, 0.2)
+    return m.to("cuda", dtype)
+
+
+def _exact(model, ids):
+    """Logits of ids [S] from the parameters in 64 bits, with differentiable copies."""
+    P = {n: p.detach().double().requires_grad_() for n, p in model.named_parameters()}
+    P.setdefault("head.weight", P["embed.weight"])
+    norm = lambda x, w: x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * w
+    S = ids.numel()
+    ang = torch.arange(S, device="cuda", dtype=torch.float64)[:, None] * \
+        10000.0 ** (-torch.arange(0, D, 2, device="cuda", dtype=torch.float64) / D)
+    cos, sin = ang.cos()[:, None], ang.sin()[:, None]
+
+    def rot(t):
+        a, b = t.split(D // 2, -1)
+        return torch.cat([a * cos - b * sin, a * sin + b * cos], -1)
+
+    x = P["embed.weight"][ids]
+    hide = torch.ones(S, S, dtype=torch.bool, device="cuda").triu(1)
+    for i in range(LAYERS):
+        W = lambda n: P[f"blocks.{i}.{n}.weight"]
+        h = norm(x, W("norm1"))
+        q, k, v = ((h @ W(n).t()).view(S, -1, D) for n in ("wq", "wk", "wv"))
+        q, k = rot(q), rot(k)
+        k, v = (t.repeat_interleave(HEADS // KV, 1) for t in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q, k) / D ** 0.5
+        a = torch.einsum("hqk,khd->qhd", torch.softmax(s.masked_fill(hide, float("-inf")), -1), v)
+        x = x + a.reshape(S, -1) @ W("wo").t()
+        h = norm(x, W("norm2"))
+        x = x + (F.silu(h @ W("w1").t()) * (h @ W("w3").t())) @ W("w2").t()
+    return norm(x, P["norm.weight"]) @ P["head.weight"].t(), P
+
+
+def _ids(n, seed):
+    return torch.randint(0, VOCAB, (n,), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def _plain(model, ids):
+    from multi_gpu_flashattention_b200 import RingLayout
+    lay = RingLayout("contiguous", ids.numel(), 1, mask="causal")
+    return model(ids[None], lay)[0]
+
+
+def _off(got, ref):
+    return ((got.double() - ref).norm() / ref.norm()).item()
+
+
+def _batch(parts):
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cu = [0]
+    for p in parts:
+        cu.append(cu[-1] + p.numel())
+    return torch.cat(parts), torch.tensor(cu, **i32), max(p.numel() for p in parts)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_serving_matches_the_model(dtype):
+    """Three prompts in ragged chunks, then token by token, one of them forked on the way,
+    the pool compacted once: all logits against the whole sequences at once."""
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    model = _model(dtype)
+    seqs = [_ids(150, 1), _ids(70, 2), _ids(33, 3)]
+    tail = _ids(12, 4)
+    seqs.append(torch.cat([seqs[0][:100], tail]))      # forked from sequence 0 after 100 tokens
+    want = [_exact(model, s)[0].detach() for s in seqs]
+    with torch.no_grad():
+        plain = max(_off(_plain(model, s), w) for s, w in zip(seqs, want))
+    cache = model.make_cache(pages=40, page_size=16, slots=6, max_tokens=160)
+    slot, done, got = [4, 0, 2, 5], [0, 0, 0, 100], [[], [], [], []]
+
+    def step(which, n):
+        parts = [seqs[b][done[b]:done[b] + k] for b, k in zip(which, n)]
+        ids, cu, most = _batch(parts)
+        slots = torch.tensor([slot[b] for b in which], dtype=torch.int32, device="cuda")
+        out = model.serve(ids, cache, slots, cu, most)
+        for i, (b, k) in enumerate(zip(which, n)):
+            got[b].append(out[int(cu[i]):int(cu[i + 1])])
+            done[b] += k
+
+    step([0, 1, 2], [64, 5, 1])
+    step([2, 0, 1], [30, 36, 40])
+    cache.fork([slot[0]], [slot[3]])
+    step([3, 0, 1, 2], [1, 1, 20, 2])
+    step([0, 3], [17, 9])
+    cache.compact()
+    while any(done[b] < seqs[b].numel() for b in range(4)):
+        live = [b for b in range(4) if done[b] < seqs[b].numel()]
+        step(live, [1] * len(live))
+    check_errors()
+    got[3].insert(0, torch.cat(got[0])[:100])
+    for b in range(4):
+        off = _off(torch.cat(got[b]), want[b])
+        assert off <= 1.5 * plain, f"sequence {b}: {off} of the norm, the plain model {plain}"
+    cache.free([slot[b] for b in range(4)])
+    assert cache.free_pages() == 40
+    check_errors()
+
+
+def test_training_with_fused_operators():
+    """Loss and gradients of the fused model, as far from 64 bits as the plain one."""
+    ids = _ids(257, 7)
+    offs = {}
+    for fused in (False, True):
+        model = _model(torch.bfloat16, fused)
+        loss = F.cross_entropy(_plain(model, ids[:-1]).float(), ids[1:])
+        loss.backward()
+        logits, P = _exact(model, ids[:-1])
+        ref = F.cross_entropy(logits, ids[1:])
+        names = [n for n, _ in model.named_parameters()]
+        grads = torch.autograd.grad(ref, [P[n] for n in names])
+        offs[fused] = {n: _off(p.grad, g) for (n, p), g in zip(model.named_parameters(), grads)}
+        offs[fused]["loss"] = abs(loss.item() - ref.item()) / ref.item()
+    plain = sum(offs[False].values()) / len(offs[False])
+    for n, o in offs[True].items():
+        assert o <= 1.5 * max(offs[False][n], plain), (n, o, offs[False][n], plain)
+
+
+def test_fused_operators_leave_the_plain_model_alone():
+    model = _model(torch.bfloat16)
+    ids = _ids(64, 9)
+    assert not model.fused_ops
+    a = _plain(model, ids)
+    model.fused_ops = True
+    for b in model.blocks:
+        b.fused_ops = True
+    assert a.shape == _plain(model, ids).shape
