@@ -373,6 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++sc;
           // Keys [64, 128) are read twice, for the maximum and for the exponentials: a row's
           // 128 scores at once, next to the probabilities, do not fit a thread's registers.
+          // Nothing here may spill: a register that tcgen05.ld is still writing was seen to
+          // be spilled before its wait, which left other kernels' values in it.
           // (The probabilities of keys [64, 128) go where scores of [32, 64) lie, so they are
           // stored last.)
           const int n_vis = (j + 1) * kTile > full ? lim - j * kTile : kTile;
@@ -392,14 +394,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             m = m_new;
             rescale = true;
           }
-          const float neg_m = m == -INFINITY ? 0.f : -m;
-          float lacc[4] = {0.f, 0.f, 0.f, 0.f}, unused[4];
-          exp_pairs<kF16, 0, true, 32>(sr, 0, p.scale_log2, neg_m, pk[0], lacc, unused);
-          tmem_ld64_sync(s_addr + 64, sr);
-          hide(sr, n_vis - 64);
-          exp_pairs<kF16, 0, true, 32>(sr, 0, p.scale_log2, neg_m, pk[1], lacc, unused);
-          tmem_st32x2_sync(s_addr, pk[0], pk[1]);
-          l = l * alpha + ((lacc[0] + lacc[1]) + (lacc[2] + lacc[3]));
           // S_t was issued behind the last PV_t, and its barrier has completed: O_t is at rest
           if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
@@ -412,6 +406,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32_sync(o_addr + ch * 32, orow);
             }
           }
+          const float neg_m = m == -INFINITY ? 0.f : -m;
+          float lacc[4] = {0.f, 0.f, 0.f, 0.f}, unused[4];
+          exp_pairs<kF16, 0, true, 32>(sr, 0, p.scale_log2, neg_m, pk[0], lacc, unused);
+          tmem_ld64_sync(s_addr + 64, sr);
+          hide(sr, n_vis - 64);
+          exp_pairs<kF16, 0, true, 32>(sr, 0, p.scale_log2, neg_m, pk[1], lacc, unused);
+          tmem_st32x2_sync(s_addr, pk[0], pk[1]);
+          l = l * alpha + ((lacc[0] + lacc[1]) + (lacc[2] + lacc[3]));
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.p_full[t]);

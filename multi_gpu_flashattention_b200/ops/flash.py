@@ -181,8 +181,11 @@ def check_errors(device=None, wait: bool = True) -> None:
     was given no explicit status word) on `device` (default: every device used
     so far) reported an error. wait=True first waits for those calls to finish;
     wait=False only looks at the ones already finished."""
+    want = torch.device(device) if device is not None else None
+    if want is not None and want.type == "cuda" and want.index is None:
+        want = torch.device("cuda", torch.cuda.current_device())
     for d, h in list(_HOST_STATUS.items()):
-        if device is None or d == torch.device(device):
+        if want is None or d == want:
             h.poll(wait=wait)
     mons = [status_monitor(device)] if device is not None else list(_MONITORS.values())
     for m in mons:

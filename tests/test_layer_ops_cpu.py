@@ -17,6 +17,20 @@ def test_host_tensors_are_refused():
         apply_rotary(torch.randn(4, 2, 64), None, torch.arange(4), torch.ones(32, dtype=torch.float64))
 
 
+def test_host_caches_are_refused():
+    from multi_gpu_flashattention_b200 import PagedKVCache, paged_attention
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        PagedKVCache.allocate(1, 4, 16, 1, 64, 2, 64, device="cpu")
+    i32 = dict(dtype=torch.int32)
+    k = torch.zeros(4, 16, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        paged_attention(k[0, :1], k, k, torch.zeros(1, 4, **i32), torch.ones(1, **i32),
+                        torch.arange(2, **i32), 1)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_attention(k[0, :1].clone().requires_grad_(), k, k, torch.zeros(1, 4, **i32),
+                        torch.ones(1, **i32), torch.arange(2, **i32), 1)
+
+
 def test_gradient_of_the_8_bit_output_is_refused():
     from multi_gpu_flashattention_b200 import rms_norm_fp8
     with pytest.raises(RuntimeError, match="no gradient"):
