@@ -28,11 +28,13 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kMaxSeqs = 4096;
 
+static_assert(kMaxSeqs <= kCacheMaxSlots, "owner[] takes an entry a sequence too");
+
 struct PlanSmem {
   int first[kMaxSeqs + 1];     // pages needed by the sequences before b
-  int owner[kCacheMaxSlots];   // the first b that names the slot
+  int owner[kCacheMaxSlots];   // the first b that names the slot; then (reserve) the place
+                               // of sequence b's first new token
   int sums[kPlanWarps];
-  int done;
 };
 
 // Exclusive scan over the CTA's threads of `mine`; `total` gets the sum.
@@ -139,9 +141,9 @@ __device__ __forceinline__ int token_position(const CacheState& c, const int* sl
                                               int seqs, int t) {
   if (t < __ldg(cu) || t >= __ldg(cu + seqs)) return 0;
   const int b = token_seq(cu, seqs, t), slot = __ldg(slots + b);
-  if (slot < 0 || slot >= c.slots) return 0;
   const int n = __ldg(cu + b + 1) - __ldg(cu + b);
-  // a sequence that could not grow: where its tokens would have gone
+  if (slot < 0 || slot >= c.slots) return t - __ldg(cu + b);
+  // a sequence that could not grow: where its tokens would have gone (as in the plan)
   const int old = c.grown[slot] == n ? c.lens[slot] - n : c.lens[slot];
   return old + t - __ldg(cu + b);
 }
@@ -201,9 +203,22 @@ __global__ void __launch_bounds__(kPlanThreads)
     c.lens[slot] = old + n;
   }
   if (tokens > kPositionsInPlan) return;  // cache_positions_kernel
+  // From here on first[] is cu and owner[b] what has to be added to a row's number.
   __syncthreads();
-  for (int t = threadIdx.x; t < tokens; t += kPlanThreads)
-    positions[t] = token_position(c, slots, cu, seqs, t);
+  for (int b = threadIdx.x; b <= seqs; b += kPlanThreads) s.first[b] = cu[b];
+  __syncthreads();
+  for (int b = threadIdx.x; b < seqs; b += kPlanThreads) {
+    const int slot = slots[b], n = s.first[b + 1] - s.first[b];
+    const bool known = slot >= 0 && slot < c.slots;
+    const int old = known ? c.lens[slot] - (c.grown[slot] == n ? n : 0) : 0;
+    s.owner[b] = old - s.first[b];
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < tokens; t += kPlanThreads) {
+    const int b = plan_find(s, seqs, t);
+    const bool in = t >= s.first[0] && t < s.first[seqs];
+    positions[t] = in ? s.owner[b] + t : 0;
+  }
 }
 
 __global__ void cache_positions_kernel(const CacheState c, const int* slots, const int* cu,

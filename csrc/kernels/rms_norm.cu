@@ -78,22 +78,24 @@ struct Share {
       vec[j] = v;
     }
     if constexpr (kLay == kShifted) {
+      constexpr int kBits = 8 * sizeof(E);
+      constexpr Raw kOne = (Raw(1) << kBits) - 1;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int c = col(j, shift);
         if (!live || c >= dim || whole(c, dim)) continue;
-        uint16_t* half = reinterpret_cast<uint16_t*>(&vec[j]);
+        if (last && c + V > dim) {
+          float e[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const bool in = c + i >= 0 && c + i < dim;
-          if constexpr (sizeof(E) == 2) {
-            uint16_t x = half[i];
-            if (last && c + V > dim && in) x = reinterpret_cast<const uint16_t*>(row)[c + i];
-            half[i] = in ? x : uint16_t(0);
-          } else {
-            float x = reinterpret_cast<float*>(&vec[j])[i];
-            if (last && c + V > dim && in) x = reinterpret_cast<const float*>(row)[c + i];
-            reinterpret_cast<float*>(&vec[j])[i] = in ? x : 0.f;
+          for (int i = 0; i < V; ++i) e[i] = c + i >= 0 && c + i < dim ? to_f(row[c + i]) : 0.f;
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) raw[j * V / 2 + i] = P::narrow(f2_pack(e[2 * i], e[2 * i + 1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            const uint32_t a = uint32_t(c + 2 * i);
+            raw[j * V / 2 + i] &= (a < uint32_t(dim) ? kOne : Raw(0)) |
+                                  (a + 1 < uint32_t(dim) ? kOne << kBits : Raw(0));
           }
         }
       }
