@@ -10,10 +10,11 @@
 // only the stored h, belong to the same stream. All sums are in fp32.
 //
 // Bound by memory: every tensor is read or written once. At 16384 x 4096 bf16 with a
-// residual the forward takes 85 us (6.3 TB/s) and the backward 112 us (4.8 TB/s, with
-// 9 us for dw's parts). A row stays in the registers of the T threads that own it (N
+// residual the forward takes 84 us (6.4 TB/s) and the backward 111 us (4.8 TB/s, with
+// 9 us for dw's parts); without the packed pairs and with the weights in registers they
+// took 120 and 210 us. A row stays in the registers of the T threads that own it (N
 // vectors each), so the statistics and the output need one pass. A vector is 16 bytes,
-// also where the width is no multiple of that (kShifted: 16384 x 4095 takes 219 + 359
+// also where the width is no multiple of that (kShifted: 16384 x 4095 takes 152 + 245
 // us, by single elements 255 + 374), and one element for other strides; T grows with the
 // row, which leaves a thread 8 to 16 elements up to a width of 4096, and 32 beyond.
 #include "rms_norm.cuh"
@@ -464,7 +465,8 @@ void with_shape(int lay, int n, F f) {
 // CTAs for all rows, `most` a SM at a time; kShifted: a multiple of the vectors' elements.
 int64_t ctas_of(const Shape& sh, int layout, int v, int64_t rows, int64_t most) {
   const int64_t sets = (rows + sh.block.y - 1) / sh.block.y, apart = layout == kShifted ? v : 1;
-  return (std::min(sets, most) + apart - 1) / apart * apart;
+  // no more than run at once: a CTA left over would take as long again
+  return std::min((sets + apart - 1) / apart, std::max<int64_t>(1, most / apart)) * apart;
 }
 
 template <class E>
