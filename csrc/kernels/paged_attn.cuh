@@ -267,6 +267,7 @@ __device__ __forceinline__ bool paged_whole(const PagedParams& p, int id, PagedU
 __device__ __forceinline__ void paged_join(const PagedShare& share, const PagedUnit& u, bool any,
                                            uint64_t begin, uint64_t end) {
   const PagedParams& p = share.p;
+  if (!p.join) return;  // one share: nothing is left
   int4 j = make_int4(0, 0, 0, 0);
   if (any && u.first >= begin && u.first + uint32_t(u.tiles) > end) {
     int n = u.s.n - u.unit * p.block_tokens;

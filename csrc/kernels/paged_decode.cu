@@ -12,8 +12,8 @@
 // running maximum, sum and output of its own in registers, so the loop has no barrier
 // but the tile's; the four are added when a unit ends. 32 sequences of 8192 keys (8 key
 // heads of 128, pages of 16) take 171 us for 1.07 GB, 6.3 TB/s; one of 131072 keys 86 us,
-// and 9 us for joining 296 parts. With a shift of the work towards few CTAs (one token
-// over 100 to 320 keys) the time is latency: 9.6 us.
+// and 9 us for joining 296 parts. For short sequences the time is latency: one token each
+// over 100 to 320 keys takes 9.6 us.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 

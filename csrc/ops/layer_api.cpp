@@ -45,10 +45,12 @@ torch::Tensor as_rows(const torch::Tensor& t) {
 }
 
 // Whether row i of r starts i * dim elements behind a 16-byte boundary, up to whole
-// vectors of v elements.
+// vectors of v elements. A width that is no multiple of a vector has its rows' edges read
+// with their neighbours', so the rows must not overlap.
 bool rows_vec(const torch::Tensor& r, int64_t dim, int v) {
   return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 &&
-         (r.size(0) <= 1 || (r.stride(0) - dim) % v == 0);
+         (r.size(0) <= 1 ||
+          ((r.stride(0) - dim) % v == 0 && (dim % v == 0 || r.stride(0) >= dim)));
 }
 
 // NormFwdParams::layout of rows (of undefined tensors: none); the outputs are packed. A

@@ -53,7 +53,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     page_size a power of two from 16 to 1024, heads a multiple of kv_heads (up to 128
     times). page_table int32 [rows, width] names each sequence's pages, kv_lens int32
     [rows] its tokens, the new ones included; `slots` int32 [sequences] gives the row of
-    each sequence (default: row b). Up to 4096 sequences.
+    each sequence (default: row b). Up to 4096 sequences; the int32 tensors contiguous.
+    max_seqlen_q also decides between the kernels for few and for many rows.
 
     The new tokens are the sequence's last: token i of n sees keys [0, kv_len - n + i],
     or with causal=False all kv_len. A token that sees no key gets 0, and -inf for its

@@ -109,6 +109,16 @@ def test_strided_and_misaligned_inputs(dim):
            four(dh).transpose(0, 2))
 
 
+@pytest.mark.parametrize("width", [9, 16, 33])
+def test_rows_that_overlap(width):
+    """A sliding window over one tensor: rows one element apart."""
+    flat = torch.randn(400, device="cuda").bfloat16()
+    x = flat.unfold(0, width, 1)
+    _, w, r, dy, dh = _make(x.shape[0], width, torch.bfloat16, True)
+    assert x.stride() == (1, 1)
+    _check(x, w, r, dy, dh)
+
+
 def test_gradients_that_do_not_arrive():
     """Only h used, only y used, only some inputs differentiable."""
     from multi_gpu_flashattention_b200 import rms_norm

@@ -136,6 +136,12 @@ def test_chunk_group_sizes(group):
     _both(Problem([35, 3], [100, 200], group, 1, 64, 16))
 
 
+@pytest.mark.parametrize("n", [9, 10, 17, 31])
+def test_chunk_of_fewer_tokens_than_a_tile(n):
+    _both(Problem([n], [n + 700], 4, 1, 128, 64))
+    _both(Problem([n], [n + 3000], 8, 2, 64, 16))
+
+
 def test_chunk_split_over_ctas():
     _both(Problem([64], [30000], 4, 1, 128, 64))
     _both(Problem([200, 50], [9000, 60], 8, 2, 128, 16))
