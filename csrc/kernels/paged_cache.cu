@@ -250,6 +250,11 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const WriteParams p) {
   if (t >= p.tokens || t < __ldg(p.cu) || t >= __ldg(p.cu + p.seqs)) return;
   const int b = token_seq(p.cu, p.seqs, t), slot = __ldg(p.slots + b);
   if (slot < 0 || slot >= p.c.slots) return;
+  // a slot named again, with as many tokens, would pass the test below too: its first
+  // sequence alone has grown
+  bool again = false;
+  for (int i = lane; i < b; i += 32) again |= __ldg(p.slots + i) == slot;
+  if (__any_sync(0xffffffffu, again)) return;
   const int q0 = __ldg(p.cu + b), n = __ldg(p.cu + b + 1) - q0;
   if (p.c.grown[slot] != n || t - q0 >= n) return;  // it could not grow
   const int pos = p.c.lens[slot] - n + t - q0;

@@ -310,6 +310,16 @@ def test_slots_out_of_range_or_named_twice():
     _errors(True)
 
 
+@pytest.mark.parametrize("n", [1, 20])
+def test_slot_named_twice_with_as_many_tokens(n):
+    """The first naming's keys and values are the ones that are kept."""
+    p = Pair(layers=1)
+    p.append([0, 1], [5, 7])
+    p.append([1, 0, 1, 2, 1], [n, 1, n, n, n])
+    p.check()
+    _errors(True)
+
+
 def test_cu_seqlens_that_make_no_sense():
     p = Pair()
     p.append([0, 1], [20, 20])
