@@ -116,8 +116,14 @@ __device__ __forceinline__ int paged_units(const PagedParams& p, const PagedSeq&
   return (s.n + p.block_tokens - 1) / p.block_tokens;
 }
 
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+  const uint32_t v = a + b;
+  return v < a ? 0xffffffffu : v;
+}
+
 // prefix[b] = tiles of one key head's units of the sequences before b; prefix[seqs] the
-// total. Called by all kThreads threads of the CTA; `sums` holds kThreads / 32 values.
+// total, which is 0, and an error, where it does not fit 32 bits: nothing is done then.
+// Called by all kThreads threads of the CTA; `sums` holds kThreads / 32 values.
 template <int kThreads>
 __device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* prefix,
                                              uint32_t* sums) {
@@ -131,13 +137,13 @@ __device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* pre
       const PagedSeq s = paged_seq(p, b);
       bad |= s.bad;
       const int units = paged_units(p, s);
-      for (int u = 0; u < units; ++u) mine += uint32_t(paged_unit_tiles(p, s, u));
+      for (int u = 0; u < units; ++u) mine = add_sat(mine, uint32_t(paged_unit_tiles(p, s, u)));
     }
     uint32_t scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += v;
+      if (lane >= o) scan = add_sat(scan, v);
     }
     if (lane == 31) sums[warp] = scan;
     __syncthreads();
@@ -145,12 +151,16 @@ __device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* pre
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       const uint32_t v = sums[w];
-      if (w < warp) here += v;
-      all += v;
+      if (w < warp) here = add_sat(here, v);
+      all = add_sat(all, v);
     }
-    if (b < p.seqs) prefix[b] = here + scan - mine;
+    if (b < p.seqs) prefix[b] = add_sat(here, scan - mine);
     before = all;
     __syncthreads();
+  }
+  if (before == 0xffffffffu) {
+    bad = true;
+    before = 0;
   }
   if (threadIdx.x == 0) prefix[p.seqs] = before;
   if (bad && blockIdx.x == 0 && p.status) record_error(p.status, kErrBadArgument, 60, 0);

@@ -119,7 +119,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   MGFA_CHECK(Hk >= 1 && Hq >= 1 && Hq % Hk == 0, "query heads must be a multiple of kv heads");
   const int64_t group = Hq / Hk;
   MGFA_CHECK(group <= kPagedMaxGroup, "at most ", kPagedMaxGroup, " query heads a kv head");
-  MGFA_CHECK(pages >= 1 && pages < (int64_t(1) << 31) && T < (int64_t(1) << 30), "too many pages or tokens, or no page");
+  MGFA_CHECK(pages >= 1 && pages < (int64_t(1) << 30) && T < (int64_t(1) << 30), "too many pages or tokens, or no page");
   check_ints(page_table, k, 2, "page_table");
   check_ints(kv_lens, k, 1, "kv_lens");
   check_ints(cu_q, k, 1, "cu_seqlens_q");
@@ -281,7 +281,7 @@ void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::T
   MGFA_CHECK(power_of_two(k.size(2)) && k.size(2) >= 16 && k.size(2) <= 1024,
              "the page size must be a power of two from 16 to 1024, got ", k.size(2));
   MGFA_CHECK(k.size(0) >= 1 && k.size(1) >= 1 && k.size(3) >= 1, "a cache needs layers, pages and heads");
-  MGFA_CHECK(k.size(1) < (int64_t(1) << 31), "too many pages");
+  MGFA_CHECK(k.size(1) < (int64_t(1) << 30), "too many pages");
   check_ints(table, k, 2, "page_table");
   check_ints(lens, k, 1, "lens");
   check_ints(refs, k, 1, "refs");
@@ -289,6 +289,8 @@ void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::T
   const int64_t slots = table.size(0);
   MGFA_CHECK(slots >= 1 && slots <= kCacheMaxSlots, "page_table must have 1 to ", kCacheMaxSlots, " rows");
   MGFA_CHECK(table.size(1) >= 1 && table.size(1) * k.size(2) < (int64_t(1) << 30), "page_table is empty or too wide");
+  // a call's pages are counted in 32 bits
+  MGFA_CHECK(table.numel() < (int64_t(1) << 31), "page_table has too many entries");
   MGFA_CHECK(lens.size(0) == slots && grown.size(0) == slots, "lens and grown must have an entry for each row of page_table");
   MGFA_CHECK(refs.size(0) == k.size(1), "refs must have an entry for each page");
 }
@@ -299,7 +301,7 @@ torch::Tensor cache_reserve(torch::Tensor k, torch::Tensor table, torch::Tensor 
   const int n = check_slots(slots, k, "slots");
   check_ints(cu, k, 1, "cu_seqlens");
   MGFA_CHECK(cu.size(0) == n + 1, "cu_seqlens must be [sequences + 1]");
-  MGFA_CHECK(tokens >= 0 && tokens < (int64_t(1) << 31), "n_tokens is out of range");
+  MGFA_CHECK(tokens >= 0 && tokens < (int64_t(1) << 30), "n_tokens is out of range");
   c10::cuda::CUDAGuard guard(k.device());
   torch::Tensor pos = torch::empty({tokens}, lens.options());
   const CacheState c = cache_state(k, table, lens, refs, grown, status);
@@ -325,7 +327,7 @@ void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::T
   MGFA_CHECK(new_k.scalar_type() == k.scalar_type() && new_v.scalar_type() == k.scalar_type() &&
                  new_k.device() == k.device() && new_v.device() == k.device(),
              "new_k and new_v must have the cache's dtype and device");
-  MGFA_CHECK(new_k.size(0) < (int64_t(1) << 31), "too many tokens");
+  MGFA_CHECK(new_k.size(0) < (int64_t(1) << 30), "too many tokens");
   if (n == 0 || new_k.size(0) == 0) return;
   c10::cuda::CUDAGuard guard(k.device());
   const CacheState c = cache_state(k, table, lens, refs, grown, status);

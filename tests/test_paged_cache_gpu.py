@@ -363,6 +363,27 @@ def test_refusals():
     _errors(False)
 
 
+def test_counts_beyond_32_bits_are_refused():
+    """Where the sums of pages, tiles and tokens would not fit (memory is reserved, not touched)."""
+    from multi_gpu_flashattention_b200 import PagedKVCache, paged_attention
+    c = Pair().c
+    i32 = dict(dtype=torch.int32, device="cuda")
+    zeros = lambda n: torch.zeros(n, **i32)
+    with pytest.raises(RuntimeError, match="out of range"):
+        c.reserve([0], [0, 1], 1 << 30)
+    with pytest.raises(RuntimeError, match="too many entries"):
+        PagedKVCache(c.k, c.v, torch.empty(4096, 1 << 19, **i32), zeros(4096), c.refs, zeros(4096))
+    # 257 sequences of 2^24 tiles of 64 keys: nothing is computed, and the error is reported
+    k = torch.zeros(2, 1024, H, D, device="cuda", dtype=torch.bfloat16)
+    wide = zeros((1 << 20) - 1)[None]
+    q = torch.zeros(257, H, D, device="cuda", dtype=torch.bfloat16)
+    out = torch.ones_like(q)
+    for lens, wrong in ((0, False), (wide.numel() * 1024, True)):
+        paged_attention(q, k, k, wide, zeros(1) + lens, torch.arange(258, **i32), 1, slots=zeros(257), out=out)
+        _errors(wrong)
+        assert (out == 0).all()                 # of the empty sequences
+
+
 def test_an_error_is_raised_by_the_next_call(monkeypatch):
     monkeypatch.undo()
     from multi_gpu_flashattention_b200.ops.flash import KernelStatusError
