@@ -52,7 +52,8 @@ def _frequencies(head_dim: int, device: torch.device) -> torch.Tensor:
     module's buffer would follow it to 16 bits)."""
     key = (head_dim, device)
     if key not in _INV_FREQ:
-        _INV_FREQ[key] = rotary_frequencies(head_dim, device=device)[0]
+        with torch.inference_mode(False):  # training saves it for backward
+            _INV_FREQ[key] = rotary_frequencies(head_dim, device=device)[0]
     return _INV_FREQ[key]
 
 

@@ -69,3 +69,13 @@ def test_frequencies_refused(kw):
     from multi_gpu_flashattention_b200 import rotary_frequencies
     with pytest.raises(ValueError):
         rotary_frequencies(**kw)
+
+
+def test_frequencies_made_under_inference_mode_serve_training():
+    from multi_gpu_flashattention_b200.models.transformer import _frequencies
+    with torch.inference_mode():
+        f = _frequencies(6, torch.device("cpu"))
+    assert not f.is_inference()
+    x = torch.ones(3, dtype=torch.float64, requires_grad=True)
+    (x * f).sum().backward()  # saves f
+    assert torch.equal(x.grad, f)
