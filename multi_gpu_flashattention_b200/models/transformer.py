@@ -188,7 +188,8 @@ class RingTransformerLM(nn.Module):
         x = self.embed(ids)
         h = rms_norm(x, self.blocks[0].norm1.weight, eps=self.blocks[0].norm1.eps)
         for i, blk in enumerate(self.blocks):
-            q, k, v = (w(h).view(ids.numel(), -1, blk.d) for w in (blk.wq, blk.wk, blk.wv))
+            q, k, v = (w(h).view(ids.numel(), n, blk.d)
+                       for w, n in ((blk.wq, blk.h), (blk.wk, blk.hkv), (blk.wv, blk.hkv)))
             q, k = apply_rotary(q, k, pos, inv_freq)
             cache.write(i, k, v, slots, cu_seqlens)
             a = cache.attend(i, q, slots, cu_seqlens, max_seqlen)

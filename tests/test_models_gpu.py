@@ -149,3 +149,17 @@ def test_fused_operators_leave_the_plain_model_alone():
     for b in model.blocks:
         b.fused_ops = True
     assert a.shape == _plain(model, ids).shape
+
+
+def test_serving_steps_without_tokens():
+    """No sequence at all, and sequences that get no token: empty logits, an unchanged cache."""
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    model = _model(torch.bfloat16)
+    cache = model.make_cache(pages=8, page_size=16, slots=3, max_tokens=64)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    prompt = _ids(20, 5)
+    model.serve(prompt, cache, torch.tensor([1], **i32), torch.tensor([0, 20], **i32), 20)
+    for slots, cu in (([], [0]), ([1, 2], [0, 0, 0])):
+        out = model.serve(prompt[:0], cache, torch.tensor(slots, **i32), torch.tensor(cu, **i32), 0)
+        assert out.shape == (0, VOCAB) and cache.lens.tolist() == [0, 20, 0]
+    check_errors()
