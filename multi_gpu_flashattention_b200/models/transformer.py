@@ -100,7 +100,8 @@ class RingAttentionBlock(nn.Module):
                            group=group, layout=layout, backend=backend)
         a = self.wo(a.reshape(B, L, self.h * self.d).to(x.dtype))
         if fused:
-            h, x = rms_norm(a, self.norm2.weight, residual=x, eps=self.norm2.eps)
+            # under autocast the stream is wider than the branch
+            h, x = rms_norm(a.to(x.dtype), self.norm2.weight, residual=x, eps=self.norm2.eps)
         else:
             x = x + a
             h = self.norm2(x)

@@ -163,3 +163,21 @@ def test_serving_steps_without_tokens():
         out = model.serve(prompt[:0], cache, torch.tensor(slots, **i32), torch.tensor(cu, **i32), 0)
         assert out.shape == (0, VOCAB) and cache.lens.tolist() == [0, 20, 0]
     check_errors()
+
+
+def test_training_with_fused_operators_under_autocast():
+    """A stream in 32 bits, products in 16: gradients as far from 64 bits as the plain model's."""
+    ids = _ids(130, 11)
+    offs = {}
+    for fused in (False, True):
+        model = _model(torch.float32, fused)
+        with torch.autocast("cuda", torch.bfloat16):
+            out = _plain(model, ids[:-1])
+        F.cross_entropy(out.float(), ids[1:]).backward()
+        logits, P = _exact(model, ids[:-1])
+        names = [n for n, _ in model.named_parameters()]
+        grads = torch.autograd.grad(F.cross_entropy(logits, ids[1:]), [P[n] for n in names])
+        offs[fused] = {n: _off(p.grad, g) for (n, p), g in zip(model.named_parameters(), grads)}
+    plain = sum(offs[False].values()) / len(offs[False])
+    for n, o in offs[True].items():
+        assert o <= 1.5 * max(offs[False][n], plain), (n, o, offs[False][n], plain)
