@@ -9,7 +9,7 @@
 // Bound by memory: a byte written or moved is read once and written once. Moving 534 MB
 // of pages takes 83 us (6.4 TB/s), the plan over 2048 pages before it 5 us. A step that
 // reserves and writes 2100 tokens of 16 sequences (18 MB) is bound by two launches and
-// their chains of look-ups: 18 us.
+// their chains of look-ups: 19 us.
 //
 // A sequence is served whole or not at all: where its pages do not suffice, its slot is
 // named twice or out of range, or its row is too short, it stays as it was (its `grown`

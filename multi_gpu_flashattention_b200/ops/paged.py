@@ -20,7 +20,9 @@ graph) are left alone: outputs keep what they held there.
 What goes wrong on the device (a slot out of range or named twice, a row of the page
 table that is too short, too few free pages, a page that is not in the pool) leaves the
 sequence concerned as it was, faults nothing and raises KernelStatusError at a later
-call on the device or in check_errors().
+call on the device or in check_errors(). A slot that a batch names twice is the first
+naming's. A cache has less than 2^30 pages and 2^31 page table entries, a batch less
+than 2^30 rows.
 """
 from __future__ import annotations
 
@@ -142,7 +144,9 @@ class PagedKVCache:
         """Sequence dst[i] becomes a copy of src[i]. Full pages are held by both, and the
         tokens of a last page that is not full are copied to a page of dst's own, in all
         layers; share=False copies every page. dst has to be empty, and none of the
-        call's sources; a source may be forked several times."""
+        call's sources; a source may be forked several times. Tokens that are reserved but
+        not yet written in a layer are copied as they are: fork before reserve(), or after
+        the last layer's write()."""
         self._status.poll()
         C().cache_fork(self.k, self.v, *self._state, self._ints(src), self._ints(dst), share)
 
