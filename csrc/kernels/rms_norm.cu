@@ -40,7 +40,9 @@ constexpr int max_threads(int elements) { return elements <= 16 ? 256 : 512; }
 enum : int {
   kAligned = 0,  // rows start on 16-byte boundaries and dim is a multiple of a vector
   kShifted = 1,  // row r starts r * dim elements behind one: the vectors are the aligned ones
-                 // that cover the row, and its first and last are taken by elements
+                 // that cover the row, and its first and last are taken by elements; for
+                 // widths from a vector less one element on, so that the vectors end inside
+                 // the next row
   kSingle = 2,   // single elements, for any strides
 };
 

@@ -42,6 +42,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rms_norm(
 std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> rms_norm_fp8(
     torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps,
     int64_t group);
+int64_t norm_layout_of(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> apply_rotary(
     torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
     torch::Tensor inv_freq, bool interleaved, double magnitude);
@@ -108,6 +109,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("status") = py::none());
   m.def("rms_norm", &mgfa::rms_norm);
   m.def("rms_norm_fp8", &mgfa::rms_norm_fp8);
+  m.def("norm_layout_of", &mgfa::norm_layout_of);
   m.def("apply_rotary", &mgfa::apply_rotary);
   m.def("paged_attention", &mgfa::paged_attention);
   m.def("host_status_word", &mgfa::host_status_word);

@@ -61,8 +61,9 @@ int norm_layout(int64_t dim, std::initializer_list<const torch::Tensor*> rows,
   const int v = 16 / int(x.element_size());
   for (const torch::Tensor* r : rows)
     if (r->defined() && !rows_vec(*r, dim, v)) return 2;
-  // a shifted row covers up to v - 1 columns more
-  if (dim % v) return dim + v - 1 <= kNormMaxDim ? 1 : 2;
+  // A shifted row's vectors reach up to v - 1 columns into its neighbours: it has to fit a
+  // block with them, and the row behind it has to hold them.
+  if (dim % v) return dim >= v - 1 && dim + v - 1 <= kNormMaxDim ? 1 : 2;
   return weight.scalar_type() != x.scalar_type() ||
                  reinterpret_cast<uintptr_t>(weight.data_ptr()) % 16 == 0
              ? 0 : 1;
@@ -260,6 +261,13 @@ std::tuple<torch::Tensor, OptTensor> rms_norm(torch::Tensor x, torch::Tensor wei
   }
   NormFwd o = norm_fwd(x, weight, residual, eps, false, false, 0);
   return {o.y, opt(o.h)};
+}
+
+// How the kernels read the rows of x, weight and residual (NormFwdParams::layout), on any
+// device: for tests of the rule.
+int64_t norm_layout_of(torch::Tensor x, torch::Tensor weight, OptTensor residual) {
+  const torch::Tensor xr = as_rows(x), rr = residual.has_value() ? as_rows(*residual) : torch::Tensor();
+  return norm_layout(x.size(-1), {&xr, &rr}, weight);
 }
 
 // ------------------------------------------------------------------ rotary positions

@@ -79,3 +79,25 @@ def test_frequencies_made_under_inference_mode_serve_training():
     x = torch.ones(3, dtype=torch.float64, requires_grad=True)
     (x * f).sum().backward()  # saves f
     assert torch.equal(x.grad, f)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_norm_reads_no_further_than_its_rows(dtype):
+    """Shifted rows are read in the aligned 16-byte vectors that cover them, the very last
+    row's last vector by elements: every other row's vectors have to end inside the tensor."""
+    from multi_gpu_flashattention_b200._ext import C
+    v = 128 // torch.finfo(dtype).bits
+    shifted = set()
+    for dim in range(1, 4 * v + 2):
+        for rows in range(1, 2 * v + 2):
+            for apart in (dim, dim + v):
+                flat = torch.zeros((rows - 1) * apart + dim, dtype=dtype)
+                assert flat.data_ptr() % 16 == 0
+                x = flat.as_strided((rows, dim), (apart, 1))
+                if C().norm_layout_of(x, torch.ones(dim, dtype=dtype), None) != 1:
+                    continue
+                shifted.add(dim)
+                for r in range(rows - 1):
+                    end = r * apart + dim
+                    assert end + -end % v <= flat.numel(), (dim, rows, apart, r)
+    assert {v - 1, v + 1, 2 * v - 1, 3 * v + 2} <= shifted  # the wider ones keep their vectors

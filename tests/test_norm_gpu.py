@@ -83,6 +83,13 @@ def test_forward_and_gradients(rows, dim, dtype, residual):
     _check(*_make(rows, dim, dtype, residual, seed=rows + dim))
 
 
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", [(2, 3), (3, 1), (4, 2), (9, 1), (7, 5), (17, 3), (6, 4), (5, 6)])
+def test_rows_shorter_than_a_vector(rows, dim, dtype, residual):
+    _check(*_make(rows, dim, dtype, residual, seed=rows + dim))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_float32_weight(dtype):
     x, w, r, dy, dh = _make(130, 768, dtype, True, wdtype=torch.float32)
