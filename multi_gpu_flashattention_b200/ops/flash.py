@@ -145,8 +145,9 @@ class HostStatus:
     """The status word of the paged-cache calls that pass none, for one device, in
     pinned host memory: kernels write it across the bus, only where they have an error
     to report, and the host reads it like any variable. A call costs no read-back, and a
-    replayed CUDA graph reports as an eager call does. The next such call on the device
-    (and check_errors()) raises KernelStatusError for a non-zero word and re-arms it."""
+    replayed CUDA graph reports as an eager call does. The next call on the device that
+    leaves nothing half done by raising (and check_errors()) raises KernelStatusError for a
+    non-zero word and re-arms it."""
 
     def __init__(self, device):
         self.device = torch.device(device)

@@ -19,9 +19,12 @@ graph) are left alone: outputs keep what they held there.
 
 What goes wrong on the device (a slot out of range or named twice, a row of the page
 table that is too short, too few free pages, a page that is not in the pool) leaves the
-sequence concerned as it was, faults nothing and raises KernelStatusError at a later
-call on the device or in check_errors(). A slot that a batch names twice is the first
-naming's. A cache has less than 2^30 pages and 2^31 page table entries, a batch less
+sequence concerned as it was and faults nothing; the batch's other sequences are served.
+It raises KernelStatusError at a later call on the device, of this or another cache, or
+in check_errors(): reserve() raises before it changes anything, so the call can be made
+again; free(), fork() and compact() raise after they have done their own work; write()
+and attend(), in the middle of a step, do not raise it. A slot that a batch names twice
+is the first naming's. A cache has less than 2^30 pages and 2^31 page table entries, a batch less
 than 2^30 rows.
 """
 from __future__ import annotations
@@ -128,7 +131,6 @@ class PagedKVCache:
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: Ints, cu_seqlens: Ints) -> None:
         """The keys and values [tokens, kv_heads, D] of the batch that reserve() made room
         for, with the same slots and cu_seqlens."""
-        self._status.poll()
         C().cache_write(self.k, self.v, *self._state, layer, k, v, self._ints(slots), self._ints(cu_seqlens))
 
     def attend(self, layer: int, q: torch.Tensor, slots: Ints, cu_seqlens: Ints, max_seqlen_q: int,
@@ -138,7 +140,8 @@ class PagedKVCache:
         k, v = self._layers[layer]
         return paged_attention(q, k, v, self.page_table, self.lens, self._ints(cu_seqlens),
                                max_seqlen_q, slots=self._ints(slots), causal=causal,
-                               softmax_scale=softmax_scale, out=out, return_lse=return_lse)
+                               softmax_scale=softmax_scale, out=out, return_lse=return_lse,
+                               status=self._status.word)
 
     def fork(self, src: Ints, dst: Ints, share: bool = True) -> None:
         """Sequence dst[i] becomes a copy of src[i]. Full pages are held by both, and the
@@ -147,19 +150,19 @@ class PagedKVCache:
         call's sources; a source may be forked several times. Tokens that are reserved but
         not yet written in a layer are copied as they are: fork before reserve(), or after
         the last layer's write()."""
-        self._status.poll()
         C().cache_fork(self.k, self.v, *self._state, self._ints(src), self._ints(dst), share)
+        self._status.poll()
 
     def free(self, slots: Ints) -> None:
         """Empties the sequences; pages that no other holds become free."""
-        self._status.poll()
         C().cache_free(self.k, *self._state, self._ints(slots))
+        self._status.poll()
 
     def compact(self) -> None:
         """Moves the pages in use to the front of the pool, in all layers, and changes the
         page table to match; the free pages are the last ones then."""
-        self._status.poll()
         C().cache_compact(self.k, self.v, *self._state)
+        self._status.poll()
 
     def free_pages(self) -> int:
         """How many pages are free (waits for the device)."""

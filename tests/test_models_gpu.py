@@ -181,3 +181,52 @@ def test_training_with_fused_operators_under_autocast():
     plain = sum(offs[False].values()) / len(offs[False])
     for n, o in offs[True].items():
         assert o <= 1.5 * max(offs[False][n], plain), (n, o, offs[False][n], plain)
+
+
+def test_a_sequence_without_room_leaves_the_others_whole(monkeypatch):
+    """One of a step's sequences gets no pages, and its error is known before the first
+    layer's write: the others' logits, keys and values are those of a step in which all had
+    room, and the refused sequence is served once there is."""
+    from multi_gpu_flashattention_b200 import KernelStatusError, PagedKVCache
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    model = _model(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    slots = torch.tensor([0, 1, 2], **i32)
+    first, cu1, most1 = _batch([_ids(20, 1), _ids(3, 2), _ids(10, 3)])
+    ids, cu, most = _batch([_ids(1, 4), _ids(40, 5), _ids(6, 6)])  # 0, 2 and 0 pages more
+    write = PagedKVCache.write
+
+    def late(self, *a):  # what reserve() reported has arrived
+        torch.cuda.synchronize()
+        return write(self, *a)
+
+    monkeypatch.setattr(PagedKVCache, "write", late)
+    runs = {}
+    for pages in (16, 5):
+        cache = model.make_cache(pages=pages, page_size=16, slots=4, max_tokens=96)
+        model.serve(first, cache, slots, cu1, most1)
+        torch.cuda.synchronize()
+        check_errors()
+        runs[pages] = model.serve(ids, cache, slots, cu, most), cache
+    (got, short), (want, roomy) = runs[5], runs[16]
+    with pytest.raises(KernelStatusError, match="too few free pages"):
+        model.serve(ids[1:41], short, slots[1:2], torch.tensor([0, 40], **i32), 40)
+    assert short.lens.tolist() == [21, 3, 16, 0] and roomy.lens.tolist() == [21, 43, 16, 0]
+    check_errors()
+    for rows in (slice(0, 1), slice(41, 47)):
+        assert torch.equal(got[rows], want[rows])
+
+    def held(cache, slot):
+        n = int(cache.lens[slot])
+        rows = cache.page_table[slot, :-(-n // 16)].long()
+        return [pool[:, rows].flatten(1, 2)[:, :n] for pool in (cache.k, cache.v)]
+
+    for slot in (0, 2):
+        for a, b in zip(held(short, slot), held(roomy, slot)):
+            assert torch.equal(a, b)
+    short.free([0])
+    again = model.serve(ids[1:41], short, slots[1:2], torch.tensor([0, 40], **i32), 40)
+    ref = _exact(model, torch.cat([_ids(3, 2), ids[1:41]]))[0].detach()[3:]
+    plain = _off(_plain(model, torch.cat([_ids(3, 2), ids[1:41]]))[3:].detach(), ref)
+    assert _off(again, ref) <= 1.5 * plain
+    check_errors()
