@@ -151,6 +151,23 @@ __device__ __forceinline__ int token_position(const CacheState& c, const int* sl
   return old + t - __ldg(cu + b);
 }
 
+// Whether reserve() has made room for row t of the batch, which is row t - q0 of the n that
+// sequence `slot` has grown by. Called by a whole warp, for cu[0] <= t < cu[seqs].
+__device__ __forceinline__ bool row_grew(const CacheState& c, const int* slots, const int* cu,
+                                         int seqs, int t, int lane, int& slot, int& q0, int& n) {
+  const int b = token_seq(cu, seqs, t);
+  slot = __ldg(slots + b);
+  if (slot < 0 || slot >= c.slots) return false;
+  // a slot named again, with as many tokens, would pass the test below too: its first
+  // sequence alone has grown
+  bool again = false;
+  for (int i = lane; i < b; i += 32) again |= __ldg(slots + i) == slot;
+  if (__any_sync(0xffffffffu, again)) return false;
+  q0 = __ldg(cu + b);
+  n = __ldg(cu + b + 1) - q0;
+  return c.grown[slot] == n && t - q0 < n;
+}
+
 constexpr int kPositionsInPlan = 4096;
 
 __global__ void __launch_bounds__(kPlanThreads)
@@ -248,15 +265,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const WriteParams p) {
   const int t = int(id >> 1), lane = threadIdx.x & 31;
   const bool value = id & 1;
   if (t >= p.tokens || t < __ldg(p.cu) || t >= __ldg(p.cu + p.seqs)) return;
-  const int b = token_seq(p.cu, p.seqs, t), slot = __ldg(p.slots + b);
-  if (slot < 0 || slot >= p.c.slots) return;
-  // a slot named again, with as many tokens, would pass the test below too: its first
-  // sequence alone has grown
-  bool again = false;
-  for (int i = lane; i < b; i += 32) again |= __ldg(p.slots + i) == slot;
-  if (__any_sync(0xffffffffu, again)) return;
-  const int q0 = __ldg(p.cu + b), n = __ldg(p.cu + b + 1) - q0;
-  if (p.c.grown[slot] != n || t - q0 >= n) return;  // it could not grow
+  int slot, q0, n;
+  if (!row_grew(p.c, p.slots, p.cu, p.seqs, t, lane, slot, q0, n)) return;
   const int pos = p.c.lens[slot] - n + t - q0;
   if (pos < 0 || pos >= int64_t(p.c.width) * p.c.page) return;
   const int page = p.c.table[int64_t(slot) * p.c.width + pos / p.c.page];
@@ -276,6 +286,18 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const WriteParams p) {
     *reinterpret_cast<uint4*>(dst + h * stride[3] + c) =
         *reinterpret_cast<const uint4*>(src + h * from[1] + c);
   }
+}
+
+// One warp per row: whether it belongs to a sequence that reserve() left as it was.
+__global__ void __launch_bounds__(256)
+    cache_refused_kernel(const CacheState c, const int* slots, const int* cu, int seqs,
+                         bool* refused, int tokens) {
+  const int t = int((int64_t(blockIdx.x) * 256 + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+  if (t >= tokens) return;
+  int slot, q0, n;
+  const bool in = t >= __ldg(cu) && t < __ldg(cu + seqs);
+  const bool no = in && !row_grew(c, slots, cu, seqs, t, lane, slot, q0, n);
+  if (lane == 0) refused[t] = no;
 }
 
 // One CTA per entry; a slot named again is freed once.
@@ -489,6 +511,12 @@ void cache_reserve_launch(const CacheState& c, const int* slots, const int* cu, 
   cache_reserve_kernel<<<1, kPlanThreads, sizeof(PlanSmem), s>>>(c, slots, cu, seqs, positions, tokens);
   if (tokens > kPositionsInPlan)
     cache_positions_kernel<<<(tokens + 255) / 256, 256, 0, s>>>(c, slots, cu, seqs, positions, tokens);
+  cuda_ok(cudaGetLastError());
+}
+
+void cache_refused_launch(const CacheState& c, const int* slots, const int* cu, int seqs,
+                          bool* refused, int tokens, cudaStream_t s) {
+  cache_refused_kernel<<<unsigned((int64_t(tokens) + 7) / 8), 256, 0, s>>>(c, slots, cu, seqs, refused, tokens);
   cuda_ok(cudaGetLastError());
 }
 

@@ -37,6 +37,9 @@ struct PageMove {
 
 void cache_reserve_launch(const CacheState& c, const int* slots, const int* cu, int seqs,
                           int* positions, int tokens, cudaStream_t stream);
+// refused[t]: whether row t belongs to a sequence that the reserve before left as it was.
+void cache_refused_launch(const CacheState& c, const int* slots, const int* cu, int seqs,
+                          bool* refused, int tokens, cudaStream_t stream);
 void cache_write_launch(const CacheState& c, const CachePool& pool, const void* k, const void* v,
                         const int64_t* k_stride, const int64_t* v_stride, const int* slots,
                         const int* cu, int seqs, int tokens, cudaStream_t stream);

@@ -57,6 +57,9 @@ void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::T
 torch::Tensor cache_reserve(torch::Tensor k, torch::Tensor table, torch::Tensor lens,
                             torch::Tensor refs, torch::Tensor grown, torch::Tensor status,
                             torch::Tensor slots, torch::Tensor cu, int64_t tokens);
+torch::Tensor cache_refused(torch::Tensor k, torch::Tensor table, torch::Tensor lens,
+                            torch::Tensor refs, torch::Tensor grown, torch::Tensor status,
+                            torch::Tensor slots, torch::Tensor cu, int64_t tokens);
 void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                  torch::Tensor refs, torch::Tensor grown, torch::Tensor status, int64_t layer,
                  torch::Tensor new_k, torch::Tensor new_v, torch::Tensor slots, torch::Tensor cu);
@@ -115,6 +118,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("host_status_word", &mgfa::host_status_word);
   m.def("cache_check", &mgfa::cache_check);
   m.def("cache_reserve", &mgfa::cache_reserve);
+  m.def("cache_refused", &mgfa::cache_refused);
   m.def("cache_write", &mgfa::cache_write);
   m.def("cache_free", &mgfa::cache_free);
   m.def("cache_fork", &mgfa::cache_fork);

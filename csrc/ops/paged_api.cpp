@@ -313,6 +313,26 @@ torch::Tensor cache_reserve(torch::Tensor k, torch::Tensor table, torch::Tensor 
   return pos;
 }
 
+// bool [tokens]: the rows of sequences that cache_reserve, called with the same slots and
+// cu, left as they were.
+torch::Tensor cache_refused(torch::Tensor k, torch::Tensor table, torch::Tensor lens,
+                            torch::Tensor refs, torch::Tensor grown, torch::Tensor status,
+                            torch::Tensor slots, torch::Tensor cu, int64_t tokens) {
+  const int n = check_slots(slots, k, "slots");
+  check_ints(cu, k, 1, "cu_seqlens");
+  MGFA_CHECK(cu.size(0) == n + 1, "cu_seqlens must be [sequences + 1]");
+  MGFA_CHECK(tokens >= 0 && tokens < (int64_t(1) << 30), "n_tokens is out of range");
+  c10::cuda::CUDAGuard guard(k.device());
+  torch::Tensor refused = torch::empty({tokens}, lens.options().dtype(at::kBool));
+  if (n > 0 && tokens > 0)
+    cache_refused_launch(cache_state(k, table, lens, refs, grown, status), slots.data_ptr<int>(),
+                         cu.data_ptr<int>(), n, refused.data_ptr<bool>(), int(tokens),
+                         at::cuda::getCurrentCUDAStream());
+  else
+    refused.zero_();
+  return refused;
+}
+
 void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                  torch::Tensor refs, torch::Tensor grown, torch::Tensor status, int64_t layer,
                  torch::Tensor new_k, torch::Tensor new_v, torch::Tensor slots, torch::Tensor cu) {

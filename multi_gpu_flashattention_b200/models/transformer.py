@@ -183,7 +183,8 @@ class RingTransformerLM(nn.Module):
         ids[cu_seqlens[b]:cu_seqlens[b + 1]], at most max_seqlen, the first of a prompt,
         a chunk of one, or single tokens. They join the cache and see all that it holds of
         their sequence (slots, cu_seqlens: int32 CUDA tensors). Rows outside every sequence
-        hold nothing. bfloat16 or float16 parameters, head_dim 64 or 128."""
+        hold nothing; those of a sequence that got no room in the cache, which stays as it
+        was, are NaN. bfloat16 or float16 parameters, head_dim 64 or 128."""
         pos = cache.reserve(slots, cu_seqlens, ids.numel())
         inv_freq = _frequencies(self.blocks[0].d, ids.device)
         x = self.embed(ids)
@@ -197,6 +198,7 @@ class RingTransformerLM(nn.Module):
             h, x = rms_norm(blk.wo(a.flatten(1)), blk.norm2.weight, residual=x, eps=blk.norm2.eps)
             after = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm
             h, x = rms_norm(blk.mlp(h), after.weight, residual=x, eps=after.eps)
+        h.masked_fill_(cache.refused(slots, cu_seqlens, ids.numel())[:, None], float("nan"))
         return self.head(h)
 
     def loss(self, ids: torch.Tensor, targets: torch.Tensor, layout: RingLayout, rank: int = 0,

@@ -124,9 +124,15 @@ class PagedKVCache:
         """Room for the batch's new tokens: sequence slots[b] grows by cu_seqlens[b + 1] -
         cu_seqlens[b] tokens, and gets pages for them. Returns the new tokens' positions,
         int32 [n_tokens] (0 for rows outside every sequence). A sequence that cannot get
-        all its pages does not grow."""
+        all its pages does not grow: refused() tells its rows."""
         self._status.poll()
         return C().cache_reserve(self.k, *self._state, self._ints(slots), self._ints(cu_seqlens), n_tokens)
+
+    def refused(self, slots: Ints, cu_seqlens: Ints, n_tokens: int) -> torch.Tensor:
+        """Which rows of the batch belong to a sequence that reserve(), called with the same
+        arguments just before, left as it was: bool [n_tokens], on the device. What attend()
+        returns for these rows stands for nothing."""
+        return C().cache_refused(self.k, *self._state, self._ints(slots), self._ints(cu_seqlens), n_tokens)
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: Ints, cu_seqlens: Ints) -> None:
         """The keys and values [tokens, kv_heads, D] of the batch that reserve() made room

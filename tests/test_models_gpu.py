@@ -230,3 +230,23 @@ def test_a_sequence_without_room_leaves_the_others_whole(monkeypatch):
     plain = _off(_plain(model, torch.cat([_ids(3, 2), ids[1:41]]))[3:].detach(), ref)
     assert _off(again, ref) <= 1.5 * plain
     check_errors()
+
+
+def test_logits_of_a_sequence_without_room_are_nan():
+    """It stays as it was, and what its rows hold cannot be taken for an answer."""
+    from multi_gpu_flashattention_b200 import KernelStatusError
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    model = _model(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = model.make_cache(pages=3, page_size=16, slots=4, max_tokens=64)
+    ids, cu, most = _batch([_ids(5, 1), _ids(33, 2), _ids(7, 3), _ids(7, 4)])
+    tail = torch.cat([ids, _ids(3, 5)])  # rows of no sequence
+    # 1 page, 3 pages of the 2 left, a slot out of range, a slot named again
+    out = model.serve(tail, cache, torch.tensor([2, 0, 4, 2], **i32), cu, most)
+    with pytest.raises(KernelStatusError):
+        check_errors()
+    assert cache.lens.tolist() == [0, 0, 5, 0]
+    assert torch.isfinite(out[:5]).all() and out[5:52].isnan().all()
+    out = model.serve(ids[:5], cache, torch.tensor([2], **i32), torch.tensor([0, 5], **i32), 5)
+    assert torch.isfinite(out).all()
+    check_errors()

@@ -310,6 +310,23 @@ def test_slots_out_of_range_or_named_twice():
     _errors(True)
 
 
+def test_rows_of_refused_sequences():
+    p = Pair(pages=6, layers=1)
+    cu = [1, 4, 8, 28, 31, 31, 100, 103]
+    slots = [3, 12, 1, 3, 0, 2, 5]   # slot 12 there is none, 3 again, 0 with no token, too many for 2
+    p.c.reserve(slots, cu, 105)
+    got = p.c.refused(slots, cu, 105)
+    assert got.dtype == torch.bool
+    want = torch.zeros(105, dtype=torch.bool)
+    want[4:8] = want[28:31] = want[31:103] = True  # pages are given in order: 5 gets none
+    assert p.c.lens.tolist()[:6] == [0, 20, 0, 3, 0, 0]
+    assert torch.equal(got.cpu(), want)
+    assert p.c.refused([], [0], 4).tolist() == [False] * 4 and p.c.refused([1], [0, 0], 0).shape == (0,)
+    with pytest.raises(RuntimeError):
+        p.c.refused([1], [0], 4)
+    _errors(True)
+
+
 @pytest.mark.parametrize("n", [1, 20])
 def test_slot_named_twice_with_as_many_tokens(n):
     """The first naming's keys and values are the ones that are kept."""
