@@ -73,6 +73,24 @@ struct PagedParams {
 #ifdef __CUDACC__
 namespace dev {
 
+// A row's probabilities are 2^(score - base) with base = its running maximum - kLift. Their
+// rounding to 16 bits for the product with V (half a step of the type) is relative, as the
+// output's own, down to the type's smallest normal number: 2^-126 in bf16, but 2^-14 in fp16,
+// where weights of 2^-25 would vanish beside the largest, while the fp32 sum counts them. So
+// fp16's are lifted to just below its largest number, 65504: up to 2^(kLift + kStale) = 2^15,
+// kStale the powers of two by which the kernel lets its maximum lag. The common factor goes
+// out with the sum, and the rest of the kernels sees base as the maximum. Both roundings are
+// upwards, so that no probability passes 2^15 (and, at scores whose last place is worth
+// more than a power of two, infinity).
+template <bool kF16, int kStale>
+struct PagedBase {
+  static constexpr float kLift = kF16 ? 15.f - kStale : 0.f;
+  static __device__ __forceinline__ float of(float top, float scale_log2) {
+    if constexpr (kF16) return __fadd_ru(__fmul_ru(top, scale_log2), -kLift);
+    return top * scale_log2;
+  }
+};
+
 // Sequence b as the kernels use it, whatever the arrays say: n new tokens from row q0,
 // all inside [0, tokens) and at most max_new; kv within the table's row. `bad` says that
 // something had to be cut.

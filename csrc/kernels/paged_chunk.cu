@@ -21,8 +21,9 @@
 // 32 heads over 32768 keys (8 key heads of 128, causal) take 1.06 ms, 1.01 PFLOP/s, and
 // 1.25 ms (0.85) under the power cap of a long run; units of few rows are bound by memory:
 // 16 tokens of 8 sequences over 8192 keys take 90 us for 268 MB.
-// O is rescaled only when the running maximum grows by more than 2^8: with the stale
-// one P stays below 2^8, whose 16-bit rounding is relative, and sums are fp32.
+// O is rescaled only when the running maximum grows by more than 2^8 (fp16: 2^4, which
+// leaves 2^11 for PagedBase's lift): with the stale one P stays below 2^8 (2^15). Sums are
+// fp32.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 #include "softmax_exp.cuh"
@@ -39,7 +40,8 @@ constexpr int kTile = 128;
 constexpr int kHalfBytes = kTile * 64 * 2;  // one 128 x 64 16-bit swizzled box
 constexpr int kWarps = 10;
 constexpr int kThreads = kWarps * 32;
-constexpr float kRescaleThreshold = 8.0f;   // log2 units
+// How far the running maximum may lag, in powers of two.
+constexpr int stale(bool f16) { return f16 ? 4 : 8; }
 
 template <int kD>
 struct __align__(1024) ChunkSmem {
@@ -388,12 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           float m_new = row_max<64>(sr);
           tmem_ld64_sync(s_addr, sr);
           hide(sr, n_vis);
-          m_new = fmaxf(m, fmaxf(m_new, row_max<64>(sr)) * p.scale_log2);
+          m_new = fmaxf(m, PagedBase<kF16, stale(kF16)>::of(fmaxf(m_new, row_max<64>(sr)), p.scale_log2));
           float alpha = 1.f;
           bool rescale = false;
           if (j == j0) {
             m = m_new;
-          } else if (m_new > m + kRescaleThreshold) {
+          } else if (kF16 ? m_new - m > stale(kF16) : m_new > m + stale(kF16)) {
             alpha = ex2_approx(m - m_new);
             m = m_new;
             rescale = true;

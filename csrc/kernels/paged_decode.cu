@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                             fmaxf(sc[m][1][2 * h], sc[m][1][2 * h + 1]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float now = fmaxf(mx[m][h], top * p.scale_log2);
+          const float now = fmaxf(mx[m][h], PagedBase<kF16, 0>::of(top, p.scale_log2));
           const float base = now == -INFINITY ? 0.f : now;
           const float keep = ex2_approx(mx[m][h] - base);  // -inf: 0, nothing was kept
           mx[m][h] = now;
@@ -269,8 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        // the 16-bit probabilities' rounding (half a step of p <= 1) is below the
-        // output's own; the sum above keeps them in fp32
+        // rounded to 16 bits (PagedBase); the sum above keeps them in fp32
         pf[m][0] = pack16<kF16>(sc[m][0][0], sc[m][0][1]);
         pf[m][1] = pack16<kF16>(sc[m][0][2], sc[m][0][3]);
         pf[m][2] = pack16<kF16>(sc[m][1][0], sc[m][1][1]);

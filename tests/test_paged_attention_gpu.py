@@ -200,6 +200,66 @@ def test_large_scores(new):
     p.check(out, lse, scale=0.35)
 
 
+class Shared(Problem):
+    """`seqs` sequences over the same pages, with keys (x, 0, ..., 0) for x of `first`, and
+    queries (1, 0, ..., 0), so that scores are x * scale; enough of them that a CTA goes
+    over a sequence's keys without a cut."""
+
+    def __init__(self, first, values, new, seqs, dtype):
+        super().__init__([new], [first.numel()], 1, 1, 64, 64, dtype)
+        self.new, self.kv = [new] * seqs, [first.numel()] * seqs
+        k = torch.zeros(first.numel(), 1, 64, device="cuda", dtype=dtype)
+        k[:, 0, 0] = first
+        v = values[:, None, None].expand(-1, 1, 64).to(dtype)
+        for t, pool in ((k, self.k), (v, self.v)):
+            for j, i in enumerate(self.table[0].tolist()):
+                part = t[j * 64:(j + 1) * 64]
+                pool[i, :part.shape[0]] = part
+        self.keys, self.values = [k] * seqs, [v] * seqs
+        self.table = self.table.expand(seqs, -1).contiguous()
+        self.lens = self.lens.expand(seqs).contiguous()
+        self.cu = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * new
+        self.q = torch.zeros(seqs * new, 1, 64, device="cuda", dtype=dtype)
+        self.q[..., 0] = 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", [0, 20000])
+@pytest.mark.parametrize("new,seqs", [(1, 320), (40, 160)])
+def test_many_small_weights_beside_a_large_one(new, seqs, at, dtype):
+    """One key with the value 0 and 32767 with the value 1 and 2^-25.2 of its weight, which
+    fp16 has no step for. Beyond the tolerance of a weight's relative rounding, an fp16 weight
+    may be off by 2^-36 of the largest: fp16's step at its small end, 2^-24, is 2^-35 of the
+    2^11 that the largest is given at least."""
+    n = 32768
+    first, values = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    first[at], values[at] = 16.0, 0.0
+    p = Shared(first, values, new, seqs, dtype)
+    out, lse = p.run(causal=False, softmax_scale=25.2 * math.log(2) / 16)
+    w = 2.0 ** -25.2
+    total = 1 + (n - 1) * w
+    want, u = (n - 1) * w / total, torch.finfo(dtype).eps / 2
+    bound = u * want + (u + 4e-5) * want + (n - 1) * 2.0 ** -36 + 2.0 ** -25
+    assert (out.double() - want).abs().max().item() <= bound
+    ref = 25.2 * math.log(2) + math.log(total)
+    assert (lse.double() - ref).abs().max().item() <= 2e-5 * (1 + ref)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("step", [0.4, 1.7, 3.9, 4.1, 8.1])
+@pytest.mark.parametrize("new,seqs", [(1, 320), (40, 160)])
+def test_a_maximum_that_creeps_up(new, seqs, step, dtype):
+    """Scores that grow by `step` powers of two every 128 keys: by less and by more than a
+    kernel lets its maximum lag. No weight may pass the type's largest number."""
+    n = 8000
+    tile = torch.arange(n, device="cuda") // 128
+    g = torch.Generator("cuda").manual_seed(3)
+    p = Shared(tile.float(), torch.randn(n, device="cuda", generator=g), new, seqs, dtype)
+    scale = step * math.log(2)
+    out, lse = p.run(causal=False, softmax_scale=scale)
+    p.check(out, lse, causal=False, scale=scale)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_nan_in_a_query_stays_in_its_row(new):
     p = Problem([new, new], [90, 300], 4, 2, 64, 16)
