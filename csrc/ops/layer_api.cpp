@@ -11,6 +11,7 @@
 #include <tuple>
 #include <vector>
 
+#include "forward_ad.hpp"
 #include "../kernels/rms_norm.cuh"
 #include "../kernels/rotary.cuh"
 
@@ -158,6 +159,7 @@ std::tuple<torch::Tensor, torch::Tensor, OptTensor> rms_norm_fp8(torch::Tensor x
                                                                  torch::Tensor weight,
                                                                  OptTensor residual, double eps,
                                                                  int64_t group) {
+  refuse_tangents("rms_norm_fp8", {x, weight, residual.value_or(torch::Tensor())});
   NormFwd o = norm_fwd(x, weight, residual, eps, false, true, group);
   return {o.y, o.scale, opt(o.h)};
 }
@@ -239,6 +241,7 @@ struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
     const bool res = grads.size() > 1;
     const torch::Tensor dy = grads[0], dh = res ? grads[1] : torch::Tensor();
     if (!dy.defined() && !dh.defined()) return {{}, {}, {}, {}};
+    refuse_tangents("rms_norm's gradient", {dy, dh});
     const variable_list saved = ctx->get_saved_variables();
     auto [dx, dw] = norm_bwd(dy, dh, saved[0], saved[1], saved[2], ctx->needs_input_grad(1));
     return once({ctx->needs_input_grad(0) ? dx : torch::Tensor(), dw,
@@ -255,6 +258,7 @@ bool wants_grad(const torch::Tensor& a, const OptTensor& b) {
 // y and h (with a residual); differentiable.
 std::tuple<torch::Tensor, OptTensor> rms_norm(torch::Tensor x, torch::Tensor weight,
                                               OptTensor residual, double eps) {
+  refuse_tangents("rms_norm", {x, weight, residual.value_or(torch::Tensor())});
   if (wants_grad(x, residual) || wants_grad(weight, {})) {
     variable_list o = RmsNormFn::apply(x, weight, residual, eps);
     return {o[0], o.size() > 1 ? OptTensor(o[1]) : OptTensor()};
@@ -370,6 +374,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const torch::Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : torch::Tensor();
     if (!dq.defined() && !dk.defined()) return {{}, {}, {}, {}, {}, {}};
+    refuse_tangents("apply_rotary's gradient", {dq, dk});
     const variable_list saved = ctx->get_saved_variables();
     const bool il = ctx->saved_data["interleaved"].toBool();
     const double mag = ctx->saved_data["magnitude"].toDouble();
@@ -385,6 +390,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
 std::tuple<torch::Tensor, OptTensor> apply_rotary(torch::Tensor q, OptTensor k,
                                                   torch::Tensor positions, torch::Tensor inv_freq,
                                                   bool interleaved, double magnitude) {
+  refuse_tangents("apply_rotary", {q, k.value_or(torch::Tensor()), inv_freq});
   if (wants_grad(q, k)) {
     variable_list o = RotaryFn::apply(q, k, positions, inv_freq, interleaved, magnitude);
     return {o[0], o.size() > 1 ? OptTensor(o[1]) : OptTensor()};

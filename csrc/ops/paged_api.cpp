@@ -11,6 +11,7 @@
 #include <cstring>
 #include <tuple>
 
+#include "forward_ad.hpp"
 #include "../kernels/paged_attn.cuh"
 #include "../kernels/paged_cache.cuh"
 #include "../kernels/tma_host.hpp"
@@ -104,6 +105,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new, OptTensor slots, bool causal,
     double scale, OptTensor out_in, bool want_lse, torch::Tensor status, int64_t wait_limit_ns) {
+  refuse_tangents("paged_attention", {q, k, v});
   check_rows16(q, 3, "q");
   check_rows16(k, 4, "k_pages");
   check_rows16(v, 4, "v_pages");
@@ -336,6 +338,7 @@ torch::Tensor cache_refused(torch::Tensor k, torch::Tensor table, torch::Tensor 
 void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                  torch::Tensor refs, torch::Tensor grown, torch::Tensor status, int64_t layer,
                  torch::Tensor new_k, torch::Tensor new_v, torch::Tensor slots, torch::Tensor cu) {
+  refuse_tangents("PagedKVCache.write", {new_k, new_v});
   MGFA_CHECK(layer >= 0 && layer < k.size(0), "layer ", layer, " is not one of the cache's ", k.size(0));
   const int n = check_slots(slots, k, "slots");
   check_ints(cu, k, 1, "cu_seqlens");

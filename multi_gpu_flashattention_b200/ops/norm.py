@@ -20,7 +20,8 @@ from .._ext import C
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6):
-    """y, or (y, h) with a residual; differentiable (once) in x, weight and residual."""
+    """y, or (y, h) with a residual; differentiable (once, in reverse mode) in x, weight and
+    residual."""
     y, h = C().rms_norm(x, weight, residual, eps)
     return y if h is None else (y, h)
 

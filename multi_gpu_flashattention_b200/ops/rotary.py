@@ -61,7 +61,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                  inv_freq: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0):
-    """q and k (k may be None) with rotary positions; differentiable (once) in q and k.
+    """q and k (k may be None) with rotary positions; differentiable (once, in reverse
+    mode) in q and k.
 
     q, k: [tokens, heads, head_dim] or [batch, tokens, heads, head_dim], bfloat16, float16
     or float32, head_dim up to 256, of one dtype; they may be strided, the results are

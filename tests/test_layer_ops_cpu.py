@@ -101,3 +101,28 @@ def test_norm_reads_no_further_than_its_rows(dtype):
                     end = r * apart + dim
                     assert end + -end % v <= flat.numel(), (dim, rows, apart, r)
     assert {v - 1, v + 1, 2 * v - 1, 3 * v + 2} <= shifted  # the wider ones keep their vectors
+
+
+def test_forward_mode_derivatives_are_refused():
+    """They would be lost without a word."""
+    import torch.autograd.forward_ad as fwd
+    from multi_gpu_flashattention_b200 import apply_rotary, paged_attention, rms_norm, rms_norm_fp8
+    x, w, f = torch.randn(4, 64), torch.ones(64), torch.ones(32, dtype=torch.float64)
+    q, pos, i32 = torch.randn(4, 2, 64), torch.arange(4), dict(dtype=torch.int32)
+    k = torch.zeros(4, 16, 1, 64, dtype=torch.bfloat16)
+    ints = torch.zeros(1, 4, **i32), torch.ones(1, **i32), torch.arange(2, **i32), 1
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        calls = [lambda: rms_norm(dual(x), w), lambda: rms_norm(x, dual(w)),
+                 lambda: rms_norm(x, w, residual=dual(x)), lambda: rms_norm_fp8(dual(x), w),
+                 lambda: apply_rotary(dual(q), None, pos, f), lambda: apply_rotary(q, dual(q), pos, f),
+                 lambda: apply_rotary(q, None, pos, dual(f)),
+                 lambda: paged_attention(dual(k[0, :1]), k, k, *ints),
+                 lambda: paged_attention(k[0, :1], k, dual(k), *ints)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+            with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+                call()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: rms_norm(t, w), (x,), (x,))

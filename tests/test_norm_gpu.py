@@ -294,3 +294,15 @@ def test_refusals():
                 lambda: rms_norm_fp8(x.requires_grad_(), w)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_tangents_of_a_gradient_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from multi_gpu_flashattention_b200 import rms_norm
+    x, w, _, dy, _ = _make(4, 64, torch.float32, False)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            rms_norm(fwd.make_dual(x, dy), w)
+        y = rms_norm(x.requires_grad_(), w)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.autograd.grad([y], [x], [fwd.make_dual(dy, dy)])
