@@ -383,6 +383,8 @@ void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const Pag
 // More rows: tcgen05 tiles.
 void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                         const PagedParams& p, cudaStream_t stream);
+// The most local memory a thread of its forms was compiled with, which has to be none.
+int64_t paged_chunk_local_bytes();
 // Joins the parts; launched behind either.
 void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
 

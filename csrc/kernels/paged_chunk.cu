@@ -28,6 +28,7 @@
 #include "sm100_ptx.cuh"
 #include "softmax_exp.cuh"
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 
@@ -58,6 +59,7 @@ struct __align__(1024) ChunkSmem {
   uint64_t drain;
   uint32_t tmem_base;
   uint32_t abort_flag;
+  uint32_t never;  // 0: the flag of the last waits, which nothing ends early
   uint32_t sums[kWarps];
   // The runs, which the producer finds a few ahead: run number i in slot i & 3.
   struct Run {
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t warp = warp_id(), lane = lane_id();
   AbortState ab{&s.abort_flag, p.status, p.wait_limit_ns};
   if (threadIdx.x == 0) {
-    s.abort_flag = 0;
+    s.abort_flag = s.never = 0;
     mbar_init(&s.q_full, 1);
     mbar_init(&s.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
@@ -210,8 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s.v_empty[st], ph, ab, 72)))) {
           // K of this tile is on its way all the same
-          volatile uint32_t never = 0;
-          AbortState drain{&never, nullptr, p.wait_limit_ns};
+          AbortState drain{&s.never, nullptr, p.wait_limit_ns};
           mbar_wait(&s.k_full[st], (it >> 1) & 1, drain, 0);
           break;
         }
@@ -227,8 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok) publish(-1);
     if (lane == 0) at.leave(p, prefix);
     // Never leave with a copy outstanding.
-    volatile uint32_t never = 0;
-    AbortState drain{&never, nullptr, p.wait_limit_ns};
+    AbortState drain{&s.never, nullptr, p.wait_limit_ns};
     if (seg > 0) mbar_wait(&s.q_full, (seg - 1) & 1, drain, 0);
     for (uint32_t i = it > 2 ? it - 2 : 0; i < it; ++i) {
       mbar_wait(&s.k_full[i & 1], (i >> 1) & 1, drain, 0);
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       return ok;
     };
-    uint32_t it = 0, seg = 0, pc[2] = {0, 0};  // phases used so far
+    uint32_t it = 0, seg = 0, pc0 = 0, pc1 = 0;  // phases used so far
     bool ok = true;
     // K tile number i has arrived; V tile number i has, and is cut behind the sequence's end
     auto wait_k = [&](uint32_t i) { return wait(&s.k_full[i & 1], (i >> 1) & 1, 81); };
@@ -290,7 +290,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
     // A unit's first P_t also says that the warps have read the last unit's O_t.
-    auto wait_p = [&](int t) { return wait(&s.p_full[t], pc[t]++ & 1, 85 + t); };
+    auto wait_p = [&](int t) {
+      const uint32_t used = t ? pc1++ : pc0++;
+      return wait(&s.p_full[t], used & 1, 85 + t);
+    };
     for (;; ++run) {
       if (!(ok = wait(&s.run_full[run & 3], (run >> 2) & 1, 88))) break;
       const auto& u = s.runs[run & 3];
@@ -339,8 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Every issued MMA has finished before TMEM is released.
     if (lane == 0) {
       mma_commit(&s.drain);
-      volatile uint32_t never = 0;
-      AbortState drain{&never, nullptr, p.wait_limit_ns};
+      AbortState drain{&s.never, nullptr, p.wait_limit_ns};
       mbar_wait(&s.drain, 0, drain, 0);
     }
   } else {
@@ -380,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           // Keys [64, 128) are read twice, for the maximum and for the exponentials: a row's
           // 128 scores at once, next to the probabilities, do not fit a thread's registers.
           // Nothing here may spill: a register that tcgen05.ld is still writing was seen to
-          // be spilled before its wait, which left other kernels' values in it.
+          // be spilled before its wait, which left other kernels' values in it. (The launch
+          // refuses a kernel that has any local memory.)
           // (The probabilities of keys [64, 128) go where scores of [32, 64) lie, so they are
           // stored last.)
           const int n_vis = (j + 1) * kTile > full ? lim - j * kTile : kTile;
@@ -521,10 +524,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int kD, bool kF16>
+int64_t chunk_local_bytes() {
+  cudaFuncAttributes a;
+  const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<kD, kF16>);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
+  return int64_t(a.localSizeBytes);
+}
+
+template <int kD, bool kF16>
 void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                   const PagedParams& p, cudaStream_t s) {
   const int smem = int(sizeof(ChunkSmem<kD>)) + 1024 + 4 * (p.seqs + 1);
   auto fn = paged_chunk_kernel<kD, kF16>;
+  static const int64_t local = chunk_local_bytes<kD, kF16>();
+  if (local != 0)
+    throw std::runtime_error("paged attention: the chunk kernel was compiled with " + std::to_string(local) +
+                             " bytes of local memory; its scores must not be spilled");
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = paged_allow_smem(fn, allowed);
   if (e == cudaSuccess) {
@@ -535,6 +550,11 @@ void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
 }
 
 }  // namespace
+
+int64_t paged_chunk_local_bytes() {
+  return std::max(std::max(chunk_local_bytes<64, false>(), chunk_local_bytes<64, true>()),
+                  std::max(chunk_local_bytes<128, false>(), chunk_local_bytes<128, true>()));
+}
 
 void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                         const PagedParams& p, cudaStream_t s) {

@@ -51,6 +51,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new,
     c10::optional<torch::Tensor> slots, bool causal, double scale,
     c10::optional<torch::Tensor> out, bool want_lse, torch::Tensor status, int64_t wait_limit_ns);
+int64_t paged_chunk_local_bytes();
 torch::Tensor host_status_word();
 void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                  torch::Tensor refs, torch::Tensor grown);
@@ -115,6 +116,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_layout_of", &mgfa::norm_layout_of);
   m.def("apply_rotary", &mgfa::apply_rotary);
   m.def("paged_attention", &mgfa::paged_attention);
+  m.def("paged_chunk_local_bytes", &mgfa::paged_chunk_local_bytes);
   m.def("host_status_word", &mgfa::host_status_word);
   m.def("cache_check", &mgfa::cache_check);
   m.def("cache_reserve", &mgfa::cache_reserve);

@@ -170,6 +170,12 @@ def test_again_between_other_kernels(new, kv):
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
 
 
+def test_chunk_kernel_spills_nothing():
+    """Its launch refuses a build in which a score could be spilled while it is being loaded."""
+    from multi_gpu_flashattention_b200._ext import C
+    assert C().paged_chunk_local_bytes() == 0
+
+
 # ------------------------------------------------------------------ rows and masks
 @pytest.mark.parametrize("new,heads", [([4, 3], 4), ([60, 50], 4)])
 def test_tokens_without_a_visible_key(new, heads):
