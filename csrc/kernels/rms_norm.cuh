@@ -13,7 +13,7 @@ enum class NormType : int { kBf16 = 0, kF16 = 1, kF32 = 2 };
 struct NormFwdParams {
   const void* x = nullptr;
   const void* residual = nullptr;  // null: h = x
-  const void* weight = nullptr;    // [dim], x's type or (weight_f32) fp32
+  const void* weight = nullptr;    // [dim], x's type or (weight_f32, where that is another) fp32
   void* y = nullptr;               // [rows, dim] packed, x's type; or 8-bit when scale is set
   void* h = nullptr;               // [rows, dim] packed, written when residual is set
   float* rstd = nullptr;           // [rows], written when set

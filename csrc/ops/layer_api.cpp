@@ -127,7 +127,7 @@ NormFwd norm_fwd(const torch::Tensor& x, const torch::Tensor& weight_in, const O
   NormFwdParams p;
   p.x = xr.data_ptr();
   p.weight = weight.data_ptr();
-  p.weight_f32 = weight.scalar_type() == at::kFloat;
+  p.weight_f32 = weight.scalar_type() != x.scalar_type();
   p.y = out.y.data_ptr();
   p.rows = xr.size(0);
   p.x_stride = xr.stride(0);
@@ -196,7 +196,7 @@ std::tuple<torch::Tensor, torch::Tensor> norm_bwd(const torch::Tensor& dy, const
     p.dh_stride = dhr.stride(0);
   }
   p.weight = weight.data_ptr();
-  p.weight_f32 = weight.scalar_type() == at::kFloat;
+  p.weight_f32 = weight.scalar_type() != h.scalar_type();
   p.rstd = rstd.data_ptr<float>();
   p.dx = dx.data_ptr();
   p.rows = hr.size(0);

@@ -116,6 +116,16 @@ def test_strided_and_misaligned_inputs(dim):
            four(dh).transpose(0, 2))
 
 
+@pytest.mark.parametrize("dim", [4, 128, 1028, 4096, 8192])
+def test_float32_rows_and_weights(dim):
+    """Weights that are read in vectors, and those that are off their boundary."""
+    x, w, r, dy, dh = _make(9, dim + 8, torch.float32, True, seed=dim)
+    cut = lambda t, o: t[..., o:o + dim]
+    for o in (0, 4, 1):
+        _check(cut(x, 0), cut(w, o), cut(r, 4), cut(dy, 0), cut(dh, 8))
+    _check(cut(x, 3), cut(w, 0), cut(r, 0), cut(dy, 0), cut(dh, 0))
+
+
 @pytest.mark.parametrize("width", [9, 16, 33])
 def test_rows_that_overlap(width):
     """A sliding window over one tensor: rows one element apart."""
