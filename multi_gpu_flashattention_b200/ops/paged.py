@@ -143,6 +143,8 @@ class PagedKVCache:
                causal: bool = True, softmax_scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """paged_attention of the batch's queries [tokens, heads, D] over a layer's cache."""
+        if not 0 <= layer < len(self._layers):
+            raise IndexError(f"layer {layer} is not one of the cache's {len(self._layers)}")
         k, v = self._layers[layer]
         return paged_attention(q, k, v, self.page_table, self.lens, self._ints(cu_seqlens),
                                max_seqlen_q, slots=self._ints(slots), causal=causal,

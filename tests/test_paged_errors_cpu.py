@@ -59,3 +59,12 @@ def test_an_earlier_error_skips_no_call(cache, name, args):
     assert cache.calls == [name]
     getattr(cache, name)(*args)
     assert cache.calls == [name, name]
+
+
+@pytest.mark.parametrize("layer", [-1, 3, 99])
+def test_attend_takes_the_cache_s_layers_only(cache, layer):
+    """As write() does: -1 is not the last layer."""
+    x = torch.zeros(1, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(IndexError, match="not one of the cache's 3"):
+        cache.attend(layer, x, [0], [0, 1], 1)
+    assert cache.calls == []
