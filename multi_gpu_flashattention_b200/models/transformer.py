@@ -174,6 +174,17 @@ class RingTransformerLM(nn.Module):
         return PagedKVCache.allocate(len(self.blocks), pages, page_size, self.blocks[0].hkv,
                                      self.blocks[0].d, slots, max_tokens, dtype=w.dtype, device=w.device)
 
+    def _check_served(self, ids: torch.Tensor, cache: PagedKVCache, max_seqlen: int) -> None:
+        """What a layer would refuse, before the cache grows."""
+        w, blk, k = self.embed.weight, self.blocks[0], cache.k
+        if ids.dim() != 1 or max_seqlen < 0:
+            raise ValueError(f"ids must be [tokens] and max_seqlen not negative, got {list(ids.shape)} and {max_seqlen}")
+        if k.shape[0] < len(self.blocks) or tuple(k.shape[3:]) != (blk.hkv, blk.d) or \
+                k.dtype != w.dtype or k.device != w.device:
+            raise ValueError("the cache does not fit the model: see make_cache()")
+        if blk.h % blk.hkv or blk.h // blk.hkv > 128:
+            raise ValueError("heads must be a multiple of kv heads, up to 128 times")
+
     @torch.no_grad()
     def serve(self, ids: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
               cu_seqlens: torch.Tensor, max_seqlen: int) -> torch.Tensor:
@@ -185,6 +196,7 @@ class RingTransformerLM(nn.Module):
         their sequence (slots, cu_seqlens: int32 CUDA tensors). Rows outside every sequence
         hold nothing; those of a sequence that got no room in the cache, which stays as it
         was, are NaN. bfloat16 or float16 parameters, head_dim 64 or 128."""
+        self._check_served(ids, cache, max_seqlen)
         pos = cache.reserve(slots, cu_seqlens, ids.numel())
         inv_freq = _frequencies(self.blocks[0].d, ids.device)
         x = self.embed(ids)

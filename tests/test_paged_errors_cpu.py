@@ -68,3 +68,32 @@ def test_attend_takes_the_cache_s_layers_only(cache, layer):
     with pytest.raises(IndexError, match="not one of the cache's 3"):
         cache.attend(layer, x, [0], [0, 1], 1)
     assert cache.calls == []
+
+
+def _lm(**kw):
+    from multi_gpu_flashattention_b200 import RingTransformerLM
+    a = dict(vocab=20, d_model=32, n_layers=2, n_heads=2, n_kv_heads=1, head_dim=64, mlp_mult=1)
+    return RingTransformerLM(**dict(a, **kw)).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("why", ["layers", "heads", "head_dim", "dtype", "ids", "max", "group"])
+def test_serve_refuses_before_the_cache_grows(cache, why):
+    """What would end the step in one of its layers, with the cache grown for it."""
+    model, ids, most = _lm(), torch.zeros(2, dtype=torch.int64), 1
+    if why == "layers":
+        model = _lm(n_layers=4)  # the cache has 3
+    elif why == "heads":
+        model = _lm(n_kv_heads=2)
+    elif why == "head_dim":
+        model = _lm(head_dim=128)
+    elif why == "dtype":
+        model = _lm().float()
+    elif why == "ids":
+        ids = ids[None]
+    elif why == "max":
+        most = -1
+    else:
+        model = _lm(n_heads=129, d_model=16)
+    with pytest.raises(ValueError):
+        model.serve(ids, cache, torch.zeros(2, dtype=torch.int32), torch.arange(3, dtype=torch.int32), most)
+    assert cache.calls == []
