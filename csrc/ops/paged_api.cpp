@@ -137,7 +137,8 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   }
   MGFA_CHECK(page_table.size(1) * page < (int64_t(1) << 30), "page_table is too wide");
   MGFA_CHECK(max_new >= 0, "max_seqlen_q must not be negative");
-  MGFA_CHECK(scale > 0.0 && std::isfinite(scale), "softmax_scale must be positive");
+  const float scale_log2 = float(scale * 1.4426950408889634);  // the kernels' own
+  MGFA_CHECK(scale_log2 > 0.f && std::isfinite(scale_log2), "softmax_scale must be positive (in float32)");
   c10::cuda::CUDAGuard guard(q.device());
   torch::Tensor out, lse;
   if (out_in.has_value()) {
@@ -177,7 +178,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   p.head_dim = int(D);
   p.causal = causal ? 1 : 0;
   p.fp16 = q.scalar_type() == at::kHalf;
-  p.scale_log2 = float(scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.wait_limit_ns = uint64_t(wait_limit_ns);
   const int sms = device_sm_count(q.get_device());
   // Up to 32 rows a key head pad to 16 or 32 on mma.sync; more fill 128-row tiles.

@@ -389,6 +389,16 @@ def test_refusals():
         call(q=p.q.clone().requires_grad_())
 
 
+def test_scales_outside_float32_are_refused():
+    """As a float they are 0 or infinite, and 0 times a hidden score is NaN."""
+    p = Problem([1], [30], 4, 2, 64, 16)
+    for scale in (1e-50, 1e39, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="softmax_scale must be positive"):
+            p.run(softmax_scale=scale)
+    out, lse = p.run(softmax_scale=1e-30)
+    p.check(out, lse, scale=1e-30)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_wrong_contents_are_reported(new):
     """Pages that are not in the pool, lengths beyond the table, slots out of range, rows
