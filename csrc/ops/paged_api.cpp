@@ -47,12 +47,13 @@ int* host_words() {
 }
 std::atomic<int> host_words_used{0};
 
-uint32_t* status_ptr(const torch::Tensor& t) {
+uint32_t* status_ptr(const torch::Tensor& t, const torch::Tensor& like) {
   MGFA_CHECK(t.scalar_type() == at::kInt && t.numel() >= 1, "status must be an int32 tensor");
   int* p = t.data_ptr<int>();
   // asking the driver about a pointer costs as much as a launch
   if (!t.is_cuda() && !(host_words_used.load() && p >= host_words() && p < host_words() + kHostWords))
     MGFA_CHECK(t.is_pinned(), "status must be in CUDA or pinned host memory");
+  MGFA_CHECK(!t.is_cuda() || t.device() == like.device(), "status must be on q's device or in pinned host memory");
   return reinterpret_cast<uint32_t*>(p);
 }
 
@@ -151,7 +152,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   }
   if (want_lse) lse = torch::empty({Hq, T}, q.options().dtype(at::kFloat));
   PagedParams p;
-  p.status = status_ptr(status);
+  p.status = status_ptr(status, q);
   p.max_new = int(std::min(max_new, T));
   if (seqs == 0 || p.max_new == 0) return {out, want_lse ? OptTensor(lse) : OptTensor()};
   p.q = q.data_ptr();
@@ -248,7 +249,7 @@ CacheState cache_state(const torch::Tensor& k, const torch::Tensor& table, const
   c.width = int(table.size(1));
   c.pages = int(k.size(1));
   c.page = int(k.size(2));
-  c.status = status_ptr(status);
+  c.status = status_ptr(status, k);
   return c;
 }
 

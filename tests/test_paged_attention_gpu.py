@@ -399,6 +399,29 @@ def test_scales_outside_float32_are_refused():
     p.check(out, lse, scale=1e-30)
 
 
+@pytest.mark.parametrize("pinned", [False, True])
+def test_a_status_word_of_the_caller(pinned):
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    p = Problem([1], [30], 4, 2, 64, 16)
+    word = torch.zeros(1, dtype=torch.int32)
+    word = word.pin_memory() if pinned else word.cuda()
+    out, lse = p.run(status=word)
+    p.check(out, lse)
+    assert int(word) == 0
+    p.table[0, 0] = -1
+    p.run(status=word)
+    torch.cuda.synchronize()
+    assert int(word) & 0xff == 4
+    check_errors()
+
+
+@pytest.mark.multigpu
+def test_a_status_word_of_another_device_is_refused():
+    p = Problem([1], [30], 4, 2, 64, 16)
+    with pytest.raises(RuntimeError, match="status must be on q's device"):
+        p.run(status=torch.zeros(1, dtype=torch.int32, device="cuda:1"))
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_wrong_contents_are_reported(new):
     """Pages that are not in the pool, lengths beyond the table, slots out of range, rows
