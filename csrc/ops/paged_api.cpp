@@ -203,13 +203,17 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
     p.grid = sms;
   }
   const int64_t tiles = std::max<int64_t>(1, (int64_t(p.width) * page + p.tile - 1) / p.tile);
+  p.max_units = (p.max_new + p.block_tokens - 1) / p.block_tokens;
+  const int64_t allowed = seqs * Hk * p.max_units;  // units, by max_new
   // Tables of at most 8 tiles a sequence: the units are dealt out whole, which takes neither
   // the lengths' sum nor a join. One token each over 100 to 320 keys: 9.6 us, in shares
-  // 15.4 us; 64 chunks of 128 tokens over 128 keys: 61 us, in shares 76 us.
-  p.whole = tiles <= 8;
-  p.max_units = (p.max_new + p.block_tokens - 1) / p.block_tokens;
-  MGFA_CHECK(seqs * Hk * p.max_units < (int64_t(1) << 30), "too many sequences, heads and tokens");
-  p.units = int(seqs * Hk * p.max_units);
+  // 15.4 us; 64 chunks of 128 tokens over 128 keys: 61 us, in shares 76 us. A CTA looks at
+  // every unit that max_new allows, though (0.3 us each), so not where these are many times
+  // those that there can be: one chunk of 1000 tokens and 255 of one, 15 times as many, 206 us, in
+  // shares 220 us; 512 chunks of 100 announced as up to 3200, 19 times, 671 us and 325 us,
+  // announced as up to the batch's 51200, 7199 us and 325 us.
+  p.whole = tiles <= 8 && allowed <= 16 * units && allowed < (int64_t(1) << 30);
+  p.units = p.whole ? int(allowed) : 0;
   p.grid = int(std::min<int64_t>(p.grid, p.whole ? p.units : (units * tiles + p.min_share - 1) / p.min_share));
   torch::Tensor work;
   const bool parts = p.grid > 1 && !p.whole;

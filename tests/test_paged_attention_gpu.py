@@ -176,6 +176,33 @@ def test_chunk_kernel_spills_nothing():
     assert C().paged_chunk_local_bytes() == 0
 
 
+@pytest.mark.parametrize("new,kv", [([100] * 64, [100] * 64), ([40, 0, 33, 1], [300, 5, 33, 900])])
+def test_max_seqlen_far_above_the_longest(new, kv):
+    """Short tables, whose units are dealt out by max_seqlen_q where it is close."""
+    p = Problem(new, kv, 4, 2, 64, 16)
+    for most in (max(new), 8 * max(new), sum(new), 1 << 40):
+        out, lse = p.run(max_new=most)
+        p.check(out, lse)
+
+
+def test_max_seqlen_that_only_bounds_the_batch_costs_little():
+    """512 chunks of 100 tokens over 100 keys, announced as up to 51200 tokens each."""
+    p = Problem([100] * 512, [100] * 512, 32, 8, 128, 64)
+    times = {}
+    for most in (100, sum(p.new)):
+        p.run(max_new=most)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        best = float("inf")
+        for _ in range(5):
+            a.record()
+            p.run(max_new=most)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        times[most] = best
+    assert times[51200] < 3 * times[100], times  # it was 23 times as long
+
+
 # ------------------------------------------------------------------ rows and masks
 @pytest.mark.parametrize("new,heads", [([4, 3], 4), ([60, 50], 4)])
 def test_tokens_without_a_visible_key(new, heads):
