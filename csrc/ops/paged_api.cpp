@@ -183,7 +183,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   p.wait_limit_ns = uint64_t(wait_limit_ns);
   const int sms = device_sm_count(q.get_device());
   // Up to 32 rows a key head pad to 16 or 32 on mma.sync; more fill 128-row tiles.
-  const bool few = p.max_new * p.group <= 32;
+  const bool few = int64_t(p.max_new) * p.group <= 32;
   int64_t units;  // at most
   if (few) {
     p.block_tokens = p.max_new;

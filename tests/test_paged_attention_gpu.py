@@ -492,6 +492,18 @@ def test_more_tokens_than_announced_are_reported():
         check_errors()
 
 
+def test_rows_beyond_32_bits():
+    """Tokens times query heads a key head pass 2^31 (overlapping rows, none of them used)."""
+    tokens, heads = 1 << 25, 64
+    q = torch.zeros(tokens * 8 + heads * 64, device="cuda", dtype=torch.bfloat16)
+    q = q.as_strided((tokens, heads, 64), (8, 64, 1))
+    p = Problem([1], [30], 64, 1, 64, 16)
+    p.q, p.max_new = q, tokens
+    p.cu.zero_()
+    p.run(out=q, return_lse=False)
+    assert not q[::1 << 20].any()
+
+
 def test_empty_batches():
     p = Problem([0, 0], [5, 6], 4, 2, 64, 16, tail=3)
     out = torch.full_like(p.q, 3.0)
