@@ -64,6 +64,8 @@ class RingAttentionBlock(nn.Module):
     embeddings run on the kernels, for CUDA tensors; each rounds its result once, where
     the plain ops round between."""
 
+    fused_ops = False  # of modules that were saved whole without one
+
     def __init__(self, d_model: int, n_heads: int, n_kv_heads: Optional[int] = None,
                  head_dim: int = 128, mlp_mult: int = 4, causal: bool = True,
                  fused_ops: bool = False):
@@ -139,6 +141,8 @@ class RingTransformerLM(nn.Module):
     replicated, so after `loss(...).backward()` the gradients are summed over
     the group (all-reduce, as in data parallelism) to give the unsharded
     model's gradients."""
+
+    fused_ops = False  # of modules that were saved whole without one
 
     def __init__(self, vocab: int, d_model: int, n_layers: int, n_heads: int,
                  n_kv_heads: Optional[int] = None, head_dim: int = 128, mlp_mult: int = 4,

@@ -84,3 +84,17 @@ def test_lm_loss_and_grads_match_unsharded_zigzag():
 
 def test_lm_loss_and_grads_match_unsharded_contiguous_3_ranks():
     run_ranks(_lm_case, 3, "contiguous")
+
+
+def test_a_model_saved_whole_before_the_flag_still_runs():
+    """torch.save(model) keeps the instance's attributes only: fused_ops is off without one."""
+    from multi_gpu_flashattention_b200.models import RingTransformerLM
+    from multi_gpu_flashattention_b200.parallel.layouts import RingLayout
+    torch.manual_seed(0)
+    model = RingTransformerLM(vocab=50, d_model=32, n_layers=1, n_heads=2, head_dim=16, mlp_mult=2)
+    lay = RingLayout("contiguous", 24, 1, mask="causal")
+    ids = torch.arange(24)[None]
+    want = model(ids, lay, backend="torch")
+    for m in [model, *model.blocks]:
+        del m.__dict__["fused_ops"]
+    assert torch.equal(model(ids, lay, backend="torch"), want)
