@@ -250,3 +250,41 @@ def test_logits_of_a_sequence_without_room_are_nan():
     out = model.serve(ids[:5], cache, torch.tensor([2], **i32), torch.tensor([0, 5], **i32), 5)
     assert torch.isfinite(out).all()
     check_errors()
+
+
+def test_the_plain_model_computes_the_plain_formulas():
+    """Without fused_ops, to the bit: norms and rotary positions in torch, attention as
+    ring_attention gives it; with it, other roundings of the same values."""
+    from multi_gpu_flashattention_b200 import RingLayout, ring_attention
+    model, ids = _model(torch.bfloat16), _ids(200, 9)
+    lay = RingLayout("contiguous", 200, 1, mask="causal")
+    norm = lambda x, w: (x.float() * torch.rsqrt(x.float().pow(2).mean(-1, keepdim=True) + 1e-6)).to(x.dtype) * w
+    inv = 10000.0 ** (-torch.arange(0, D // 2, device="cuda", dtype=torch.float32) * 2 / D)
+    ang = torch.arange(200, device="cuda", dtype=torch.float32)[:, None] * inv
+
+    def rot(t):
+        a, b = t[..., :D // 2].float(), t[..., D // 2:].float()
+        c, s = ang.cos()[None, :, None], ang.sin()[None, :, None]
+        return torch.cat([a * c - b * s, a * s + b * c], -1).to(t.dtype)
+
+    with torch.no_grad():
+        x = model.embed(ids[None])
+        for blk in model.blocks:
+            h = norm(x, blk.norm1.weight)
+            q, k, v = (w(h).view(1, 200, -1, D) for w in (blk.wq, blk.wk, blk.wv))
+            a = ring_attention(rot(q), rot(k), v.contiguous(), causal=True, layout=lay)
+            x = x + blk.wo(a.reshape(1, 200, -1))
+            h = norm(x, blk.norm2.weight)
+            x = x + blk.w2(F.silu(blk.w1(h)) * blk.w3(h))
+        want = model.head(norm(x, model.norm.weight))
+        plain = model(ids[None], lay)
+        assert torch.equal(plain, want)
+        for m in [model, *model.blocks]:
+            m.fused_ops = True
+        fused = model(ids[None], lay)
+        assert not torch.equal(fused, plain)
+        ref = _exact(model, ids)[0]
+        assert _off(fused[0], ref) <= 1.5 * _off(plain[0], ref)
+        for m in [model, *model.blocks]:
+            m.fused_ops = False
+        assert torch.equal(model(ids[None], lay), want)
