@@ -288,3 +288,50 @@ def test_the_plain_model_computes_the_plain_formulas():
         for m in [model, *model.blocks]:
             m.fused_ops = False
         assert torch.equal(model(ids[None], lay), want)
+
+
+def test_serving_steps_in_a_graph():
+    """A decode step captured once and replayed, a sequence running out of pages on the way:
+    the same logits and the same cache as step by step, NaN from the refused step on."""
+    from multi_gpu_flashattention_b200 import KernelStatusError
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    model = _model(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    slots, cu = torch.tensor([2, 0], **i32), torch.tensor([0, 1, 2], **i32)
+    first, cu1, most1 = _batch([_ids(14, 1), _ids(3, 2)])
+    runs = []
+    for graphed in (False, True):
+        cache = model.make_cache(pages=3, page_size=16, slots=3, max_tokens=64)  # one page to spare
+        model.serve(first, cache, slots, cu1, most1)
+        ids, got = _ids(2, 3), []
+        if graphed:
+            saved = [t.clone() for t in (cache.page_table, cache.lens, cache.refs, cache.grown)]
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                model.serve(ids, cache, slots, cu, 1)
+                for t, u in zip((cache.page_table, cache.lens, cache.refs, cache.grown), saved):
+                    t.copy_(u)
+            torch.cuda.current_stream().wait_stream(s)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = model.serve(ids, cache, slots, cu, 1)
+        for i in range(20):  # sequence 2 grows into the last page, sequence 0 stays at 16 tokens
+            ids.copy_(_ids(2, 10 + i))
+            if graphed:
+                graph.replay()
+            else:
+                try:
+                    out = model.serve(ids, cache, slots, cu, 1)
+                except KernelStatusError:
+                    out = model.serve(ids, cache, slots, cu, 1)
+            got.append(out.clone())
+        with pytest.raises(KernelStatusError, match="too few free pages"):
+            check_errors()
+        assert cache.lens.tolist() == [16, 0, 32]
+        runs.append(torch.stack(got))
+    bad = runs[0].isnan().all(-1)
+    assert torch.equal(bad, runs[1].isnan().all(-1))
+    assert bad[:, 0].tolist() == [False] * 18 + [True] * 2 and bad[:, 1].tolist() == [False] * 13 + [True] * 7
+    assert torch.equal(runs[0].nan_to_num(), runs[1].nan_to_num())
+    check_errors()
