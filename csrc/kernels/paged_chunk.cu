@@ -19,8 +19,11 @@
 // 128 keys takes 1.25 us, the two products and their hand-overs 1.1 us, so a key tile of
 // both halves takes 2.4 us where the tensor cores alone would need 1.5 us. 2048 tokens of
 // 32 heads over 32768 keys (8 key heads of 128, causal) take 1.06 ms, 1.01 PFLOP/s, and
-// 1.25 ms (0.85) under the power cap of a long run; units of few rows are bound by memory:
-// 16 tokens of 8 sequences over 8192 keys take 90 us for 268 MB.
+// 1.25 ms (0.85) under the power cap of a long run. Units of few rows are bound by the same
+// chain, with two tiles of K and V on their way, and not by memory: 16 tokens of 8 sequences
+// over 8192 keys take 87 us for 268 MB, 3.1 TB/s, where the decode kernel reaches 6.3. So do
+// single tokens that share a call with a chunk: 512 tokens and 60 sequences of one over 4096
+// keys take 329 us together, 77 and 179 us (on the decode kernel) apart.
 // O is rescaled only when the running maximum grows by more than 2^8 (fp16: 2^4, which
 // leaves 2^11 for PagedBase's lift): with the stale one P stays below 2^8 (2^15). Sums are
 // fp32.
@@ -379,9 +382,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = j0; j < t1; j += step) {
           if (!(ok = wait(&s.s_full[t], sc & 1, 90 + t))) break;
           ++sc;
-          // Keys [64, 128) are read twice, for the maximum and for the exponentials: a row's
-          // 128 scores at once, next to the probabilities, do not fit a thread's registers.
-          // Nothing here may spill: a register that tcgen05.ld is still writing was seen to
+          // Keys [64, 128) are read twice, for the maximum and for the exponentials, and 64
+          // scores are held at a time, which leaves registers to spare. (flash_fwd_sm100.cu
+          // holds a row's 128, reads them once, and spills nothing in 168 registers.) Nothing
+          // here may spill: a register that tcgen05.ld is still writing was seen to
           // be spilled before its wait, which left other kernels' values in it. (The launch
           // refuses a kernel that has any local memory.)
           // (The probabilities of keys [64, 128) go where scores of [32, 64) lie, so they are

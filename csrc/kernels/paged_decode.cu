@@ -12,7 +12,9 @@
 // running maximum, sum and output of its own in registers, so the loop has no barrier
 // but the tile's; the four are added when a unit ends. 32 sequences of 8192 keys (8 key
 // heads of 128, pages of 16) take 171 us for 1.07 GB, 6.3 TB/s; one of 131072 keys 86 us,
-// and 9 us for joining 296 parts. For short sequences the time is latency: one token each
+// and 9 us for joining 296 parts; with 4 new tokens each (16 rows) the 32 sequences take
+// 1.03 times as long, with 8 (32 rows, whose second block of 16 spills 468 bytes at head_dim
+// 128) 1.3 times. For short sequences the time is latency: one token each
 // over 100 to 320 keys takes 9.6 us.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"

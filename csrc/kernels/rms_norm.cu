@@ -12,11 +12,16 @@
 // Bound by memory: every tensor is read or written once. At 16384 x 4096 bf16 with a
 // residual the forward takes 84 us (6.4 TB/s) and the backward 111 us (4.8 TB/s, with
 // 9 us for dw's parts); without the packed pairs and with the weights in registers they
-// took 120 and 210 us. A row stays in the registers of the T threads that own it (N
-// vectors each), so the statistics and the output need one pass. A vector is 16 bytes,
-// also where the width is no multiple of that (kShifted: 16384 x 4095 takes 152 + 245
-// us, by single elements 255 + 374), and one element for other strides; T grows with the
-// row, which leaves a thread 8 to 16 elements up to a width of 4096, and 32 beyond.
+// took 120 and 210 us. A row stays with the T threads that own it (N vectors each), so the
+// statistics and the output need one pass. A vector is 16 bytes, also where the width is no
+// multiple of that (kShifted: 16384 x 4095 takes 150 + 241 us, half the aligned rate; by
+// single elements 255 + 374), and one element for other strides. T grows with the row, which
+// leaves a thread 8 to 16 elements up to a width of 4096, and 32 beyond: there the backward's
+// three tensors do not fit 128 registers (392 bytes of spills in 16 bits, 608 in fp32), and
+// 8192 x 8192 takes 90 us forward and 123 us back in bf16, 160 and 222 us in fp32, against
+// 82 and 164 us of each at the copy's rate. The 8-bit output of 16384 x 4096 takes 111 us
+// with a scale a row and 129 us with one for each 128 columns (72 us for its bytes): the
+// division of every value by its scale comes on top.
 #include "rms_norm.cuh"
 
 #include <cuda_bf16.h>

@@ -30,7 +30,8 @@ enum : int {
 
 // Heads whose loads a thread has under way. At 32768 tokens of 32 + 8 heads of 128 in
 // bf16 (671 MB moved) 2, 3 and 4 take 121, 120 and 117 us (halves) and 174, 149 and
-// 121 us (neighbours); 8 spill.
+// 121 us (neighbours). At 4 CTAs an SM a thread has 64 registers: 4 heads spill 176 bytes in
+// the 16-bit halves and none in the neighbours, 8 more than they gain.
 constexpr int kBatch = 4;
 
 __host__ __device__ inline int units_of(int mode, int v, int head_dim, int rotary_dim) {

@@ -261,10 +261,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 
 // Load and wait in one asm statement: the destination registers are defined
-// only when the statement ends, after tcgen05.wait::ld, so the compiler can
-// neither use nor copy nor spill them while the load is still in flight (an
-// empty fence after a separate wait orders later uses, not a copy or spill
-// the compiler places between the load and the wait).
+// only when the statement ends, after tcgen05.wait::ld, so the front end
+// places no use or copy of them between the load and the wait (an empty fence
+// after a separate wait orders later uses only). It does not keep ptxas, which
+// sees two instructions, from spilling a destination register in between: a
+// version of paged_chunk.cu that spilled scores, in this very form, was seen to
+// return other kernels' values. A kernel that loads scores must not spill them.
 __device__ __forceinline__ void tmem_ld32_sync(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
