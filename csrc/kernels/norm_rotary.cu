@@ -1,0 +1,694 @@
+// Root-mean-square norm of each query and key head with the rotary positions in the same
+// pass, its gradients, and the same on the way into a paged cache:
+//
+//   n = x * rstd * w,  rstd = 1 / sqrt(mean(x^2) + eps) over the head,  y = R(t) n
+//
+// R(t) rotates the pairs of the first rotary_dim columns (rotary.cu). Back, with
+// g = R(-t) dy (the transpose):
+//
+//   dw = sum over tokens and heads of g * x * rstd
+//   dx = rstd * (g w - x * rstd^2 * mean(g w x))
+//
+// Bound by memory: forward reads x and writes y, back reads x and dy and writes dx. A
+// head's sums stay within the 1 to 32 lanes that hold it, so neither pass waits for more
+// than shuffles; rstd is computed again from x in the backward pass, which reads x anyway.
+// The weights are folded into the sines and cosines where that saves work, and each
+// thread keeps its columns' in registers.
+#include "norm_rotary.cuh"
+
+#include <algorithm>
+
+#include "pairs.cuh"
+#include "paged_attn.cuh"
+
+namespace mgfa {
+namespace {
+
+using namespace mgfa::dev;
+
+constexpr int kThreads = 256;
+constexpr int kFwdBatch = 4;  // heads whose loads a thread has under way
+constexpr int kBwdBatch = 2;  // (of x and dy)
+
+// How a head's columns are cut (V elements are 16 bytes):
+enum : int {
+  kHalves = 0,      // a lane has V columns of either half of the pairs, then V others
+  kNeighbours = 1,  // V columns with the pairs (2i, 2i + 1) inside
+  kAny = 2,         // V columns; each one's partner is fetched by itself (from L1)
+};
+
+inline int lanes_of(int mode, int v, int head_dim, int rotary_dim) {
+  return mode == kHalves ? rotary_dim / 2 / v + (head_dim - rotary_dim) / v : head_dim / v;
+}
+
+// A CTA's threads: `tile` tokens, of each slots[0] + slots[1] + slots[2] groups of
+// 2^lanes_log threads, for query, key and (append) value heads. Group i of n takes heads
+// i, i + n, ... of its kind, `batch` of them in each of `rounds`.
+struct Cut {
+  int tile, threads, lanes, lanes_log, rounds;
+  int slots[3];
+};
+
+Cut make_cut(int lanes, const int (&heads)[3], int batch, int64_t tokens, int sm_count) {
+  Cut c;
+  c.lanes = lanes;
+  c.lanes_log = 0;
+  while (1 << c.lanes_log < lanes) ++c.lanes_log;
+  const int most = kThreads >> c.lanes_log;
+  int want[3], sum = 0, total = 0;
+  for (int i = 0; i < 3; ++i) sum += want[i] = (heads[i] + batch - 1) / batch;
+  for (int i = 0; i < 3; ++i) {
+    c.slots[i] = sum <= most ? want[i] : want[i] ? std::max<int>(1, int64_t(most) * want[i] / sum) : 0;
+    total += c.slots[i];
+  }
+  for (; total > most; --total) --*std::max_element(c.slots, c.slots + 3);
+  c.rounds = 0;
+  for (int i = 0; i < 3; ++i)
+    if (c.slots[i]) c.rounds = std::max(c.rounds, (heads[i] + c.slots[i] * batch - 1) / (c.slots[i] * batch));
+  c.tile = int(std::max<int64_t>(1, std::min<int64_t>(most / std::max(1, total), tokens / (2 * sm_count))));
+  c.threads = ((c.tile * total << c.lanes_log) + 31) / 32 * 32;
+  return c;
+}
+
+// A thread's place: token `t` of the tile, lane u of the group for head `slot` and every
+// `step`-th behind it, of `kind`. live: it has columns of a head; its first is c0 and, in
+// kHalves, its second vector's c1 (rotates: c0 and c1 are pairs, otherwise c1 alone).
+template <int kMode, int V>
+struct Place {
+  int t, u, kind, slot, step, c0, c1;
+  bool live, rotates;
+  __device__ __forceinline__ Place(const RotaryParams& p, const Cut& cut) {
+    const int group = threadIdx.x >> cut.lanes_log, all = cut.slots[0] + cut.slots[1] + cut.slots[2];
+    u = threadIdx.x & ((1 << cut.lanes_log) - 1);
+    t = group / all;
+    slot = group - t * all;
+    kind = 0;
+    if (slot >= cut.slots[0]) {
+      slot -= cut.slots[0];
+      kind = 1;
+      if (slot >= cut.slots[1]) {
+        slot -= cut.slots[1];
+        kind = 2;
+      }
+    }
+    step = cut.slots[kind];
+    live = t < cut.tile && u < cut.lanes;
+    const int half = p.rotary_dim >> 1;
+    rotates = kMode != kHalves || u < half / V;
+    c0 = live ? u * V : 0;
+    c1 = kMode != kHalves ? c0 : rotates ? c0 + half : p.rotary_dim + (u - half / V) * V;
+  }
+};
+
+// The sum over the 2^log lanes of a group.
+__device__ __forceinline__ float group_sum(float v, int log) {
+  for (int o = 0; o < log; ++o) v += __shfl_xor_sync(0xffffffffu, v, 1 << o);
+  return v;
+}
+
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
+__device__ __forceinline__ uint64_t swapped(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return f2_pack(b, a);
+}
+
+// The partners of columns c and c + 1 (pairs (i, i + half)).
+__device__ __forceinline__ int partner(int c, int half) {
+  return c >= 2 * half ? c : c < half ? c + half : c - half;
+}
+
+__device__ __forceinline__ float weight_at(const NormRotaryParams& p, int kind, int c, bool half_type) {
+  if (p.weight_f32) return static_cast<const float*>(p.weight[kind])[c];
+  return half_type ? __half2float(static_cast<const __half*>(p.weight[kind])[c])
+                   : __bfloat162float(static_cast<const __nv_bfloat16*>(p.weight[kind])[c]);
+}
+
+// out = own * co + partner * si for columns c0.. of a token whose angles are `cs`.
+template <int kMode, int kPairs>
+__device__ __forceinline__ void column_angles(const RotaryParams& p, const float2* cs, int c0,
+                                              uint64_t (&co)[kPairs], uint64_t (&si)[kPairs]) {
+  const int half = p.rotary_dim >> 1;
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k) {
+    const int c = c0 + 2 * k;
+    co[k] = f2_pack(1.f, 1.f);
+    si[k] = 0;
+    if (c >= p.rotary_dim) continue;
+    if (kMode == kNeighbours) {
+      const float2 f = cs[c >> 1];
+      co[k] = f2_pack(f.x, f.x);
+      si[k] = f2_pack(-f.y, f.y);
+    } else {
+      const float2 f = cs[c < half ? c : c - half], g = cs[c + 1 < half ? c + 1 : c + 1 - half];
+      co[k] = f2_pack(f.x, g.x);
+      si[k] = f2_pack(c < half ? -f.y : f.y, c + 1 < half ? -g.y : g.y);
+    }
+  }
+}
+
+// Where a new token's keys and values go, in elements; < 0: nowhere. Called by a whole warp.
+struct AppendPlace {
+  int64_t k, v;
+};
+__device__ __forceinline__ AppendPlace append_place(const CacheAppendParams& p, int t, int lane) {
+  AppendPlace none{-1, -1};
+  if (t < __ldg(p.cu) || t >= __ldg(p.cu + p.seqs)) return none;
+  int slot, q0, n;
+  if (!row_grew(p.c, p.slots, p.cu, p.seqs, t, lane, slot, q0, n)) return none;
+  const int pos = p.c.lens[slot] - n + t - q0;
+  if (pos < 0 || pos >= int64_t(p.c.width) * p.c.page) return none;
+  const int page = p.c.table[int64_t(slot) * p.c.width + pos / p.c.page];
+  if (page < 0 || page >= p.c.pages) {
+    if (lane == 0) record_error(p.c.status, kErrBadArgument, 67, 0);
+    return none;
+  }
+  const int row = pos % p.c.page;
+  return {page * p.k_stride[0] + row * p.k_stride[1], page * p.v_stride[0] + row * p.v_stride[1]};
+}
+
+// kNorm: with the norm. P: NormRotaryParams, or CacheAppendParams to write into a cache.
+template <class E, int kMode, bool kNorm, class P>
+__global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, const Cut cut) {
+  constexpr bool kAppend = std::is_same_v<P, CacheAppendParams>;
+  constexpr int V = 16 / sizeof(E), kPairs = V / 2;
+  using Pair = PairOf<E>;
+  union Vec {
+    uint4 v;
+    typename Pair::Raw w[kPairs];
+  };
+  extern __shared__ float2 cs[];  // [tile][rotary_dim / 2], then (append) [tile] places
+  const int half = p.rotary_dim >> 1;
+  const int64_t first = int64_t(blockIdx.x) * cut.tile, all = p.batch * p.tokens;
+  const int here = int(all - first < cut.tile ? all - first : cut.tile);
+  AppendPlace* const places = reinterpret_cast<AppendPlace*>(cs + (cut.tile * half + 1) / 2 * 2);
+  const Place<kMode, V> at(p, cut);
+  const int64_t token = first + at.t, b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
+  RotaryTensor x = p.x[at.kind & 1];
+  if constexpr (kAppend)
+    if (at.kind == 2) x = p.v;
+  const int heads = at.live && at.t < here ? x.heads : 0;
+  const E* const in = static_cast<const E*>(x.in) + b * x.stride_b + l * x.stride_t;
+
+  Vec x0[kFwdBatch], x1[kMode == kHalves ? kFwdBatch : 1];
+  uint64_t other[kMode == kAny ? kFwdBatch : 1][kPairs];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kFwdBatch; ++i) {
+      const int h = h0 + i * at.step;
+      x0[i].v = make_uint4(0, 0, 0, 0);
+      if constexpr (kMode == kHalves) x1[i].v = x0[i].v;
+      if (h < heads) {
+        const E* row = in + h * x.stride_h;
+        if (at.rotates) x0[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c0));
+        if constexpr (kMode == kHalves) x1[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c1));
+        if constexpr (kMode == kAny) {
+#pragma unroll
+          for (int k = 0; k < kPairs; ++k) {
+            const int c = at.c0 + 2 * k;
+            other[i][k] = f2_pack(to_f(row[partner(c, half)]), to_f(row[partner(c + 1, half)]));
+          }
+        }
+      }
+    }
+  };
+  load(at.slot);
+
+  if constexpr (kAppend) {
+    for (int i = threadIdx.x >> 5; i < here; i += blockDim.x >> 5) {
+      const AppendPlace to = append_place(p, int(first) + i, threadIdx.x & 31);
+      if ((threadIdx.x & 31) == 0) places[i] = to;
+    }
+  }
+  for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
+    const int tt = i / half;
+    cs[i] = rotary_angle(p, first + tt, i - tt * half);
+  }
+  __syncthreads();
+
+  E* out = nullptr;
+  int64_t out_h = p.head_dim;
+  if (heads > 0) {
+    if (!kAppend || at.kind == 0) out = static_cast<E*>(x.out) + token * x.heads * p.head_dim;
+    if constexpr (kAppend) {
+      if (at.kind == 1 && places[at.t].k >= 0) out = static_cast<E*>(p.k_pool) + places[at.t].k;
+      if (at.kind == 2 && places[at.t].v >= 0) out = static_cast<E*>(p.v_pool) + places[at.t].v;
+      if (at.kind) out_h = at.kind == 1 ? p.k_stride[2] : p.v_stride[2];
+    }
+  }
+  // out0 = n0 * co0 + partner * si0, and in kHalves out1 = n1 * co1 + n0 * si1; the weights
+  // are inside
+  constexpr int kTwo = kMode == kHalves ? kPairs : 1;
+  uint64_t co0[kPairs], si0[kPairs], co1[kTwo], si1[kTwo];
+  {
+    const float2* angles = cs + (at.t < here ? at.t * half : 0);
+    column_angles<kMode>(p, angles, kMode == kHalves && !at.rotates ? p.rotary_dim : at.c0, co0, si0);
+#pragma unroll
+    for (int k = 0; k < kTwo; ++k) {
+      co1[k] = co0[k];
+      si1[k] = at.rotates ? f2_sub(0, si0[k]) : 0;
+    }
+    if constexpr (kNorm) {
+      constexpr bool kHalfType = std::is_same_v<E, __half>;
+      auto pair_of_weights = [&](int c, int d) {
+        return f2_pack(weight_at(p, at.kind, c, kHalfType), weight_at(p, at.kind, d, kHalfType));
+      };
+      if (at.live && at.kind < 2) {
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const int c = at.c0 + 2 * k;
+          const uint64_t w = pair_of_weights(c, c + 1);
+          co0[k] = f2_mul(co0[k], w);
+          if constexpr (kMode == kNeighbours) si0[k] = f2_mul(si0[k], swapped(w));
+          if constexpr (kMode == kAny)
+            si0[k] = f2_mul(si0[k], pair_of_weights(partner(c, half), partner(c + 1, half)));
+          if constexpr (kMode == kHalves) {
+            const uint64_t w1 = pair_of_weights(at.c1 + 2 * k, at.c1 + 2 * k + 1);
+            si0[k] = f2_mul(si0[k], w1);
+            co1[k] = f2_mul(co1[k], w1);
+            si1[k] = f2_mul(si1[k], w);
+          }
+        }
+      }
+    }
+  }
+  const bool turns = !kAppend || at.kind < 2;
+  for (int r = 0; r < cut.rounds; ++r) {
+    const int h0 = at.slot + r * kFwdBatch * at.step;
+    if (r) load(h0);
+#pragma unroll
+    for (int i = 0; i < kFwdBatch; ++i) {
+      uint64_t a[kPairs], d[kPairs], scale = f2_pack(1.f, 1.f);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        a[k] = Pair::wide(x0[i].w[k]);
+        if constexpr (kMode == kHalves) d[k] = Pair::wide(x1[i].w[k]);
+        if constexpr (kMode == kNeighbours) d[k] = swapped(a[k]);
+        if constexpr (kMode == kAny) d[k] = other[i][k];
+      }
+      if constexpr (kNorm) {
+        uint64_t sq = 0;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          sq = f2_fma(a[k], a[k], sq);
+          if constexpr (kMode == kHalves) sq = f2_fma(d[k], d[k], sq);
+        }
+        const float mean = group_sum(pair_sum(sq), cut.lanes_log) / float(p.head_dim);
+        const float rstd = rsqrtf(mean + p.eps);
+        scale = f2_pack(rstd, rstd);
+      }
+      const int h = h0 + i * at.step;
+      if (h >= heads || !out) continue;
+      if (turns) {
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          if constexpr (kNorm) {
+            a[k] = f2_mul(a[k], scale);
+            d[k] = f2_mul(d[k], scale);
+          }
+          // without the norm the columns behind rotary_dim are copies, bit for bit
+          if (kNorm || (kMode == kHalves ? at.rotates : at.c0 + 2 * k < p.rotary_dim))
+            x0[i].w[k] = Pair::narrow(f2_fma(a[k], co0[k], f2_mul(d[k], si0[k])));
+          if constexpr (kMode == kHalves)
+            if (kNorm || at.rotates) x1[i].w[k] = Pair::narrow(f2_fma(d[k], co1[k], f2_mul(a[k], si1[k])));
+        }
+      }
+      E* row = out + h * out_h;
+      if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0[i].v;
+      if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1[i].v;
+    }
+  }
+}
+
+// Gradients. A CTA takes every gridDim.x-th tile, and keeps its columns' share of the
+// weights' gradients in registers; the shares are added in the groups' order.
+template <class E, int kMode>
+__global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const NormRotaryParams p, const Cut cut) {
+  constexpr int V = 16 / sizeof(E), kPairs = V / 2, kTwo = kMode == kHalves ? kPairs : 1;
+  using Pair = PairOf<E>;
+  union Vec {
+    uint4 v;
+    typename Pair::Raw w[kPairs];
+  };
+  extern __shared__ float2 cs[];  // [tile][rotary_dim / 2]; at the end the weights' gradients
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int half = p.rotary_dim >> 1;
+  const int64_t all = p.batch * p.tokens;
+  const Place<kMode, V> at(p, cut);
+  const RotaryTensor x = p.x[at.kind], y = p.dy[at.kind];
+  constexpr bool kHalfType = std::is_same_v<E, __half>;
+  uint64_t w0[kPairs], w1[kTwo], acc0[kPairs], acc1[kTwo];
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k) {
+    acc0[k] = w0[k] = 0;
+    if (at.live)
+      w0[k] = f2_pack(weight_at(p, at.kind, at.c0 + 2 * k, kHalfType), weight_at(p, at.kind, at.c0 + 2 * k + 1, kHalfType));
+    if constexpr (kMode == kHalves) {
+      acc1[k] = w1[k] = 0;
+      if (at.live)
+        w1[k] = f2_pack(weight_at(p, at.kind, at.c1 + 2 * k, kHalfType), weight_at(p, at.kind, at.c1 + 2 * k + 1, kHalfType));
+    }
+  }
+  for (int64_t first = int64_t(blockIdx.x) * cut.tile; first < all; first += int64_t(gridDim.x) * cut.tile) {
+    const int here = int(all - first < cut.tile ? all - first : cut.tile);
+    const int64_t token = first + at.t, b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
+    const int heads = at.live && at.t < here ? x.heads : 0;
+    const E* const in = static_cast<const E*>(x.in) + b * x.stride_b + l * x.stride_t;
+    const E* const dy = static_cast<const E*>(y.in) + b * y.stride_b + l * y.stride_t;
+    E* const dx = static_cast<E*>(x.out) + token * x.heads * p.head_dim;
+    Vec x0[kBwdBatch], x1[kMode == kHalves ? kBwdBatch : 1], y0[kBwdBatch], y1[kMode == kHalves ? kBwdBatch : 1];
+    uint64_t other[kMode == kAny ? kBwdBatch : 1][kPairs];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int i = 0; i < kBwdBatch; ++i) {
+        const int h = h0 + i * at.step;
+        x0[i].v = y0[i].v = make_uint4(0, 0, 0, 0);
+        if constexpr (kMode == kHalves) x1[i].v = y1[i].v = x0[i].v;
+        if constexpr (kMode == kAny) {
+#pragma unroll
+          for (int k = 0; k < kPairs; ++k) other[i][k] = 0;
+        }
+        if (h < heads) {
+          const E* row = in + h * x.stride_h;
+          const E* back = dy + h * y.stride_h;
+          if (at.rotates) {
+            x0[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c0));
+            y0[i].v = __ldg(reinterpret_cast<const uint4*>(back + at.c0));
+          }
+          if constexpr (kMode == kHalves) {
+            x1[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c1));
+            y1[i].v = __ldg(reinterpret_cast<const uint4*>(back + at.c1));
+          }
+          if constexpr (kMode == kAny) {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+              const int c = at.c0 + 2 * k;
+              other[i][k] = f2_pack(to_f(back[partner(c, half)]), to_f(back[partner(c + 1, half)]));
+            }
+          }
+        }
+      }
+    };
+    load(at.slot);
+    __syncthreads();  // the last tile's angles have been read
+    for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
+      const int tt = i / half;
+      cs[i] = rotary_angle(p, first + tt, i - tt * half);
+    }
+    __syncthreads();
+    uint64_t co[kPairs], si[kPairs];
+    column_angles<kMode>(p, cs + (at.t < here ? at.t * half : 0),
+                         kMode == kHalves && !at.rotates ? p.rotary_dim : at.c0, co, si);
+    for (int r = 0; r < cut.rounds; ++r) {
+      const int h0 = at.slot + r * kBwdBatch * at.step;
+      if (r) load(h0);
+#pragma unroll
+      for (int i = 0; i < kBwdBatch; ++i) {
+        // g in g0, g1 and x in a, d
+        uint64_t g0[kPairs], g1[kTwo], sq = 0, dot = 0;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const uint64_t e = Pair::wide(y0[i].w[k]), a = Pair::wide(x0[i].w[k]);
+          uint64_t f = 0;
+          if constexpr (kMode == kHalves) f = Pair::wide(y1[i].w[k]);
+          if constexpr (kMode == kNeighbours) f = swapped(e);
+          if constexpr (kMode == kAny) f = other[i][k];
+          g0[k] = f2_fma(e, co[k], f2_mul(f, si[k]));
+          sq = f2_fma(a, a, sq);
+          dot = f2_fma(f2_mul(g0[k], w0[k]), a, dot);
+          if constexpr (kMode == kHalves) {
+            const uint64_t d = Pair::wide(x1[i].w[k]);
+            g1[k] = f2_sub(f2_mul(f, co[k]), f2_mul(e, si[k]));
+            sq = f2_fma(d, d, sq);
+            dot = f2_fma(f2_mul(g1[k], w1[k]), d, dot);
+          }
+        }
+        const float inv = 1.f / float(p.head_dim);
+        const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
+        const float along = group_sum(pair_sum(dot), cut.lanes_log) * inv * rstd * rstd;
+        const int h = h0 + i * at.step;
+        if (h >= heads) continue;
+        const uint64_t scale = f2_pack(rstd, rstd), minus = f2_pack(-along, -along);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const uint64_t a = Pair::wide(x0[i].w[k]);
+          acc0[k] = f2_fma(g0[k], f2_mul(a, scale), acc0[k]);
+          x0[i].w[k] = Pair::narrow(f2_mul(scale, f2_fma(g0[k], w0[k], f2_mul(a, minus))));
+          if constexpr (kMode == kHalves) {
+            const uint64_t d = Pair::wide(x1[i].w[k]);
+            acc1[k] = f2_fma(g1[k], f2_mul(d, scale), acc1[k]);
+            x1[i].w[k] = Pair::narrow(f2_mul(scale, f2_fma(g1[k], w1[k], f2_mul(d, minus))));
+          }
+        }
+        E* row = dx + h * p.head_dim;
+        if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0[i].v;
+        if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1[i].v;
+      }
+    }
+  }
+  if (!p.dw_part) return;
+  // [group][head_dim]
+  float* const sums = reinterpret_cast<float*>(cs);
+  __syncthreads();
+  if (at.live) {
+    float* mine = sums + (threadIdx.x >> cut.lanes_log) * p.head_dim;
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+      if (at.rotates) f2_unpack(acc0[k], mine[at.c0 + 2 * k], mine[at.c0 + 2 * k + 1]);
+      if constexpr (kMode == kHalves) f2_unpack(acc1[k], mine[at.c1 + 2 * k], mine[at.c1 + 2 * k + 1]);
+    }
+  }
+  __syncthreads();
+  const int step = cut.slots[0] + cut.slots[1];
+  for (int i = threadIdx.x; i < 2 * p.head_dim; i += blockDim.x) {
+    const int kind = i / p.head_dim, c = i - kind * p.head_dim;
+    float sum = 0.f;
+    for (int t = 0; t < cut.tile; ++t)
+      for (int j = 0; j < cut.slots[kind]; ++j)
+        sum += sums[(t * step + (kind ? cut.slots[0] : 0) + j) * p.head_dim + c];
+    p.dw_part[int64_t(blockIdx.x) * 2 * p.head_dim + i] = sum;
+  }
+}
+
+// Heads that start or end off a 16-byte boundary, or need more than 32 lanes: a warp a head,
+// its columns lane by lane, a CTA a token (back: every gridDim.x-th). head_dim is at most 256.
+constexpr int kPerLane = 8;
+
+template <class E, bool kBack>
+__global__ void __launch_bounds__(kThreads) norm_rotary_element_kernel(const NormRotaryParams p) {
+  extern __shared__ float2 cs[];  // [rotary_dim / 2]; at the end the weights' gradients
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int kWarps = kThreads / 32;
+  constexpr bool kHalfType = std::is_same_v<E, __half>;
+  const int half = p.rotary_dim >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float inv = 1.f / float(p.head_dim);
+  float acc[kBack ? 2 : 1][kPerLane] = {};
+  for (int64_t token = blockIdx.x; token < p.batch * p.tokens; token += gridDim.x) {
+    const int64_t b = token / p.tokens, l = token - b * p.tokens;
+    __syncthreads();
+    for (int i = threadIdx.x; i < half; i += kThreads) cs[i] = rotary_angle(p, token, i);
+    __syncthreads();
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const RotaryTensor& x = p.x[kind];
+      const RotaryTensor& y = p.dy[kind];
+      for (int h = warp; h < x.heads; h += kWarps) {
+        const E* row = static_cast<const E*>(x.in) + b * x.stride_b + l * x.stride_t + h * x.stride_h;
+        const E* back = kBack ? static_cast<const E*>(y.in) + b * y.stride_b + l * y.stride_t + h * y.stride_h : row;
+        E* out = static_cast<E*>(x.out) + (token * x.heads + h) * p.head_dim;
+        float sq = 0.f, dot = 0.f, v[kPerLane], g[kPerLane], w[kPerLane];
+#pragma unroll
+        for (int k = 0; k < kPerLane; ++k) {
+          const int c = lane + 32 * k;
+          v[k] = g[k] = w[k] = 0.f;
+          if (c >= p.head_dim) continue;
+          v[k] = to_f(row[c]);
+          w[k] = weight_at(p, kind, c, kHalfType);
+          sq += v[k] * v[k];
+          // the rotation's own and partner's terms: of the weighted inputs, or of dy
+          const bool turns = c < p.rotary_dim, second = p.interleaved ? c & 1 : c >= half;
+          const int pair = p.interleaved ? c >> 1 : second ? c - half : c;
+          const int o = p.interleaved ? c ^ 1 : second ? c - half : c + half;
+          g[k] = kBack ? to_f(back[c]) : v[k] * w[k];
+          if (turns) {
+            const float2 f = cs[pair];
+            const float other = to_f(back[o]) * (kBack ? 1.f : weight_at(p, kind, o, kHalfType));
+            g[k] = g[k] * f.x + other * (second ? f.y : -f.y);
+          }
+          if (kBack) dot += g[k] * w[k] * v[k];
+        }
+        const float rstd = rsqrtf(group_sum(sq, 5) * inv + p.eps);
+        const float along = kBack ? group_sum(dot, 5) * inv * rstd * rstd : 0.f;
+#pragma unroll
+        for (int k = 0; k < kPerLane; ++k) {
+          const int c = lane + 32 * k;
+          if (c >= p.head_dim) continue;
+          if (kBack) acc[kBack ? kind : 0][k] += g[k] * (v[k] * rstd);
+          out[c] = from_f<E>(kBack ? rstd * (g[k] * w[k] - v[k] * along) : rstd * g[k]);
+        }
+      }
+    }
+  }
+  if constexpr (kBack) {
+    if (!p.dw_part) return;
+    float* const sums = reinterpret_cast<float*>(cs);  // [warp][2][head_dim]
+    __syncthreads();
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+      for (int k = 0; k < kPerLane; ++k)
+        if (lane + 32 * k < p.head_dim) sums[(warp * 2 + kind) * p.head_dim + lane + 32 * k] = acc[kind][k];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * p.head_dim; i += kThreads) {
+      float sum = 0.f;
+      for (int j = 0; j < kWarps; ++j) sum += sums[j * 2 * p.head_dim + i];
+      p.dw_part[int64_t(blockIdx.x) * 2 * p.head_dim + i] = sum;
+    }
+  }
+}
+
+// dw from the CTAs' parts, in an order that `parts` alone decides: warp j of a CTA adds
+// parts j, j + kDwWarps, ... of 32 columns, then the warps' sums are added.
+constexpr int kDwWarps = 16;
+template <class E>
+__global__ void __launch_bounds__(kDwWarps * 32) norm_rotary_dw_kernel(const NormRotaryParams p, int parts) {
+  __shared__ float sums[kDwWarps][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+  const int columns = 2 * p.head_dim;
+  float sum = 0.f;
+  if (i < columns) {
+#pragma unroll 8
+    for (int j = warp; j < parts; j += kDwWarps) sum += p.dw_part[int64_t(j) * columns + i];
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp || i >= columns) return;
+  sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < kDwWarps; ++j) sum += sums[j][lane];
+  const int kind = i / p.head_dim, c = i - kind * p.head_dim;
+  if (!p.dw[kind]) return;
+  if (p.weight_f32) static_cast<float*>(p.dw[kind])[c] = sum;
+  else static_cast<E*>(p.dw[kind])[c] = from_f<E>(sum);
+}
+
+// The widest accesses that the pairs' layout and (p.vec) the strides allow; < 0: by elements.
+template <class E>
+int mode_of(const RotaryParams& p) {
+  constexpr int V = 16 / sizeof(E);
+  if (!p.vec) return -1;
+  const int pairs = p.rotary_dim / 2;
+  const int mode = p.interleaved ? kNeighbours
+                   : pairs % V == 0 && (p.head_dim - p.rotary_dim) % V == 0 ? kHalves : kAny;
+  return lanes_of(mode, V, p.head_dim, p.rotary_dim) <= 32 ? mode : -1;
+}
+
+template <class E, int kMode, bool kNorm, class P>
+void fwd_mode(const P& p, int sm_count, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(E);
+  constexpr bool kAppend = std::is_same_v<P, CacheAppendParams>;
+  int heads[3] = {p.x[0].heads, p.x[1].heads, 0};
+  if constexpr (kAppend) heads[2] = p.v.heads;
+  const int64_t all = p.batch * p.tokens;
+  const Cut cut = make_cut(lanes_of(kMode, V, p.head_dim, p.rotary_dim), heads, kFwdBatch, all, sm_count);
+  const size_t smem = (size_t(cut.tile) * (p.rotary_dim / 2) + 1) / 2 * 2 * sizeof(float2) +
+                      (kAppend ? cut.tile * sizeof(AppendPlace) : 0);
+  norm_rotary_kernel<E, kMode, kNorm, P>
+      <<<unsigned((all + cut.tile - 1) / cut.tile), cut.threads, smem, s>>>(p, cut);
+}
+
+template <class E, bool kNorm, class P>
+void fwd_e(const P& p, int sm_count, cudaStream_t s) {
+  switch (mode_of<E>(p)) {
+    case kHalves: return fwd_mode<E, kHalves, kNorm>(p, sm_count, s);
+    case kNeighbours: return fwd_mode<E, kNeighbours, kNorm>(p, sm_count, s);
+    case kAny: return fwd_mode<E, kAny, kNorm>(p, sm_count, s);
+    default: break;
+  }
+  if constexpr (!std::is_same_v<P, CacheAppendParams>)
+    norm_rotary_element_kernel<E, false>
+        <<<unsigned(p.batch * p.tokens), kThreads, (p.rotary_dim / 2) * sizeof(float2), s>>>(p);
+}
+
+template <class E>
+Cut bwd_cut(const NormRotaryParams& p, int mode, int sm_count) {
+  return make_cut(lanes_of(mode, 16 / sizeof(E), p.head_dim, p.rotary_dim),
+                  {p.x[0].heads, p.x[1].heads, 0}, kBwdBatch, p.batch * p.tokens, sm_count);
+}
+
+// Two CTAs an SM, each with every parts-th tile.
+template <class E>
+int bwd_parts(const NormRotaryParams& p, int sm_count) {
+  const int mode = mode_of<E>(p);
+  const int64_t tiles = mode < 0 ? p.batch * p.tokens
+                                 : (p.batch * p.tokens + bwd_cut<E>(p, mode, sm_count).tile - 1) / bwd_cut<E>(p, mode, sm_count).tile;
+  return int(std::min<int64_t>(tiles, 2 * sm_count));
+}
+
+template <class E, int kMode>
+void bwd_mode(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
+  const Cut cut = bwd_cut<E>(p, kMode, sm_count);
+  const size_t angles = size_t(cut.tile) * (p.rotary_dim / 2) * sizeof(float2);
+  const size_t sums = p.dw_part ? size_t(cut.threads >> cut.lanes_log) * p.head_dim * sizeof(float) : 0;
+  norm_rotary_bwd_kernel<E, kMode><<<parts, cut.threads, std::max(angles, sums), s>>>(p, cut);
+}
+
+template <class E>
+void bwd_e(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
+  switch (mode_of<E>(p)) {
+    case kHalves: bwd_mode<E, kHalves>(p, parts, sm_count, s); break;
+    case kNeighbours: bwd_mode<E, kNeighbours>(p, parts, sm_count, s); break;
+    case kAny: bwd_mode<E, kAny>(p, parts, sm_count, s); break;
+    default:
+      norm_rotary_element_kernel<E, true>
+          <<<parts, kThreads, std::max(p.rotary_dim / 2 * sizeof(float2), 2 * kThreads / 32 * p.head_dim * sizeof(float)), s>>>(p);
+  }
+  if (!p.dw_part) return;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((2 * p.head_dim + 31) / 32);
+  cfg.blockDim = dim3(kDwWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, norm_rotary_dw_kernel<E>, p, parts);
+}
+
+}  // namespace
+
+void norm_rotary_launch(RotaryType t, const NormRotaryParams& p, int sm_count, cudaStream_t s) {
+  switch (t) {
+    case RotaryType::kBf16: return fwd_e<__nv_bfloat16, true>(p, sm_count, s);
+    case RotaryType::kF16: return fwd_e<__half, true>(p, sm_count, s);
+    default: return fwd_e<float, true>(p, sm_count, s);
+  }
+}
+
+int norm_rotary_bwd_parts(RotaryType t, const NormRotaryParams& p, int sm_count) {
+  return t == RotaryType::kF32 ? bwd_parts<float>(p, sm_count) : bwd_parts<__half>(p, sm_count);
+}
+
+void norm_rotary_bwd_launch(RotaryType t, const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
+  switch (t) {
+    case RotaryType::kBf16: return bwd_e<__nv_bfloat16>(p, parts, sm_count, s);
+    case RotaryType::kF16: return bwd_e<__half>(p, parts, sm_count, s);
+    default: return bwd_e<float>(p, parts, sm_count, s);
+  }
+}
+
+void cache_append_launch(RotaryType t, const CacheAppendParams& p, int sm_count, cudaStream_t s) {
+  if (t == RotaryType::kBf16)
+    p.norm ? fwd_e<__nv_bfloat16, true>(p, sm_count, s) : fwd_e<__nv_bfloat16, false>(p, sm_count, s);
+  else
+    p.norm ? fwd_e<__half, true>(p, sm_count, s) : fwd_e<__half, false>(p, sm_count, s);
+}
+
+}  // namespace mgfa

@@ -129,16 +129,6 @@ __device__ __forceinline__ int plan_pages(PlanSmem& s, const CacheState& c, int 
   return found < wanted ? found : wanted;
 }
 
-__device__ __forceinline__ int token_seq(const int* cu, int seqs, int t) {
-  int lo = 0, hi = seqs;  // the last b with cu[b] <= t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // Position of row t of the batch: behind what its sequence held before it grew.
 __device__ __forceinline__ int token_position(const CacheState& c, const int* slots, const int* cu,
                                               int seqs, int t) {
@@ -149,23 +139,6 @@ __device__ __forceinline__ int token_position(const CacheState& c, const int* sl
   // a sequence that could not grow: where its tokens would have gone (as in the plan)
   const int old = c.grown[slot] == n ? c.lens[slot] - n : c.lens[slot];
   return old + t - __ldg(cu + b);
-}
-
-// Whether reserve() has made room for row t of the batch, which is row t - q0 of the n that
-// sequence `slot` has grown by. Called by a whole warp, for cu[0] <= t < cu[seqs].
-__device__ __forceinline__ bool row_grew(const CacheState& c, const int* slots, const int* cu,
-                                         int seqs, int t, int lane, int& slot, int& q0, int& n) {
-  const int b = token_seq(cu, seqs, t);
-  slot = __ldg(slots + b);
-  if (slot < 0 || slot >= c.slots) return false;
-  // a slot named again, with as many tokens, would pass the test below too: its first
-  // sequence alone has grown
-  bool again = false;
-  for (int i = lane; i < b; i += 32) again |= __ldg(slots + i) == slot;
-  if (__any_sync(0xffffffffu, again)) return false;
-  q0 = __ldg(cu + b);
-  n = __ldg(cu + b + 1) - q0;
-  return c.grown[slot] == n && t - q0 < n;
 }
 
 constexpr int kPositionsInPlan = 4096;

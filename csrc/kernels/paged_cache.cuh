@@ -35,6 +35,39 @@ struct PageMove {
   int from, to, tokens;
 };
 
+#ifdef __CUDACC__
+namespace dev {
+
+__device__ __forceinline__ int token_seq(const int* cu, int seqs, int t) {
+  int lo = 0, hi = seqs;  // the last b with cu[b] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(cu + mid) <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Whether reserve() has made room for row t of the batch, which is row t - q0 of the n that
+// sequence `slot` has grown by. Called by a whole warp, for cu[0] <= t < cu[seqs].
+__device__ __forceinline__ bool row_grew(const CacheState& c, const int* slots, const int* cu,
+                                         int seqs, int t, int lane, int& slot, int& q0, int& n) {
+  const int b = token_seq(cu, seqs, t);
+  slot = __ldg(slots + b);
+  if (slot < 0 || slot >= c.slots) return false;
+  // a slot named again, with as many tokens, would pass the test below too: its first
+  // sequence alone has grown
+  bool again = false;
+  for (int i = lane; i < b; i += 32) again |= __ldg(slots + i) == slot;
+  if (__any_sync(0xffffffffu, again)) return false;
+  q0 = __ldg(cu + b);
+  n = __ldg(cu + b + 1) - q0;
+  return c.grown[slot] == n && t - q0 < n;
+}
+
+}  // namespace dev
+#endif
+
 void cache_reserve_launch(const CacheState& c, const int* slots, const int* cu, int seqs,
                           int* positions, int tokens, cudaStream_t stream);
 // refused[t]: whether row t belongs to a sequence that the reserve before left as it was.

@@ -38,19 +38,6 @@ __host__ __device__ inline int units_of(int mode, int v, int head_dim, int rotar
   return mode == kHalves ? rotary_dim / 2 / v + (head_dim - rotary_dim) / v : head_dim / v;
 }
 
-// (cos, sin) * magnitude of pair f at a token.
-__device__ __forceinline__ float2 angle(const RotaryParams& p, int64_t token, int f) {
-  const int64_t b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
-  const int64_t at = b * p.pos_stride_b + l * p.pos_stride_t;
-  const double pos = p.positions64 ? double(static_cast<const int64_t*>(p.positions)[at])
-                                   : double(static_cast<const int32_t*>(p.positions)[at]);
-  double turns = pos * p.inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
-  turns -= rint(turns);
-  float s, c;
-  sincospif(float(2.0 * turns), &s, &c);
-  return make_float2(c * p.magnitude, s * p.magnitude * p.sign);
-}
-
 // CTA: `tile` tokens; of each, `slots` groups of `units` threads, each of which takes
 // every slots-th head, at the same columns c0 (and c1) throughout. So a thread reads its
 // columns' sines and cosines once from shared memory, and its first loads are under way
@@ -107,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
 
   for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
     const int tt = i / half;
-    cs[i] = angle(p, first + tt, i - tt * half);
+    cs[i] = rotary_angle(p, first + tt, i - tt * half);
   }
   __syncthreads();
   if (slot >= heads) return;
@@ -167,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) rotary_element_kernel(const RotaryPa
   extern __shared__ float2 cs[];  // [rotary_dim / 2]
   const int half = p.rotary_dim >> 1;
   const int64_t token = blockIdx.x, b = token / p.tokens, l = token - b * p.tokens;
-  for (int i = threadIdx.x; i < half; i += kThreads) cs[i] = angle(p, token, i);
+  for (int i = threadIdx.x; i < half; i += kThreads) cs[i] = rotary_angle(p, token, i);
   __syncthreads();
   for (int k = 0; k < 2; ++k) {
     const RotaryTensor& x = p.x[k];

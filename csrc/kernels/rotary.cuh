@@ -1,4 +1,5 @@
-// Launch interface of the rotary position kernel (rotary.cu).
+// Launch interface of the rotary position kernel (rotary.cu), and a pair's angle, which
+// norm_rotary.cu uses too.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -31,6 +32,25 @@ struct RotaryParams {
   float magnitude = 1.f; // factor on the rotated values
   float sign = 1.f;      // -1: the transpose, for gradients
 };
+
+#ifdef __CUDACC__
+namespace dev {
+
+// (cos, sin) * magnitude of pair f at a token.
+__device__ __forceinline__ float2 rotary_angle(const RotaryParams& p, int64_t token, int f) {
+  const int64_t b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
+  const int64_t at = b * p.pos_stride_b + l * p.pos_stride_t;
+  const double pos = p.positions64 ? double(static_cast<const int64_t*>(p.positions)[at])
+                                   : double(static_cast<const int32_t*>(p.positions)[at]);
+  double turns = pos * p.inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
+  turns -= rint(turns);
+  float s, c;
+  sincospif(float(2.0 * turns), &s, &c);
+  return make_float2(c * p.magnitude, s * p.magnitude * p.sign);
+}
+
+}  // namespace dev
+#endif
 
 void rotary_launch(RotaryType t, const RotaryParams& p, int sm_count, cudaStream_t stream);
 

@@ -46,6 +46,10 @@ int64_t norm_layout_of(torch::Tensor x, torch::Tensor weight, c10::optional<torc
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> apply_rotary(
     torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
     torch::Tensor inv_freq, bool interleaved, double magnitude);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> apply_norm_rotary(
+    torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
+    torch::Tensor inv_freq, torch::Tensor q_weight, c10::optional<torch::Tensor> k_weight,
+    double eps, bool interleaved, double magnitude);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new,
@@ -64,6 +68,13 @@ torch::Tensor cache_refused(torch::Tensor k, torch::Tensor table, torch::Tensor 
 void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                  torch::Tensor refs, torch::Tensor grown, torch::Tensor status, int64_t layer,
                  torch::Tensor new_k, torch::Tensor new_v, torch::Tensor slots, torch::Tensor cu);
+torch::Tensor cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                           torch::Tensor refs, torch::Tensor grown, torch::Tensor status,
+                           int64_t layer, torch::Tensor q, torch::Tensor new_k, torch::Tensor new_v,
+                           torch::Tensor positions, torch::Tensor inv_freq, torch::Tensor slots,
+                           torch::Tensor cu, c10::optional<torch::Tensor> q_weight,
+                           c10::optional<torch::Tensor> k_weight, double eps, bool interleaved,
+                           double magnitude);
 void cache_free(torch::Tensor k, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
                 torch::Tensor grown, torch::Tensor status, torch::Tensor slots);
 void cache_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
@@ -115,6 +126,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_fp8", &mgfa::rms_norm_fp8);
   m.def("norm_layout_of", &mgfa::norm_layout_of);
   m.def("apply_rotary", &mgfa::apply_rotary);
+  m.def("apply_norm_rotary", &mgfa::apply_norm_rotary);
   m.def("paged_attention", &mgfa::paged_attention);
   m.def("paged_chunk_local_bytes", &mgfa::paged_chunk_local_bytes);
   m.def("host_status_word", &mgfa::host_status_word);
@@ -122,6 +134,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cache_reserve", &mgfa::cache_reserve);
   m.def("cache_refused", &mgfa::cache_refused);
   m.def("cache_write", &mgfa::cache_write);
+  m.def("cache_append", &mgfa::cache_append);
   m.def("cache_free", &mgfa::cache_free);
   m.def("cache_fork", &mgfa::cache_fork);
   m.def("cache_compact", &mgfa::cache_compact);

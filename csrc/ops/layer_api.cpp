@@ -1,7 +1,7 @@
 // Torch-facing entry points of the per-token operators of a decoder layer:
-// root-mean-square norm (rms_norm.cu) and rotary positions (rotary.cu).
+// root-mean-square norm (rms_norm.cu), rotary positions (rotary.cu) and both at once on
+// each head (norm_rotary.cu).
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/types.h>
 #include "../common/check.hpp"
 #include <ATen/cuda/CUDAContext.h>
@@ -12,8 +12,9 @@
 #include <vector>
 
 #include "forward_ad.hpp"
+#include "rotary_args.hpp"
+#include "../kernels/norm_rotary.cuh"
 #include "../kernels/rms_norm.cuh"
-#include "../kernels/rotary.cuh"
 
 namespace mgfa {
 
@@ -218,16 +219,6 @@ std::tuple<torch::Tensor, torch::Tensor> norm_bwd(const torch::Tensor& dy, const
   return {dx, dw};
 }
 
-// Gradients that cannot be differentiated again: an error where that is tried.
-variable_list once(variable_list grads) {
-  if (!at::GradMode::is_enabled()) return grads;
-  for (auto& g : grads)
-    if (g.defined()) g = g.detach().requires_grad_(true);
-  auto node = std::make_shared<torch::autograd::DelayedError>(
-      "this operator's gradient has no gradient of its own", int(grads.size()));
-  return (*node)(std::move(grads));
-}
-
 struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& x,
                                const torch::Tensor& weight, const OptTensor& residual, double eps) {
@@ -277,83 +268,24 @@ int64_t norm_layout_of(torch::Tensor x, torch::Tensor weight, OptTensor residual
 // ------------------------------------------------------------------ rotary positions
 namespace {
 
-RotaryTensor rotary_tensor(const torch::Tensor& t, torch::Tensor& out, const char* name) {
-  MGFA_CHECK(t.dim() == 3 || t.dim() == 4, name,
-             " must be [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]");
-  RotaryTensor r;
-  out = torch::empty(t.sizes(), t.options());
-  r.in = t.data_ptr();
-  r.out = out.data_ptr();
-  r.stride_b = t.dim() == 4 ? t.stride(0) : 0;
-  r.stride_t = t.stride(-3);
-  r.stride_h = t.stride(-2);
-  r.heads = int(t.size(-2));
-  return r;
-}
-
-}  // namespace
-
-namespace {
-
 // q (and k) with rotary positions; sign -1 rotates back (the gradient).
 std::tuple<torch::Tensor, torch::Tensor> rotary(torch::Tensor q, const OptTensor& k_in,
                                                 const torch::Tensor& positions,
                                                 const torch::Tensor& inv_freq, bool interleaved,
                                                 double magnitude, double sign) {
-  const NormType t = norm_type(q, "q");
-  MGFA_CHECK(q.dim() == 3 || q.dim() == 4,
-             "q must be [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]");
-  const int64_t D = q.size(-1), L = q.size(-3), B = q.dim() == 4 ? q.size(0) : 1;
-  MGFA_CHECK(D >= 2 && D <= 256, "head_dim must be 2 to 256, got ", D);
-  MGFA_CHECK(inv_freq.is_cuda() && inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 &&
-                 inv_freq.is_contiguous() && inv_freq.device() == q.device(),
-             "inv_freq must be a contiguous float64 CUDA tensor [rotary_dim / 2] on q's device");
-  MGFA_CHECK(inv_freq.numel() >= 1 && 2 * inv_freq.numel() <= D,
-             "inv_freq has ", inv_freq.numel(), " entries for head_dim ", D);
-  MGFA_CHECK(positions.is_cuda() && positions.device() == q.device() &&
-                 (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong),
-             "positions must be an int32 or int64 CUDA tensor on q's device");
-  MGFA_CHECK((positions.dim() == 1 && positions.size(0) == L) ||
-                 (q.dim() == 4 && positions.dim() == 2 && positions.size(0) == B &&
-                  positions.size(1) == L),
-             "positions must be [tokens], or [batch, tokens] for a batch");
-  torch::Tensor k, qo, ko;
-  if (q.stride(-1) != 1) q = q.contiguous();
-  if (k_in.has_value()) {
-    k = *k_in;
-    MGFA_CHECK(k.is_cuda() && k.device() == q.device() && k.scalar_type() == q.scalar_type() &&
-                   k.dim() == q.dim() && k.size(-1) == D && k.size(-3) == L &&
-                   (k.dim() == 3 || k.size(0) == B),
-               "k must match q in all but the number of heads");
-    if (k.stride(-1) != 1) k = k.contiguous();
-  }
-  c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor k = k_in.value_or(torch::Tensor()), qo, ko;
   RotaryParams p;
-  p.x[0] = rotary_tensor(q, qo, "q");
-  if (k.defined()) p.x[1] = rotary_tensor(k, ko, "k");
-  p.positions = positions.data_ptr();
-  p.positions64 = positions.scalar_type() == at::kLong;
-  p.pos_stride_b = positions.dim() == 2 ? positions.stride(0) : 0;
-  p.pos_stride_t = positions.stride(-1);
-  p.inv_freq = inv_freq.data_ptr<double>();
-  p.batch = B;
-  p.tokens = L;
-  p.head_dim = int(D);
-  p.rotary_dim = int(2 * inv_freq.numel());
-  p.interleaved = interleaved;
-  p.magnitude = float(magnitude);
+  const RotaryType t = rotary_args(p, q, k, positions, inv_freq, interleaved, magnitude);
+  c10::cuda::CUDAGuard guard(q.device());
+  qo = torch::empty(q.sizes(), q.options());
+  p.x[0].out = qo.data_ptr();
+  if (k.defined()) {
+    ko = torch::empty(k.sizes(), k.options());
+    p.x[1].out = ko.data_ptr();
+  }
   p.sign = float(sign);
-  const int v = t == NormType::kF32 ? 4 : 8;
-  auto vec_tensor = [&](const RotaryTensor& r) {
-    return reinterpret_cast<uintptr_t>(r.in) % 16 == 0 && r.stride_b % v == 0 &&
-           r.stride_t % v == 0 && r.stride_h % v == 0;
-  };
-  p.vec = D % v == 0 && vec_tensor(p.x[0]) && (!k.defined() || vec_tensor(p.x[1]));
-  MGFA_CHECK(p.x[0].heads + int64_t(p.x[1].heads) <= 4096, "at most 4096 heads");
-  MGFA_CHECK(B * L < (int64_t(1) << 31), "too many tokens");
-  if (B * L > 0 && p.x[0].heads + p.x[1].heads > 0) {
-    rotary_launch(RotaryType(int(t)), p, device_sm_count(q.get_device()),
-                  at::cuda::getCurrentCUDAStream());
+  if (p.batch * p.tokens > 0 && p.x[0].heads + p.x[1].heads > 0) {
+    rotary_launch(t, p, device_sm_count(q.get_device()), at::cuda::getCurrentCUDAStream());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   return {qo, ko};
@@ -396,6 +328,127 @@ std::tuple<torch::Tensor, OptTensor> apply_rotary(torch::Tensor q, OptTensor k,
     return {o[0], o.size() > 1 ? OptTensor(o[1]) : OptTensor()};
   }
   auto [qo, ko] = rotary(q, k, positions, inv_freq, interleaved, magnitude, 1.0);
+  return {qo, opt(ko)};
+}
+
+// ------------------------------------------------- heads normed and rotated in one pass
+namespace {
+
+// q' and k' (undefined without a k).
+std::tuple<torch::Tensor, torch::Tensor> norm_rotary(torch::Tensor q, torch::Tensor k,
+                                                     const torch::Tensor& positions,
+                                                     const torch::Tensor& inv_freq,
+                                                     const torch::Tensor& q_weight,
+                                                     const OptTensor& k_weight, double eps,
+                                                     bool interleaved, double magnitude) {
+  NormRotaryParams p;
+  const RotaryType t = rotary_args(p, q, k, positions, inv_freq, interleaved, magnitude);
+  c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor w[2], qo = torch::empty(q.sizes(), q.options()), ko;
+  norm_weight_args(p, q, k, q_weight, k_weight, eps, w);
+  p.x[0].out = qo.data_ptr();
+  if (k.defined()) {
+    ko = torch::empty(k.sizes(), k.options());
+    p.x[1].out = ko.data_ptr();
+  }
+  if (p.batch * p.tokens > 0 && p.x[0].heads + p.x[1].heads > 0) {
+    norm_rotary_launch(t, p, device_sm_count(q.get_device()), at::cuda::getCurrentCUDAStream());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return {qo, ko};
+}
+
+struct NormRotaryFn : torch::autograd::Function<NormRotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& q,
+                               const torch::Tensor& q_weight, const OptTensor& k,
+                               const OptTensor& k_weight, const torch::Tensor& positions,
+                               const torch::Tensor& inv_freq, double eps, bool interleaved,
+                               double magnitude) {
+    const torch::Tensor none;
+    auto [qo, ko] = norm_rotary(q, k.value_or(none), positions, inv_freq, q_weight, k_weight, eps,
+                                interleaved, magnitude);
+    ctx->save_for_backward({q, q_weight, k.value_or(none), k_weight.value_or(none), positions, inv_freq});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->set_materialize_grads(false);
+    if (!ko.defined()) return {qo};
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list none(9);
+    torch::Tensor dy[2] = {grads[0], grads.size() > 1 ? grads[1] : torch::Tensor()};
+    if (!dy[0].defined() && !dy[1].defined()) return none;
+    refuse_tangents("apply_norm_rotary's gradient", {dy[0], dy[1]});
+    const variable_list saved = ctx->get_saved_variables();
+    torch::Tensor x[2] = {saved[0], saved[2]};
+    c10::cuda::CUDAGuard guard(x[0].device());
+    NormRotaryParams p;
+    const RotaryType t = rotary_args(p, x[0], x[1], saved[4], saved[5], ctx->saved_data["interleaved"].toBool(),
+                                     ctx->saved_data["magnitude"].toDouble());
+    torch::Tensor w[2], dx[2], dw[2], part;
+    norm_weight_args(p, x[0], x[1], saved[1], opt(saved[3]), ctx->saved_data["eps"].toDouble(), w);
+    p.sign = -1.f;
+    bool need_dw = false;
+    for (int i = 0; i < 2; ++i) {
+      if (!dy[i].defined()) {  // nothing reaches this side
+        p.x[i].heads = 0;
+        continue;
+      }
+      const bool needs_x = ctx->needs_input_grad(2 * i), needs_w = ctx->needs_input_grad(2 * i + 1);
+      if (!needs_x && !needs_w) {
+        p.x[i].heads = 0;
+        continue;
+      }
+      if (dy[i].stride(-1) != 1) dy[i] = dy[i].contiguous();
+      p.dy[i] = rotary_tensor(dy[i]);
+      p.vec = p.vec && rotary_vec(p.dy[i], dy[i]);
+      dx[i] = torch::empty(x[i].sizes(), x[i].options());
+      p.x[i].out = dx[i].data_ptr();
+      if (needs_w) {
+        dw[i] = torch::empty(w[i].sizes(), w[i].options());
+        p.dw[i] = dw[i].data_ptr();
+        need_dw = true;
+      }
+    }
+    if (p.batch * p.tokens > 0 && p.x[0].heads + p.x[1].heads > 0) {
+      const int sms = device_sm_count(x[0].get_device());
+      const int parts = norm_rotary_bwd_parts(t, p, sms);
+      if (need_dw) {
+        part = torch::empty({parts, 2, p.head_dim}, x[0].options().dtype(at::kFloat));
+        p.dw_part = part.data_ptr<float>();
+      }
+      norm_rotary_bwd_launch(t, p, parts, sms, at::cuda::getCurrentCUDAStream());
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+    } else {
+      for (torch::Tensor& g : dw)
+        if (g.defined()) g.zero_();
+    }
+    for (int i = 0; i < 2; ++i) {
+      if (!dx[i].defined()) continue;
+      if (ctx->needs_input_grad(2 * i)) none[2 * i] = dx[i];
+      none[2 * i + 1] = dw[i];
+    }
+    return once(std::move(none));
+  }
+};
+
+}  // namespace
+
+std::tuple<torch::Tensor, OptTensor> apply_norm_rotary(torch::Tensor q, OptTensor k,
+                                                       torch::Tensor positions, torch::Tensor inv_freq,
+                                                       torch::Tensor q_weight, OptTensor k_weight,
+                                                       double eps, bool interleaved, double magnitude) {
+  refuse_tangents("apply_norm_rotary", {q, k.value_or(torch::Tensor()), q_weight,
+                                        k_weight.value_or(torch::Tensor()), inv_freq});
+  MGFA_CHECK(k.has_value() == k_weight.has_value(), "k and k_weight come together");
+  if (wants_grad(q, k) || wants_grad(q_weight, k_weight)) {
+    variable_list o = NormRotaryFn::apply(q, q_weight, k, k_weight, positions, inv_freq, eps,
+                                          interleaved, magnitude);
+    return {o[0], o.size() > 1 ? OptTensor(o[1]) : OptTensor()};
+  }
+  auto [qo, ko] = norm_rotary(q, k.value_or(torch::Tensor()), positions, inv_freq, q_weight, k_weight,
+                              eps, interleaved, magnitude);
   return {qo, opt(ko)};
 }
 

@@ -12,6 +12,7 @@
 #include <tuple>
 
 #include "forward_ad.hpp"
+#include "rotary_args.hpp"
 #include "../kernels/paged_attn.cuh"
 #include "../kernels/paged_cache.cuh"
 #include "../kernels/tma_host.hpp"
@@ -366,6 +367,57 @@ void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::T
   const int64_t ks[2] = {new_k.stride(0), new_k.stride(1)}, vs[2] = {new_v.stride(0), new_v.stride(1)};
   cache_write_launch(c, pool, new_k.data_ptr(), new_v.data_ptr(), ks, vs, slots.data_ptr<int>(),
                      cu.data_ptr<int>(), n, int(new_k.size(0)), at::cuda::getCurrentCUDAStream());
+}
+
+// q with its heads normed (with weights) and rotated; k's, treated alike, and v go to the
+// pages of the batch that cache_reserve made room for.
+torch::Tensor cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                           torch::Tensor refs, torch::Tensor grown, torch::Tensor status,
+                           int64_t layer, torch::Tensor q, torch::Tensor new_k, torch::Tensor new_v,
+                           torch::Tensor positions, torch::Tensor inv_freq, torch::Tensor slots,
+                           torch::Tensor cu, OptTensor q_weight, OptTensor k_weight, double eps,
+                           bool interleaved, double magnitude) {
+  const torch::Tensor none;
+  refuse_tangents("PagedKVCache.append", {q, new_k, new_v, inv_freq, q_weight.value_or(none), k_weight.value_or(none)});
+  MGFA_CHECK(layer >= 0 && layer < k.size(0), "layer ", layer, " is not one of the cache's ", k.size(0));
+  const int n = check_slots(slots, k, "slots");
+  check_ints(cu, k, 1, "cu_seqlens");
+  MGFA_CHECK(cu.size(0) == n + 1, "cu_seqlens must be [sequences + 1]");
+  check_rows16(q, 3, "q");
+  check_rows16(new_k, 3, "new_k");
+  check_rows16(new_v, 3, "new_v");
+  MGFA_CHECK(new_k.sizes() == new_v.sizes() && new_k.size(1) == k.size(3) && new_k.size(2) == k.size(4),
+             "new_k and new_v must be [tokens, kv_heads, head_dim] as in the cache");
+  MGFA_CHECK(q.size(0) == new_k.size(0) && q.size(2) == k.size(4), "q must be [tokens, heads, head_dim] with new_k's tokens and head_dim");
+  for (const torch::Tensor* t : {&q, &new_k, &new_v})
+    MGFA_CHECK(t->scalar_type() == k.scalar_type() && t->device() == k.device(),
+               "q, new_k and new_v must have the cache's dtype and device");
+  MGFA_CHECK(q.size(0) < (int64_t(1) << 30), "too many tokens");
+  MGFA_CHECK(q_weight.has_value() == k_weight.has_value(), "q_weight and k_weight come together");
+  c10::cuda::CUDAGuard guard(k.device());
+  CacheAppendParams p;
+  const RotaryType t = rotary_args(p, q, new_k, positions, inv_freq, interleaved, magnitude);
+  torch::Tensor w[2], out = torch::empty(q.sizes(), q.options());
+  if (q_weight.has_value()) {
+    norm_weight_args(p, q, new_k, *q_weight, k_weight, eps, w);
+    p.norm = 1;
+  }
+  if (q.size(0) == 0) return out;
+  p.x[0].out = out.data_ptr();
+  p.v = rotary_tensor(new_v);
+  p.c = cache_state(k, table, lens, refs, grown, status);
+  p.k_pool = static_cast<uint16_t*>(k.data_ptr()) + layer * k.stride(0);
+  p.v_pool = static_cast<uint16_t*>(v.data_ptr()) + layer * v.stride(0);
+  for (int i = 0; i < 3; ++i) {
+    p.k_stride[i] = k.stride(i + 1);
+    p.v_stride[i] = v.stride(i + 1);
+  }
+  p.slots = slots.data_ptr<int>();
+  p.cu = cu.data_ptr<int>();
+  p.seqs = n;
+  cache_append_launch(t, p, device_sm_count(k.get_device()), at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
 }
 
 void cache_free(torch::Tensor k, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,

@@ -17,8 +17,10 @@ rms_norm(x, weight, residual=None), rms_norm_fp8(...)
     output in 8 bits with scales.
 apply_rotary(q, k, positions, inv_freq), rotary_frequencies(rotary_dim, ...)
     Rotary positions in both layouts (differentiable), and their (scaled) frequencies.
+apply_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight)
+    The same behind a root-mean-square norm of each head, in one pass (differentiable).
 PagedKVCache, paged_attention(q, k_pages, v_pages, page_table, kv_lens, ...)
-    A paged cache of keys and values (reserve, write, fork, free, compact) and the
+    A paged cache of keys and values (reserve, write, append, fork, free, compact) and the
     attention of new tokens over it, from one token a sequence to long chunks.
 RingHealth, PeerLostError
     Liveness gate for ring calls (`ring_attention(..., health=RingHealth())`).
@@ -32,6 +34,6 @@ from .parallel.health import PeerLostError, RingHealth  # noqa: F401
 from .ops.flash import KernelStatusError, flash_attn, flash_attn_bwd, flash_attn_fwd  # noqa: F401
 from .ops.norm import rms_norm, rms_norm_fp8  # noqa: F401
 from .ops.paged import PagedKVCache, paged_attention  # noqa: F401
-from .ops.rotary import apply_rotary, rotary_frequencies  # noqa: F401
+from .ops.rotary import apply_norm_rotary, apply_rotary, rotary_frequencies  # noqa: F401
 from .ops.graphs import GraphedAttention  # noqa: F401
 from .models import RingAttentionBlock, RingTransformerLM, shard_targets  # noqa: F401

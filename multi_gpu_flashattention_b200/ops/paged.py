@@ -139,6 +139,22 @@ class PagedKVCache:
         for, with the same slots and cu_seqlens."""
         C().cache_write(self.k, self.v, *self._state, layer, k, v, self._ints(slots), self._ints(cu_seqlens))
 
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               positions: torch.Tensor, inv_freq: torch.Tensor, slots: Ints, cu_seqlens: Ints,
+               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, interleaved: bool = False, magnitude: float = 1.0) -> torch.Tensor:
+        """write() with the rotary positions applied on the way, in one pass: q [tokens,
+        heads, D] and k [tokens, kv_heads, D] become what apply_rotary or, with weights,
+        apply_norm_rotary makes of them; k's and v go to the pages of the batch that
+        reserve() made room for, and q's are returned (of all rows). positions int32 or int64
+        [tokens], as reserve() returns them; the rest as in those functions. Inference only:
+        there is no gradient."""
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_weight, k_weight)):
+            raise RuntimeError("append has no gradient: call it under torch.no_grad()")
+        return C().cache_append(self.k, self.v, *self._state, layer, q, k, v, positions, inv_freq,
+                                self._ints(slots), self._ints(cu_seqlens), q_weight, k_weight, eps,
+                                interleaved, magnitude)
+
     def attend(self, layer: int, q: torch.Tensor, slots: Ints, cu_seqlens: Ints, max_seqlen_q: int,
                causal: bool = True, softmax_scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, return_lse: bool = False):

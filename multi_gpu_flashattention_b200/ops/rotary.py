@@ -1,5 +1,5 @@
 """Rotary positions on the sm_100a kernel: interleaved and half layouts, part of the
-head, scaled for long contexts.
+head, scaled for long contexts; alone, or behind a norm of each head in the same pass.
 
 A head's first rotary_dim elements form pairs, (i, i + rotary_dim / 2) or, interleaved,
 (2i, 2i + 1); pair i of the token at position t is rotated by t * inv_freq[i] and
@@ -69,4 +69,20 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     contiguous. positions: int32 or int64 [tokens], or [batch, tokens]. inv_freq:
     float64 [rotary_dim / 2] (rotary_frequencies). Returns (q', k'), or q' alone."""
     qo, ko = C().apply_rotary(q, k, positions, inv_freq, interleaved, magnitude)
+    return qo if ko is None else (qo, ko)
+
+
+def apply_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                      inv_freq: torch.Tensor, q_weight: torch.Tensor,
+                      k_weight: Optional[torch.Tensor], eps: float = 1e-6,
+                      interleaved: bool = False, magnitude: float = 1.0):
+    """apply_rotary of q and k with each head normed first, in one pass:
+
+        n = x * rsqrt(mean(x^2) + eps) * weight     over the head's elements, in float32
+
+    and rounded once, behind the rotation. q_weight, k_weight: [head_dim], of q's dtype or
+    float32 (both alike). The rest is as in apply_rotary (k and k_weight may be None);
+    differentiable (once, in reverse mode) in q, k and the weights."""
+    qo, ko = C().apply_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved,
+                                   magnitude)
     return qo if ko is None else (qo, ko)

@@ -62,6 +62,7 @@ if which in ("all", "cuda"):
                 "csrc/kernels/legacy_fp32.cu",
                 "csrc/kernels/rms_norm.cu",
                 "csrc/kernels/rotary.cu",
+                "csrc/kernels/norm_rotary.cu",
                 "csrc/kernels/paged_decode.cu",
                 "csrc/kernels/paged_chunk.cu",
                 "csrc/kernels/paged_cache.cu",
