@@ -50,6 +50,8 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> apply_norm_rotary(
     torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
     torch::Tensor inv_freq, torch::Tensor q_weight, c10::optional<torch::Tensor> k_weight,
     double eps, bool interleaved, double magnitude);
+std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>>
+token_logprobs(torch::Tensor logits, torch::Tensor targets, int64_t top, int64_t ignore, torch::Tensor status);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new,
@@ -127,6 +129,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_layout_of", &mgfa::norm_layout_of);
   m.def("apply_rotary", &mgfa::apply_rotary);
   m.def("apply_norm_rotary", &mgfa::apply_norm_rotary);
+  m.def("token_logprobs", &mgfa::token_logprobs);
   m.def("paged_attention", &mgfa::paged_attention);
   m.def("paged_chunk_local_bytes", &mgfa::paged_chunk_local_bytes);
   m.def("host_status_word", &mgfa::host_status_word);

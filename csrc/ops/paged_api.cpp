@@ -48,6 +48,9 @@ int* host_words() {
 }
 std::atomic<int> host_words_used{0};
 
+}  // namespace
+
+// The kernels' status word in `t`, which is on `like`'s device or in pinned host memory.
 uint32_t* status_ptr(const torch::Tensor& t, const torch::Tensor& like) {
   MGFA_CHECK(t.scalar_type() == at::kInt && t.numel() >= 1, "status must be an int32 tensor");
   int* p = t.data_ptr<int>();
@@ -57,6 +60,8 @@ uint32_t* status_ptr(const torch::Tensor& t, const torch::Tensor& like) {
   MGFA_CHECK(!t.is_cuda() || t.device() == like.device(), "status must be on q's device or in pinned host memory");
   return reinterpret_cast<uint32_t*>(p);
 }
+
+namespace {
 
 // 16-bit values, head_dim 64 or 128 (the last dimension, contiguous), every row on a
 // 16-byte boundary.

@@ -22,6 +22,9 @@ apply_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight)
 PagedKVCache, paged_attention(q, k_pages, v_pages, page_table, kv_lens, ...)
     A paged cache of keys and values (reserve, write, append, fork, free, compact) and the
     attention of new tokens over it, from one token a sequence to long chunks.
+token_logprobs(logits, targets, top=0)
+    Log probabilities of given tokens and the entropy (both differentiable), and the
+    likeliest alternatives.
 RingHealth, PeerLostError
     Liveness gate for ring calls (`ring_attention(..., health=RingHealth())`).
 RingAttentionBlock, RingTransformerLM, shard_targets
@@ -32,6 +35,7 @@ from .parallel.layouts import RingLayout, make_layout  # noqa: F401
 from .parallel.api import ring_attention  # noqa: F401
 from .parallel.health import PeerLostError, RingHealth  # noqa: F401
 from .ops.flash import KernelStatusError, flash_attn, flash_attn_bwd, flash_attn_fwd  # noqa: F401
+from .ops.logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from .ops.norm import rms_norm, rms_norm_fp8  # noqa: F401
 from .ops.paged import PagedKVCache, paged_attention  # noqa: F401
 from .ops.rotary import apply_norm_rotary, apply_rotary, rotary_frequencies  # noqa: F401

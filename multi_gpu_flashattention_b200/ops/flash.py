@@ -142,7 +142,7 @@ def status_monitor(device) -> StatusMonitor:
 
 
 class HostStatus:
-    """The status word of the paged-cache calls that pass none, for one device, in
+    """The status word of the paged-cache calls that pass none and of token_logprobs, for one device, in
     pinned host memory: kernels write it across the bus, only where they have an error
     to report, and the host reads it like any variable. A call costs no read-back, and a
     replayed CUDA graph reports as an eager call does. The next call on the device that
@@ -163,10 +163,11 @@ class HostStatus:
         v = int(self._value[0]) & 0xFFFFFFFF
         if v:
             self._value[0] = 0
-            raise _status_error(v, "paged cache")
+            raise _status_error(v, _HOST_STATUS_SITES.get((v >> 8) & 0xFF, "paged cache"))
 
 
 _HOST_STATUS: dict = {}
+_HOST_STATUS_SITES = {68: "token_logprobs (a target outside the vocab)"}
 
 
 def host_status(device) -> HostStatus:

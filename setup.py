@@ -54,6 +54,7 @@ if which in ("all", "cuda"):
                 "csrc/ops/attn_api.cpp",
                 "csrc/ops/layer_api.cpp",
                 "csrc/ops/paged_api.cpp",
+                "csrc/ops/loss_api.cpp",
                 "csrc/kernels/umma_probe.cu",
                 "csrc/kernels/flash_fwd_sm100.cu",
                 "csrc/kernels/attn_fwd_persistent.cu",
@@ -63,6 +64,7 @@ if which in ("all", "cuda"):
                 "csrc/kernels/rms_norm.cu",
                 "csrc/kernels/rotary.cu",
                 "csrc/kernels/norm_rotary.cu",
+                "csrc/kernels/token_logprobs.cu",
                 "csrc/kernels/paged_decode.cu",
                 "csrc/kernels/paged_chunk.cu",
                 "csrc/kernels/paged_cache.cu",
