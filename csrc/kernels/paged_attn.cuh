@@ -64,11 +64,34 @@ struct PagedParams {
   // parts of share c are 2 c (a unit that an earlier share began) and 2 c + 1
   float* part_o = nullptr;
   float2* part_ml = nullptr;
+  // sequences that share a prefix (paged_shared.cu): sequences [0, own) come without the
+  // first[b] tokens that their group shares, and behind them the groups, each the new tokens
+  // of its sequences over the shared[g] tokens before; `seqs` counts both
+  const int* first = nullptr;   // [own]; null: nothing is shared
+  const int* groups = nullptr;  // [seqs - own + 1] sequences
+  const int* shared = nullptr;  // [seqs - own] tokens
+  int own = 0;
+  int no_own = 0;                        // this launch leaves the sequences' own keys to another
+  int64_t least_rows = 0, most_rows = 0;  // of a group a key head: those that it takes
+  float* acc_o = nullptr;    // [2 (own, shared)][tokens][heads][head_dim]: rows of whole units,
+  float2* acc_ml = nullptr;  // as parts
+  int2* desc = nullptr;      // of the units (paged_desc): the shares that have parts of it, first
+                             // and last, or -1 where it is whole
   int4* join = nullptr;  // [grid] of the unit that share c began and others go on with:
                          // its first row of q, first head, rows (0: none), last share
   uint32_t* status = nullptr;
   uint64_t wait_limit_ns = 0;
 };
+
+// Entries of PagedParams::desc a key head, of `seqs` sequences or groups. Their units are
+// numbered by their rows (two sequences' never meet, as every sequence before adds one); the
+// groups' come behind the sequences'.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline int64_t paged_desc_rows(const PagedParams& p, int seqs) {
+  return int64_t(p.tokens) / p.block_tokens + seqs + 1;
+}
 
 #ifdef __CUDACC__
 namespace dev {
@@ -92,22 +115,43 @@ struct PagedBase {
 };
 
 // Sequence b as the kernels use it, whatever the arrays say: n new tokens from row q0,
-// all inside [0, tokens) and at most max_new; kv within the table's row. `bad` says that
-// something had to be cut.
+// all inside [0, tokens) and at most max_new; kv within the table's row, behind `skip` pages;
+// new token i sees keys [0, base + i], those below kv. `bad` says that something had to be
+// cut.
 struct PagedSeq {
-  int q0, n, kv, row;
+  int q0, n, kv, base, row, skip;
   bool bad;
 };
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+// Group g (PagedParams::groups) as a sequence.
+__device__ __forceinline__ PagedSeq paged_group(const PagedParams& p, int g) {
   PagedSeq s;
+  s.n = s.kv = s.base = s.q0 = s.row = s.skip = 0;
+  const int a = __ldg(p.groups + g), e = __ldg(p.groups + g + 1), kv = __ldg(p.shared + g);
+  s.bad = a < 0 || e < a || e > p.own || kv < 0 || kv > int64_t(p.width) * p.page || kv % p.page;
+  if (s.bad || kv == 0 || a == e) return s;
+  const int q0 = __ldg(p.cu_q + a), end = __ldg(p.cu_q + e), row = p.slots ? __ldg(p.slots + a) : a;
+  s.bad = q0 < 0 || end < q0 || end > p.tokens || row < 0 || row >= p.rows;
+  const int64_t rows = int64_t(end - q0) * p.group;
+  if (s.bad || rows < p.least_rows || rows > p.most_rows) return s;
+  s.n = end - q0;
+  s.q0 = q0;
+  s.kv = s.base = kv;
+  s.row = row;
+  return s;
+}
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+  if (p.first && b >= p.own) return paged_group(p, b - p.own);
+  PagedSeq s;
+  s.skip = 0;
   s.q0 = __ldg(p.cu_q + b);
   int end = __ldg(p.cu_q + b + 1);
   s.row = p.slots ? __ldg(p.slots + b) : b;
   s.bad = s.q0 < 0 || end < s.q0 || end > p.tokens || end - s.q0 > p.max_new || s.row < 0 ||
           s.row >= p.rows;
   if (s.bad) {
-    s.n = s.kv = s.q0 = s.row = 0;
+    s.n = s.kv = s.base = s.q0 = s.row = 0;
     return s;
   }
   s.n = end - s.q0;
@@ -117,6 +161,18 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     s.bad = true;
     s.kv = s.kv < 0 ? 0 : int(most);
   }
+  if (p.first) {
+    const int first = __ldg(p.first + b);
+    if (first < 0 || first > s.kv || first % p.page) {
+      s.bad = true;
+      s.n = 0;
+    } else {
+      s.skip = first / p.page;
+      s.kv -= first;
+    }
+    if (p.no_own) s.n = 0;
+  }
+  s.base = p.causal ? s.kv - s.n : s.kv;
   return s;
 }
 
@@ -125,7 +181,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
 __device__ __forceinline__ int paged_unit_tiles(const PagedParams& p, const PagedSeq& s, int unit) {
   int last = (unit + 1) * p.block_tokens;
   last = last < s.n ? last : s.n;
-  int seen = p.causal ? s.kv - s.n + last : s.kv;
+  int seen = s.base + last;
   seen = seen < s.kv ? seen : s.kv;
   return seen > 0 ? (seen + p.tile - 1) / p.tile : 1;
 }
@@ -231,6 +287,12 @@ __device__ __forceinline__ void paged_next(const PagedParams& p, const uint32_t*
     }
   }
   u.tiles = paged_unit_tiles(p, u.s, u.unit);
+}
+
+// The place of a unit in PagedParams::desc.
+__device__ __forceinline__ int64_t paged_desc(const PagedParams& p, const PagedSeq& s, int b, int unit, int hk) {
+  const int64_t at = b < p.own ? b : paged_desc_rows(p, p.own) + b - p.own;
+  return (at + s.q0 / p.block_tokens + unit) * p.kv_heads + hk;
 }
 
 struct PagedShare {
@@ -357,6 +419,16 @@ struct PagedWalk {
   __device__ __forceinline__ bool complete() const { return t0 == 0 && t1 == u.tiles; }
   // The workspace's part that takes an incomplete run.
   __device__ __forceinline__ int64_t part() const { return 2 * int64_t(blockIdx.x) + (t0 > 0 ? 0 : 1); }
+  // With desc: of each run, by one thread.
+  __device__ __forceinline__ void note(const PagedParams& p, const uint32_t* prefix) const {
+    if (!p.desc || t0 > 0) return;
+    p.desc[paged_desc(p, u.s, u.b, u.unit, u.hk)] =
+        complete() ? make_int2(-1, -1) : make_int2(int(blockIdx.x), PagedShare(p, prefix).last(u));
+  }
+  // A complete unit's row in acc_o and acc_ml.
+  __device__ __forceinline__ int64_t acc_row(const PagedParams& p, int token, int head) const {
+    return ((u.b < p.own ? 0 : int64_t(p.tokens)) + token) * p.heads + head;
+  }
   // After the last run, by one thread.
   __device__ __forceinline__ void leave(const PagedParams& p, const uint32_t* prefix) const {
     if (!p.whole) paged_join(PagedShare(p, prefix), u, true, begin, end);
@@ -381,11 +453,19 @@ cudaError_t paged_allow_smem(Fn fn, std::atomic<uint64_t>& done) {
 void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
                          cudaStream_t stream);
 // More rows: tcgen05 tiles.
+// early: may begin while the launch before, which it does not need, still runs.
 void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                        const PagedParams& p, cudaStream_t stream);
+                        const PagedParams& p, cudaStream_t stream, bool early = false);
 // The most local memory a thread of its forms was compiled with, which has to be none.
 int64_t paged_chunk_local_bytes();
 // Joins the parts; launched behind either.
 void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
+// Sequences that share a prefix: `shared`, `first` and `member` ([own]: its group, or -1) from
+// the page table, for the groups of p. (Nothing but the arrays of the problem is read.)
+void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t stream);
+// Joins own and shared parts, behind the launch `a` that took the sequences' own keys and, with
+// groups of c.least_rows rows and more, `c`.
+void paged_shared_launch(const PagedParams& a, const PagedParams& c, bool two, const int* member,
+                         cudaStream_t stream);
 
 }  // namespace mgfa

@@ -67,7 +67,7 @@ struct __align__(1024) ChunkSmem {
   // The runs, which the producer finds a few ahead: run number i in slot i & 3.
   struct Run {
     PagedSeq s;
-    int hk, unit, t0, t1, complete, part;  // t1 < 0: there is none
+    int hk, unit, t0, t1, complete, part, acc;  // t1 < 0: there is none; acc: of acc_o's halves
   } runs[4];
   uint64_t run_full[4], run_empty[4];
 };
@@ -137,8 +137,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.drain, 1);
     fence_mbar_init();
   }
+  // A launch that began early ends behind the one before it, so that what waits for this one
+  // sees the results of both.
+  auto behind = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   PagedWalk at;
-  if (!at.start<kThreads>(p, prefix, s.sums)) return;  // the whole CTA
+  if (!at.start<kThreads>(p, prefix, s.sums)) return behind();  // the whole CTA
   if (warp == 0) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
@@ -167,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         r.t1 = t1;
         r.complete = at.complete();
         r.part = int(at.part());
+        r.acc = at.u.b >= p.own;
         mbar_arrive(&s.run_full[run & 3]);
       }
       ++run;
@@ -177,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const PagedUnit& u = at.u;
       const int tok0 = u.unit * p.block_tokens;
       const int tiles = u.s.n - tok0 > tile_tokens ? 2 : 1;
+      if (lane == 0) at.note(p, prefix);
       if (!(ok = publish(at.t1))) break;
       ok = __all_sync(0xffffffffu, mbar_wait(&s.q_empty, (seg & 1) ^ 1, ab, 70));
       if (!ok) break;
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d(s.q[t][hf], &map_q, &s.q_full, hf * 64, u.hk * p.group,
                         u.s.q0 + tok0 + t * tile_tokens, 0);
       }
-      const int* row = p.page_table + int64_t(u.s.row) * p.table_stride;
+      const int* row = p.page_table + int64_t(u.s.row) * p.table_stride + u.s.skip;
       for (int j = at.t0; j < at.t1; ++j, ++it) {
         const int st = it & 1;
         const uint32_t ph = ((it >> 1) & 1) ^ 1;
@@ -375,9 +380,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       {
         // keys that this row sees, and those that the tile's first row, hence each, does
         const int tok = tok0 + r / p.group;
-        int lim = p.causal ? kv - n + tok + 1 : kv;
+        int lim = u.s.base + tok + 1;
         lim = r >= tile_tokens * p.group || tok >= n ? 0 : lim < kv ? lim : kv;
-        int full = p.causal ? kv - n + tok0 + 1 : kv;
+        int full = u.s.base + tok0 + 1;
         full = full < kv ? full : kv;
         for (int j = j0; j < t1; j += step) {
           if (!(ok = wait(&s.s_full[t], sc & 1, 90 + t))) break;
@@ -456,12 +461,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             l = l * w0 + o.y * w1;
             m = top;
           }
-          const bool done = u.complete;
+          const bool whole = u.complete, done = whole && !p.acc_o;
           const int tok = tok0 + r / p.group, r_head = r % p.group;
           const bool valid = r < tile_tokens * p.group && tok < u.s.n;
           const int64_t row_tok = u.s.q0 + tok, head = int64_t(u.hk) * p.group + r_head;
-          const int64_t part = int64_t(u.part) * p.unit_rows +
-                               (tok - u.unit * p.block_tokens) * p.group + r_head;
+          const int64_t part = whole ? ((u.acc ? int64_t(p.tokens) : 0) + row_tok) * p.heads + head
+                                     : int64_t(u.part) * p.unit_rows +
+                                           (tok - u.unit * p.block_tokens) * p.group + r_head;
           if (done) {
             const float scale = l == 0.f ? 0.f : 1.f / l;
             w0 *= scale;
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint8_t* to = done ? reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) +
                                                           row_tok * p.o_stride_t + head * p.o_stride_h)
-                             : reinterpret_cast<uint8_t*>(p.part_o + part * kD);
+                             : reinterpret_cast<uint8_t*>((whole ? p.acc_o : p.part_o) + part * kD);
           // one copy of the code for all columns: fetching it takes longer than running it
 #pragma unroll 1
           for (int ch = 0; ch < kOChunks; ++ch) {
@@ -510,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (valid) {
-            if (!done) p.part_ml[part] = make_float2(m, l);
+            if (!done) (whole ? p.acc_ml : p.part_ml)[part] = make_float2(m, l);
             else if (p.lse)
               p.lse[head * p.tokens + row_tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
@@ -525,6 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc<512>(tmem);
+  behind();
 }
 
 template <int kD, bool kF16>
@@ -537,7 +544,7 @@ int64_t chunk_local_bytes() {
 
 template <int kD, bool kF16>
 void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                  const PagedParams& p, cudaStream_t s) {
+                  const PagedParams& p, cudaStream_t s, bool early) {
   const int smem = int(sizeof(ChunkSmem<kD>)) + 1024 + 4 * (p.seqs + 1);
   auto fn = paged_chunk_kernel<kD, kF16>;
   static const int64_t local = chunk_local_bytes<kD, kF16>();
@@ -547,8 +554,17 @@ void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = paged_allow_smem(fn, allowed);
   if (e == cudaSuccess) {
-    fn<<<p.grid, kThreads, smem, s>>>(mq, mk, mv, p);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, fn, mq, mk, mv, p);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
 }
@@ -561,9 +577,11 @@ int64_t paged_chunk_local_bytes() {
 }
 
 void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                        const PagedParams& p, cudaStream_t s) {
-  if (p.head_dim == 64) p.fp16 ? chunk_launch<64, true>(mq, mk, mv, p, s) : chunk_launch<64, false>(mq, mk, mv, p, s);
-  else p.fp16 ? chunk_launch<128, true>(mq, mk, mv, p, s) : chunk_launch<128, false>(mq, mk, mv, p, s);
+                        const PagedParams& p, cudaStream_t s, bool early) {
+  if (p.head_dim == 64)
+    p.fp16 ? chunk_launch<64, true>(mq, mk, mv, p, s, early) : chunk_launch<64, false>(mq, mk, mv, p, s, early);
+  else
+    p.fp16 ? chunk_launch<128, true>(mq, mk, mv, p, s, early) : chunk_launch<128, false>(mq, mk, mv, p, s, early);
 }
 
 }  // namespace mgfa

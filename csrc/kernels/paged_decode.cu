@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     bool ok = true;
     do {
       const PagedUnit& u = at.u;
-      const int* row = p.page_table + int64_t(u.s.row) * p.table_stride;
+      const int* row = p.page_table + int64_t(u.s.row) * p.table_stride + u.s.skip;
+      if (lane == 0) at.note(p, prefix);
       for (int t = at.t0; t < at.t1; ++t, ++it) {
         const int st = it % kStages;
         if (!__all_sync(0xffffffffu, mbar_wait(&s.empty[st], ((it / kStages) & 1) ^ 1, ab, 61))) {
@@ -165,14 +166,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   bool ok = true;
   do {
     const PagedUnit& u = at.u;
-    const int rows = u.s.n * p.group;
+    // the sequence's or, of a group (PagedParams::groups), the unit's
+    const int tok0 = u.unit * p.block_tokens, left = u.s.n - tok0;
+    const int rows = (left < p.block_tokens ? left : p.block_tokens) * p.group, q0 = u.s.q0 + tok0;
     // queries: row r = token r / group, head r % group
     for (int i = threadIdx.x; i < kR * (kD / 8); i += kConsumers * 32) {
       const int r = i / (kD / 8), c = (i % (kD / 8)) * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < rows)
         v = *reinterpret_cast<const uint4*>(
-            static_cast<const uint16_t*>(p.q) + int64_t(u.s.q0 + r / p.group) * p.q_stride_t +
+            static_cast<const uint16_t*>(p.q) + int64_t(q0 + r / p.group) * p.q_stride_t +
             int64_t(u.hk * p.group + r % p.group) * p.q_stride_h + c);
       *reinterpret_cast<uint4*>(&s.q[r][c]) = v;
     }
@@ -190,11 +193,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = m * 16 + h * 8 + (lane >> 2);
-        int l = p.causal ? u.s.kv - u.s.n + r / p.group + 1 : u.s.kv;
+        int l = u.s.base + tok0 + r / p.group + 1;
         l = l < u.s.kv ? l : u.s.kv;
         lim[m][h] = r < rows ? l : 0;
       }
-    const int full_keys = (p.causal ? u.s.kv - u.s.n + 1 : u.s.kv);  // seen by every row
+    const int full_keys = u.s.base + tok0 + 1;  // seen by every row, those below kv
     float o[kMT][kD / 8][4], mx[kMT][2], sum[kMT][2];
 #pragma unroll
     for (int m = 0; m < kMT; ++m) {
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
       const int key0 = t * kKeys + warp * 16;
-      const bool whole = key0 + 16 <= full_keys;
+      const bool whole = key0 + 16 <= full_keys && key0 + 16 <= u.s.kv;
       uint32_t pf[kMT][4];
 #pragma unroll
       for (int m = 0; m < kMT; ++m) {
@@ -361,9 +364,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int k = 0; k < kConsumers; ++k) total += s.ml[k][r].y * ex2_approx(s.ml[k][r].x - base);
       const float* a = &s.acc[r][c];
-      if (done) {
+      const int tok = q0 + r / p.group, head = u.hk * p.group + r % p.group;
+      if (done && !p.acc_o) {
         const float inv = total == 0.f ? 0.f : 1.f / total;  // 0: no visible key
-        const int tok = u.s.q0 + r / p.group, head = u.hk * p.group + r % p.group;
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + int64_t(tok) * p.o_stride_t +
                                   int64_t(head) * p.o_stride_h + c) =
             make_uint4(pack16<kF16>(a[0] * inv, a[1] * inv), pack16<kF16>(a[2] * inv, a[3] * inv),
@@ -372,10 +375,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           p.lse[int64_t(head) * p.tokens + tok] =
               total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
       } else {
-        float* dst = p.part_o + (slot * p.unit_rows + r) * kD + c;
+        const int64_t to = done ? at.acc_row(p, tok, head) : slot * p.unit_rows + r;
+        float* dst = (done ? p.acc_o : p.part_o) + to * kD + c;
         *reinterpret_cast<float4*>(dst) = make_float4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<float4*>(dst + 4) = make_float4(a[4], a[5], a[6], a[7]);
-        if (c == 0) p.part_ml[slot * p.unit_rows + r] = make_float2(top, total);
+        if (c == 0) (done ? p.acc_ml : p.part_ml)[to] = make_float2(top, total);
       }
     }
     if (threadIdx.x == 0) s.stop = *ab.flag;

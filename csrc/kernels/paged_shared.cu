@@ -1,0 +1,296 @@
+// Attention of sequences that share a prefix: what they share, and the join of their parts.
+//
+// Sequences that were forked from one prompt hold the same pages for its full ones. A group
+// is a run of the batch's sequences; its first shared[g] tokens are read once for the new
+// tokens of all of them, as one more sequence whose every row sees every key, and each
+// sequence's own keys are read for itself. Both come as (O, m, l): O = sum 2^(s - m) v,
+// l = sum 2^(s - m), unnormalised in fp32, from paged_decode.cu and paged_chunk.cu, whose
+// shares may cut them further. A row's result is
+//
+//   out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,   M = max m_i
+//
+// over its own parts and its group's, in that order: one softmax over all keys, whose two
+// halves are never rounded to 16 bits.
+#include "paged_attn.cuh"
+#include "sm100_ptx.cuh"
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+namespace mgfa {
+namespace {
+
+using namespace mgfa::dev;
+namespace cg = cooperative_groups;
+
+// ---------------------------------------------------------------------- what is shared
+constexpr int kPlanThreads = 512;
+constexpr int kPlanCtas = 8;  // of a group, a cluster
+
+// shared[g]: the leading pages that all of the group's sequences name alike, as far as these
+// are full and hold none of their new tokens; 0 for a sequence alone, which reads them once
+// anyway. Invalid groups share nothing, and neither do all others of the call then.
+__global__ void __launch_bounds__(kPlanThreads)
+    paged_plan_kernel(const PagedParams p, int* shared, int* first, int* member) {
+  const int g = blockIdx.x / kPlanCtas, cta = blockIdx.x % kPlanCtas, n_groups = p.seqs - p.own;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool bad = false;
+  for (int i = threadIdx.x; i < n_groups; i += kPlanThreads) {
+    const int a = __ldg(p.groups + i), e = __ldg(p.groups + i + 1);
+    bad |= a < 0 || e < a || e > p.own;
+  }
+  bad = __syncthreads_or(bad);
+  const int from = bad ? 0 : __ldg(p.groups + g), to = bad ? 0 : __ldg(p.groups + g + 1);
+  __shared__ int least;
+  if (threadIdx.x == 0) least = to - from > 1 ? p.width : 0;
+  __syncthreads();
+  auto row_of = [&](int b) { return p.slots ? __ldg(p.slots + b) : b; };
+  if (to - from > 1) {
+    const int lead = row_of(from);
+    const bool lead_ok = lead >= 0 && lead < p.rows;
+    for (int b = from + cta * (kPlanThreads / 32) + warp; b < to; b += kPlanCtas * (kPlanThreads / 32)) {
+      const int row = row_of(b), n = __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b);
+      int pages = 0;
+      if (lead_ok && row >= 0 && row < p.rows && n >= 0) {
+        const int64_t kv = std::min<int64_t>(__ldg(p.kv_lens + row), int64_t(p.width) * p.page);
+        pages = int(std::max<int64_t>(kv - n, 0) / p.page);
+        const int* mine = p.page_table + int64_t(row) * p.table_stride;
+        const int* theirs = p.page_table + int64_t(lead) * p.table_stride;
+        for (int j0 = 0; j0 < pages; j0 += 32 * 4) {
+          bool differ[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int j = j0 + k * 32 + lane;
+            differ[k] = false;
+            if (j < pages) {
+              const int page = __ldg(mine + j);
+              differ[k] = page != __ldg(theirs + j) || page < 0;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = __ballot_sync(0xffffffffu, differ[k]);
+            if (at) pages = std::min(pages, j0 + k * 32 + __ffs(at) - 1);
+          }
+        }
+      }
+      if (lane == 0) atomicMin(&least, pages);
+    }
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  int all = least;
+  for (int i = 0; i < kPlanCtas; ++i) all = std::min(all, *cluster.map_shared_rank(&least, i));
+  cluster.sync();
+  const int id = cta * kPlanThreads + int(threadIdx.x), step = kPlanCtas * kPlanThreads;
+  for (int b = from + id; b < to; b += step) {
+    first[b] = all * p.page;
+    member[b] = g;
+  }
+  if (id == 0) shared[g] = all * p.page;
+  if (g == 0) {  // sequences of no group
+    const int begin = bad ? p.own : __ldg(p.groups), end = bad ? p.own : __ldg(p.groups + n_groups);
+    for (int b = id; b < p.own; b += step)
+      if (b < begin || b >= end) {
+        first[b] = 0;
+        member[b] = -1;
+      }
+    if (bad && id == 0) record_error(p.status, kErrBadArgument, 69, 0);
+  }
+}
+
+// ---------------------------------------------------------------------- the join
+constexpr int kJoinWarps = 16;
+
+// A row's parts of one kind: whole, or those of shares [c, last].
+struct RowParts {
+  const float* o;
+  const float2* ml;
+  int64_t row;   // of acc_o, or r of the unit
+  int c, n;
+  int unit_rows;  // 0: whole
+  __device__ __forceinline__ int64_t at(int i) const {
+    return unit_rows ? (2 * int64_t(c + i) + (i == 0 ? 1 : 0)) * unit_rows + row : row;
+  }
+};
+
+__device__ __forceinline__ RowParts row_parts(const PagedParams& p, const PagedSeq& s, int b, int hk, int i, int head) {
+  const int unit = i / p.block_tokens;
+  const int2 d = p.desc[paged_desc(p, s, b, unit, hk)];
+  RowParts r;
+  r.c = d.x;
+  if (d.x < 0) {
+    r.o = p.acc_o;
+    r.ml = p.acc_ml;
+    r.row = ((b < p.own ? 0 : int64_t(p.tokens)) + s.q0 + i) * p.heads + head;
+    r.n = 1;
+    r.unit_rows = 0;
+  } else {
+    r.o = p.part_o;
+    r.ml = p.part_ml;
+    r.row = (i - unit * p.block_tokens) * p.group + head - hk * p.group;
+    // (of a unit that a wait which ran out has left alone: none)
+    r.n = d.y >= d.x && d.y < p.grid ? d.y - d.x + 1 : 0;
+    r.unit_rows = p.unit_rows;
+  }
+  return r;
+}
+
+// CTA (b * kv_heads + hk, y): every gridDim.y-th block of rows of sequence b and key head hk.
+// kSplit warps share a row, as in paged_merge_kernel.
+template <int kD, bool kF16, int kSplit>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    paged_shared_kernel(const PagedParams a, const PagedParams c, int two, const int* member) {
+  constexpr int kE = kD / 32, kRows = kJoinWarps / kSplit;
+  __shared__ float sh[kSplit > 1 ? kJoinWarps : 1][kD];
+  const int b = blockIdx.x / a.kv_heads, hk = blockIdx.x - b * a.kv_heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
+  const PagedSeq own = paged_seq(a, b);
+  const int rows = own.n * a.group;  // (at most max_new * group)
+  // the group, and which launch took it
+  PagedSeq over;
+  over.n = 0;
+  bool second = false;
+  int g = -1;
+  if (own.skip > 0) {
+    g = member[b];
+    if (g >= 0 && g < a.seqs - a.own) {
+      over = paged_group(a, g);
+      if (over.n == 0 && two) {
+        over = paged_group(c, g);
+        second = true;
+      }
+      const bool inside = own.q0 >= over.q0 && own.q0 + own.n <= over.q0 + over.n;
+      if (!inside || over.kv != own.skip * a.page) over.n = 0;
+    }
+    if (over.n == 0 && blockIdx.y == 0 && hk == 0 && threadIdx.x == 0)
+      record_error(a.status, kErrBadArgument, 69, 0);  // first[] and the groups do not fit
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
+    const int r = r0 + warp / kSplit;
+    const bool live = r < rows;
+    const int i = live ? r / a.group : 0, head = hk * a.group + (live ? r - i * a.group : 0);
+    float top = -INFINITY, total = 0.f, acc[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[e] = 0.f;
+    if (live) {
+      RowParts side[2];
+      side[0] = row_parts(a, own, b, hk, i, head);
+      side[1].n = 0;
+      if (over.n > 0)
+        side[1] = row_parts(second ? c : a, over, a.own + g, hk, own.q0 + i - over.q0, head);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        for (int j = lane; j < side[k].n; j += 32) top = fmaxf(top, side[k].ml[side[k].at(j)].x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        for (int j0 = 0; j0 < side[k].n; j0 += 32) {
+          float2 ml = make_float2(-INFINITY, 0.f);
+          if (j0 + lane < side[k].n) ml = side[k].ml[side[k].at(j0 + lane)];
+          const float wt = ex2_approx(ml.x - base);
+          total += ml.y * wt;
+          const int n = side[k].n - j0 < 32 ? side[k].n - j0 : 32;
+#pragma unroll 8
+          for (int j = part; j < n; j += kSplit) {
+            const float f = __shfl_sync(0xffffffffu, wt, j);
+            const float* src = side[k].o + side[k].at(j0 + j) * kD + lane * kE;
+            if constexpr (kE == 4) {
+              const float4 v = *reinterpret_cast<const float4*>(src);
+              acc[0] = fmaf(f, v.x, acc[0]);
+              acc[1] = fmaf(f, v.y, acc[1]);
+              acc[2] = fmaf(f, v.z, acc[2]);
+              acc[3] = fmaf(f, v.w, acc[3]);
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(src);
+              acc[0] = fmaf(f, v.x, acc[0]);
+              acc[1] = fmaf(f, v.y, acc[1]);
+            }
+          }
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if constexpr (kSplit > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kE; ++e) sh[warp][lane * kE + e] = acc[e];
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int k = 1; k < kSplit; ++k)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) acc[e] += sh[warp + k][lane * kE + e];
+      }
+    }
+    if (!live || part) continue;
+    const float base = top == -INFINITY ? 0.f : top;
+    const float inv = total == 0.f ? 0.f : 1.f / total;  // 0: no visible key
+    const int tok = own.q0 + i;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + int64_t(tok) * a.o_stride_t +
+                    int64_t(head) * a.o_stride_h + lane * kE;
+    if constexpr (kE == 4)
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack16<kF16>(acc[0] * inv, acc[1] * inv), pack16<kF16>(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out) = pack16<kF16>(acc[0] * inv, acc[1] * inv);
+    if (a.lse && lane == 0)
+      a.lse[int64_t(head) * a.tokens + tok] =
+          total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
+  }
+}
+
+void cuda_ok(cudaError_t e) {
+  if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
+}
+
+template <int kD, bool kF16>
+void join_launch(const PagedParams& a, const PagedParams& c, bool two, const int* member, cudaStream_t s) {
+  // Few rows have many parts each, many rows few.
+  const int64_t rows = int64_t(a.max_new) * a.group;
+  const bool few = int64_t(a.own) * rows * a.kv_heads <= 1024;
+  const int per = few ? kJoinWarps / 4 : kJoinWarps;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.own * a.kv_heads, unsigned(std::min<int64_t>((rows + per - 1) / per, 64)));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cuda_ok(cudaLaunchKernelEx(&cfg, few ? paged_shared_kernel<kD, kF16, 4> : paged_shared_kernel<kD, kF16, 1>, a, c,
+                             int(two), member));
+}
+
+}  // namespace
+
+void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.seqs - p.own) * kPlanCtas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kPlanCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cuda_ok(cudaLaunchKernelEx(&cfg, paged_plan_kernel, p, shared, first, member));
+}
+
+void paged_shared_launch(const PagedParams& a, const PagedParams& c, bool two, const int* member,
+                         cudaStream_t s) {
+  if (a.head_dim == 64)
+    a.fp16 ? join_launch<64, true>(a, c, two, member, s) : join_launch<64, false>(a, c, two, member, s);
+  else
+    a.fp16 ? join_launch<128, true>(a, c, two, member, s) : join_launch<128, false>(a, c, two, member, s);
+}
+
+}  // namespace mgfa

@@ -56,7 +56,11 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new,
     c10::optional<torch::Tensor> slots, bool causal, double scale,
-    c10::optional<torch::Tensor> out, bool want_lse, torch::Tensor status, int64_t wait_limit_ns);
+    c10::optional<torch::Tensor> out, bool want_lse, torch::Tensor status, int64_t wait_limit_ns,
+    c10::optional<torch::Tensor> groups, c10::optional<torch::Tensor> plan);
+torch::Tensor shared_prefix(torch::Tensor page_table, torch::Tensor kv_lens, torch::Tensor cu_q,
+                            torch::Tensor groups, int64_t page, c10::optional<torch::Tensor> slots,
+                            torch::Tensor status);
 int64_t paged_chunk_local_bytes();
 torch::Tensor host_status_word();
 void cache_check(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
@@ -131,6 +135,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("apply_norm_rotary", &mgfa::apply_norm_rotary);
   m.def("token_logprobs", &mgfa::token_logprobs);
   m.def("paged_attention", &mgfa::paged_attention);
+  m.def("shared_prefix", &mgfa::shared_prefix);
   m.def("paged_chunk_local_bytes", &mgfa::paged_chunk_local_bytes);
   m.def("host_status_word", &mgfa::host_status_word);
   m.def("cache_check", &mgfa::cache_check);

@@ -108,10 +108,130 @@ torch::Tensor host_status_word() {
   return torch::from_blob(host_words() + i, {1}, torch::TensorOptions().dtype(at::kInt));
 }
 
+namespace {
+
+// How many groups cu_groups counts of a batch of `seqs` sequences.
+int64_t check_groups(const torch::Tensor& groups, const torch::Tensor& like, int64_t seqs) {
+  check_ints(groups, like, 1, "cu_groups");
+  MGFA_CHECK(groups.size(0) >= 1, "cu_groups must be [groups + 1]");
+  const int64_t n = groups.size(0) - 1;
+  MGFA_CHECK(seqs + n <= kPagedMaxSeqs, "at most ", kPagedMaxSeqs, " sequences and groups a call");
+  return n;
+}
+
+// A group's rows a key head up to which its prefix goes to the decode kernel, in units of 16
+// or 32 rows that each read it (all but the first from L2); above, to 128-row tiles.
+constexpr int64_t kGroupFewRows = 64;
+
+// The launches for sequences that share prefixes (paged_shared.cu).
+void attend_shared(PagedParams p, bool few, const torch::Tensor& q, const torch::Tensor& k,
+                   const torch::Tensor& v, const torch::Tensor& groups, const torch::Tensor& plan, int sms) {
+  const int64_t T = p.tokens, Hk = p.kv_heads, D = p.head_dim, n_groups = groups.size(0) - 1;
+  p.own = p.seqs;
+  p.seqs += int(n_groups);
+  p.groups = groups.data_ptr<int>();
+  p.shared = plan.data_ptr<int>();
+  p.first = p.shared + n_groups;
+  const int* member = p.first + p.own;
+  const auto f32 = q.options().dtype(at::kFloat);
+  // one of these each for what is a sequence's own and what its group shares
+  torch::Tensor acc = torch::empty({2 * T * p.heads * (D + 2)}, f32), work[2];
+  p.acc_o = acc.data_ptr<float>();
+  p.acc_ml = reinterpret_cast<float2*>(p.acc_o + 2 * T * p.heads * D);
+  PagedParams c = p;
+  // with few rows a sequence the groups' sizes decide, of which the host knows the bound
+  const bool two = few && T * p.group > kGroupFewRows;
+  p.most_rows = two ? kGroupFewRows : INT64_MAX;
+  c.least_rows = kGroupFewRows + 1;
+  c.most_rows = INT64_MAX;
+  c.no_own = 1;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  for (int i = 0; i < (two ? 2 : 1); ++i) {
+    PagedParams& l = i ? c : p;
+    const bool decode = few && i == 0;
+    if (decode) {
+      l.block_tokens = std::max(l.max_new, (l.max_new * l.group <= 16 ? 16 : 32) / l.group);
+      l.tile = 64;
+      l.grid = 2 * sms;
+    } else {
+      l.block_tokens = 2 * std::max(1, 128 / l.group);
+      l.tile = 128;
+      l.snap = 4;
+      l.grid = sms;
+    }
+    l.unit_rows = l.block_tokens * l.group;
+    l.min_share = 2;
+    const int64_t units = (T / l.block_tokens + n_groups + (i ? 0 : T / l.block_tokens + l.own)) * Hk;
+    const int64_t tiles = std::max<int64_t>(1, (int64_t(l.width) * l.page + l.tile - 1) / l.tile);
+    l.grid = int(std::min<int64_t>(l.grid, (units * tiles + l.min_share - 1) / l.min_share));
+    const int64_t rows = 2 * int64_t(l.grid) * l.unit_rows;
+    const int64_t descs = (paged_desc_rows(l, l.own) + paged_desc_rows(l, int(n_groups))) * Hk;
+    work[i] = torch::empty({rows * (D + 2) + 2 * descs}, f32);
+    l.part_o = work[i].data_ptr<float>();
+    l.part_ml = reinterpret_cast<float2*>(l.part_o + rows * D);
+    l.desc = reinterpret_cast<int2*>(l.part_ml + rows);
+    const uint32_t chunk = uint32_t(std::min<int64_t>(l.page, l.tile));
+    const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, 1, 1});
+    const CUtensorMap mv = map16(v, {3, 1, 2, 0}, {64, chunk, 1, 1});
+    if (decode) {
+      paged_decode_launch(mk, mv, l, stream);
+    } else {
+      const CUtensorMap mq = map16(q, {2, 1, 0, -1}, {64, uint32_t(l.group), uint32_t(l.block_tokens / 2), 1});
+      paged_chunk_launch(mq, mk, mv, l, stream, i == 1);
+    }
+  }
+  paged_shared_launch(p, c, two, member, stream);
+}
+
+}  // namespace
+
+// int32 [groups + 2 * sequences]: the tokens that each group shares, then for each sequence
+// those that its group shares and its group, or -1.
+torch::Tensor shared_prefix(torch::Tensor page_table, torch::Tensor kv_lens, torch::Tensor cu_q,
+                            torch::Tensor groups, int64_t page, OptTensor slots, torch::Tensor status) {
+  MGFA_CHECK(page_table.is_cuda(), "page_table must be a CUDA tensor");
+  check_ints(page_table, page_table, 2, "page_table");
+  check_ints(kv_lens, page_table, 1, "kv_lens");
+  check_ints(cu_q, page_table, 1, "cu_seqlens_q");
+  MGFA_CHECK(power_of_two(page) && page >= 16 && page <= 1024,
+             "the page size must be a power of two from 16 to 1024, got ", page);
+  MGFA_CHECK(page_table.size(1) * page < (int64_t(1) << 30), "page_table is too wide");
+  MGFA_CHECK(kv_lens.size(0) == page_table.size(0), "kv_lens must have an entry for each row of page_table");
+  MGFA_CHECK(cu_q.size(0) >= 1, "cu_seqlens_q must be [sequences + 1]");
+  const int64_t seqs = cu_q.size(0) - 1;
+  if (slots.has_value()) {
+    check_ints(*slots, page_table, 1, "slots");
+    MGFA_CHECK(slots->size(0) == seqs, "slots must have an entry for each sequence");
+  } else {
+    MGFA_CHECK(page_table.size(0) >= seqs, "page_table must have a row for each sequence");
+  }
+  const int64_t n = check_groups(groups, page_table, seqs);
+  c10::cuda::CUDAGuard guard(page_table.device());
+  torch::Tensor plan = torch::empty({n + 2 * seqs}, page_table.options());
+  PagedParams p;
+  p.status = status_ptr(status, page_table);
+  if (n == 0) return plan;
+  p.page_table = page_table.data_ptr<int>();
+  p.table_stride = page_table.stride(0);
+  p.kv_lens = kv_lens.data_ptr<int>();
+  p.slots = slots.has_value() ? slots->data_ptr<int>() : nullptr;
+  p.cu_q = cu_q.data_ptr<int>();
+  p.groups = groups.data_ptr<int>();
+  p.own = int(seqs);
+  p.seqs = int(seqs + n);
+  p.rows = int(page_table.size(0));
+  p.width = int(page_table.size(1));
+  p.page = int(page);
+  int* shared = plan.data_ptr<int>();
+  paged_plan_launch(p, shared, shared + n, shared + n + seqs, at::cuda::getCurrentCUDAStream());
+  return plan;
+}
+
 std::tuple<torch::Tensor, OptTensor> paged_attention(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
     torch::Tensor kv_lens, torch::Tensor cu_q, int64_t max_new, OptTensor slots, bool causal,
-    double scale, OptTensor out_in, bool want_lse, torch::Tensor status, int64_t wait_limit_ns) {
+    double scale, OptTensor out_in, bool want_lse, torch::Tensor status, int64_t wait_limit_ns,
+    OptTensor groups, OptTensor plan) {
   refuse_tangents("paged_attention", {q, k, v});
   check_rows16(q, 3, "q");
   check_rows16(k, 4, "k_pages");
@@ -144,6 +264,11 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   }
   MGFA_CHECK(page_table.size(1) * page < (int64_t(1) << 30), "page_table is too wide");
   MGFA_CHECK(max_new >= 0, "max_seqlen_q must not be negative");
+  const int64_t n_groups = groups.has_value() ? check_groups(*groups, k, seqs) : 0;
+  if (n_groups) {
+    check_ints(*plan, k, 1, "the plan");
+    MGFA_CHECK(plan->size(0) == n_groups + 2 * seqs, "the plan of the shared prefixes is of another batch");
+  }
   const float scale_log2 = float(scale * 1.4426950408889634);  // the kernels' own
   MGFA_CHECK(scale_log2 > 0.f && std::isfinite(scale_log2), "softmax_scale must be positive (in float32)");
   c10::cuda::CUDAGuard guard(q.device());
@@ -190,6 +315,10 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   const int sms = device_sm_count(q.get_device());
   // Up to 32 rows a key head pad to 16 or 32 on mma.sync; more fill 128-row tiles.
   const bool few = int64_t(p.max_new) * p.group <= 32;
+  if (n_groups) {
+    attend_shared(p, few, q, k, v, *groups, *plan, sms);
+    return {out, want_lse ? OptTensor(lse) : OptTensor()};
+  }
   int64_t units;  // at most
   if (few) {
     p.block_tokens = p.max_new;

@@ -22,6 +22,8 @@ apply_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight)
 PagedKVCache, paged_attention(q, k_pages, v_pages, page_table, kv_lens, ...)
     A paged cache of keys and values (reserve, write, append, fork, free, compact) and the
     attention of new tokens over it, from one token a sequence to long chunks.
+shared_prefix(page_table, kv_lens, cu_seqlens_q, cu_groups, page_size)
+    The plan with which that attention reads what forked sequences share once for all.
 token_logprobs(logits, targets, top=0)
     Log probabilities of given tokens and the entropy (both differentiable), and the
     likeliest alternatives.
@@ -37,7 +39,7 @@ from .parallel.health import PeerLostError, RingHealth  # noqa: F401
 from .ops.flash import KernelStatusError, flash_attn, flash_attn_bwd, flash_attn_fwd  # noqa: F401
 from .ops.logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from .ops.norm import rms_norm, rms_norm_fp8  # noqa: F401
-from .ops.paged import PagedKVCache, paged_attention  # noqa: F401
+from .ops.paged import PagedKVCache, SharedPrefix, paged_attention, shared_prefix  # noqa: F401
 from .ops.rotary import apply_norm_rotary, apply_rotary, rotary_frequencies  # noqa: F401
 from .ops.graphs import GraphedAttention  # noqa: F401
 from .models import RingAttentionBlock, RingTransformerLM, shard_targets  # noqa: F401

@@ -30,7 +30,7 @@ than 2^30 rows.
 from __future__ import annotations
 
 import math
-from typing import Optional, Sequence, Union
+from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -44,12 +44,50 @@ def _scale(head_dim: int, softmax_scale: Optional[float]) -> float:
     return softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
 
 
+class SharedPrefix(NamedTuple):
+    """What the sequences of a batch share (shared_prefix()): cu_groups, the groups; plan, int32,
+    the tokens that each group shares, then each sequence's, then its group."""
+    cu_groups: torch.Tensor
+    plan: torch.Tensor
+
+    @property
+    def lens(self) -> torch.Tensor:
+        """int32 [groups]: how many tokens each group shares."""
+        return self.plan[:self.cu_groups.shape[0] - 1]
+
+
+def _status_word(device, status: Optional[torch.Tensor]) -> torch.Tensor:
+    if status is not None:
+        return status
+    h = host_status(device)
+    h.poll()  # an error of an earlier call surfaces here
+    return h.word
+
+
+def shared_prefix(page_table: torch.Tensor, kv_lens: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                  cu_groups: torch.Tensor, page_size: int, slots: Optional[torch.Tensor] = None,
+                  status: Optional[torch.Tensor] = None) -> SharedPrefix:
+    """The plan with which paged_attention reads what sequences share once for all of them.
+
+    cu_groups int32 [groups + 1]: group g is the batch's sequences [cu_groups[g],
+    cu_groups[g + 1]), neighbours, as forks of one prompt. They share the leading pages that
+    the page table names alike for all of them, as far as these are full and hold none of
+    their new tokens; a sequence alone, or outside every group, shares nothing. The other
+    arguments are those of paged_attention, whose batch the plan is of: it holds until the
+    lengths or the page table change, hence for all layers of a step. Up to 4096 sequences
+    and groups. Everything stays on the device. cu_groups that fall or leave the batch are
+    reported as an error, and nothing is shared."""
+    plan = C().shared_prefix(page_table, kv_lens, cu_seqlens_q, cu_groups, page_size, slots,
+                             _status_word(page_table.device, status))
+    return SharedPrefix(cu_groups, plan)
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     page_table: torch.Tensor, kv_lens: torch.Tensor, cu_seqlens_q: torch.Tensor,
                     max_seqlen_q: int, slots: Optional[torch.Tensor] = None, causal: bool = True,
                     softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                     return_lse: bool = False, status: Optional[torch.Tensor] = None,
-                    wait_limit_ns: int = DEFAULT_WAIT_LIMIT_NS):
+                    wait_limit_ns: int = DEFAULT_WAIT_LIMIT_NS, shared: Optional[SharedPrefix] = None):
     """Attention of each sequence's new tokens over its paged keys and values.
 
     q [tokens, heads, D] (bfloat16 or float16, D = 64 or 128), the sequences' new tokens
@@ -59,7 +97,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     times). page_table int32 [rows, width] names each sequence's pages, kv_lens int32
     [rows] its tokens, the new ones included; `slots` int32 [sequences] gives the row of
     each sequence (default: row b). Up to 4096 sequences; the int32 tensors contiguous.
-    max_seqlen_q also decides between the kernels for few and for many rows.
+    max_seqlen_q also decides between the kernels for few and for many rows. shared: the
+    batch's shared_prefix(), with which keys and values that sequences share are read once.
 
     The new tokens are the sequence's last: token i of n sees keys [0, kv_len - n + i],
     or with causal=False all kv_len. A token that sees no key gets 0, and -inf for its
@@ -70,13 +109,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     written. Inference only: there is no gradient."""
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError("paged_attention has no gradient: call it under torch.no_grad()")
-    if status is None:
-        h = host_status(q.device)
-        h.poll()  # an error of an earlier call surfaces here
-        status = h.word
+    status = _status_word(q.device, status)
     o, lse = C().paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens_q,
                                  max_seqlen_q, slots, causal, _scale(q.shape[-1], softmax_scale),
-                                 out, return_lse, status, wait_limit_ns)
+                                 out, return_lse, status, wait_limit_ns, *(shared or (None, None)))
     return (o, lse) if return_lse else o
 
 
@@ -157,15 +193,24 @@ class PagedKVCache:
 
     def attend(self, layer: int, q: torch.Tensor, slots: Ints, cu_seqlens: Ints, max_seqlen_q: int,
                causal: bool = True, softmax_scale: Optional[float] = None,
-               out: Optional[torch.Tensor] = None, return_lse: bool = False):
-        """paged_attention of the batch's queries [tokens, heads, D] over a layer's cache."""
+               out: Optional[torch.Tensor] = None, return_lse: bool = False,
+               shared: Optional[SharedPrefix] = None):
+        """paged_attention of the batch's queries [tokens, heads, D] over a layer's cache;
+        shared: the batch's shared_prefix()."""
         if not 0 <= layer < len(self._layers):
             raise IndexError(f"layer {layer} is not one of the cache's {len(self._layers)}")
         k, v = self._layers[layer]
         return paged_attention(q, k, v, self.page_table, self.lens, self._ints(cu_seqlens),
                                max_seqlen_q, slots=self._ints(slots), causal=causal,
                                softmax_scale=softmax_scale, out=out, return_lse=return_lse,
-                               status=self._status.word)
+                               status=self._status.word, shared=shared)
+
+    def shared_prefix(self, slots: Ints, cu_seqlens: Ints, cu_groups: Ints) -> SharedPrefix:
+        """shared_prefix() of a batch that reserve() has made room for: cu_groups [groups + 1]
+        says which of its sequences, neighbours, were forked from one another. For attend()
+        in every layer of the step."""
+        return shared_prefix(self.page_table, self.lens, self._ints(cu_seqlens), self._ints(cu_groups),
+                             self.page_size, slots=self._ints(slots), status=self._status.word)
 
     def fork(self, src: Ints, dst: Ints, share: bool = True) -> None:
         """Sequence dst[i] becomes a copy of src[i]. Full pages are held by both, and the

@@ -67,6 +67,7 @@ if which in ("all", "cuda"):
                 "csrc/kernels/token_logprobs.cu",
                 "csrc/kernels/paged_decode.cu",
                 "csrc/kernels/paged_chunk.cu",
+                "csrc/kernels/paged_shared.cu",
                 "csrc/kernels/paged_cache.cu",
                 "csrc/comm/symmetric.cpp",
                 "csrc/comm/ring_engine.cpp",
