@@ -33,6 +33,13 @@ namespace mgfa {
 constexpr int kPagedMaxSeqs = 4096;
 constexpr int kPagedMaxGroup = 128;
 
+// Forms of the decode kernel that a launch may ask for; otherwise the rows of a unit decide.
+enum : int {
+  kPagedByRows = 0,
+  kPagedHeadsApart = 1,  // units of four key heads, up to 16 rows each
+  kPagedRowsApart = 2,   // units of up to 32 rows, which eight warps share
+};
+
 struct PagedParams {
   // problem
   const void* q = nullptr;      // [tokens, heads, head_dim], strides in elements
@@ -59,7 +66,8 @@ struct PagedParams {
   int units = 0;         // seqs * kv_heads * max_units
   int whole = 0;         // 1: the units are dealt out whole: no shares, no parts
   int grid = 0;          // CTAs
-  int unit_rows = 0;     // rows of a part in the workspace
+  int unit_rows = 0;     // rows of a part in the workspace (kPagedHeadsApart: of each of its heads)
+  int form = kPagedByRows;
   // workspace: parts [2 * grid][unit_rows][head_dim] and their (max, sum), log2 units; the
   // parts of share c are 2 c (a unit that an earlier share began) and 2 c + 1
   float* part_o = nullptr;
@@ -295,6 +303,10 @@ __device__ __forceinline__ int64_t paged_desc(const PagedParams& p, const PagedS
   return (at + s.q0 / p.block_tokens + unit) * p.kv_heads + hk;
 }
 
+// At the end of a launch that may have begun early: it ends behind the one before it, so that
+// what waits for this one sees the results of both.
+__device__ __forceinline__ void paged_behind() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct PagedShare {
   const PagedParams& p;
   const uint32_t* prefix;
@@ -450,10 +462,10 @@ cudaError_t paged_allow_smem(Fn fn, std::atomic<uint64_t>& done) {
 }
 
 // Few rows a key head (max_new * group <= 32).
-void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
-                         cudaStream_t stream);
-// More rows: tcgen05 tiles.
 // early: may begin while the launch before, which it does not need, still runs.
+void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
+                         cudaStream_t stream, bool early = false);
+// More rows: tcgen05 tiles.
 void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                         const PagedParams& p, cudaStream_t stream, bool early = false);
 // The most local memory a thread of its forms was compiled with, which has to be none.
@@ -463,9 +475,13 @@ void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
 // Sequences that share a prefix: `shared`, `first` and `member` ([own]: its group, or -1) from
 // the page table, for the groups of p. (Nothing but the arrays of the problem is read.)
 void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t stream);
-// Joins own and shared parts, behind the launch `a` that took the sequences' own keys and, with
-// groups of c.least_rows rows and more, `c`.
-void paged_shared_launch(const PagedParams& a, const PagedParams& c, bool two, const int* member,
-                         cudaStream_t stream);
+// Joins own and shared parts, behind the launches that left them.
+struct PagedSharedParams {
+  PagedParams own;          // of the sequences' own keys
+  PagedParams over[2];      // of the groups' prefixes, by their rows
+  int launches = 0;         // of over
+  const int* member = nullptr;  // [sequences] group, or -1
+};
+void paged_shared_launch(const PagedSharedParams& p, cudaStream_t stream);
 
 }  // namespace mgfa

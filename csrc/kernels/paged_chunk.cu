@@ -137,11 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.drain, 1);
     fence_mbar_init();
   }
-  // A launch that began early ends behind the one before it, so that what waits for this one
-  // sees the results of both.
-  auto behind = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   PagedWalk at;
-  if (!at.start<kThreads>(p, prefix, s.sums)) return behind();  // the whole CTA
+  if (!at.start<kThreads>(p, prefix, s.sums)) return paged_behind();  // the whole CTA
   if (warp == 0) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
@@ -531,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc<512>(tmem);
-  behind();
+  paged_behind();
 }
 
 template <int kD, bool kF16>

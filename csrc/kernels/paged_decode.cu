@@ -27,19 +27,33 @@ namespace {
 using namespace mgfa::dev;
 
 constexpr int kConsumers = 4;
-constexpr int kThreads = (kConsumers + 1) * 32;
-constexpr int kKeys = 64;
+constexpr int kKeys = 64;  // of a tile, or 16 of each of four heads
 
-template <int kD, int kMT>
+// How the consumer warps share a unit.
+enum : int {
+  kKeysOfOne = 0,  // four warps: 16 of a tile's 64 keys each, up to 16 rows
+  kKeysOfTwo = 1,  // the same with up to 32 rows a warp
+  kRowsApart = 2,  // eight warps: 16 keys and half of up to 32 rows each
+  kHeadsApart = 3, // four warps: 16 keys of four key heads, a head each, up to 16 rows
+};
+constexpr int kFourHeads = 4;
+
+template <int kD, int kForm>
 struct __align__(1024) DecodeSmem {
   static constexpr int kHalves = kD / 64;
-  static constexpr int kStages = kD == 64 ? 6 : (kMT == 1 ? 3 : 2);
+  static constexpr int kMT = kForm == kKeysOfTwo ? 2 : 1;        // blocks of 16 rows of a warp
+  static constexpr int kBlocks = kForm == kRowsApart ? 2 : 1;    // of a CTA's groups of four warps
+  static constexpr int kWarps = kConsumers * kBlocks;
+  static constexpr int kRows = 16 * kMT * kBlocks;
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kCtas = kBlocks == 1 ? 2 : 1;             // of an SM
+  static constexpr int kStages = (kD == 64 ? 6 : (kMT == 1 ? 3 : 2)) * kBlocks;
   uint16_t kv[kStages][2][kHalves][kKeys * 64];  // [stage][K, V][64 columns][key][column]
   union {  // the queries are last read before a unit's results are added
-    uint16_t q[16 * kMT][kD + 8];
-    float acc[16 * kMT][kD + 4];
+    uint16_t q[kRows][kD + 8];
+    float acc[kRows][kD + 4];
   };
-  float2 ml[kConsumers][16 * kMT];
+  float2 ml[kConsumers][kRows];
   uint64_t full[kStages], empty[kStages];
   uint32_t abort_flag, stop;
   uint32_t sums[kThreads / 32];
@@ -75,15 +89,20 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int kWarps>
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
-// kD head_dim, kF16 type, kMT blocks of 16 rows.
-template <int kD, bool kF16, int kMT>
-__global__ void __launch_bounds__(kThreads, 2)
+// kD head_dim, kF16 type. With kHeadsApart p.kv_heads counts fours of key heads, and p.tile
+// is 16.
+template <int kD, bool kF16, int kForm>
+__global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD, kForm>::kCtas)
     paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
-  using Smem = DecodeSmem<kD, kMT>;
-  constexpr int kStages = Smem::kStages, kHalves = kD / 64, kR = 16 * kMT;
+  using Smem = DecodeSmem<kD, kForm>;
+  constexpr int kStages = Smem::kStages, kHalves = kD / 64, kMT = Smem::kMT, kR = Smem::kRows;
+  constexpr int kWarps = Smem::kWarps, kThreads = Smem::kThreads;
+  constexpr bool kApart = kForm == kHeadsApart;
+  constexpr int kTileKeys = kApart ? 16 : kKeys;
   extern __shared__ uint8_t raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint32_t* prefix = reinterpret_cast<uint32_t*>(&s + 1);
@@ -94,21 +113,22 @@ __global__ void __launch_bounds__(kThreads, 2)
     s.abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], kConsumers);
+      mbar_init(&s.empty[i], kWarps);
     }
     fence_mbar_init();
   }
   PagedWalk at;
-  if (!at.start<kThreads>(p, prefix, s.sums)) return;  // the whole CTA
+  if (!at.start<kThreads>(p, prefix, s.sums)) return paged_behind();  // the whole CTA
   uint32_t it = 0;
 
-  if (warp == kConsumers) {
+  if (warp == kWarps) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&map_k);
       tma_prefetch_desc(&map_v);
     }
-    const int chunk = p.page < kKeys ? p.page : kKeys;  // keys of one box
+    const int chunk = p.page < kTileKeys ? p.page : kTileKeys;  // keys of one box
+    constexpr int kBoxHeads = kApart ? kFourHeads : 1;
     bool ok = true;
     do {
       const PagedUnit& u = at.u;
@@ -121,13 +141,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           break;
         }
         // boxes that hold a key below kv; the others' keys are masked
-        const int left = u.s.kv - t * kKeys;
-        const int boxes = left <= 0 ? 0 : ((left < kKeys ? left : kKeys) + chunk - 1) / chunk;
+        const int left = u.s.kv - t * kTileKeys;
+        const int boxes = left <= 0 ? 0 : ((left < kTileKeys ? left : kTileKeys) + chunk - 1) / chunk;
         if (lane == 0)
-          mbar_arrive_expect_tx(&s.full[st], uint32_t(boxes * chunk * kD * 2 * 2));
+          mbar_arrive_expect_tx(&s.full[st], uint32_t(boxes * chunk * kBoxHeads * kD * 2 * 2));
         __syncwarp();
         for (int c = lane; c < boxes; c += 32) {
-          const int key = t * kKeys + c * chunk;
+          const int key = t * kTileKeys + c * chunk;
           int page = __ldg(row + key / p.page);
           if (page < 0 || page >= p.pages) {
             record_error(p.status, kErrBadArgument, 62, 0);
@@ -136,9 +156,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int hf = 0; hf < kHalves; ++hf) {
             tma_load_4d(&s.kv[st][0][hf][c * chunk * 64], &map_k, &s.full[st], hf * 64,
-                        key % p.page, u.hk, page);
+                        key % p.page, u.hk * kBoxHeads, page);
             tma_load_4d(&s.kv[st][1][hf][c * chunk * 64], &map_v, &s.full[st], hf * 64,
-                        key % p.page, u.hk, page);
+                        key % p.page, u.hk * kBoxHeads, page);
           }
         }
         __syncwarp();
@@ -150,15 +170,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     AbortState drain{&never, nullptr, p.wait_limit_ns};
     for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
       mbar_wait(&s.full[i % kStages], (i / kStages) & 1, drain, 0);
-    return;
+    return paged_behind();
   }
 
   // -------------------------------------------------------------- consumers
   const int mi = lane >> 3, lr = lane & 7;  // matrix and row of this lane's ldmatrix address
+  const uint32_t quarter = warp % kConsumers;  // of a tile's 64 rows of K and V
+  const int block = kForm == kRowsApart ? int(warp / kConsumers) * 16 : 0;  // the warp's first row of the unit's
   // K: matrices (keys 0-7, 8 columns), (keys 0-7, next 8), (keys 8-15, ..) twice
-  const uint32_t k_row = warp * 16 + (mi >> 1) * 8 + lr, k_col = (mi & 1) * 8;
+  const uint32_t k_row = quarter * 16 + (mi >> 1) * 8 + lr, k_col = (mi & 1) * 8;
   // V, transposed: (keys 0-7), (keys 8-15), then the next 8 columns
-  const uint32_t v_row = warp * 16 + (mi & 1) * 8 + lr, v_col = (mi >> 1) * 8;
+  const uint32_t v_row = quarter * 16 + (mi & 1) * 8 + lr, v_col = (mi >> 1) * 8;
   const uint32_t kv_base = smem_u32(&s.kv[0][0][0][0]);
   constexpr uint32_t kHalfBytes = kKeys * 128;
   // A wait that ran out must not leave the other warps in a barrier: such a warp goes on
@@ -166,25 +188,43 @@ __global__ void __launch_bounds__(kThreads, 2)
   bool ok = true;
   do {
     const PagedUnit& u = at.u;
-    // the sequence's or, of a group (PagedParams::groups), the unit's
-    const int tok0 = u.unit * p.block_tokens, left = u.s.n - tok0;
-    const int rows = (left < p.block_tokens ? left : p.block_tokens) * p.group, q0 = u.s.q0 + tok0;
-    // queries: row r = token r / group, head r % group
-    for (int i = threadIdx.x; i < kR * (kD / 8); i += kConsumers * 32) {
-      const int r = i / (kD / 8), c = (i % (kD / 8)) * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows)
-        v = *reinterpret_cast<const uint4*>(
-            static_cast<const uint16_t*>(p.q) + int64_t(q0 + r / p.group) * p.q_stride_t +
-            int64_t(u.hk * p.group + r % p.group) * p.q_stride_h + c);
-      *reinterpret_cast<uint4*>(&s.q[r][c]) = v;
-    }
-    consumers_sync();
-    const uint32_t q_addr = smem_u32(&s.q[(mi & 1) * 8 + lr][(mi >> 1) * 8]);
+    // the sequence's or, of a group (PagedParams::groups, kRowsApart), the unit's
+    const int tok0 = kForm == kRowsApart ? u.unit * p.block_tokens : 0, left = u.s.n - tok0;
+    const int rows = (kForm == kRowsApart && left > p.block_tokens ? p.block_tokens : left) * p.group;
+    const int q0 = u.s.q0 + tok0;
+    // queries: row r = token r / group, head r % group of the key head's
+    const int hk = kApart ? u.hk * kFourHeads + int(quarter) : u.hk;
+    auto query = [&](int r) {
+      return static_cast<const uint16_t*>(p.q) + int64_t(q0 + r / p.group) * p.q_stride_t +
+             int64_t(hk * p.group + r % p.group) * p.q_stride_h;
+    };
     uint32_t qf[kMT == 1 ? kD / 16 : 1][4];
-    if constexpr (kMT == 1) {
+    uint32_t q_addr = 0;
+    if constexpr (kApart) {
+      // straight to where mma.sync wants them: nothing here waits for another warp
 #pragma unroll
-      for (int ks = 0; ks < kD / 16; ++ks) ldsm4(q_addr + ks * 32, qf[ks]);
+      for (int h = 0; h < 2; ++h) {
+        const int r = h * 8 + int(lane >> 2);
+        const uint16_t* at_row = r < rows ? query(r) : nullptr;
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            qf[ks][c * 2 + h] = at_row ? __ldg(reinterpret_cast<const uint32_t*>(at_row + ks * 16 + c * 8 + (lane & 3) * 2)) : 0u;
+      }
+    } else {
+      for (int i = threadIdx.x; i < kR * (kD / 8); i += kWarps * 32) {
+        const int r = i / (kD / 8), c = (i % (kD / 8)) * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows) v = *reinterpret_cast<const uint4*>(query(r) + c);
+        *reinterpret_cast<uint4*>(&s.q[r][c]) = v;
+      }
+      consumers_sync<kWarps>();
+      q_addr = smem_u32(&s.q[block + (mi & 1) * 8 + lr][(mi >> 1) * 8]);
+      if constexpr (kMT == 1) {
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks) ldsm4(q_addr + ks * 32, qf[ks]);
+      }
     }
     // keys seen by this thread's rows (lane / 4 and that + 8 of each block)
     int lim[kMT][2];
@@ -192,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int m = 0; m < kMT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = m * 16 + h * 8 + (lane >> 2);
+        const int r = block + m * 16 + h * 8 + (lane >> 2);
         int l = u.s.base + tok0 + r / p.group + 1;
         l = l < u.s.kv ? l : u.s.kv;
         lim[m][h] = r < rows ? l : 0;
@@ -234,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
       }
-      const int key0 = t * kKeys + warp * 16;
+      const int key0 = t * kTileKeys + (kApart ? 0 : int(quarter) * 16);
       const bool whole = key0 + 16 <= full_keys && key0 + 16 <= u.s.kv;
       uint32_t pf[kMT][4];
 #pragma unroll
@@ -309,6 +349,40 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[st]);
     }
+    if constexpr (kApart) {
+      const bool done = at.complete();
+      const int64_t slot = at.part();
+      // each warp has whole rows
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float total = sum[0][h];
+        total += __shfl_xor_sync(0xffffffffu, total, 1);
+        total += __shfl_xor_sync(0xffffffffu, total, 2);
+        const int r = h * 8 + int(lane >> 2);
+        if (r >= rows || !ok) continue;
+        const int tok = q0 + r / p.group, head = hk * p.group + r % p.group, c0 = int(lane & 3) * 2;
+        const float top = mx[0][h], base = top == -INFINITY ? 0.f : top;
+        if (done && !p.acc_o) {
+          const float inv = total == 0.f ? 0.f : 1.f / total;  // 0: no visible key
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.o_stride_t + int64_t(head) * p.o_stride_h + c0;
+#pragma unroll
+          for (int n = 0; n < kD / 8; ++n)
+            *reinterpret_cast<uint32_t*>(dst + n * 8) = pack16<kF16>(o[0][n][2 * h] * inv, o[0][n][2 * h + 1] * inv);
+          if (p.lse && c0 == 0)
+            p.lse[int64_t(head) * p.tokens + tok] =
+                total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
+        } else {
+          const int64_t to = done ? at.acc_row(p, tok, head) : (slot * kFourHeads + quarter) * p.unit_rows + r;
+          float* dst = (done ? p.acc_o : p.part_o) + to * kD + c0;
+#pragma unroll
+          for (int n = 0; n < kD / 8; ++n)
+            *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[0][n][2 * h], o[0][n][2 * h + 1]);
+          if (c0 == 0) (done ? p.acc_ml : p.part_ml)[to] = make_float2(top, total);
+        }
+      }
+      if (!ok) break;
+      continue;
+    }
     // ---- the four warps' results, in the warps' order
 #pragma unroll
     for (int m = 0; m < kMT; ++m)
@@ -317,27 +391,27 @@ __global__ void __launch_bounds__(kThreads, 2)
         sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
         sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
         if ((lane & 3) == 0)
-          s.ml[warp][m * 16 + h * 8 + (lane >> 2)] = make_float2(mx[m][h], sum[m][h]);
+          s.ml[quarter][block + m * 16 + h * 8 + (lane >> 2)] = make_float2(mx[m][h], sum[m][h]);
       }
-    consumers_sync();
+    consumers_sync<kWarps>();
     float weight[kMT][2];
 #pragma unroll
     for (int m = 0; m < kMT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = m * 16 + h * 8 + (lane >> 2);
+        const int r = block + m * 16 + h * 8 + (lane >> 2);
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kConsumers; ++i) top = fmaxf(top, s.ml[i][r].x);
         weight[m][h] = ex2_approx(mx[m][h] - (top == -INFINITY ? 0.f : top));
       }
     for (int i = 0; i < kConsumers; ++i) {
-      if (int(warp) == i) {
+      if (int(quarter) == i) {
 #pragma unroll
         for (int m = 0; m < kMT; ++m)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int r = m * 16 + h * 8 + (lane >> 2);
+            const int r = block + m * 16 + h * 8 + (lane >> 2);
 #pragma unroll
             for (int n = 0; n < kD / 8; ++n) {
               float2* at = reinterpret_cast<float2*>(&s.acc[r][n * 8 + (lane & 3) * 2]);
@@ -350,11 +424,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
       }
-      consumers_sync();
+      consumers_sync<kWarps>();
     }
     const bool done = at.complete();
     const int64_t slot = at.part();
-    for (int i = threadIdx.x; i < kR * (kD / 8); i += kConsumers * 32) {
+    for (int i = threadIdx.x; i < kR * (kD / 8); i += kWarps * 32) {
       const int r = i / (kD / 8), c = (i % (kD / 8)) * 8;
       if (r >= rows || *ab.flag) continue;
       float top = -INFINITY, total = 0.f;
@@ -383,8 +457,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     if (threadIdx.x == 0) s.stop = *ab.flag;
-    consumers_sync();  // q, acc and ml are free again
-  } while (!s.stop && at.next(p, prefix));
+    consumers_sync<kWarps>();  // q, acc and ml are free again
+  } while (!(kApart ? *ab.flag : s.stop) && at.next(p, prefix));
+  paged_behind();
 }
 
 // ---------------------------------------------------------------------- joining the parts
@@ -473,28 +548,44 @@ void cuda_ok(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
 }
 
-template <int kD, bool kF16, int kMT>
-void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s) {
-  const int smem = int(sizeof(DecodeSmem<kD, kMT>)) + 1024 + 4 * (p.seqs + 1);
-  auto fn = paged_decode_kernel<kD, kF16, kMT>;
+template <int kD, bool kF16, int kForm>
+void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s, bool early) {
+  using Smem = DecodeSmem<kD, kForm>;
+  auto fn = paged_decode_kernel<kD, kF16, kForm>;
   static std::atomic<uint64_t> allowed{0};
   cuda_ok(paged_allow_smem(fn, allowed));
-  fn<<<p.grid, kThreads, smem, s>>>(mk, mv, p);
-  cuda_ok(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(Smem::kThreads);
+  cfg.dynamicSmemBytes = int(sizeof(Smem)) + 1024 + 4 * (p.seqs + 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  cuda_ok(cudaLaunchKernelEx(&cfg, fn, mk, mv, p));
 }
 
 template <int kD, bool kF16>
-void decode_rows(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s) {
-  if (p.unit_rows <= 16) decode_launch<kD, kF16, 1>(mk, mv, p, s);
-  else decode_launch<kD, kF16, 2>(mk, mv, p, s);
+void decode_rows(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s, bool early) {
+  switch (p.form) {
+    case kPagedHeadsApart: return decode_launch<kD, kF16, kHeadsApart>(mk, mv, p, s, early);
+    case kPagedRowsApart: return decode_launch<kD, kF16, kRowsApart>(mk, mv, p, s, early);
+    default: break;
+  }
+  if (p.unit_rows <= 16) decode_launch<kD, kF16, kKeysOfOne>(mk, mv, p, s, early);
+  else decode_launch<kD, kF16, kKeysOfTwo>(mk, mv, p, s, early);
 }
 
 }  // namespace
 
 void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
-                         cudaStream_t s) {
-  if (p.head_dim == 64) p.fp16 ? decode_rows<64, true>(mk, mv, p, s) : decode_rows<64, false>(mk, mv, p, s);
-  else p.fp16 ? decode_rows<128, true>(mk, mv, p, s) : decode_rows<128, false>(mk, mv, p, s);
+                         cudaStream_t s, bool early) {
+  if (p.head_dim == 64)
+    p.fp16 ? decode_rows<64, true>(mk, mv, p, s, early) : decode_rows<64, false>(mk, mv, p, s, early);
+  else
+    p.fp16 ? decode_rows<128, true>(mk, mv, p, s, early) : decode_rows<128, false>(mk, mv, p, s, early);
 }
 
 template <int kD, bool kF16>

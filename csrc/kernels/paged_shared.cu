@@ -28,7 +28,8 @@ namespace cg = cooperative_groups;
 
 // ---------------------------------------------------------------------- what is shared
 constexpr int kPlanThreads = 512;
-constexpr int kPlanCtas = 8;  // of a group, a cluster
+constexpr int kPlanCtas = 8;   // of a group, a cluster
+constexpr int kPlanLoads = 8;  // of each table that a lane has under way
 
 // shared[g]: the leading pages that all of the group's sequences name alike, as far as these
 // are full and hold none of their new tokens; 0 for a sequence alone, which reads them once
@@ -59,10 +60,10 @@ __global__ void __launch_bounds__(kPlanThreads)
         pages = int(std::max<int64_t>(kv - n, 0) / p.page);
         const int* mine = p.page_table + int64_t(row) * p.table_stride;
         const int* theirs = p.page_table + int64_t(lead) * p.table_stride;
-        for (int j0 = 0; j0 < pages; j0 += 32 * 4) {
-          bool differ[4];
+        for (int j0 = 0; j0 < pages; j0 += 32 * kPlanLoads) {
+          bool differ[kPlanLoads];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < kPlanLoads; ++k) {
             const int j = j0 + k * 32 + lane;
             differ[k] = false;
             if (j < pages) {
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(kPlanThreads)
             }
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < kPlanLoads; ++k) {
             const uint32_t at = __ballot_sync(0xffffffffu, differ[k]);
             if (at) pages = std::min(pages, j0 + k * 32 + __ffs(at) - 1);
           }
@@ -105,84 +106,81 @@ __global__ void __launch_bounds__(kPlanThreads)
 // ---------------------------------------------------------------------- the join
 constexpr int kJoinWarps = 16;
 
-// A row's parts of one kind: whole, or those of shares [c, last].
+// A row's parts of one kind: whole, or those of shares [c, c + n).
 struct RowParts {
   const float* o;
   const float2* ml;
-  int64_t row;   // of acc_o, or r of the unit
-  int c, n;
-  int unit_rows;  // 0: whole
-  __device__ __forceinline__ int64_t at(int i) const {
-    return unit_rows ? (2 * int64_t(c + i) + (i == 0 ? 1 : 0)) * unit_rows + row : row;
-  }
+  int64_t row, first, step;  // part i: at `row` (n == 1), or first + i * step
+  int n;
+  __device__ __forceinline__ int64_t at(int i) const { return i ? first + i * step : row; }
 };
 
-__device__ __forceinline__ RowParts row_parts(const PagedParams& p, const PagedSeq& s, int b, int hk, int i, int head) {
-  const int unit = i / p.block_tokens;
-  const int2 d = p.desc[paged_desc(p, s, b, unit, hk)];
+// Of row (i, head) of sequence or group b, whose keys launch p took; heads: key heads of a unit.
+__device__ __forceinline__ RowParts row_parts(const PagedParams& p, const PagedSeq& s, int b, int i, int head) {
+  const int heads = p.form == kPagedHeadsApart ? 4 : 1, hk = head / p.group;
+  const int unit = i / p.block_tokens, tok = i - unit * p.block_tokens;
+  const int2 d = p.desc[paged_desc(p, s, b, unit, hk / heads)];
   RowParts r;
-  r.c = d.x;
+  r.first = r.step = 0;
   if (d.x < 0) {
     r.o = p.acc_o;
     r.ml = p.acc_ml;
     r.row = ((b < p.own ? 0 : int64_t(p.tokens)) + s.q0 + i) * p.heads + head;
     r.n = 1;
-    r.unit_rows = 0;
   } else {
+    // share c's parts are 2 c and 2 c + 1, which is the one of the unit that it begins
+    const int64_t at = int64_t(hk % heads) * p.unit_rows + tok * p.group + head - hk * p.group;
     r.o = p.part_o;
     r.ml = p.part_ml;
-    r.row = (i - unit * p.block_tokens) * p.group + head - hk * p.group;
+    r.step = 2 * int64_t(heads) * p.unit_rows;
+    r.first = d.x * r.step + at;
+    r.row = r.first + r.step / 2;
     // (of a unit that a wait which ran out has left alone: none)
     r.n = d.y >= d.x && d.y < p.grid ? d.y - d.x + 1 : 0;
-    r.unit_rows = p.unit_rows;
   }
   return r;
 }
 
-// CTA (b * kv_heads + hk, y): every gridDim.y-th block of rows of sequence b and key head hk.
+// CTA (b, y): every gridDim.y-th block of rows of sequence b, a row for each new token and head.
 // kSplit warps share a row, as in paged_merge_kernel.
 template <int kD, bool kF16, int kSplit>
-__global__ void __launch_bounds__(kJoinWarps * 32)
-    paged_shared_kernel(const PagedParams a, const PagedParams c, int two, const int* member) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_shared_kernel(const __grid_constant__ PagedSharedParams p) {
   constexpr int kE = kD / 32, kRows = kJoinWarps / kSplit;
   __shared__ float sh[kSplit > 1 ? kJoinWarps : 1][kD];
-  const int b = blockIdx.x / a.kv_heads, hk = blockIdx.x - b * a.kv_heads;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
+  const PagedParams& a = p.own;
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
   const PagedSeq own = paged_seq(a, b);
-  const int rows = own.n * a.group;  // (at most max_new * group)
+  const int64_t rows = int64_t(own.n) * a.heads;
   // the group, and which launch took it
   PagedSeq over;
   over.n = 0;
-  bool second = false;
-  int g = -1;
+  int taken = 0, g = -1;
   if (own.skip > 0) {
-    g = member[b];
+    g = p.member[b];
     if (g >= 0 && g < a.seqs - a.own) {
-      over = paged_group(a, g);
-      if (over.n == 0 && two) {
-        over = paged_group(c, g);
-        second = true;
+      for (; taken < p.launches; ++taken) {
+        over = paged_group(p.over[taken], g);
+        if (over.n > 0) break;
       }
       const bool inside = own.q0 >= over.q0 && own.q0 + own.n <= over.q0 + over.n;
       if (!inside || over.kv != own.skip * a.page) over.n = 0;
     }
-    if (over.n == 0 && blockIdx.y == 0 && hk == 0 && threadIdx.x == 0)
+    if (over.n == 0 && blockIdx.y == 0 && threadIdx.x == 0)
       record_error(a.status, kErrBadArgument, 69, 0);  // first[] and the groups do not fit
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
-    const int r = r0 + warp / kSplit;
+  for (int64_t r0 = int64_t(blockIdx.y) * kRows; r0 < rows; r0 += int64_t(gridDim.y) * kRows) {
+    const int64_t r = r0 + warp / kSplit;
     const bool live = r < rows;
-    const int i = live ? r / a.group : 0, head = hk * a.group + (live ? r - i * a.group : 0);
+    const int i = live ? int(r / a.heads) : 0, head = live ? int(r - int64_t(i) * a.heads) : 0;
     float top = -INFINITY, total = 0.f, acc[kE];
 #pragma unroll
     for (int e = 0; e < kE; ++e) acc[e] = 0.f;
     if (live) {
       RowParts side[2];
-      side[0] = row_parts(a, own, b, hk, i, head);
+      side[0] = row_parts(a, own, b, i, head);
       side[1].n = 0;
-      if (over.n > 0)
-        side[1] = row_parts(second ? c : a, over, a.own + g, hk, own.q0 + i - over.q0, head);
+      if (over.n > 0) side[1] = row_parts(p.over[taken], over, a.own + g, own.q0 + i - over.q0, head);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         for (int j = lane; j < side[k].n; j += 32) top = fmaxf(top, side[k].ml[side[k].at(j)].x);
@@ -251,13 +249,13 @@ void cuda_ok(cudaError_t e) {
 }
 
 template <int kD, bool kF16>
-void join_launch(const PagedParams& a, const PagedParams& c, bool two, const int* member, cudaStream_t s) {
-  // Few rows have many parts each, many rows few.
-  const int64_t rows = int64_t(a.max_new) * a.group;
-  const bool few = int64_t(a.own) * rows * a.kv_heads <= 1024;
+void join_launch(const PagedSharedParams& p, cudaStream_t s) {
+  // Few rows may have many parts each, many rows have few.
+  const int64_t rows = int64_t(p.own.max_new) * p.own.heads;
+  const bool few = int64_t(p.own.own) * rows <= 1024;
   const int per = few ? kJoinWarps / 4 : kJoinWarps;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.own * a.kv_heads, unsigned(std::min<int64_t>((rows + per - 1) / per, 64)));
+  cfg.gridDim = dim3(p.own.own, unsigned(std::min<int64_t>((rows + per - 1) / per, 256)));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -265,8 +263,7 @@ void join_launch(const PagedParams& a, const PagedParams& c, bool two, const int
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cuda_ok(cudaLaunchKernelEx(&cfg, few ? paged_shared_kernel<kD, kF16, 4> : paged_shared_kernel<kD, kF16, 1>, a, c,
-                             int(two), member));
+  cuda_ok(cudaLaunchKernelEx(&cfg, few ? paged_shared_kernel<kD, kF16, 4> : paged_shared_kernel<kD, kF16, 1>, p));
 }
 
 }  // namespace
@@ -285,12 +282,9 @@ void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* membe
   cuda_ok(cudaLaunchKernelEx(&cfg, paged_plan_kernel, p, shared, first, member));
 }
 
-void paged_shared_launch(const PagedParams& a, const PagedParams& c, bool two, const int* member,
-                         cudaStream_t s) {
-  if (a.head_dim == 64)
-    a.fp16 ? join_launch<64, true>(a, c, two, member, s) : join_launch<64, false>(a, c, two, member, s);
-  else
-    a.fp16 ? join_launch<128, true>(a, c, two, member, s) : join_launch<128, false>(a, c, two, member, s);
+void paged_shared_launch(const PagedSharedParams& p, cudaStream_t s) {
+  if (p.own.head_dim == 64) p.own.fp16 ? join_launch<64, true>(p, s) : join_launch<64, false>(p, s);
+  else p.own.fp16 ? join_launch<128, true>(p, s) : join_launch<128, false>(p, s);
 }
 
 }  // namespace mgfa

@@ -119,40 +119,41 @@ int64_t check_groups(const torch::Tensor& groups, const torch::Tensor& like, int
   return n;
 }
 
-// A group's rows a key head up to which its prefix goes to the decode kernel, in units of 16
-// or 32 rows that each read it (all but the first from L2); above, to 128-row tiles.
-constexpr int64_t kGroupFewRows = 64;
+// A group's rows a key head up to which its prefix goes to the decode kernel (32 of its rows
+// read it at once); above, to 128-row tiles.
+constexpr int64_t kGroupFewRows = 32;
 
 // The launches for sequences that share prefixes (paged_shared.cu).
-void attend_shared(PagedParams p, bool few, const torch::Tensor& q, const torch::Tensor& k,
+void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q, const torch::Tensor& k,
                    const torch::Tensor& v, const torch::Tensor& groups, const torch::Tensor& plan, int sms) {
-  const int64_t T = p.tokens, Hk = p.kv_heads, D = p.head_dim, n_groups = groups.size(0) - 1;
+  const int64_t T = problem.tokens, D = problem.head_dim, n_groups = groups.size(0) - 1;
+  const auto f32 = q.options().dtype(at::kFloat);
+  PagedSharedParams j;
+  PagedParams& p = j.own;
+  p = problem;
   p.own = p.seqs;
   p.seqs += int(n_groups);
   p.groups = groups.data_ptr<int>();
   p.shared = plan.data_ptr<int>();
   p.first = p.shared + n_groups;
-  const int* member = p.first + p.own;
-  const auto f32 = q.options().dtype(at::kFloat);
-  // one of these each for what is a sequence's own and what its group shares
-  torch::Tensor acc = torch::empty({2 * T * p.heads * (D + 2)}, f32), work[2];
+  p.most_rows = -1;  // no groups
+  j.member = p.first + p.own;
+  // rows of whole units, of what is a sequence's own and of what its group shares
+  torch::Tensor acc = torch::empty({2 * T * p.heads * (D + 2)}, f32), work[3];
   p.acc_o = acc.data_ptr<float>();
   p.acc_ml = reinterpret_cast<float2*>(p.acc_o + 2 * T * p.heads * D);
-  PagedParams c = p;
-  // with few rows a sequence the groups' sizes decide, of which the host knows the bound
-  const bool two = few && T * p.group > kGroupFewRows;
-  p.most_rows = two ? kGroupFewRows : INT64_MAX;
-  c.least_rows = kGroupFewRows + 1;
-  c.most_rows = INT64_MAX;
-  c.no_own = 1;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  for (int i = 0; i < (two ? 2 : 1); ++i) {
-    PagedParams& l = i ? c : p;
-    const bool decode = few && i == 0;
+  int launched = 0;
+  auto launch = [&](PagedParams& l, bool decode, int64_t units) {
+    uint32_t heads = 1;
     if (decode) {
-      l.block_tokens = std::max(l.max_new, (l.max_new * l.group <= 16 ? 16 : 32) / l.group);
       l.tile = 64;
-      l.grid = 2 * sms;
+      l.grid = l.form == kPagedRowsApart ? sms : 2 * sms;
+      if (l.form == kPagedHeadsApart) {
+        heads = 4;
+        l.tile = 16;
+        l.kv_heads /= 4;
+      }
     } else {
       l.block_tokens = 2 * std::max(1, 128 / l.group);
       l.tile = 128;
@@ -161,26 +162,50 @@ void attend_shared(PagedParams p, bool few, const torch::Tensor& q, const torch:
     }
     l.unit_rows = l.block_tokens * l.group;
     l.min_share = 2;
-    const int64_t units = (T / l.block_tokens + n_groups + (i ? 0 : T / l.block_tokens + l.own)) * Hk;
+    units = (units + T / l.block_tokens) * l.kv_heads;
     const int64_t tiles = std::max<int64_t>(1, (int64_t(l.width) * l.page + l.tile - 1) / l.tile);
     l.grid = int(std::min<int64_t>(l.grid, (units * tiles + l.min_share - 1) / l.min_share));
-    const int64_t rows = 2 * int64_t(l.grid) * l.unit_rows;
-    const int64_t descs = (paged_desc_rows(l, l.own) + paged_desc_rows(l, int(n_groups))) * Hk;
-    work[i] = torch::empty({rows * (D + 2) + 2 * descs}, f32);
-    l.part_o = work[i].data_ptr<float>();
+    const int64_t rows = 2 * int64_t(l.grid) * l.unit_rows * heads;
+    const int64_t descs = (paged_desc_rows(l, l.own) + paged_desc_rows(l, int(n_groups))) * l.kv_heads;
+    work[launched] = torch::empty({rows * (D + 2) + 2 * descs}, f32);
+    l.part_o = work[launched].data_ptr<float>();
     l.part_ml = reinterpret_cast<float2*>(l.part_o + rows * D);
     l.desc = reinterpret_cast<int2*>(l.part_ml + rows);
     const uint32_t chunk = uint32_t(std::min<int64_t>(l.page, l.tile));
-    const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, 1, 1});
-    const CUtensorMap mv = map16(v, {3, 1, 2, 0}, {64, chunk, 1, 1});
+    const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, heads, 1});
+    const CUtensorMap mv = map16(v, {3, 1, 2, 0}, {64, chunk, heads, 1});
     if (decode) {
-      paged_decode_launch(mk, mv, l, stream);
+      paged_decode_launch(mk, mv, l, stream, launched > 0);
     } else {
       const CUtensorMap mq = map16(q, {2, 1, 0, -1}, {64, uint32_t(l.group), uint32_t(l.block_tokens / 2), 1});
-      paged_chunk_launch(mq, mk, mv, l, stream, i == 1);
+      paged_chunk_launch(mq, mk, mv, l, stream, launched > 0);
     }
+    ++launched;
+  };
+  // The groups, by their rows, of which the host knows the bounds; the longest work, on 128-row
+  // tiles, first.
+  if (T * p.group > kGroupFewRows) {
+    PagedParams& l = j.over[j.launches++] = p;
+    l.no_own = 1;
+    l.least_rows = kGroupFewRows + 1;
+    l.most_rows = INT64_MAX;
+    launch(l, false, n_groups);
   }
-  paged_shared_launch(p, c, two, member, stream);
+  if (p.group <= kGroupFewRows) {
+    PagedParams& l = j.over[j.launches++] = p;
+    l.no_own = 1;
+    l.least_rows = 0;
+    l.most_rows = kGroupFewRows;
+    l.form = kPagedRowsApart;
+    l.block_tokens = int(kGroupFewRows) / l.group;
+    launch(l, true, n_groups);
+  }
+  if (few) {
+    p.block_tokens = p.max_new;
+    if (p.max_new * p.group <= 16 && p.kv_heads % 4 == 0) p.form = kPagedHeadsApart;
+  }
+  launch(p, few, p.own);
+  paged_shared_launch(j, stream);
 }
 
 }  // namespace
