@@ -12,9 +12,12 @@
 // by shuffles, through shared memory and, where few rows share the SMs, across the CTAs of
 // a cluster. Exponents are of base 2: sums hold W = sum (x - m) log2(e) e^(x - m).
 //
-// The alternatives are kept by each warp, one a lane, as 64-bit keys that order by value
-// and then by lower index, so that any order of work gives the same ones. A NaN counts as
-// the largest value; it makes its row's sums NaN.
+// The alternatives are 64-bit keys that order by value and then by lower index, so that any
+// order of work gives the same ones. Of a segment's threads, `top` have a largest key that is
+// not below the top-th largest of these; so none of the segment's alternatives is below it,
+// and few other elements are above: these are gathered in shared memory and ranked by
+// counting, together with those of the segments before. A NaN counts as the largest value;
+// it makes its row's sums NaN.
 #include "token_logprobs.cuh"
 
 #include <cooperative_groups.h>
@@ -79,6 +82,22 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, int index) {
   return uint64_t(order) << 32 | uint32_t(~index);
 }
 
+constexpr int kGather = 256;  // keys of a segment that are gathered at once
+
+// What the threads that share a row (a CTA, or a warp) need for its alternatives.
+struct Gather {
+  uint64_t keys[kGather + 32];  // lanes' largest, then candidates
+  uint64_t list[32];            // the alternatives so far, the largest first; 0: none
+  uint64_t floor;
+  int count;
+};
+
+template <int kT>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (kT == 32) __syncwarp();
+  else __syncthreads();
+}
+
 // The largest of the warp's keys.
 __device__ __forceinline__ uint64_t warp_top(uint64_t key) {
   const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(key >> 32));
@@ -105,6 +124,17 @@ struct Logits {
     vecs = int((int64_t(head) + n + V - 1) / V);
   }
   __device__ __forceinline__ bool inside(int64_t v) const { return v * V >= head && (v + 1) * V <= int64_t(head) + vocab; }
+  // The largest element, NaN where one is: 16-bit ones in pairs as they lie.
+  static __device__ __forceinline__ float largest(const Vec& a) {
+    if constexpr (sizeof(E) == 4) {
+      return max_nan(max_nan(a.e[0], a.e[1]), max_nan(a.e[2], a.e[3]));
+    } else {
+      using E2 = std::conditional_t<std::is_same_v<E, __half>, __half2, __nv_bfloat162>;
+      auto pair = [&](int k) { return *reinterpret_cast<const E2*>(&a.w[k]); };
+      const E2 m = __hmax2_nan(__hmax2_nan(pair(0), pair(1)), __hmax2_nan(pair(2), pair(3)));
+      return max_nan(to_f(m.x), to_f(m.y));
+    }
+  }
   // -inf outside the row, whose first and last elements are read by themselves
   __device__ __forceinline__ void load(int64_t v, Vec& to) const {
     if (inside(v)) {
@@ -159,6 +189,125 @@ __device__ __forceinline__ void put_top(const LogprobParams& p, int64_t row, int
   p.top_indices[row * p.top + rank] = int64_t(uint32_t(~uint32_t(key)));
 }
 
+// Adds a segment's elements to the alternatives of the threads that share the row: `at` are a
+// thread's vectors, n of them in use, `top` its largest element.
+template <class E, int kWarps>
+__device__ __forceinline__ void add_segment(const Logits<E>& x, const typename Logits<E>::Vec (&at)[kVecs], int64_t first,
+                                            int n, float top, int want, Gather& g) {
+  constexpr int V = Logits<E>::V, kT = kWarps * 32;
+  const int lane = threadIdx.x & 31, warp = kWarps == 1 ? 0 : int(threadIdx.x) >> 5, tid = warp * 32 + lane;
+  using L = Logits<E>;
+  using Vec = typename L::Vec;
+  // calls take(key) for the elements of a vector of the thread
+  auto each = [&](const Vec& v, int i, auto take) {
+    const int64_t c0 = (first + i * kT + tid) * V - x.head;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (c0 + j >= 0 && c0 + j < x.vocab) take(key_of(order_of(to_f(v.e[j])), int(c0) + j));
+  };
+  const bool any = first + tid < x.vecs;  // (a vector may hold nothing of the row but at its ends)
+  uint32_t order = any ? order_of(top) : 0;
+  // A bound that is quick to have: in each warp, a want / kWarps-th of the threads is not below.
+  uint32_t bound = 0;
+  if constexpr (kWarps > 1) {
+    __shared__ uint32_t bounds[kWarps];
+    uint32_t left = order;
+    for (int j = (want + kWarps - 1) / kWarps; j > 0; --j) {
+      bound = __reduce_max_sync(0xffffffffu, left);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, left == bound)) - 1) left = 0;
+    }
+    if (lane == 0) bounds[warp] = bound;
+    if (tid == 0) g.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kWarps; ++j) bound = bounds[j] < bound ? bounds[j] : bound;
+  } else {
+    if (lane == 0) g.count = 0;
+    __syncwarp();
+  }
+  // The want-th largest of the threads' largest keys.
+  uint64_t mine = 0;
+  const bool offers = any && order >= bound;
+  if (offers) {
+    // it is in the first vector whose largest element it is
+    Vec in = at[0];
+    int which = 0;
+#pragma unroll
+    for (int i = kVecs - 1; i > 0; --i)
+      if (i < n && order_of(L::largest(at[i])) == order) {
+        in = at[i];
+        which = i;
+      }
+    if (order_of(L::largest(at[0])) == order) {
+      in = at[0];
+      which = 0;
+    }
+    each(in, which, [&](uint64_t key) { mine = key > mine ? key : mine; });
+    if (mine) g.keys[atomicAdd(&g.count, 1)] = mine;
+  }
+  if (tid == 0) g.floor = 0;
+  group_sync<kT>();
+  const int offered = g.count;
+  if (tid < offered) {
+    const uint64_t key = g.keys[tid];
+    int above = 0;
+    for (int i = 0; i < offered; ++i) above += g.keys[i] > key;
+    if (above == want - 1) g.floor = key;
+  }
+  group_sync<kT>();
+  const uint64_t floor = g.floor > g.list[want - 1] ? g.floor : g.list[want - 1];
+  if (tid == 0) g.count = 0;
+  group_sync<kT>();
+  // Only a thread whose largest key is not below the floor has others that are not.
+  if (mine >= floor && mine) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (i < n && order_of(L::largest(at[i])) >= uint32_t(floor >> 32))
+        each(at[i], i, [&](uint64_t key) {
+          if (key >= floor) {
+            const int to = atomicAdd(&g.count, 1);
+            if (to < kGather) g.keys[to] = key;
+          }
+        });
+  }
+  group_sync<kT>();
+  int gathered = g.count;
+  if (gathered > kGather) {
+    // Too many (a few threads with all that is large): the largest, the next one, and so on.
+    __shared__ uint64_t tops[kWarpsCta];
+    uint64_t below = ~uint64_t(0);
+    for (int r = 0; r < want; ++r) {
+      uint64_t key = 0;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        if (i < n) each(at[i], i, [&](uint64_t k) { key = k < below && k > key ? k : key; });
+      key = warp_top(key);
+      if constexpr (kWarps > 1) {
+        if (lane == 0) tops[warp] = key;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kWarps; ++j) key = tops[j] > key ? tops[j] : key;
+        __syncthreads();
+      }
+      if (tid == 0) g.keys[r] = key;
+      below = key;
+    }
+    gathered = want;
+  }
+  // The list so far joins them (its keys are others: of columns before).
+  const uint64_t kept = tid < 32 ? g.list[tid] : 0;
+  if (tid < 32) g.keys[gathered + tid] = kept;
+  group_sync<kT>();
+  const int all = gathered + 32;
+  for (int c = tid; c < all; c += kT) {
+    const uint64_t key = g.keys[c];
+    int above = key ? 0 : 32;
+    for (int i = 0; i < all; ++i) above += g.keys[i] > key;
+    if (above < 32) g.list[above] = key;
+  }
+  group_sync<kT>();
+}
+
 // kWarps 8: a row for a cluster of CTAs, which take its segments in turn; 1: a row a warp.
 template <class E, int kWarps, bool kTop>
 __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(const LogprobParams p, int ctas) {
@@ -173,7 +322,11 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
   const L x(p.x, row * p.stride, p.vocab);
   const Given given = given_of<E>(p, row);
   Sums mine{-INFINITY, 0.f, 0.f};
-  uint64_t best = 0;  // the lane's of the warp's alternatives, the largest in lane 0
+  __shared__ Gather gathers[kTop ? kWarpsCta / kWarps : 1];
+  Gather* const gather = kTop ? &gathers[kWarps == 1 ? warp : 0] : nullptr;
+  if constexpr (kTop) {
+    if (tid < 32) gather->list[tid] = 0;
+  }
   for (int64_t first = int64_t(rank) * kVecs * kT; first < x.vecs; first += int64_t(ctas) * kVecs * kT) {
     typename L::Vec at[kVecs];
 #pragma unroll
@@ -181,17 +334,13 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
     // vectors of a thread that the row reaches
     const int n = x.vecs - first < kVecs * kT ? int((x.vecs - first + kT - 1) / kT) : kVecs;
     // the maximum
-    float m = mine.m;
+    float m = mine.m, top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       if (i >= n) break;
-#pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        float a, b;
-        f2_unpack(P::wide(at[i].w[k]), a, b);
-        m = max_nan(m, max_nan(a, b));
-      }
+      top = max_nan(top, L::largest(at[i]));
     }
+    m = max_nan(m, top);
     const float base = m == -INFINITY ? 0.f : m;
     uint64_t s = f2_pack(0.f, 0.f), w = s;
     if (m != mine.m && mine.m != -INFINITY) {
@@ -222,71 +371,21 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
     f2_unpack(w, a, b);
     mine.w += a + b;
     if constexpr (kTop) {
-      // Each lane offers its largest element that has not been taken; the warp's largest is
-      // put in its place in the list, while it is above the last one there.
-      uint64_t tops[kVecs];
-      auto top_of = [&](int i, uint64_t below) {
-        uint64_t t = 0;
-        const int64_t v = first + i * kT + tid;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int64_t c = v * V + j - x.head;
-          const uint64_t key = key_of(order_of(to_f(at[i].e[j])), int(c));
-          if (c >= 0 && c < x.vocab && key < below && key > t) t = key;
-        }
-        return t;
-      };
-      uint64_t offer = 0;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        tops[i] = i < n ? top_of(i, ~uint64_t(0)) : 0;
-        offer = tops[i] > offer ? tops[i] : offer;
-      }
-      for (;;) {
-        const uint64_t key = warp_top(offer);
-        if (key <= __shfl_sync(0xffffffffu, best, p.top - 1)) break;
-        const int place = __popc(__ballot_sync(0xffffffffu, best > key));
-        const uint64_t up = __shfl_up_sync(0xffffffffu, best, 1);
-        best = lane < place ? best : lane == place ? key : up;
-        if (offer == key) {
-          offer = 0;
-#pragma unroll
-          for (int i = 0; i < kVecs; ++i) {
-            if (tops[i] == key) tops[i] = top_of(i, key);
-            offer = tops[i] > offer ? tops[i] : offer;
-          }
-        }
-      }
+      add_segment<E, kWarps>(x, at, first, n, top, p.top, *gather);
     }
   }
   mine = warp_join(mine);
   if constexpr (kWarps == 1) {
     if (lane == 0) finish(p, row, mine, given);
-    if (kTop && lane < p.top) put_top(p, row, lane, best, mine.m, logf(mine.s));
+    if constexpr (kTop) {
+      if (lane < p.top) put_top(p, row, lane, gather->list[lane], mine.m, logf(mine.s));
+    }
   } else {
     __shared__ Sums sums[kWarps];
-    __shared__ uint64_t tops[kTop ? kThreads : 1];  // of the CTA's warps, then of the cluster's CTAs
-    __shared__ uint64_t list[kTop ? 32 : 1];        // the CTA's, in order
     if (lane == 0) sums[warp] = mine;
-    if constexpr (kTop) {
-      tops[threadIdx.x] = lane < p.top ? best : 0;
-      if (threadIdx.x < 32) list[threadIdx.x] = 0;
-    }
     __syncthreads();
     Sums all = lane < kWarps ? sums[lane] : Sums{-INFINITY, 0.f, 0.f};
     all = warp_join(all);
-    // the place of a thread's key among `tops`, or 32
-    auto place = [&](uint64_t key) {
-      int n = key ? 0 : 32;
-      for (int i = 0; i < kThreads; ++i) n += tops[i] > key;
-      return n < 32 ? n : 32;
-    };
-    if constexpr (kTop) {
-      const uint64_t key = tops[threadIdx.x];
-      const int n = place(key);
-      if (n < p.top) list[n] = key;
-      __syncthreads();
-    }
     if (ctas > 1) {
       cg::cluster_group cluster = cg::this_cluster();
       __shared__ Sums cta_sums;
@@ -295,17 +394,26 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
       if (rank == 0) {
         all = lane < ctas ? *cluster.map_shared_rank(&cta_sums, lane) : Sums{-INFINITY, 0.f, 0.f};
         all = warp_join(all);
-        if constexpr (kTop) tops[threadIdx.x] = warp < ctas ? cluster.map_shared_rank(list, warp)[lane] : 0;
+        if constexpr (kTop) gather->keys[threadIdx.x] = warp < ctas ? cluster.map_shared_rank(gather, warp)->list[lane] : 0;
       }
       cluster.sync();  // nobody leaves before the first CTA has read its results
       if (rank) return;
       if constexpr (kTop) {
-        const uint64_t key = tops[threadIdx.x];
-        const int n = place(key);
-        if (n < p.top) put_top(p, row, n, key, all.m, logf(all.s));
+        // the CTAs' lists: a key's place is how many are above it in each of them
+        const uint64_t key = gather->keys[threadIdx.x];
+        int place = key ? 0 : 32;
+#pragma unroll
+        for (int l = 0; l < kWarps; ++l) {
+          const uint64_t* list = gather->keys + l * 32;
+          int above = 0;
+#pragma unroll
+          for (int step = 16; step > 0; step >>= 1) above += list[above + step - 1] > key ? step : 0;
+          place += above + (list[above] > key);
+        }
+        if (place < p.top) put_top(p, row, place, key, all.m, logf(all.s));
       }
     } else if constexpr (kTop) {
-      if (int(threadIdx.x) < p.top) put_top(p, row, threadIdx.x, list[threadIdx.x], all.m, logf(all.s));
+      if (int(threadIdx.x) < p.top) put_top(p, row, threadIdx.x, gather->list[threadIdx.x], all.m, logf(all.s));
     }
     if (threadIdx.x == 0) finish(p, row, all, given);
   }
@@ -391,7 +499,7 @@ void launch_e(const LogprobParams& p, int sm_count, cudaStream_t s) {
   // SMs four times over.
   const int64_t segments = (vecs + kThreads * kVecs - 1) / (kThreads * kVecs);
   int ctas = 1;
-  while (ctas < 8 && ctas < segments && p.rows * ctas < 16 * sm_count) ctas *= 2;
+  while (ctas < 8 && ctas < segments && p.rows * ctas < (kTop ? 1 : 16) * sm_count) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid_of(p.rows * ctas));
   cfg.blockDim = dim3(kThreads);

@@ -321,3 +321,19 @@ def test_large_offsets():
     close(r.logprobs[-2:], d["logprobs"], d["logprobs_err"])
     close(dx[-2:], d["dx"], d["dx_err"])
     assert torch.equal(r.top_indices[-2:], top_of(x.detach()[-2:], 2)[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [2000, 16000, 150000])
+def test_alternatives_that_few_threads_hold(V, dtype):
+    """All that is large lies in the vectors of `n` threads, more than is gathered at once; and in
+    those of one thread."""
+    per = 16 // torch.empty(0, dtype=dtype).element_size()
+    threads = 32 if V < 2048 else 256
+    lane = torch.arange(V, device="cuda") // per % threads
+    x = torch.randn(8, V, device="cuda")
+    for row, n in enumerate((1, 5, 15, 20, 31, 32, 64, 2)):
+        x[row] += 20 * (lane < n) if row % 2 else 20 * (lane >= threads - n)
+    t = torch.randint(0, V, (8,), device="cuda")
+    for top in (1, 20, 32):
+        check(x.to(dtype), t, top=top, grads=False)
