@@ -13,11 +13,10 @@
 // a cluster. Exponents are of base 2: sums hold W = sum (x - m) log2(e) e^(x - m).
 //
 // The alternatives are 64-bit keys that order by value and then by lower index, so that any
-// order of work gives the same ones. Of a segment's threads, `top` have a largest key that is
-// not below the top-th largest of these; so none of the segment's alternatives is below it,
-// and few other elements are above: these are gathered in shared memory and ranked by
-// counting, together with those of the segments before. A NaN counts as the largest value;
-// it makes its row's sums NaN.
+// order of work gives the same ones. What is not below a bound that the threads' largest
+// elements give is gathered in shared memory and ranked by counting, together with the
+// alternatives of the segments before. A NaN counts as the largest value; it makes its row's
+// sums NaN.
 #include "token_logprobs.cuh"
 
 #include <cooperative_groups.h>
@@ -86,7 +85,7 @@ constexpr int kGather = 256;  // keys of a segment that are gathered at once
 
 // What the threads that share a row (a CTA, or a warp) need for its alternatives.
 struct Gather {
-  uint64_t keys[kGather + 32];  // lanes' largest, then candidates
+  uint64_t keys[kGather + 32];
   uint64_t list[32];            // the alternatives so far, the largest first; 0: none
   uint64_t floor;
   int count;
@@ -135,6 +134,15 @@ struct Logits {
       return max_nan(to_f(m.x), to_f(m.y));
     }
   }
+  static __device__ __forceinline__ float element(const Vec& a, int j) {
+    if constexpr (sizeof(E) == 4) {
+      return j & 2 ? (j & 1 ? a.e[3] : a.e[2]) : (j & 1 ? a.e[1] : a.e[0]);
+    } else {
+      const uint32_t w = j & 4 ? (j & 2 ? a.w[3] : a.w[2]) : (j & 2 ? a.w[1] : a.w[0]);
+      const uint16_t h = uint16_t(j & 1 ? w >> 16 : w);
+      return to_f(*reinterpret_cast<const E*>(&h));
+    }
+  }
   // -inf outside the row, whose first and last elements are read by themselves
   __device__ __forceinline__ void load(int64_t v, Vec& to) const {
     if (inside(v)) {
@@ -160,13 +168,15 @@ __device__ __forceinline__ int64_t target_of(const LogprobParams& p, int64_t row
 
 // A row's given token: its logit, and whether it has one.
 struct Given {
-  float x;
-  bool ignored, known;
+  float x = 0.f;
+  bool ignored = true, known = false;
 };
 template <class E>
 __device__ __forceinline__ Given given_of(const LogprobParams& p, int64_t row) {
   const int64_t t = target_of(p, row);
-  Given g{0.f, t == p.ignore, t >= 0 && t < p.vocab};
+  Given g;
+  g.ignored = t == p.ignore;
+  g.known = t >= 0 && t < p.vocab;
   if (g.known) g.x = to_f(static_cast<const E*>(p.x)[row * p.stride + t]);
   return g;
 }
@@ -189,26 +199,30 @@ __device__ __forceinline__ void put_top(const LogprobParams& p, int64_t row, int
   p.top_indices[row * p.top + rank] = int64_t(uint32_t(~uint32_t(key)));
 }
 
-// Adds a segment's elements to the alternatives of the threads that share the row: `at` are a
-// thread's vectors, n of them in use, `top` its largest element.
-template <class E, int kWarps>
-__device__ __forceinline__ void add_segment(const Logits<E>& x, const typename Logits<E>::Vec (&at)[kVecs], int64_t first,
-                                            int n, float top, int want, Gather& g) {
-  constexpr int V = Logits<E>::V, kT = kWarps * 32;
-  const int lane = threadIdx.x & 31, warp = kWarps == 1 ? 0 : int(threadIdx.x) >> 5, tid = warp * 32 + lane;
-  using L = Logits<E>;
-  using Vec = typename L::Vec;
-  // calls take(key) for the elements of a vector of the thread
-  auto each = [&](const Vec& v, int i, auto take) {
-    const int64_t c0 = (first + i * kT + tid) * V - x.head;
+// The elements of vector v, each as take(key).
+template <class E, class Take>
+__device__ __forceinline__ void each_key(const Logits<E>& x, const typename Logits<E>::Vec& a, int64_t v, Take take) {
+  constexpr int V = Logits<E>::V;
+  const int64_t c0 = v * V - x.head;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (c0 + j >= 0 && c0 + j < x.vocab) take(key_of(order_of(to_f(v.e[j])), int(c0) + j));
-  };
-  const bool any = first + tid < x.vecs;  // (a vector may hold nothing of the row but at its ends)
-  uint32_t order = any ? order_of(top) : 0;
-  // A bound that is quick to have: in each warp, a want / kWarps-th of the threads is not below.
+  for (int j = 0; j < V; ++j)
+    if (c0 + j >= 0 && c0 + j < x.vocab) take(key_of(order_of(to_f(a.e[j])), int(c0) + j));
+}
+
+// A segment's elements join the alternatives of the threads that share the row, in two steps.
+// First all that is not below a bound is gathered, which is quick to have: in each warp a
+// want / kWarps-th of the threads have a largest element (`top`, of the n vectors `at` in use)
+// that is not below it, so that the segment's `want` largest are among them. (A NaN bound, of
+// a segment with fewer threads, takes all.)
+template <class E, int kWarps>
+__device__ __forceinline__ void gather_segment(const Logits<E>& x, const typename Logits<E>::Vec (&at)[kVecs],
+                                               int64_t first, int n, float top, int want, Gather& g) {
+  using L = Logits<E>;
+  constexpr int V = L::V, kT = kWarps * 32;
+  const int lane = threadIdx.x & 31, warp = kWarps == 1 ? 0 : int(threadIdx.x) >> 5, tid = warp * 32 + lane;
+  const uint32_t order = first + tid < x.vecs ? order_of(top) : 0;
   uint32_t bound = 0;
+  if (tid == 0) g.count = 0;
   if constexpr (kWarps > 1) {
     __shared__ uint32_t bounds[kWarps];
     uint32_t left = order;
@@ -217,91 +231,108 @@ __device__ __forceinline__ void add_segment(const Logits<E>& x, const typename L
       if (lane == __ffs(__ballot_sync(0xffffffffu, left == bound)) - 1) left = 0;
     }
     if (lane == 0) bounds[warp] = bound;
-    if (tid == 0) g.count = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kWarps; ++j) bound = bounds[j] < bound ? bounds[j] : bound;
   } else {
-    if (lane == 0) g.count = 0;
     __syncwarp();
-  }
-  // The want-th largest of the threads' largest keys.
-  uint64_t mine = 0;
-  const bool offers = any && order >= bound;
-  if (offers) {
-    // it is in the first vector whose largest element it is
-    Vec in = at[0];
-    int which = 0;
+    int above = 0;  // lanes before this one in the order of their largest elements
 #pragma unroll
-    for (int i = kVecs - 1; i > 0; --i)
-      if (i < n && order_of(L::largest(at[i])) == order) {
-        in = at[i];
-        which = i;
-      }
-    if (order_of(L::largest(at[0])) == order) {
-      in = at[0];
-      which = 0;
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t other = __shfl_sync(0xffffffffu, order, j);
+      above += other > order || (other == order && j < lane);
     }
-    each(in, which, [&](uint64_t key) { mine = key > mine ? key : mine; });
-    if (mine) g.keys[atomicAdd(&g.count, 1)] = mine;
+    bound = __shfl_sync(0xffffffffu, order, __ffs(__ballot_sync(0xffffffffu, above == want - 1)) - 1);
   }
-  if (tid == 0) g.floor = 0;
-  group_sync<kT>();
-  const int offered = g.count;
-  if (tid < offered) {
-    const uint64_t key = g.keys[tid];
-    int above = 0;
-    for (int i = 0; i < offered; ++i) above += g.keys[i] > key;
-    if (above == want - 1) g.floor = key;
-  }
-  group_sync<kT>();
-  const uint64_t floor = g.floor > g.list[want - 1] ? g.floor : g.list[want - 1];
-  if (tid == 0) g.count = 0;
-  group_sync<kT>();
-  // Only a thread whose largest key is not below the floor has others that are not.
-  if (mine >= floor && mine) {
+  const float least = value_of(bound);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (i < n && order_of(L::largest(at[i])) >= uint32_t(floor >> 32))
-        each(at[i], i, [&](uint64_t key) {
-          if (key >= floor) {
-            const int to = atomicAdd(&g.count, 1);
-            if (to < kGather) g.keys[to] = key;
-          }
-        });
+  for (int i = 0; i < kVecs; ++i) {
+    if (i >= n) break;
+    if (L::largest(at[i]) < least) continue;
+    uint32_t mask = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) mask |= uint32_t(!(to_f(at[i].e[j]) < least)) << j;
+    const int64_t c0 = (first + i * kT + tid) * V - x.head;
+    for (; mask; mask &= mask - 1) {
+      const int j = __ffs(mask) - 1;
+      if (c0 + j < 0 || c0 + j >= x.vocab) continue;
+      const int to = atomicAdd(&g.count, 1);
+      if (to < kGather) g.keys[to] = key_of(order_of(L::element(at[i], j)), int(c0) + j);
+    }
   }
   group_sync<kT>();
+}
+
+// Then they are ranked together with the list so far. Where too many were gathered (equal
+// logits, a few threads with all that is large), the segment is read again.
+template <class E, int kWarps>
+__device__ __forceinline__ void rank_segment(const Logits<E>& x, int64_t first, int n, int want, Gather& g) {
+  using L = Logits<E>;
+  constexpr int kT = kWarps * 32;
+  const int lane = threadIdx.x & 31, warp = kWarps == 1 ? 0 : int(threadIdx.x) >> 5, tid = warp * 32 + lane;
   int gathered = g.count;
   if (gathered > kGather) {
-    // Too many (a few threads with all that is large): the largest, the next one, and so on.
-    __shared__ uint64_t tops[kWarpsCta];
-    uint64_t below = ~uint64_t(0);
-    for (int r = 0; r < want; ++r) {
-      uint64_t key = 0;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-        if (i < n) each(at[i], i, [&](uint64_t k) { key = k < below && k > key ? k : key; });
-      key = warp_top(key);
-      if constexpr (kWarps > 1) {
-        if (lane == 0) tops[warp] = key;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kWarps; ++j) key = tops[j] > key ? tops[j] : key;
-        __syncthreads();
+    group_sync<kT>();
+    auto each = [&](auto take) {
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        typename L::Vec a;
+        x.load(first + i * kT + tid, a);
+        each_key<E>(x, a, first + i * kT + tid, take);
       }
-      if (tid == 0) g.keys[r] = key;
-      below = key;
+    };
+    // The want-th largest of the threads' largest keys is a better bound.
+    uint64_t mine = 0;
+    each([&](uint64_t key) { mine = key > mine ? key : mine; });
+    g.keys[tid] = mine;
+    if (tid == 0) {
+      g.count = 0;
+      g.floor = 0;
     }
-    gathered = want;
+    group_sync<kT>();
+    int above = 0;
+    for (int i = 0; i < kT; ++i) above += g.keys[i] > mine;
+    if (mine && above == want - 1) g.floor = mine;
+    group_sync<kT>();
+    const uint64_t floor = g.floor;
+    if (mine >= floor)
+      each([&](uint64_t key) {
+        if (key >= floor) {
+          const int to = atomicAdd(&g.count, 1);
+          if (to < kGather) g.keys[to] = key;
+        }
+      });
+    group_sync<kT>();
+    gathered = g.count;
+    if (gathered > kGather) {
+      // Still too many: the largest, the next one, and so on.
+      __shared__ uint64_t tops[kWarpsCta];
+      uint64_t below = ~uint64_t(0);
+      for (int r = 0; r < want; ++r) {
+        uint64_t key = 0;
+        each([&](uint64_t k) { key = k < below && k > key ? k : key; });
+        key = warp_top(key);
+        if constexpr (kWarps > 1) {
+          if (lane == 0) tops[warp] = key;
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < kWarps; ++j) key = tops[j] > key ? tops[j] : key;
+          __syncthreads();
+        }
+        if (tid == 0) g.keys[r] = key;
+        below = key;
+      }
+      gathered = want;
+    }
   }
-  // The list so far joins them (its keys are others: of columns before).
-  const uint64_t kept = tid < 32 ? g.list[tid] : 0;
-  if (tid < 32) g.keys[gathered + tid] = kept;
+  // (the list's keys are others: of columns before)
+  if (tid < 32) g.keys[gathered + tid] = g.list[tid];
   group_sync<kT>();
   const int all = gathered + 32;
   for (int c = tid; c < all; c += kT) {
     const uint64_t key = g.keys[c];
     int above = key ? 0 : 32;
+#pragma unroll 4
     for (int i = 0; i < all; ++i) above += g.keys[i] > key;
     if (above < 32) g.list[above] = key;
   }
@@ -320,17 +351,23 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
   const int64_t row = kWarps == 1 ? int64_t(blockIdx.x) * kWarpsCta + warp : int64_t(blockIdx.x / unsigned(ctas));
   if (kWarps == 1 && row >= p.rows) return;  // the whole warp, which no other waits for
   const L x(p.x, row * p.stride, p.vocab);
-  const Given given = given_of<E>(p, row);
+  Given given;
   Sums mine{-INFINITY, 0.f, 0.f};
   __shared__ Gather gathers[kTop ? kWarpsCta / kWarps : 1];
   Gather* const gather = kTop ? &gathers[kWarps == 1 ? warp : 0] : nullptr;
   if constexpr (kTop) {
     if (tid < 32) gather->list[tid] = 0;
   }
-  for (int64_t first = int64_t(rank) * kVecs * kT; first < x.vecs; first += int64_t(ctas) * kVecs * kT) {
-    typename L::Vec at[kVecs];
+  const int64_t step = int64_t(ctas) * kVecs * kT;
+  typename L::Vec at[kVecs];
+  auto load = [&](int64_t first) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) x.load(first + i * kT + tid, at[i]);
+  };
+  if (kTop) load(int64_t(rank) * kVecs * kT);
+  for (int64_t first = int64_t(rank) * kVecs * kT; first < x.vecs; first += step) {
+    if (!kTop) load(first);
+    if (first == int64_t(rank) * kVecs * kT) given = given_of<E>(p, row);  // behind the first loads
     // vectors of a thread that the row reaches
     const int n = x.vecs - first < kVecs * kT ? int((x.vecs - first + kT - 1) / kT) : kVecs;
     // the maximum
@@ -371,7 +408,9 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
     f2_unpack(w, a, b);
     mine.w += a + b;
     if constexpr (kTop) {
-      add_segment<E, kWarps>(x, at, first, n, top, p.top, *gather);
+      gather_segment<E, kWarps>(x, at, first, n, top, p.top, *gather);
+      if (first + step < x.vecs) load(first + step);
+      rank_segment<E, kWarps>(x, first, n, p.top, *gather);
     }
   }
   mine = warp_join(mine);
@@ -419,25 +458,29 @@ __global__ void __launch_bounds__(kThreads, kTop ? 2 : 3) token_logprobs_kernel(
   }
 }
 
-// dx of a row's segments. Where x's and dx's rows lie differently to 16-byte boundaries, dx
-// is written by elements.
+// dx. A row's segments go to `parts` units of kT threads (a CTA, or a warp where rows have few
+// vectors), each of which loads its next segment before it works on one. Where x's and dx's
+// rows lie differently to 16-byte boundaries, dx is written by elements.
 constexpr int kBackVecs = 4;
-// kT threads a segment: a CTA, or a warp for rows of few vectors.
 template <class E, int kT>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const LogprobBwdParams p, int segments) {
+__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const LogprobBwdParams p, int parts) {
   using L = Logits<E>;
   using P = typename L::P;
   constexpr int V = L::V, kPairs = L::kPairs;
   const int64_t unit = kT == kThreads ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * (kThreads / kT) + threadIdx.x / kT;
-  const int64_t row = unit / segments;
+  const int64_t row = unit / parts;
   if (row >= p.rows) return;
   const int tid = threadIdx.x % kT;
-  const int64_t first = (unit - row * segments) * kBackVecs * kT;
+  const int64_t step = int64_t(parts) * kBackVecs * kT;
+  int64_t first = (unit - row * parts) * kBackVecs * kT;
   const L x(p.x, row * p.stride, p.vocab);
   E* const dx = static_cast<E*>(p.dx) + row * p.vocab;
-  typename L::Vec at[kBackVecs];
+  typename L::Vec at[kBackVecs], ahead[kBackVecs];
+  auto load = [&](int64_t from, typename L::Vec (&to)[kBackVecs]) {
 #pragma unroll
-  for (int i = 0; i < kBackVecs; ++i) x.load(first + i * kT + tid, at[i]);
+    for (int i = 0; i < kBackVecs; ++i) x.load(from + i * kT + tid, to[i]);
+  };
+  load(first, at);
   const int64_t t = target_of(p, row);
   const bool known = t != p.ignore && t >= 0 && t < p.vocab;
   const float4 stats = reinterpret_cast<const float4*>(p.stats)[row];
@@ -447,34 +490,56 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const Logp
   const float dh = p.dh && !none ? p.dh[row * p.dh_stride] : 0.f;
   const float base = none ? 0.f : m, inv = none ? 0.f : 1.f / stats.y;
   const bool alike = (reinterpret_cast<uintptr_t>(dx) - reinterpret_cast<uintptr_t>(static_cast<const E*>(p.x) + row * p.stride)) % 16 == 0;
-  const int place = known ? int(t) : -1;
+  const int64_t place = known ? t : -1;
+  // dl + dh (ln p + H) = rest + dh z
+  const float rest = fmaf(dh, h - ln_s, dl);
+  const uint64_t minus = f2_pack(-base, -base), log2e = f2_pack(kLog2e, kLog2e), inv2 = f2_pack(-inv, -inv),
+                 dh2 = f2_pack(dh, dh), rest2 = f2_pack(rest, rest);
+  for (; first < x.vecs; first += step) {
+    if (first + step < x.vecs) load(first + step, ahead);
 #pragma unroll
-  for (int i = 0; i < kBackVecs; ++i) {
-    const int64_t v = first + i * kT + tid, c0 = v * V - x.head;
-    if (v >= x.vecs) break;
+    for (int i = 0; i < kBackVecs; ++i) {
+      const int64_t v = first + i * kT + tid, c0 = v * V - x.head;
+      if (v >= x.vecs) break;
+      float d[V];
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) {
-      float z[2], d[2];
-      f2_unpack(f2_add(P::wide(at[i].w[k]), f2_pack(-base, -base)), z[0], z[1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // 2^(z log2 e) with the product in two parts: rounding it would cost up to |z| steps
-        const float y = max_nan(z[j] * kLog2e, kLeast), lo = y > kLeast ? fmaf(z[j], kLog2eRest, fmaf(z[j], kLog2e, -y)) : 0.f;
-        const float e = ex2_approx(y), prob = fmaf(e, lo * kLn2, e) * inv;
-        // where z is -inf, ln p times p is 0
-        const float lnp = max_nan(z[j], kLeast) - ln_s;
-        d[j] = -prob * fmaf(dh, lnp + h, dl);
-        if (c0 + 2 * k + j == place) d[j] += dl;
+      for (int k = 0; k < kPairs; ++k) {
+        float z[2], y[2], e[2];
+        f2_unpack(f2_add(P::wide(at[i].w[k]), minus), z[0], z[1]);
+        // (-inf would be NaN in the products below; e^kLeast is 0 already)
+        z[0] = max_nan(z[0], kLeast);
+        z[1] = max_nan(z[1], kLeast);
+        const uint64_t zz = f2_pack(z[0], z[1]), yy = f2_mul(zz, log2e);
+        f2_unpack(yy, y[0], y[1]);
+        e[0] = ex2_approx(y[0]);
+        e[1] = ex2_approx(y[1]);
+        uint64_t ee = f2_pack(e[0], e[1]);
+        if constexpr (sizeof(E) == 4) {
+          // z log2 e in two parts: rounding it costs up to |z| steps of float32 (of which 16-bit
+          // results see nothing)
+          const uint64_t minus1 = f2_pack(-1.f, -1.f), more = f2_pack(kLog2eRest, kLog2eRest), ln2 = f2_pack(kLn2, kLn2);
+          const uint64_t lo = f2_fma(zz, more, f2_fma(zz, log2e, f2_mul(yy, minus1)));
+          ee = f2_fma(ee, f2_mul(lo, ln2), ee);
+        }
+        f2_unpack(f2_mul(f2_mul(ee, inv2), f2_fma(dh2, zz, rest2)), d[2 * k], d[2 * k + 1]);
       }
-      at[i].w[k] = P::narrow(f2_pack(d[0], d[1]));
-    }
-    if (alike && x.inside(v)) {
-      *reinterpret_cast<uint4*>(dx + c0) = at[i].v;
-    } else {
+      if (place >= c0 && place < c0 + V) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (c0 + j >= 0 && c0 + j < p.vocab) dx[c0 + j] = at[i].e[j];
+        for (int j = 0; j < V; ++j)
+          if (c0 + j == place) d[j] += dl;
+      }
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) at[i].w[k] = P::narrow(f2_pack(d[2 * k], d[2 * k + 1]));
+      if (alike && x.inside(v)) {
+        *reinterpret_cast<uint4*>(dx + c0) = at[i].v;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c0 + j >= 0 && c0 + j < p.vocab) dx[c0 + j] = at[i].e[j];
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kBackVecs; ++i) at[i].v = ahead[i].v;
   }
 }
 
@@ -514,19 +579,22 @@ void launch_e(const LogprobParams& p, int sm_count, cudaStream_t s) {
 }
 
 template <class E, int kT>
-void bwd_t(const LogprobBwdParams& p, int64_t vecs, cudaStream_t s) {
+void bwd_t(const LogprobBwdParams& p, int64_t vecs, int sm_count, cudaStream_t s) {
   const int64_t segments = (vecs + kT * kBackVecs - 1) / (kT * kBackVecs);
+  // as few units as keep the SMs evenly loaded
+  int64_t parts = 1;
+  while (parts * 2 <= segments && p.rows * parts * kT < 16 * int64_t(kThreads) * sm_count * 4) parts *= 2;
   token_logprobs_bwd_kernel<E, kT>
-      <<<grid_of((p.rows * segments + kThreads / kT - 1) / (kThreads / kT)), kThreads, 0, s>>>(p, int(segments));
+      <<<grid_of((p.rows * parts + kThreads / kT - 1) / (kThreads / kT)), kThreads, 0, s>>>(p, int(parts));
   cuda_ok(cudaGetLastError());
 }
 
 template <class E>
-void bwd_e(const LogprobBwdParams& p, cudaStream_t s) {
+void bwd_e(const LogprobBwdParams& p, int sm_count, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
   const int64_t vecs = (int64_t(p.vocab) + V - 1) / V + 1;
-  if (vecs < kThreads * kBackVecs) bwd_t<E, 32>(p, vecs, s);
-  else bwd_t<E, kThreads>(p, vecs, s);
+  if (vecs < kThreads * kBackVecs) bwd_t<E, 32>(p, vecs, sm_count, s);
+  else bwd_t<E, kThreads>(p, vecs, sm_count, s);
 }
 
 }  // namespace
@@ -539,11 +607,11 @@ void token_logprobs_launch(LogitType t, const LogprobParams& p, int sm_count, cu
   }
 }
 
-void token_logprobs_bwd_launch(LogitType t, const LogprobBwdParams& p, cudaStream_t s) {
+void token_logprobs_bwd_launch(LogitType t, const LogprobBwdParams& p, int sm_count, cudaStream_t s) {
   switch (t) {
-    case LogitType::kBf16: return bwd_e<__nv_bfloat16>(p, s);
-    case LogitType::kF16: return bwd_e<__half>(p, s);
-    default: return bwd_e<float>(p, s);
+    case LogitType::kBf16: return bwd_e<__nv_bfloat16>(p, sm_count, s);
+    case LogitType::kF16: return bwd_e<__half>(p, sm_count, s);
+    default: return bwd_e<float>(p, sm_count, s);
   }
 }
 

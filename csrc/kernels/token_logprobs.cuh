@@ -37,6 +37,6 @@ struct LogprobBwdParams : LogprobParams {
 };
 
 void token_logprobs_launch(LogitType t, const LogprobParams& p, int sm_count, cudaStream_t stream);
-void token_logprobs_bwd_launch(LogitType t, const LogprobBwdParams& p, cudaStream_t stream);
+void token_logprobs_bwd_launch(LogitType t, const LogprobBwdParams& p, int sm_count, cudaStream_t stream);
 
 }  // namespace mgfa

@@ -129,7 +129,8 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
     p.dl = grad_rows(dl, p.dl_stride);
     p.dh = grad_rows(dh, p.dh_stride);
     p.dx = dx.data_ptr();
-    if (p.rows > 0) token_logprobs_bwd_launch(logit_type(x), p, at::cuda::getCurrentCUDAStream());
+    if (p.rows > 0) 
+      token_logprobs_bwd_launch(logit_type(x), p, device_sm_count(x.get_device()), at::cuda::getCurrentCUDAStream());
     return once({dx, {}, {}, {}, {}});
   }
 };
