@@ -12,11 +12,15 @@
 // Bound by memory: forward reads x and writes y, back reads x and dy and writes dx. A
 // head's sums stay within the 1 to 32 lanes that hold it, so neither pass waits for more
 // than shuffles; rstd is computed again from x in the backward pass, which reads x anyway.
-// The weights are folded into the sines and cosines where that saves work, and each
-// thread keeps its columns' in registers.
+// The sines, cosines and weights of a thread's columns take the registers that loads under
+// way would need: so each thread has a ring in shared memory, into which it copies (cp.async)
+// what it will work on 4 or 8 heads later, and no other thread waits for it.
 #include "norm_rotary.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <stdexcept>
+#include <string>
 
 #include "pairs.cuh"
 #include "paged_attn.cuh"
@@ -27,8 +31,8 @@ namespace {
 using namespace mgfa::dev;
 
 constexpr int kThreads = 256;
-constexpr int kFwdBatch = 4;  // heads whose loads a thread has under way
-constexpr int kBwdBatch = 2;  // (of x and dy)
+// Heads that a thread has under way: 64 KB of 32 and (x and dy) 64 bytes a thread in halves.
+constexpr int kFwdRing = 8, kBwdRing = 4;
 
 // How a head's columns are cut (V elements are 16 bytes):
 enum : int {
@@ -43,13 +47,16 @@ inline int lanes_of(int mode, int v, int head_dim, int rotary_dim) {
 
 // A CTA's threads: `tile` tokens, of each slots[0] + slots[1] + slots[2] groups of
 // 2^lanes_log threads, for query, key and (append) value heads. Group i of n takes heads
-// i, i + n, ... of its kind, `batch` of them in each of `rounds`.
+// i, i + n, ... of its kind, `rounds` of them at most. The CTA takes every gridDim.x-th tile.
 struct Cut {
   int tile, threads, lanes, lanes_log, rounds;
   int slots[3];
 };
 
-Cut make_cut(int lanes, const int (&heads)[3], int batch, int64_t tokens, int sm_count) {
+Cut make_cut(int lanes, const int (&heads)[3], int64_t tokens, int sm_count) {
+  // Four heads a thread share its columns' sines and weights; where tokens are few, each has
+  // threads of its own.
+  const int batch = tokens >= 4 * sm_count ? 4 : 1;
   Cut c;
   c.lanes = lanes;
   c.lanes_log = 0;
@@ -64,7 +71,7 @@ Cut make_cut(int lanes, const int (&heads)[3], int batch, int64_t tokens, int sm
   for (; total > most; --total) --*std::max_element(c.slots, c.slots + 3);
   c.rounds = 0;
   for (int i = 0; i < 3; ++i)
-    if (c.slots[i]) c.rounds = std::max(c.rounds, (heads[i] + c.slots[i] * batch - 1) / (c.slots[i] * batch));
+    if (c.slots[i]) c.rounds = std::max(c.rounds, (heads[i] + c.slots[i] - 1) / c.slots[i]);
   c.tile = int(std::max<int64_t>(1, std::min<int64_t>(most / std::max(1, total), tokens / (2 * sm_count))));
   c.threads = ((c.tile * total << c.lanes_log) + 31) / 32 * 32;
   return c;
@@ -159,9 +166,9 @@ struct AppendPlace {
 __device__ __forceinline__ AppendPlace append_place(const CacheAppendParams& p, int t, int lane) {
   AppendPlace none{-1, -1};
   if (t < __ldg(p.cu) || t >= __ldg(p.cu + p.seqs)) return none;
-  int slot, q0, n;
-  if (!row_grew(p.c, p.slots, p.cu, p.seqs, t, lane, slot, q0, n)) return none;
-  const int pos = p.c.lens[slot] - n + t - q0;
+  int slot, q0, n, len;
+  if (!row_grew(p.c, p.slots, p.cu, p.seqs, t, lane, slot, q0, n, len)) return none;
+  const int pos = len - n + t - q0;
   if (pos < 0 || pos >= int64_t(p.c.width) * p.c.page) return none;
   const int page = p.c.table[int64_t(slot) * p.c.width + pos / p.c.page];
   if (page < 0 || page >= p.c.pages) {
@@ -172,124 +179,175 @@ __device__ __forceinline__ AppendPlace append_place(const CacheAppendParams& p, 
   return {page * p.k_stride[0] + row * p.k_stride[1], page * p.v_stride[0] + row * p.v_stride[1]};
 }
 
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last n copies' groups have arrived (the thread's own).
+template <int n>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
+
+// The rows that a thread works on in turn: round r of the CTA's tile j is head slot + r * step
+// of token t of the tile. Rows are copied kDepth ahead, kIn times (kHalves: 2) 16 bytes of each;
+// vector v of ring entry i is at ring[(i * kVecs + v) * threads], and a head's lanes lie side
+// by side there.
+template <class E, int kMode, int kIn, int kDepth>
+struct Rows {
+  static constexpr int kPer = kMode == kHalves ? 2 : 1, kVecs = kIn * kPer;
+  const RotaryParams& p;
+  const Cut& cut;
+  const Place<kMode, 16 / sizeof(E)>& at;
+  const RotaryTensor* in;  // [kIn]
+  uint4* mine;
+  int64_t all, tiles;  // tokens; tiles of this CTA
+  int64_t j = 0;       // the next to copy
+  int r = 0, entry = 0;
+  const E* row[kIn];
+  bool here = false;
+
+  __device__ __forceinline__ Rows(const RotaryParams& params, const Cut& c, const Place<kMode, 16 / sizeof(E)>& place,
+                                  const RotaryTensor* tensors, uint4* ring)
+      : p(params), cut(c), at(place), in(tensors), mine(ring + threadIdx.x) {
+    all = p.batch * p.tokens;
+    const int64_t n = (all + cut.tile - 1) / cut.tile;
+    tiles = n > blockIdx.x ? (n - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    for (int i = 0; i < kDepth; ++i) next();
+  }
+  __device__ __forceinline__ int64_t first(int64_t tile) const { return (blockIdx.x + tile * gridDim.x) * cut.tile; }
+  // Starts the copy of one more row into the entry that was read last.
+  __device__ __forceinline__ void next() {
+    if (j < tiles) {
+      if (r == 0) {
+        const int64_t token = first(j) + at.t;
+        here = at.live && token < all;
+        if (here) {
+          const int64_t b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
+#pragma unroll
+          for (int i = 0; i < kIn; ++i)
+            row[i] = static_cast<const E*>(in[i].in) + b * in[i].stride_b + l * in[i].stride_t + at.slot * in[i].stride_h;
+        }
+      }
+      if (here && at.slot + r * at.step < in[0].heads) {
+        uint4* to = mine + entry * kVecs * blockDim.x;
+#pragma unroll
+        for (int i = 0; i < kIn; ++i) {
+          if (at.rotates) copy16(to + i * kPer * blockDim.x, row[i] + at.c0);
+          if constexpr (kMode == kHalves) copy16(to + (i * kPer + 1) * blockDim.x, row[i] + at.c1);
+          row[i] += at.step * in[i].stride_h;
+        }
+      }
+      if (++r == cut.rounds) {
+        r = 0;
+        ++j;
+      }
+    }
+    copies_commit();
+    entry = entry + 1 == kDepth ? 0 : entry + 1;
+  }
+  // The oldest row has arrived. (kAny reads its neighbours' columns.)
+  __device__ __forceinline__ void arrived() const {
+    copies_wait<kDepth - 1>();
+    if constexpr (kMode == kAny) __syncwarp();
+  }
+  __device__ __forceinline__ uint4 get(int v) const { return mine[(entry * kVecs + v) * blockDim.x]; }
+  // Column c of the head, of input i (kAny).
+  __device__ __forceinline__ float element(int i, int c) const {
+    return to_f(reinterpret_cast<const E*>(mine + (entry * kVecs + i * kPer) * blockDim.x - at.u)[c]);
+  }
+};
+
 // kNorm: with the norm. P: NormRotaryParams, or CacheAppendParams to write into a cache.
 template <class E, int kMode, bool kNorm, class P>
 __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, const Cut cut) {
   constexpr bool kAppend = std::is_same_v<P, CacheAppendParams>;
-  constexpr int V = 16 / sizeof(E), kPairs = V / 2;
+  constexpr int V = 16 / sizeof(E), kPairs = V / 2, kTwo = kMode == kHalves ? kPairs : 1;
   using Pair = PairOf<E>;
+  using R = Rows<E, kMode, 1, kFwdRing>;
   union Vec {
     uint4 v;
     typename Pair::Raw w[kPairs];
   };
-  extern __shared__ float2 cs[];  // [tile][rotary_dim / 2], then (append) [tile] places
-  const int half = p.rotary_dim >> 1;
-  const int64_t first = int64_t(blockIdx.x) * cut.tile, all = p.batch * p.tokens;
-  const int here = int(all - first < cut.tile ? all - first : cut.tile);
-  AppendPlace* const places = reinterpret_cast<AppendPlace*>(cs + (cut.tile * half + 1) / 2 * 2);
+  extern __shared__ uint4 ring[];  // then, twice, a tile's angles and (append) places
+  const int half = p.rotary_dim >> 1, angles = (cut.tile * half + 1) / 2 * 2;
+  float2* const cs = reinterpret_cast<float2*>(ring + kFwdRing * R::kVecs * blockDim.x);
+  AppendPlace* const places = reinterpret_cast<AppendPlace*>(cs + 2 * angles);
   const Place<kMode, V> at(p, cut);
-  const int64_t token = first + at.t, b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
   RotaryTensor x = p.x[at.kind & 1];
   if constexpr (kAppend)
     if (at.kind == 2) x = p.v;
-  const int heads = at.live && at.t < here ? x.heads : 0;
-  const E* const in = static_cast<const E*>(x.in) + b * x.stride_b + l * x.stride_t;
+  R rows(p, cut, at, &x, ring);
 
-  Vec x0[kFwdBatch], x1[kMode == kHalves ? kFwdBatch : 1];
-  uint64_t other[kMode == kAny ? kFwdBatch : 1][kPairs];
-  auto load = [&](int h0) {
-#pragma unroll
-    for (int i = 0; i < kFwdBatch; ++i) {
-      const int h = h0 + i * at.step;
-      x0[i].v = make_uint4(0, 0, 0, 0);
-      if constexpr (kMode == kHalves) x1[i].v = x0[i].v;
-      if (h < heads) {
-        const E* row = in + h * x.stride_h;
-        if (at.rotates) x0[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c0));
-        if constexpr (kMode == kHalves) x1[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c1));
-        if constexpr (kMode == kAny) {
-#pragma unroll
-          for (int k = 0; k < kPairs; ++k) {
-            const int c = at.c0 + 2 * k;
-            other[i][k] = f2_pack(to_f(row[partner(c, half)]), to_f(row[partner(c + 1, half)]));
-          }
-        }
+  // angles and places of the CTA's tile j
+  auto prepare = [&](int64_t j) {
+    const int64_t first = rows.first(j);
+    const int here = int(rows.all - first < cut.tile ? rows.all - first : cut.tile);
+    if constexpr (kAppend) {
+      for (int i = threadIdx.x >> 5; i < here; i += blockDim.x >> 5) {
+        const AppendPlace to = append_place(p, int(first) + i, threadIdx.x & 31);
+        if ((threadIdx.x & 31) == 0) places[(j & 1) * cut.tile + i] = to;
       }
+    }
+    for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
+      const int tt = i / half;
+      cs[(j & 1) * angles + i] = rotary_angle(p, first + tt, i - tt * half);
     }
   };
-  load(at.slot);
-
-  if constexpr (kAppend) {
-    for (int i = threadIdx.x >> 5; i < here; i += blockDim.x >> 5) {
-      const AppendPlace to = append_place(p, int(first) + i, threadIdx.x & 31);
-      if ((threadIdx.x & 31) == 0) places[i] = to;
-    }
-  }
-  for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
-    const int tt = i / half;
-    cs[i] = rotary_angle(p, first + tt, i - tt * half);
-  }
-  __syncthreads();
-
-  E* out = nullptr;
-  int64_t out_h = p.head_dim;
-  if (heads > 0) {
-    if (!kAppend || at.kind == 0) out = static_cast<E*>(x.out) + token * x.heads * p.head_dim;
-    if constexpr (kAppend) {
-      if (at.kind == 1 && places[at.t].k >= 0) out = static_cast<E*>(p.k_pool) + places[at.t].k;
-      if (at.kind == 2 && places[at.t].v >= 0) out = static_cast<E*>(p.v_pool) + places[at.t].v;
-      if (at.kind) out_h = at.kind == 1 ? p.k_stride[2] : p.v_stride[2];
-    }
-  }
-  // out0 = n0 * co0 + partner * si0, and in kHalves out1 = n1 * co1 + n0 * si1; the weights
-  // are inside
-  constexpr int kTwo = kMode == kHalves ? kPairs : 1;
-  uint64_t co0[kPairs], si0[kPairs], co1[kTwo], si1[kTwo];
-  {
-    const float2* angles = cs + (at.t < here ? at.t * half : 0);
-    column_angles<kMode>(p, angles, kMode == kHalves && !at.rotates ? p.rotary_dim : at.c0, co0, si0);
+  if (rows.tiles > 0) prepare(0);
+  uint64_t w0[kPairs], w1[kTwo], wo[kMode == kAny ? kPairs : 1];
+  if constexpr (kNorm) {
+    constexpr bool kHalfType = std::is_same_v<E, __half>;
+    auto weights = [&](int c, int d) {
+      return at.live && at.kind < 2 ? f2_pack(weight_at(p, at.kind, c, kHalfType), weight_at(p, at.kind, d, kHalfType))
+                                    : uint64_t(0);
+    };
 #pragma unroll
-    for (int k = 0; k < kTwo; ++k) {
-      co1[k] = co0[k];
-      si1[k] = at.rotates ? f2_sub(0, si0[k]) : 0;
-    }
-    if constexpr (kNorm) {
-      constexpr bool kHalfType = std::is_same_v<E, __half>;
-      auto pair_of_weights = [&](int c, int d) {
-        return f2_pack(weight_at(p, at.kind, c, kHalfType), weight_at(p, at.kind, d, kHalfType));
-      };
-      if (at.live && at.kind < 2) {
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-          const int c = at.c0 + 2 * k;
-          const uint64_t w = pair_of_weights(c, c + 1);
-          co0[k] = f2_mul(co0[k], w);
-          if constexpr (kMode == kNeighbours) si0[k] = f2_mul(si0[k], swapped(w));
-          if constexpr (kMode == kAny)
-            si0[k] = f2_mul(si0[k], pair_of_weights(partner(c, half), partner(c + 1, half)));
-          if constexpr (kMode == kHalves) {
-            const uint64_t w1 = pair_of_weights(at.c1 + 2 * k, at.c1 + 2 * k + 1);
-            si0[k] = f2_mul(si0[k], w1);
-            co1[k] = f2_mul(co1[k], w1);
-            si1[k] = f2_mul(si1[k], w);
-          }
-        }
-      }
+    for (int k = 0; k < kPairs; ++k) {
+      const int c = at.c0 + 2 * k;
+      w0[k] = weights(c, c + 1);
+      if constexpr (kMode == kHalves) w1[k] = weights(at.c1 + 2 * k, at.c1 + 2 * k + 1);
+      if constexpr (kMode == kAny) wo[k] = weights(partner(c, half), partner(c + 1, half));
     }
   }
   const bool turns = !kAppend || at.kind < 2;
-  for (int r = 0; r < cut.rounds; ++r) {
-    const int h0 = at.slot + r * kFwdBatch * at.step;
-    if (r) load(h0);
-#pragma unroll
-    for (int i = 0; i < kFwdBatch; ++i) {
-      uint64_t a[kPairs], d[kPairs], scale = f2_pack(1.f, 1.f);
+  const float inv = 1.f / float(p.head_dim);
+  for (int64_t j = 0; j < rows.tiles; ++j) {
+    __syncthreads();  // the tile's angles are there, and those of the tile before have been read
+    if (j + 1 < rows.tiles) prepare(j + 1);
+    const int64_t token = rows.first(j) + at.t;
+    const int heads = at.live && token < rows.all ? x.heads : 0;
+    E* out = nullptr;
+    int64_t out_h = p.head_dim;
+    if (heads > 0) {
+      if (!kAppend || at.kind == 0) out = static_cast<E*>(x.out) + token * x.heads * p.head_dim;
+      if constexpr (kAppend) {
+        const AppendPlace to = places[(j & 1) * cut.tile + at.t];
+        if (at.kind == 1 && to.k >= 0) out = static_cast<E*>(p.k_pool) + to.k;
+        if (at.kind == 2 && to.v >= 0) out = static_cast<E*>(p.v_pool) + to.v;
+        if (at.kind) out_h = at.kind == 1 ? p.k_stride[2] : p.v_stride[2];
+      }
+    }
+    uint64_t co[kPairs], si[kPairs];
+    column_angles<kMode>(p, cs + (j & 1) * angles + at.t * half,
+                         (kMode == kHalves && !at.rotates) || heads == 0 ? p.rotary_dim : at.c0, co, si);
+    for (int r = 0; r < cut.rounds; ++r) {
+      const int h = at.slot + r * at.step;
+      const bool valid = h < heads;
+      rows.arrived();
+      Vec x0, x1;
+      x0.v = x1.v = make_uint4(0, 0, 0, 0);
+      if (valid && at.rotates) x0.v = rows.get(0);
+      if constexpr (kMode == kHalves)
+        if (valid) x1.v = rows.get(1);
+      uint64_t a[kPairs], d[kPairs];
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
-        a[k] = Pair::wide(x0[i].w[k]);
-        if constexpr (kMode == kHalves) d[k] = Pair::wide(x1[i].w[k]);
+        a[k] = Pair::wide(x0.w[k]);
+        if constexpr (kMode == kHalves) d[k] = Pair::wide(x1.w[k]);
         if constexpr (kMode == kNeighbours) d[k] = swapped(a[k]);
-        if constexpr (kMode == kAny) d[k] = other[i][k];
+        if constexpr (kMode == kAny) {
+          const int c = at.c0 + 2 * k;
+          d[k] = valid ? f2_pack(rows.element(0, partner(c, half)), rows.element(0, partner(c + 1, half))) : 0;
+        }
       }
       if constexpr (kNorm) {
         uint64_t sq = 0;
@@ -298,49 +356,67 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
           sq = f2_fma(a[k], a[k], sq);
           if constexpr (kMode == kHalves) sq = f2_fma(d[k], d[k], sq);
         }
-        const float mean = group_sum(pair_sum(sq), cut.lanes_log) / float(p.head_dim);
-        const float rstd = rsqrtf(mean + p.eps);
-        scale = f2_pack(rstd, rstd);
+        const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
+        const uint64_t scale = f2_pack(rstd, rstd);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const uint64_t w = w0[k];
+          a[k] = f2_mul(f2_mul(a[k], scale), w);
+          d[k] = f2_mul(f2_mul(d[k], scale), kMode == kHalves ? w1[kMode == kHalves ? k : 0]
+                                             : kMode == kAny  ? wo[kMode == kAny ? k : 0]
+                                                              : swapped(w));
+        }
       }
-      const int h = h0 + i * at.step;
-      if (h >= heads || !out) continue;
       if (turns) {
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {
-          if constexpr (kNorm) {
-            a[k] = f2_mul(a[k], scale);
-            d[k] = f2_mul(d[k], scale);
-          }
           // without the norm the columns behind rotary_dim are copies, bit for bit
           if (kNorm || (kMode == kHalves ? at.rotates : at.c0 + 2 * k < p.rotary_dim))
-            x0[i].w[k] = Pair::narrow(f2_fma(a[k], co0[k], f2_mul(d[k], si0[k])));
+            x0.w[k] = Pair::narrow(f2_fma(a[k], co[k], f2_mul(d[k], si[k])));
           if constexpr (kMode == kHalves)
-            if (kNorm || at.rotates) x1[i].w[k] = Pair::narrow(f2_fma(d[k], co1[k], f2_mul(a[k], si1[k])));
+            if (kNorm || at.rotates)
+              x1.w[k] = Pair::narrow(at.rotates ? f2_sub(f2_mul(d[k], co[k]), f2_mul(a[k], si[k])) : d[k]);
         }
       }
-      E* row = out + h * out_h;
-      if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0[i].v;
-      if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1[i].v;
+      if (valid && out) {
+        E* row = out + h * out_h;
+        if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0.v;
+        if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1.v;
+      }
+      if constexpr (kMode == kAny) __syncwarp();
+      rows.next();
     }
   }
+  copies_wait<0>();
 }
 
-// Gradients. A CTA takes every gridDim.x-th tile, and keeps its columns' share of the
-// weights' gradients in registers; the shares are added in the groups' order.
+// Gradients. Each thread keeps its columns' share of the weights' gradients in registers; the
+// shares are added in the groups' order.
 template <class E, int kMode>
 __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const NormRotaryParams p, const Cut cut) {
   constexpr int V = 16 / sizeof(E), kPairs = V / 2, kTwo = kMode == kHalves ? kPairs : 1;
   using Pair = PairOf<E>;
+  using R = Rows<E, kMode, 2, kBwdRing>;
   union Vec {
     uint4 v;
     typename Pair::Raw w[kPairs];
   };
-  extern __shared__ float2 cs[];  // [tile][rotary_dim / 2]; at the end the weights' gradients
+  extern __shared__ uint4 ring[];  // then, twice, a tile's angles; at the end the weights' gradients
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int half = p.rotary_dim >> 1;
-  const int64_t all = p.batch * p.tokens;
+  const int half = p.rotary_dim >> 1, angles = cut.tile * half;
+  float2* const cs = reinterpret_cast<float2*>(ring + kBwdRing * R::kVecs * blockDim.x);
   const Place<kMode, V> at(p, cut);
-  const RotaryTensor x = p.x[at.kind], y = p.dy[at.kind];
+  const RotaryTensor tensors[2] = {p.x[at.kind], p.dy[at.kind]};
+  R rows(p, cut, at, tensors, ring);
+  auto prepare = [&](int64_t j) {
+    const int64_t first = rows.first(j);
+    const int here = int(rows.all - first < cut.tile ? rows.all - first : cut.tile);
+    for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
+      const int tt = i / half;
+      cs[(j & 1) * angles + i] = rotary_angle(p, first + tt, i - tt * half);
+    }
+  };
+  if (rows.tiles > 0) prepare(0);
   constexpr bool kHalfType = std::is_same_v<E, __half>;
   uint64_t w0[kPairs], w1[kTwo], acc0[kPairs], acc1[kTwo];
 #pragma unroll
@@ -354,106 +430,78 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const Norm
         w1[k] = f2_pack(weight_at(p, at.kind, at.c1 + 2 * k, kHalfType), weight_at(p, at.kind, at.c1 + 2 * k + 1, kHalfType));
     }
   }
-  for (int64_t first = int64_t(blockIdx.x) * cut.tile; first < all; first += int64_t(gridDim.x) * cut.tile) {
-    const int here = int(all - first < cut.tile ? all - first : cut.tile);
-    const int64_t token = first + at.t, b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
-    const int heads = at.live && at.t < here ? x.heads : 0;
-    const E* const in = static_cast<const E*>(x.in) + b * x.stride_b + l * x.stride_t;
-    const E* const dy = static_cast<const E*>(y.in) + b * y.stride_b + l * y.stride_t;
-    E* const dx = static_cast<E*>(x.out) + token * x.heads * p.head_dim;
-    Vec x0[kBwdBatch], x1[kMode == kHalves ? kBwdBatch : 1], y0[kBwdBatch], y1[kMode == kHalves ? kBwdBatch : 1];
-    uint64_t other[kMode == kAny ? kBwdBatch : 1][kPairs];
-    auto load = [&](int h0) {
-#pragma unroll
-      for (int i = 0; i < kBwdBatch; ++i) {
-        const int h = h0 + i * at.step;
-        x0[i].v = y0[i].v = make_uint4(0, 0, 0, 0);
-        if constexpr (kMode == kHalves) x1[i].v = y1[i].v = x0[i].v;
-        if constexpr (kMode == kAny) {
-#pragma unroll
-          for (int k = 0; k < kPairs; ++k) other[i][k] = 0;
-        }
-        if (h < heads) {
-          const E* row = in + h * x.stride_h;
-          const E* back = dy + h * y.stride_h;
-          if (at.rotates) {
-            x0[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c0));
-            y0[i].v = __ldg(reinterpret_cast<const uint4*>(back + at.c0));
-          }
-          if constexpr (kMode == kHalves) {
-            x1[i].v = __ldg(reinterpret_cast<const uint4*>(row + at.c1));
-            y1[i].v = __ldg(reinterpret_cast<const uint4*>(back + at.c1));
-          }
-          if constexpr (kMode == kAny) {
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) {
-              const int c = at.c0 + 2 * k;
-              other[i][k] = f2_pack(to_f(back[partner(c, half)]), to_f(back[partner(c + 1, half)]));
-            }
-          }
-        }
-      }
-    };
-    load(at.slot);
-    __syncthreads();  // the last tile's angles have been read
-    for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
-      const int tt = i / half;
-      cs[i] = rotary_angle(p, first + tt, i - tt * half);
-    }
-    __syncthreads();
+  const float inv = 1.f / float(p.head_dim);
+  for (int64_t j = 0; j < rows.tiles; ++j) {
+    __syncthreads();  // the tile's angles are there, and those of the tile before have been read
+    if (j + 1 < rows.tiles) prepare(j + 1);
+    const int64_t token = rows.first(j) + at.t;
+    const int heads = at.live && token < rows.all ? tensors[0].heads : 0;
+    E* const dx = static_cast<E*>(tensors[0].out) + token * tensors[0].heads * p.head_dim;
     uint64_t co[kPairs], si[kPairs];
-    column_angles<kMode>(p, cs + (at.t < here ? at.t * half : 0),
-                         kMode == kHalves && !at.rotates ? p.rotary_dim : at.c0, co, si);
+    column_angles<kMode>(p, cs + (j & 1) * angles + at.t * half,
+                         (kMode == kHalves && !at.rotates) || heads == 0 ? p.rotary_dim : at.c0, co, si);
     for (int r = 0; r < cut.rounds; ++r) {
-      const int h0 = at.slot + r * kBwdBatch * at.step;
-      if (r) load(h0);
-#pragma unroll
-      for (int i = 0; i < kBwdBatch; ++i) {
-        // g in g0, g1 and x in a, d
-        uint64_t g0[kPairs], g1[kTwo], sq = 0, dot = 0;
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-          const uint64_t e = Pair::wide(y0[i].w[k]), a = Pair::wide(x0[i].w[k]);
-          uint64_t f = 0;
-          if constexpr (kMode == kHalves) f = Pair::wide(y1[i].w[k]);
-          if constexpr (kMode == kNeighbours) f = swapped(e);
-          if constexpr (kMode == kAny) f = other[i][k];
-          g0[k] = f2_fma(e, co[k], f2_mul(f, si[k]));
-          sq = f2_fma(a, a, sq);
-          dot = f2_fma(f2_mul(g0[k], w0[k]), a, dot);
-          if constexpr (kMode == kHalves) {
-            const uint64_t d = Pair::wide(x1[i].w[k]);
-            g1[k] = f2_sub(f2_mul(f, co[k]), f2_mul(e, si[k]));
-            sq = f2_fma(d, d, sq);
-            dot = f2_fma(f2_mul(g1[k], w1[k]), d, dot);
-          }
-        }
-        const float inv = 1.f / float(p.head_dim);
-        const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
-        const float along = group_sum(pair_sum(dot), cut.lanes_log) * inv * rstd * rstd;
-        const int h = h0 + i * at.step;
-        if (h >= heads) continue;
-        const uint64_t scale = f2_pack(rstd, rstd), minus = f2_pack(-along, -along);
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-          const uint64_t a = Pair::wide(x0[i].w[k]);
-          acc0[k] = f2_fma(g0[k], f2_mul(a, scale), acc0[k]);
-          x0[i].w[k] = Pair::narrow(f2_mul(scale, f2_fma(g0[k], w0[k], f2_mul(a, minus))));
-          if constexpr (kMode == kHalves) {
-            const uint64_t d = Pair::wide(x1[i].w[k]);
-            acc1[k] = f2_fma(g1[k], f2_mul(d, scale), acc1[k]);
-            x1[i].w[k] = Pair::narrow(f2_mul(scale, f2_fma(g1[k], w1[k], f2_mul(d, minus))));
-          }
-        }
-        E* row = dx + h * p.head_dim;
-        if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0[i].v;
-        if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1[i].v;
+      const int h = at.slot + r * at.step;
+      const bool valid = h < heads;
+      rows.arrived();
+      Vec x0, x1, y0, y1;
+      x0.v = x1.v = y0.v = y1.v = make_uint4(0, 0, 0, 0);
+      if (valid && at.rotates) {
+        x0.v = rows.get(0);
+        y0.v = rows.get(R::kPer);
       }
+      if constexpr (kMode == kHalves)
+        if (valid) {
+          x1.v = rows.get(1);
+          y1.v = rows.get(3);
+        }
+      uint64_t g0[kPairs], g1[kTwo], sq = 0, dot = 0;
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const uint64_t e = Pair::wide(y0.w[k]), a = Pair::wide(x0.w[k]);
+        uint64_t f = 0;
+        if constexpr (kMode == kHalves) f = Pair::wide(y1.w[k]);
+        if constexpr (kMode == kNeighbours) f = swapped(e);
+        if constexpr (kMode == kAny) {
+          const int c = at.c0 + 2 * k;
+          if (valid) f = f2_pack(rows.element(1, partner(c, half)), rows.element(1, partner(c + 1, half)));
+        }
+        g0[k] = f2_fma(e, co[k], f2_mul(f, si[k]));
+        sq = f2_fma(a, a, sq);
+        dot = f2_fma(f2_mul(g0[k], w0[k]), a, dot);
+        if constexpr (kMode == kHalves) {
+          const uint64_t d = Pair::wide(x1.w[k]);
+          g1[k] = f2_sub(f2_mul(f, co[k]), f2_mul(e, si[k]));
+          sq = f2_fma(d, d, sq);
+          dot = f2_fma(f2_mul(g1[k], w1[k]), d, dot);
+        }
+      }
+      if constexpr (kMode == kAny) __syncwarp();
+      rows.next();
+      const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
+      const float along = group_sum(pair_sum(dot), cut.lanes_log) * inv * rstd * rstd;
+      if (!valid) continue;
+      const uint64_t scale = f2_pack(rstd, rstd), minus = f2_pack(-along, -along);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const uint64_t a = Pair::wide(x0.w[k]);
+        acc0[k] = f2_fma(g0[k], f2_mul(a, scale), acc0[k]);
+        x0.w[k] = Pair::narrow(f2_mul(scale, f2_fma(g0[k], w0[k], f2_mul(a, minus))));
+        if constexpr (kMode == kHalves) {
+          const uint64_t d = Pair::wide(x1.w[k]);
+          acc1[k] = f2_fma(g1[k], f2_mul(d, scale), acc1[k]);
+          x1.w[k] = Pair::narrow(f2_mul(scale, f2_fma(g1[k], w1[k], f2_mul(d, minus))));
+        }
+      }
+      E* row = dx + h * p.head_dim;
+      if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0.v;
+      if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1.v;
     }
   }
+  copies_wait<0>();
   if (!p.dw_part) return;
   // [group][head_dim]
-  float* const sums = reinterpret_cast<float*>(cs);
+  float* const sums = reinterpret_cast<float*>(ring);
   __syncthreads();
   if (at.live) {
     float* mine = sums + (threadIdx.x >> cut.lanes_log) * p.head_dim;
@@ -589,6 +637,19 @@ int mode_of(const RotaryParams& p) {
   return lanes_of(mode, V, p.head_dim, p.rotary_dim) <= 32 ? mode : -1;
 }
 
+void cuda_ok(cudaError_t e) {
+  if (e != cudaSuccess) throw std::runtime_error(std::string("norm and rotary positions: ") + cudaGetErrorString(e));
+}
+
+// The CTAs of a launch: as many as run at once.
+template <auto fn, class P>
+void launch_tiles(const P& p, const Cut& cut, int64_t tokens, int ctas, size_t smem, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};  // (of this kernel)
+  cuda_ok(paged_allow_smem(fn, allowed));
+  fn<<<unsigned(std::min<int64_t>((tokens + cut.tile - 1) / cut.tile, ctas)), cut.threads, smem, s>>>(p, cut);
+  cuda_ok(cudaGetLastError());
+}
+
 template <class E, int kMode, bool kNorm, class P>
 void fwd_mode(const P& p, int sm_count, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
@@ -596,11 +657,11 @@ void fwd_mode(const P& p, int sm_count, cudaStream_t s) {
   int heads[3] = {p.x[0].heads, p.x[1].heads, 0};
   if constexpr (kAppend) heads[2] = p.v.heads;
   const int64_t all = p.batch * p.tokens;
-  const Cut cut = make_cut(lanes_of(kMode, V, p.head_dim, p.rotary_dim), heads, kFwdBatch, all, sm_count);
-  const size_t smem = (size_t(cut.tile) * (p.rotary_dim / 2) + 1) / 2 * 2 * sizeof(float2) +
-                      (kAppend ? cut.tile * sizeof(AppendPlace) : 0);
-  norm_rotary_kernel<E, kMode, kNorm, P>
-      <<<unsigned((all + cut.tile - 1) / cut.tile), cut.threads, smem, s>>>(p, cut);
+  const Cut cut = make_cut(lanes_of(kMode, V, p.head_dim, p.rotary_dim), heads, all, sm_count);
+  const size_t angles = (size_t(cut.tile) * (p.rotary_dim / 2) + 1) / 2 * 2;
+  const size_t smem = sizeof(uint4) * kFwdRing * Rows<E, kMode, 1, kFwdRing>::kVecs * cut.threads +
+                      2 * angles * sizeof(float2) + (kAppend ? 2 * cut.tile * sizeof(AppendPlace) : 0);
+  launch_tiles<norm_rotary_kernel<E, kMode, kNorm, P>>(p, cut, all, 2 * sm_count, smem, s);
 }
 
 template <class E, bool kNorm, class P>
@@ -619,7 +680,7 @@ void fwd_e(const P& p, int sm_count, cudaStream_t s) {
 template <class E>
 Cut bwd_cut(const NormRotaryParams& p, int mode, int sm_count) {
   return make_cut(lanes_of(mode, 16 / sizeof(E), p.head_dim, p.rotary_dim),
-                  {p.x[0].heads, p.x[1].heads, 0}, kBwdBatch, p.batch * p.tokens, sm_count);
+                  {p.x[0].heads, p.x[1].heads, 0}, p.batch * p.tokens, sm_count);
 }
 
 // Two CTAs an SM, each with every parts-th tile.
@@ -634,9 +695,10 @@ int bwd_parts(const NormRotaryParams& p, int sm_count) {
 template <class E, int kMode>
 void bwd_mode(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
   const Cut cut = bwd_cut<E>(p, kMode, sm_count);
-  const size_t angles = size_t(cut.tile) * (p.rotary_dim / 2) * sizeof(float2);
+  const size_t ring = sizeof(uint4) * kBwdRing * Rows<E, kMode, 2, kBwdRing>::kVecs * cut.threads +
+                      2 * size_t(cut.tile) * (p.rotary_dim / 2) * sizeof(float2);
   const size_t sums = p.dw_part ? size_t(cut.threads >> cut.lanes_log) * p.head_dim * sizeof(float) : 0;
-  norm_rotary_bwd_kernel<E, kMode><<<parts, cut.threads, std::max(angles, sums), s>>>(p, cut);
+  launch_tiles<norm_rotary_bwd_kernel<E, kMode>>(p, cut, p.batch * p.tokens, parts, std::max(ring, sums), s);
 }
 
 template <class E>
@@ -659,7 +721,7 @@ void bwd_e(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, norm_rotary_dw_kernel<E>, p, parts);
+  cuda_ok(cudaLaunchKernelEx(&cfg, norm_rotary_dw_kernel<E>, p, parts));
 }
 
 }  // namespace

@@ -238,9 +238,9 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const WriteParams p) {
   const int t = int(id >> 1), lane = threadIdx.x & 31;
   const bool value = id & 1;
   if (t >= p.tokens || t < __ldg(p.cu) || t >= __ldg(p.cu + p.seqs)) return;
-  int slot, q0, n;
-  if (!row_grew(p.c, p.slots, p.cu, p.seqs, t, lane, slot, q0, n)) return;
-  const int pos = p.c.lens[slot] - n + t - q0;
+  int slot, q0, n, len;
+  if (!row_grew(p.c, p.slots, p.cu, p.seqs, t, lane, slot, q0, n, len)) return;
+  const int pos = len - n + t - q0;
   if (pos < 0 || pos >= int64_t(p.c.width) * p.c.page) return;
   const int page = p.c.table[int64_t(slot) * p.c.width + pos / p.c.page];
   if (page < 0 || page >= p.c.pages) {
@@ -267,9 +267,9 @@ __global__ void __launch_bounds__(256)
                          bool* refused, int tokens) {
   const int t = int((int64_t(blockIdx.x) * 256 + threadIdx.x) >> 5), lane = threadIdx.x & 31;
   if (t >= tokens) return;
-  int slot, q0, n;
+  int slot, q0, n, len;
   const bool in = t >= __ldg(cu) && t < __ldg(cu + seqs);
-  const bool no = in && !row_grew(c, slots, cu, seqs, t, lane, slot, q0, n);
+  const bool no = in && !row_grew(c, slots, cu, seqs, t, lane, slot, q0, n, len);
   if (lane == 0) refused[t] = no;
 }
 

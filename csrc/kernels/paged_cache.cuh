@@ -48,21 +48,37 @@ __device__ __forceinline__ int token_seq(const int* cu, int seqs, int t) {
   return lo;
 }
 
+// token_seq() by a whole warp: 32 entries a step.
+__device__ __forceinline__ int token_seq_warp(const int* cu, int seqs, int t, int lane) {
+  int lo = 0, n = seqs;  // the last b with cu[b] <= t is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lo + lane * step;
+    const bool below = lane * step < n && (lane == 0 || __ldg(cu + at) <= t);
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, below));
+    lo += last * step;
+    n = n - last * step < step ? n - last * step : step;
+  }
+  return lo;
+}
+
 // Whether reserve() has made room for row t of the batch, which is row t - q0 of the n that
-// sequence `slot` has grown by. Called by a whole warp, for cu[0] <= t < cu[seqs].
+// sequence `slot`, now of `len` tokens, has grown by. Called by a whole warp, for
+// cu[0] <= t < cu[seqs]. (Loads that do not need one another are issued together.)
 __device__ __forceinline__ bool row_grew(const CacheState& c, const int* slots, const int* cu,
-                                         int seqs, int t, int lane, int& slot, int& q0, int& n) {
-  const int b = token_seq(cu, seqs, t);
+                                         int seqs, int t, int lane, int& slot, int& q0, int& n, int& len) {
+  const int b = token_seq_warp(cu, seqs, t, lane);
   slot = __ldg(slots + b);
+  q0 = __ldg(cu + b);
+  n = __ldg(cu + b + 1) - q0;
   if (slot < 0 || slot >= c.slots) return false;
+  const int grown = c.grown[slot];
+  len = c.lens[slot];
   // a slot named again, with as many tokens, would pass the test below too: its first
   // sequence alone has grown
   bool again = false;
   for (int i = lane; i < b; i += 32) again |= __ldg(slots + i) == slot;
   if (__any_sync(0xffffffffu, again)) return false;
-  q0 = __ldg(cu + b);
-  n = __ldg(cu + b + 1) - q0;
-  return c.grown[slot] == n && t - q0 < n;
+  return grown == n && t - q0 < n;
 }
 
 }  // namespace dev
