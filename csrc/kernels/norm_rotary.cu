@@ -31,8 +31,8 @@ namespace {
 using namespace mgfa::dev;
 
 constexpr int kThreads = 256;
-// Heads that a thread has under way: 64 KB of 32 and (x and dy) 64 bytes a thread in halves.
-constexpr int kFwdRing = 8, kBwdRing = 4;
+// Heads of a unit, two units being a thread's ring (kHalves: 256 bytes either way).
+constexpr int kFwdUnit = 4, kBwdUnit = 2;
 
 // How a head's columns are cut (V elements are 16 bytes):
 enum : int {
@@ -136,25 +136,74 @@ __device__ __forceinline__ float weight_at(const NormRotaryParams& p, int kind, 
                    : __bfloat162float(static_cast<const __nv_bfloat16*>(p.weight[kind])[c]);
 }
 
-// out = own * co + partner * si for columns c0.. of a token whose angles are `cs`.
+// A tile's angles in shared memory, by token: cosines, then sines with the sign that the first
+// of a pair takes them with, each `angle_row` floats.
+__host__ __device__ inline int angle_row(int rotary_dim) { return (rotary_dim / 2 + 3) / 4 * 4; }
+
+// Those of a tile of tokens [first, first + here). turns: inv_freq / 2 pi. kFast: sine and
+// cosine of the reduced angle to 2^-21, of which 16-bit results see nothing; otherwise to two
+// steps of float32.
+template <bool kFast>
+__device__ __forceinline__ void tile_angles(const RotaryParams& p, const double* turns, int64_t first, int here, float* to) {
+  const int half = p.rotary_dim >> 1, row = angle_row(p.rotary_dim);
+  for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
+    const int tt = i / half, f = i - tt * half;
+    double t = rotary_position(p, first + tt) * turns[f];
+    t -= rint(t);
+    float s, c;
+    if constexpr (kFast) {
+      const float radians = float(t) * 6.283185307179586f;
+      s = __sinf(radians);
+      c = __cosf(radians);
+    } else {
+      sincospif(float(2.0 * t), &s, &c);
+    }
+    to[2 * tt * row + f] = c * p.magnitude;
+    to[(2 * tt + 1) * row + f] = -s * p.magnitude * p.sign;
+  }
+}
+
+// out = own * co + partner * si for columns c0.. of a token whose angles are `cs`. (kHalves: of
+// the first half's columns, or of none.)
 template <int kMode, int kPairs>
-__device__ __forceinline__ void column_angles(const RotaryParams& p, const float2* cs, int c0,
+__device__ __forceinline__ void column_angles(const RotaryParams& p, const float* cs, int c0,
                                               uint64_t (&co)[kPairs], uint64_t (&si)[kPairs]) {
   const int half = p.rotary_dim >> 1;
+  const float* const sn = cs + angle_row(p.rotary_dim);
+  if constexpr (kMode == kHalves) {
 #pragma unroll
-  for (int k = 0; k < kPairs; ++k) {
-    const int c = c0 + 2 * k;
-    co[k] = f2_pack(1.f, 1.f);
-    si[k] = 0;
-    if (c >= p.rotary_dim) continue;
-    if (kMode == kNeighbours) {
-      const float2 f = cs[c >> 1];
-      co[k] = f2_pack(f.x, f.x);
-      si[k] = f2_pack(-f.y, f.y);
-    } else {
-      const float2 f = cs[c < half ? c : c - half], g = cs[c + 1 < half ? c + 1 : c + 1 - half];
-      co[k] = f2_pack(f.x, g.x);
-      si[k] = f2_pack(c < half ? -f.y : f.y, c + 1 < half ? -g.y : g.y);
+    for (int k = 0; k < kPairs; ++k) {
+      co[k] = f2_pack(1.f, 1.f);
+      si[k] = 0;
+    }
+    if (c0 < p.rotary_dim) {
+#pragma unroll
+      for (int k = 0; k < kPairs; k += 2) {
+        const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(cs + c0 + 2 * k);
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(sn + c0 + 2 * k);
+        co[k] = u.x;
+        co[k + 1] = u.y;
+        si[k] = v.x;
+        si[k + 1] = v.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+      const int c = c0 + 2 * k;
+      co[k] = f2_pack(1.f, 1.f);
+      si[k] = 0;
+      if (c >= p.rotary_dim) continue;
+      if (kMode == kNeighbours) {
+        const float u = cs[c >> 1], v = sn[c >> 1];
+        co[k] = f2_pack(u, u);
+        si[k] = f2_pack(v, -v);
+      } else {
+        const bool second = c >= half, next = c + 1 >= half;
+        const int i = second ? c - half : c, j = next ? c + 1 - half : c + 1;
+        co[k] = f2_pack(cs[i], cs[j]);
+        si[k] = f2_pack(second ? -sn[i] : sn[i], next ? -sn[j] : sn[j]);
+      }
     }
   }
 }
@@ -187,72 +236,79 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int n>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
 
-// The rows that a thread works on in turn: round r of the CTA's tile j is head slot + r * step
-// of token t of the tile. Rows are copied kDepth ahead, kIn times (kHalves: 2) 16 bytes of each;
-// vector v of ring entry i is at ring[(i * kVecs + v) * threads], and a head's lanes lie side
-// by side there.
-template <class E, int kMode, int kIn, int kDepth>
-struct Rows {
-  static constexpr int kPer = kMode == kHalves ? 2 : 1, kVecs = kIn * kPer;
+// What a thread works on in turn: units of kUnit heads of one token, of which it has two in its
+// ring: while it works on one, it copies the next but one, head for head, into the place of
+// what it has read. Unit (tile j, pass i) of the CTA is heads slot + (i * kUnit + r) * step of
+// token t of its tile j. Of each head kIn times (kHalves: 2) 16 bytes; a head's lanes lie side
+// by side in shared memory.
+template <class E, int kMode, int kIn, int kUnit>
+struct Units {
+  static constexpr int kPer = kMode == kHalves ? 2 : 1, kVecs = kIn * kPer, kRing = 2 * kUnit;
   const RotaryParams& p;
   const Cut& cut;
   const Place<kMode, 16 / sizeof(E)>& at;
-  const RotaryTensor* in;  // [kIn]
+  const int64_t all;  // tokens
+  int64_t tiles;      // of this CTA
+  int passes;
   uint4* mine;
-  int64_t all, tiles;  // tokens; tiles of this CTA
-  int64_t j = 0;       // the next to copy
-  int r = 0, entry = 0;
+  // the unit to copy into next, and its first head's rows
+  int64_t j = 0;
+  int pass = 0, heads_left = 0;
   const E* row[kIn];
-  bool here = false;
 
-  __device__ __forceinline__ Rows(const RotaryParams& params, const Cut& c, const Place<kMode, 16 / sizeof(E)>& place,
-                                  const RotaryTensor* tensors, uint4* ring)
-      : p(params), cut(c), at(place), in(tensors), mine(ring + threadIdx.x) {
-    all = p.batch * p.tokens;
+  __device__ __forceinline__ Units(const RotaryParams& params, const Cut& c, const Place<kMode, 16 / sizeof(E)>& place,
+                                   const RotaryTensor (&in)[kIn], uint4* ring)
+      : p(params), cut(c), at(place), all(params.batch * params.tokens), mine(ring + threadIdx.x) {
     const int64_t n = (all + cut.tile - 1) / cut.tile;
     tiles = n > blockIdx.x ? (n - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
-    for (int i = 0; i < kDepth; ++i) next();
+    passes = (cut.rounds + kUnit - 1) / kUnit;
+    for (int k = 0; k < 2; ++k) {
+      begin(in);
+#pragma unroll
+      for (int r = 0; r < kUnit; ++r) copy(in, k, r);
+    }
   }
   __device__ __forceinline__ int64_t first(int64_t tile) const { return (blockIdx.x + tile * gridDim.x) * cut.tile; }
-  // Starts the copy of one more row into the entry that was read last.
-  __device__ __forceinline__ void next() {
-    if (j < tiles) {
-      if (r == 0) {
-        const int64_t token = first(j) + at.t;
-        here = at.live && token < all;
-        if (here) {
-          const int64_t b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
+  // Before a unit's copies.
+  __device__ __forceinline__ void begin(const RotaryTensor (&in)[kIn]) {
+    if (pass == 0) {
+      const int64_t token = first(j) + at.t;
+      heads_left = at.live && j < tiles && token < all ? in[0].heads - at.slot : 0;
+      if (heads_left > 0) {
+        const int64_t b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
 #pragma unroll
-          for (int i = 0; i < kIn; ++i)
-            row[i] = static_cast<const E*>(in[i].in) + b * in[i].stride_b + l * in[i].stride_t + at.slot * in[i].stride_h;
-        }
-      }
-      if (here && at.slot + r * at.step < in[0].heads) {
-        uint4* to = mine + entry * kVecs * blockDim.x;
-#pragma unroll
-        for (int i = 0; i < kIn; ++i) {
-          if (at.rotates) copy16(to + i * kPer * blockDim.x, row[i] + at.c0);
-          if constexpr (kMode == kHalves) copy16(to + (i * kPer + 1) * blockDim.x, row[i] + at.c1);
-          row[i] += at.step * in[i].stride_h;
-        }
-      }
-      if (++r == cut.rounds) {
-        r = 0;
-        ++j;
+        for (int i = 0; i < kIn; ++i)
+          row[i] = static_cast<const E*>(in[i].in) + b * in[i].stride_b + l * in[i].stride_t + at.slot * in[i].stride_h;
       }
     }
-    copies_commit();
-    entry = entry + 1 == kDepth ? 0 : entry + 1;
+    if (++pass == passes) {
+      pass = 0;
+      ++j;
+    }
   }
-  // The oldest row has arrived. (kAny reads its neighbours' columns.)
+  // Head r of the unit, into half k of the ring.
+  __device__ __forceinline__ void copy(const RotaryTensor (&in)[kIn], int k, int r) {
+    if (heads_left > 0) {
+      uint4* to = mine + (k * kUnit + r) * kVecs * blockDim.x;
+#pragma unroll
+      for (int i = 0; i < kIn; ++i) {
+        if (at.rotates) copy16(to + i * kPer * blockDim.x, row[i] + at.c0);
+        if constexpr (kMode == kHalves) copy16(to + (i * kPer + 1) * blockDim.x, row[i] + at.c1);
+        row[i] += at.step * in[i].stride_h;
+      }
+    }
+    heads_left -= at.step;
+    copies_commit();
+  }
+  // The oldest head has arrived. (kAny reads its neighbours' columns.)
   __device__ __forceinline__ void arrived() const {
-    copies_wait<kDepth - 1>();
+    copies_wait<kRing - 1>();
     if constexpr (kMode == kAny) __syncwarp();
   }
-  __device__ __forceinline__ uint4 get(int v) const { return mine[(entry * kVecs + v) * blockDim.x]; }
+  __device__ __forceinline__ uint4 get(int k, int r, int v) const { return mine[((k * kUnit + r) * kVecs + v) * blockDim.x]; }
   // Column c of the head, of input i (kAny).
-  __device__ __forceinline__ float element(int i, int c) const {
-    return to_f(reinterpret_cast<const E*>(mine + (entry * kVecs + i * kPer) * blockDim.x - at.u)[c]);
+  __device__ __forceinline__ float element(int k, int r, int i, int c) const {
+    return to_f(reinterpret_cast<const E*>(mine + ((k * kUnit + r) * kVecs + i * kPer) * blockDim.x - at.u)[c]);
   }
 };
 
@@ -262,37 +318,38 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
   constexpr bool kAppend = std::is_same_v<P, CacheAppendParams>;
   constexpr int V = 16 / sizeof(E), kPairs = V / 2, kTwo = kMode == kHalves ? kPairs : 1;
   using Pair = PairOf<E>;
-  using R = Rows<E, kMode, 1, kFwdRing>;
+  using U = Units<E, kMode, 1, kFwdUnit>;
   union Vec {
     uint4 v;
     typename Pair::Raw w[kPairs];
   };
-  extern __shared__ uint4 ring[];  // then, twice, a tile's angles and (append) places
-  const int half = p.rotary_dim >> 1, angles = (cut.tile * half + 1) / 2 * 2;
-  float2* const cs = reinterpret_cast<float2*>(ring + kFwdRing * R::kVecs * blockDim.x);
-  AppendPlace* const places = reinterpret_cast<AppendPlace*>(cs + 2 * angles);
+  // inv_freq / 2 pi; twice a tile's (append) places and angles; the ring
+  extern __shared__ uint4 shared[];
+  const int half = p.rotary_dim >> 1, angles = 2 * cut.tile * angle_row(p.rotary_dim);
+  double* const turns = reinterpret_cast<double*>(shared);
+  AppendPlace* const places = reinterpret_cast<AppendPlace*>(turns + (half + 1) / 2 * 2);
+  float* const cs = reinterpret_cast<float*>(places + (kAppend ? 2 * cut.tile : 0));
   const Place<kMode, V> at(p, cut);
-  RotaryTensor x = p.x[at.kind & 1];
+  RotaryTensor x[1] = {p.x[at.kind & 1]};
   if constexpr (kAppend)
-    if (at.kind == 2) x = p.v;
-  R rows(p, cut, at, &x, ring);
+    if (at.kind == 2) x[0] = p.v;
+  U units(p, cut, at, x, reinterpret_cast<uint4*>(cs + 2 * angles));
 
   // angles and places of the CTA's tile j
   auto prepare = [&](int64_t j) {
-    const int64_t first = rows.first(j);
-    const int here = int(rows.all - first < cut.tile ? rows.all - first : cut.tile);
+    const int64_t first = units.first(j);
+    const int here = int(units.all - first < cut.tile ? units.all - first : cut.tile);
     if constexpr (kAppend) {
       for (int i = threadIdx.x >> 5; i < here; i += blockDim.x >> 5) {
         const AppendPlace to = append_place(p, int(first) + i, threadIdx.x & 31);
         if ((threadIdx.x & 31) == 0) places[(j & 1) * cut.tile + i] = to;
       }
     }
-    for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
-      const int tt = i / half;
-      cs[(j & 1) * angles + i] = rotary_angle(p, first + tt, i - tt * half);
-    }
+    tile_angles<sizeof(E) == 2>(p, turns, first, here, cs + (j & 1) * angles);
   };
-  if (rows.tiles > 0) prepare(0);
+  for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * 0.15915494309189535;
+  __syncthreads();
+  if (units.tiles > 0) prepare(0);
   uint64_t w0[kPairs], w1[kTwo], wo[kMode == kAny ? kPairs : 1];
   if constexpr (kNorm) {
     constexpr bool kHalfType = std::is_same_v<E, __half>;
@@ -308,83 +365,90 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
       if constexpr (kMode == kAny) wo[k] = weights(partner(c, half), partner(c + 1, half));
     }
   }
-  const bool turns = !kAppend || at.kind < 2;
+  const bool rotated = !kAppend || at.kind < 2;
   const float inv = 1.f / float(p.head_dim);
-  for (int64_t j = 0; j < rows.tiles; ++j) {
+  int k = 0;  // half of the ring
+  for (int64_t j = 0; j < units.tiles; ++j) {
     __syncthreads();  // the tile's angles are there, and those of the tile before have been read
-    if (j + 1 < rows.tiles) prepare(j + 1);
-    const int64_t token = rows.first(j) + at.t;
-    const int heads = at.live && token < rows.all ? x.heads : 0;
+    if (j + 1 < units.tiles) prepare(j + 1);
+    const int64_t token = units.first(j) + at.t;
+    int left = at.live && token < units.all ? x[0].heads - at.slot : 0;  // heads from this one on
     E* out = nullptr;
     int64_t out_h = p.head_dim;
-    if (heads > 0) {
-      if (!kAppend || at.kind == 0) out = static_cast<E*>(x.out) + token * x.heads * p.head_dim;
+    uint64_t co[kPairs], si[kPairs];
+    if (left > 0) {
+      if (!kAppend || at.kind == 0) out = static_cast<E*>(x[0].out) + token * x[0].heads * p.head_dim;
       if constexpr (kAppend) {
         const AppendPlace to = places[(j & 1) * cut.tile + at.t];
         if (at.kind == 1 && to.k >= 0) out = static_cast<E*>(p.k_pool) + to.k;
         if (at.kind == 2 && to.v >= 0) out = static_cast<E*>(p.v_pool) + to.v;
         if (at.kind) out_h = at.kind == 1 ? p.k_stride[2] : p.v_stride[2];
       }
+      column_angles<kMode>(p, cs + (j & 1) * angles + 2 * at.t * angle_row(p.rotary_dim),
+                           kMode == kHalves && !at.rotates ? p.rotary_dim : at.c0, co, si);
     }
-    uint64_t co[kPairs], si[kPairs];
-    column_angles<kMode>(p, cs + (j & 1) * angles + at.t * half,
-                         (kMode == kHalves && !at.rotates) || heads == 0 ? p.rotary_dim : at.c0, co, si);
-    for (int r = 0; r < cut.rounds; ++r) {
-      const int h = at.slot + r * at.step;
-      const bool valid = h < heads;
-      rows.arrived();
-      Vec x0, x1;
-      x0.v = x1.v = make_uint4(0, 0, 0, 0);
-      if (valid && at.rotates) x0.v = rows.get(0);
-      if constexpr (kMode == kHalves)
-        if (valid) x1.v = rows.get(1);
-      uint64_t a[kPairs], d[kPairs];
+    E* row = out + at.slot * out_h;
+    for (int i = 0; i < units.passes; ++i, k ^= 1) {
+      units.begin(x);
 #pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        a[k] = Pair::wide(x0.w[k]);
-        if constexpr (kMode == kHalves) d[k] = Pair::wide(x1.w[k]);
-        if constexpr (kMode == kNeighbours) d[k] = swapped(a[k]);
-        if constexpr (kMode == kAny) {
-          const int c = at.c0 + 2 * k;
-          d[k] = valid ? f2_pack(rows.element(0, partner(c, half)), rows.element(0, partner(c + 1, half))) : 0;
-        }
-      }
-      if constexpr (kNorm) {
-        uint64_t sq = 0;
+      for (int r = 0; r < kFwdUnit; ++r) {
+        units.arrived();
+        if (i * kFwdUnit + r < cut.rounds) {
+          Vec x0, x1;
+          x0.v = x1.v = make_uint4(0, 0, 0, 0);
+          if (left > 0) {
+            if (at.rotates) x0.v = units.get(k, r, 0);
+            if constexpr (kMode == kHalves) x1.v = units.get(k, r, 1);
+          }
+          uint64_t a[kPairs], d[kPairs];
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-          sq = f2_fma(a[k], a[k], sq);
-          if constexpr (kMode == kHalves) sq = f2_fma(d[k], d[k], sq);
-        }
-        const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
-        const uint64_t scale = f2_pack(rstd, rstd);
+          for (int n = 0; n < kPairs; ++n) {
+            a[n] = Pair::wide(x0.w[n]);
+            if constexpr (kMode == kHalves) d[n] = Pair::wide(x1.w[n]);
+            if constexpr (kMode == kNeighbours) d[n] = swapped(a[n]);
+            if constexpr (kMode == kAny) {
+              const int c = at.c0 + 2 * n;
+              d[n] = left > 0 ? f2_pack(units.element(k, r, 0, partner(c, half)), units.element(k, r, 0, partner(c + 1, half))) : 0;
+            }
+          }
+          uint64_t scale = 0;
+          if constexpr (kNorm) {
+            uint64_t sq = 0;
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-          const uint64_t w = w0[k];
-          a[k] = f2_mul(f2_mul(a[k], scale), w);
-          d[k] = f2_mul(f2_mul(d[k], scale), kMode == kHalves ? w1[kMode == kHalves ? k : 0]
-                                             : kMode == kAny  ? wo[kMode == kAny ? k : 0]
-                                                              : swapped(w));
-        }
-      }
-      if (turns) {
+            for (int n = 0; n < kPairs; ++n) {
+              sq = f2_fma(a[n], a[n], sq);
+              if constexpr (kMode == kHalves) sq = f2_fma(d[n], d[n], sq);
+            }
+            const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
+            scale = f2_pack(rstd, rstd);
+          }
+          if (left > 0 && out) {
+            if (rotated) {
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-          // without the norm the columns behind rotary_dim are copies, bit for bit
-          if (kNorm || (kMode == kHalves ? at.rotates : at.c0 + 2 * k < p.rotary_dim))
-            x0.w[k] = Pair::narrow(f2_fma(a[k], co[k], f2_mul(d[k], si[k])));
-          if constexpr (kMode == kHalves)
-            if (kNorm || at.rotates)
-              x1.w[k] = Pair::narrow(at.rotates ? f2_sub(f2_mul(d[k], co[k]), f2_mul(a[k], si[k])) : d[k]);
+              for (int n = 0; n < kPairs; ++n) {
+                if constexpr (kNorm) {
+                  a[n] = f2_mul(f2_mul(a[n], scale), w0[n]);
+                  d[n] = f2_mul(f2_mul(d[n], scale), kMode == kHalves ? w1[kMode == kHalves ? n : 0]
+                                                     : kMode == kAny  ? wo[kMode == kAny ? n : 0]
+                                                                      : swapped(w0[n]));
+                }
+                // without the norm the columns behind rotary_dim are copies, bit for bit
+                if (kNorm || (kMode == kHalves ? at.rotates : at.c0 + 2 * n < p.rotary_dim))
+                  x0.w[n] = Pair::narrow(f2_fma(a[n], co[n], f2_mul(d[n], si[n])));
+                if constexpr (kMode == kHalves)
+                  if (kNorm || at.rotates)
+                    x1.w[n] = Pair::narrow(at.rotates ? f2_sub(f2_mul(d[n], co[n]), f2_mul(a[n], si[n])) : d[n]);
+              }
+            }
+            if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0.v;
+            if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1.v;
+          }
+          left -= at.step;
+          row += at.step * out_h;
         }
+        if constexpr (kMode == kAny) __syncwarp();
+        units.copy(x, k, r);
       }
-      if (valid && out) {
-        E* row = out + h * out_h;
-        if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0.v;
-        if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1.v;
-      }
-      if constexpr (kMode == kAny) __syncwarp();
-      rows.next();
     }
   }
   copies_wait<0>();
@@ -396,112 +460,125 @@ template <class E, int kMode>
 __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const NormRotaryParams p, const Cut cut) {
   constexpr int V = 16 / sizeof(E), kPairs = V / 2, kTwo = kMode == kHalves ? kPairs : 1;
   using Pair = PairOf<E>;
-  using R = Rows<E, kMode, 2, kBwdRing>;
+  using U = Units<E, kMode, 2, kBwdUnit>;
   union Vec {
     uint4 v;
     typename Pair::Raw w[kPairs];
   };
-  extern __shared__ uint4 ring[];  // then, twice, a tile's angles; at the end the weights' gradients
+  // inv_freq / 2 pi, twice a tile's angles, the ring; at the end the weights' gradients
+  extern __shared__ uint4 shared[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int half = p.rotary_dim >> 1, angles = cut.tile * half;
-  float2* const cs = reinterpret_cast<float2*>(ring + kBwdRing * R::kVecs * blockDim.x);
+  const int half = p.rotary_dim >> 1, angles = 2 * cut.tile * angle_row(p.rotary_dim);
+  double* const turns = reinterpret_cast<double*>(shared);
+  float* const cs = reinterpret_cast<float*>(turns + (half + 1) / 2 * 2);
   const Place<kMode, V> at(p, cut);
-  const RotaryTensor tensors[2] = {p.x[at.kind], p.dy[at.kind]};
-  R rows(p, cut, at, tensors, ring);
+  const RotaryTensor in[2] = {p.x[at.kind], p.dy[at.kind]};
+  U units(p, cut, at, in, reinterpret_cast<uint4*>(cs + 2 * angles));
   auto prepare = [&](int64_t j) {
-    const int64_t first = rows.first(j);
-    const int here = int(rows.all - first < cut.tile ? rows.all - first : cut.tile);
-    for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
-      const int tt = i / half;
-      cs[(j & 1) * angles + i] = rotary_angle(p, first + tt, i - tt * half);
-    }
+    const int64_t first = units.first(j);
+    const int here = int(units.all - first < cut.tile ? units.all - first : cut.tile);
+    tile_angles<sizeof(E) == 2>(p, turns, first, here, cs + (j & 1) * angles);
   };
-  if (rows.tiles > 0) prepare(0);
+  for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * 0.15915494309189535;
+  __syncthreads();
+  if (units.tiles > 0) prepare(0);
   constexpr bool kHalfType = std::is_same_v<E, __half>;
   uint64_t w0[kPairs], w1[kTwo], acc0[kPairs], acc1[kTwo];
 #pragma unroll
-  for (int k = 0; k < kPairs; ++k) {
-    acc0[k] = w0[k] = 0;
+  for (int n = 0; n < kPairs; ++n) {
+    acc0[n] = w0[n] = 0;
     if (at.live)
-      w0[k] = f2_pack(weight_at(p, at.kind, at.c0 + 2 * k, kHalfType), weight_at(p, at.kind, at.c0 + 2 * k + 1, kHalfType));
+      w0[n] = f2_pack(weight_at(p, at.kind, at.c0 + 2 * n, kHalfType), weight_at(p, at.kind, at.c0 + 2 * n + 1, kHalfType));
     if constexpr (kMode == kHalves) {
-      acc1[k] = w1[k] = 0;
+      acc1[n] = w1[n] = 0;
       if (at.live)
-        w1[k] = f2_pack(weight_at(p, at.kind, at.c1 + 2 * k, kHalfType), weight_at(p, at.kind, at.c1 + 2 * k + 1, kHalfType));
+        w1[n] = f2_pack(weight_at(p, at.kind, at.c1 + 2 * n, kHalfType), weight_at(p, at.kind, at.c1 + 2 * n + 1, kHalfType));
     }
   }
   const float inv = 1.f / float(p.head_dim);
-  for (int64_t j = 0; j < rows.tiles; ++j) {
+  int k = 0;  // half of the ring
+  for (int64_t j = 0; j < units.tiles; ++j) {
     __syncthreads();  // the tile's angles are there, and those of the tile before have been read
-    if (j + 1 < rows.tiles) prepare(j + 1);
-    const int64_t token = rows.first(j) + at.t;
-    const int heads = at.live && token < rows.all ? tensors[0].heads : 0;
-    E* const dx = static_cast<E*>(tensors[0].out) + token * tensors[0].heads * p.head_dim;
+    if (j + 1 < units.tiles) prepare(j + 1);
+    const int64_t token = units.first(j) + at.t;
+    int left = at.live && token < units.all ? in[0].heads - at.slot : 0;  // heads from this one on
+    E* row = static_cast<E*>(in[0].out) + (token * in[0].heads + at.slot) * p.head_dim;
     uint64_t co[kPairs], si[kPairs];
-    column_angles<kMode>(p, cs + (j & 1) * angles + at.t * half,
-                         (kMode == kHalves && !at.rotates) || heads == 0 ? p.rotary_dim : at.c0, co, si);
-    for (int r = 0; r < cut.rounds; ++r) {
-      const int h = at.slot + r * at.step;
-      const bool valid = h < heads;
-      rows.arrived();
-      Vec x0, x1, y0, y1;
-      x0.v = x1.v = y0.v = y1.v = make_uint4(0, 0, 0, 0);
-      if (valid && at.rotates) {
-        x0.v = rows.get(0);
-        y0.v = rows.get(R::kPer);
-      }
-      if constexpr (kMode == kHalves)
-        if (valid) {
-          x1.v = rows.get(1);
-          y1.v = rows.get(3);
-        }
-      uint64_t g0[kPairs], g1[kTwo], sq = 0, dot = 0;
+    // (lanes without columns have to add nothing to their group's sums, whatever lies there)
+    column_angles<kMode>(p, cs + (j & 1) * angles + 2 * (left > 0 ? at.t : 0) * angle_row(p.rotary_dim),
+                         left > 0 && (kMode != kHalves || at.rotates) ? at.c0 : p.rotary_dim, co, si);
+    for (int i = 0; i < units.passes; ++i, k ^= 1) {
+      units.begin(in);
 #pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        const uint64_t e = Pair::wide(y0.w[k]), a = Pair::wide(x0.w[k]);
-        uint64_t f = 0;
-        if constexpr (kMode == kHalves) f = Pair::wide(y1.w[k]);
-        if constexpr (kMode == kNeighbours) f = swapped(e);
-        if constexpr (kMode == kAny) {
-          const int c = at.c0 + 2 * k;
-          if (valid) f = f2_pack(rows.element(1, partner(c, half)), rows.element(1, partner(c + 1, half)));
+      for (int r = 0; r < kBwdUnit; ++r) {
+        units.arrived();
+        if (i * kBwdUnit + r >= cut.rounds) {
+          units.copy(in, k, r);
+          continue;
         }
-        g0[k] = f2_fma(e, co[k], f2_mul(f, si[k]));
-        sq = f2_fma(a, a, sq);
-        dot = f2_fma(f2_mul(g0[k], w0[k]), a, dot);
-        if constexpr (kMode == kHalves) {
-          const uint64_t d = Pair::wide(x1.w[k]);
-          g1[k] = f2_sub(f2_mul(f, co[k]), f2_mul(e, si[k]));
-          sq = f2_fma(d, d, sq);
-          dot = f2_fma(f2_mul(g1[k], w1[k]), d, dot);
+        Vec x0, x1, y0, y1;
+        x0.v = x1.v = y0.v = y1.v = make_uint4(0, 0, 0, 0);
+        if (left > 0) {
+          if (at.rotates) {
+            x0.v = units.get(k, r, 0);
+            y0.v = units.get(k, r, U::kPer);
+          }
+          if constexpr (kMode == kHalves) {
+            x1.v = units.get(k, r, 1);
+            y1.v = units.get(k, r, 3);
+          }
         }
-      }
-      if constexpr (kMode == kAny) __syncwarp();
-      rows.next();
-      const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
-      const float along = group_sum(pair_sum(dot), cut.lanes_log) * inv * rstd * rstd;
-      if (!valid) continue;
-      const uint64_t scale = f2_pack(rstd, rstd), minus = f2_pack(-along, -along);
+        uint64_t g0[kPairs], g1[kTwo], sq = 0, dot = 0;
 #pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        const uint64_t a = Pair::wide(x0.w[k]);
-        acc0[k] = f2_fma(g0[k], f2_mul(a, scale), acc0[k]);
-        x0.w[k] = Pair::narrow(f2_mul(scale, f2_fma(g0[k], w0[k], f2_mul(a, minus))));
-        if constexpr (kMode == kHalves) {
-          const uint64_t d = Pair::wide(x1.w[k]);
-          acc1[k] = f2_fma(g1[k], f2_mul(d, scale), acc1[k]);
-          x1.w[k] = Pair::narrow(f2_mul(scale, f2_fma(g1[k], w1[k], f2_mul(d, minus))));
+        for (int n = 0; n < kPairs; ++n) {
+          const uint64_t e = Pair::wide(y0.w[n]), a = Pair::wide(x0.w[n]);
+          uint64_t f = 0;
+          if constexpr (kMode == kHalves) f = Pair::wide(y1.w[n]);
+          if constexpr (kMode == kNeighbours) f = swapped(e);
+          if constexpr (kMode == kAny) {
+            const int c = at.c0 + 2 * n;
+            if (left > 0) f = f2_pack(units.element(k, r, 1, partner(c, half)), units.element(k, r, 1, partner(c + 1, half)));
+          }
+          g0[n] = f2_fma(e, co[n], f2_mul(f, si[n]));
+          sq = f2_fma(a, a, sq);
+          dot = f2_fma(f2_mul(g0[n], w0[n]), a, dot);
+          if constexpr (kMode == kHalves) {
+            const uint64_t d = Pair::wide(x1.w[n]);
+            g1[n] = f2_sub(f2_mul(f, co[n]), f2_mul(e, si[n]));
+            sq = f2_fma(d, d, sq);
+            dot = f2_fma(f2_mul(g1[n], w1[n]), d, dot);
+          }
         }
+        if constexpr (kMode == kAny) __syncwarp();
+        units.copy(in, k, r);
+        // (groups without a head have the sums of nothing)
+        const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
+        const float along = group_sum(pair_sum(dot), cut.lanes_log) * inv * rstd * rstd;
+        if (left > 0) {
+          const uint64_t scale = f2_pack(rstd, rstd), minus = f2_pack(-along, -along);
+#pragma unroll
+          for (int n = 0; n < kPairs; ++n) {
+            const uint64_t a = Pair::wide(x0.w[n]);
+            acc0[n] = f2_fma(g0[n], f2_mul(a, scale), acc0[n]);
+            x0.w[n] = Pair::narrow(f2_mul(scale, f2_fma(g0[n], w0[n], f2_mul(a, minus))));
+            if constexpr (kMode == kHalves) {
+              const uint64_t d = Pair::wide(x1.w[n]);
+              acc1[n] = f2_fma(g1[n], f2_mul(d, scale), acc1[n]);
+              x1.w[n] = Pair::narrow(f2_mul(scale, f2_fma(g1[n], w1[n], f2_mul(d, minus))));
+            }
+          }
+          if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0.v;
+          if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1.v;
+        }
+        left -= at.step;
+        row += at.step * p.head_dim;
       }
-      E* row = dx + h * p.head_dim;
-      if (at.rotates) *reinterpret_cast<uint4*>(row + at.c0) = x0.v;
-      if constexpr (kMode == kHalves) *reinterpret_cast<uint4*>(row + at.c1) = x1.v;
     }
   }
   copies_wait<0>();
   if (!p.dw_part) return;
   // [group][head_dim]
-  float* const sums = reinterpret_cast<float*>(ring);
+  float* const sums = reinterpret_cast<float*>(shared);
   __syncthreads();
   if (at.live) {
     float* mine = sums + (threadIdx.x >> cut.lanes_log) * p.head_dim;
@@ -641,6 +718,11 @@ void cuda_ok(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("norm and rotary positions: ") + cudaGetErrorString(e));
 }
 
+// Bytes of the frequencies and of two tiles' angles in shared memory.
+size_t turns_and_angles(const RotaryParams& p, const Cut& cut) {
+  return size_t(p.rotary_dim / 2 + 1) / 2 * 2 * sizeof(double) + 4 * size_t(cut.tile) * angle_row(p.rotary_dim) * sizeof(float);
+}
+
 // The CTAs of a launch: as many as run at once.
 template <auto fn, class P>
 void launch_tiles(const P& p, const Cut& cut, int64_t tokens, int ctas, size_t smem, cudaStream_t s) {
@@ -658,9 +740,9 @@ void fwd_mode(const P& p, int sm_count, cudaStream_t s) {
   if constexpr (kAppend) heads[2] = p.v.heads;
   const int64_t all = p.batch * p.tokens;
   const Cut cut = make_cut(lanes_of(kMode, V, p.head_dim, p.rotary_dim), heads, all, sm_count);
-  const size_t angles = (size_t(cut.tile) * (p.rotary_dim / 2) + 1) / 2 * 2;
-  const size_t smem = sizeof(uint4) * kFwdRing * Rows<E, kMode, 1, kFwdRing>::kVecs * cut.threads +
-                      2 * angles * sizeof(float2) + (kAppend ? 2 * cut.tile * sizeof(AppendPlace) : 0);
+  using U = Units<E, kMode, 1, kFwdUnit>;
+  const size_t smem = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * cut.threads +
+                      (kAppend ? 2 * cut.tile * sizeof(AppendPlace) : 0);
   launch_tiles<norm_rotary_kernel<E, kMode, kNorm, P>>(p, cut, all, 2 * sm_count, smem, s);
 }
 
@@ -695,8 +777,8 @@ int bwd_parts(const NormRotaryParams& p, int sm_count) {
 template <class E, int kMode>
 void bwd_mode(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
   const Cut cut = bwd_cut<E>(p, kMode, sm_count);
-  const size_t ring = sizeof(uint4) * kBwdRing * Rows<E, kMode, 2, kBwdRing>::kVecs * cut.threads +
-                      2 * size_t(cut.tile) * (p.rotary_dim / 2) * sizeof(float2);
+  using U = Units<E, kMode, 2, kBwdUnit>;
+  const size_t ring = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * cut.threads;
   const size_t sums = p.dw_part ? size_t(cut.threads >> cut.lanes_log) * p.head_dim * sizeof(float) : 0;
   launch_tiles<norm_rotary_bwd_kernel<E, kMode>>(p, cut, p.batch * p.tokens, parts, std::max(ring, sums), s);
 }

@@ -36,13 +36,16 @@ struct RotaryParams {
 #ifdef __CUDACC__
 namespace dev {
 
-// (cos, sin) * magnitude of pair f at a token.
-__device__ __forceinline__ float2 rotary_angle(const RotaryParams& p, int64_t token, int f) {
+__device__ __forceinline__ double rotary_position(const RotaryParams& p, int64_t token) {
   const int64_t b = p.batch == 1 ? 0 : token / p.tokens, l = token - b * p.tokens;
   const int64_t at = b * p.pos_stride_b + l * p.pos_stride_t;
-  const double pos = p.positions64 ? double(static_cast<const int64_t*>(p.positions)[at])
-                                   : double(static_cast<const int32_t*>(p.positions)[at]);
-  double turns = pos * p.inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
+  return p.positions64 ? double(static_cast<const int64_t*>(p.positions)[at])
+                       : double(static_cast<const int32_t*>(p.positions)[at]);
+}
+
+// (cos, sin) * magnitude of pair f at a token.
+__device__ __forceinline__ float2 rotary_angle(const RotaryParams& p, int64_t token, int f) {
+  double turns = rotary_position(p, token) * p.inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
   turns -= rint(turns);
   float s, c;
   sincospif(float(2.0 * turns), &s, &c);
