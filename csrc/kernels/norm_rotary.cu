@@ -109,7 +109,9 @@ struct Place {
 
 // The sum over the 2^log lanes of a group.
 __device__ __forceinline__ float group_sum(float v, int log) {
-  for (int o = 0; o < log; ++o) v += __shfl_xor_sync(0xffffffffu, v, 1 << o);
+#pragma unroll
+  for (int o = 0; o < 5; ++o)
+    if (o < log) v += __shfl_xor_sync(0xffffffffu, v, 1 << o);
   return v;
 }
 
@@ -255,6 +257,7 @@ struct Units {
   int64_t j = 0;
   int pass = 0, heads_left = 0;
   const E* row[kIn];
+  int64_t row_step[kIn];
 
   __device__ __forceinline__ Units(const RotaryParams& params, const Cut& c, const Place<kMode, 16 / sizeof(E)>& place,
                                    const RotaryTensor (&in)[kIn], uint4* ring)
@@ -262,10 +265,12 @@ struct Units {
     const int64_t n = (all + cut.tile - 1) / cut.tile;
     tiles = n > blockIdx.x ? (n - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
     passes = (cut.rounds + kUnit - 1) / kUnit;
+#pragma unroll
+    for (int i = 0; i < kIn; ++i) row_step[i] = at.step * in[i].stride_h;
     for (int k = 0; k < 2; ++k) {
       begin(in);
 #pragma unroll
-      for (int r = 0; r < kUnit; ++r) copy(in, k, r);
+      for (int r = 0; r < kUnit; ++r) copy(k, r);
     }
   }
   __device__ __forceinline__ int64_t first(int64_t tile) const { return (blockIdx.x + tile * gridDim.x) * cut.tile; }
@@ -287,14 +292,14 @@ struct Units {
     }
   }
   // Head r of the unit, into half k of the ring.
-  __device__ __forceinline__ void copy(const RotaryTensor (&in)[kIn], int k, int r) {
+  __device__ __forceinline__ void copy(int k, int r) {
     if (heads_left > 0) {
-      uint4* to = mine + (k * kUnit + r) * kVecs * blockDim.x;
+      uint4* to = mine + (k * kUnit + r) * kVecs * kThreads;
 #pragma unroll
       for (int i = 0; i < kIn; ++i) {
-        if (at.rotates) copy16(to + i * kPer * blockDim.x, row[i] + at.c0);
-        if constexpr (kMode == kHalves) copy16(to + (i * kPer + 1) * blockDim.x, row[i] + at.c1);
-        row[i] += at.step * in[i].stride_h;
+        if (at.rotates) copy16(to + i * kPer * kThreads, row[i] + at.c0);
+        if constexpr (kMode == kHalves) copy16(to + (i * kPer + 1) * kThreads, row[i] + at.c1);
+        row[i] += row_step[i];
       }
     }
     heads_left -= at.step;
@@ -305,10 +310,10 @@ struct Units {
     copies_wait<kRing - 1>();
     if constexpr (kMode == kAny) __syncwarp();
   }
-  __device__ __forceinline__ uint4 get(int k, int r, int v) const { return mine[((k * kUnit + r) * kVecs + v) * blockDim.x]; }
+  __device__ __forceinline__ uint4 get(int k, int r, int v) const { return mine[((k * kUnit + r) * kVecs + v) * kThreads]; }
   // Column c of the head, of input i (kAny).
   __device__ __forceinline__ float element(int k, int r, int i, int c) const {
-    return to_f(reinterpret_cast<const E*>(mine + ((k * kUnit + r) * kVecs + i * kPer) * blockDim.x - at.u)[c]);
+    return to_f(reinterpret_cast<const E*>(mine + ((k * kUnit + r) * kVecs + i * kPer) * kThreads - at.u)[c]);
   }
 };
 
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
           row += at.step * out_h;
         }
         if constexpr (kMode == kAny) __syncwarp();
-        units.copy(x, k, r);
+        units.copy(k, r);
       }
     }
   }
@@ -513,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const Norm
       for (int r = 0; r < kBwdUnit; ++r) {
         units.arrived();
         if (i * kBwdUnit + r >= cut.rounds) {
-          units.copy(in, k, r);
+          units.copy(k, r);
           continue;
         }
         Vec x0, x1, y0, y1;
@@ -550,10 +555,16 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const Norm
           }
         }
         if constexpr (kMode == kAny) __syncwarp();
-        units.copy(in, k, r);
+        units.copy(k, r);
         // (groups without a head have the sums of nothing)
-        const float rstd = rsqrtf(group_sum(pair_sum(sq), cut.lanes_log) * inv + p.eps);
-        const float along = group_sum(pair_sum(dot), cut.lanes_log) * inv * rstd * rstd;
+        float both[2] = {pair_sum(sq), pair_sum(dot)};
+#pragma unroll
+        for (int o = 0; o < 5; ++o)
+          if (o < cut.lanes_log) {
+            both[0] += __shfl_xor_sync(0xffffffffu, both[0], 1 << o);
+            both[1] += __shfl_xor_sync(0xffffffffu, both[1], 1 << o);
+          }
+        const float rstd = rsqrtf(both[0] * inv + p.eps), along = both[1] * inv * rstd * rstd;
         if (left > 0) {
           const uint64_t scale = f2_pack(rstd, rstd), minus = f2_pack(-along, -along);
 #pragma unroll
@@ -741,7 +752,7 @@ void fwd_mode(const P& p, int sm_count, cudaStream_t s) {
   const int64_t all = p.batch * p.tokens;
   const Cut cut = make_cut(lanes_of(kMode, V, p.head_dim, p.rotary_dim), heads, all, sm_count);
   using U = Units<E, kMode, 1, kFwdUnit>;
-  const size_t smem = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * cut.threads +
+  const size_t smem = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * kThreads +
                       (kAppend ? 2 * cut.tile * sizeof(AppendPlace) : 0);
   launch_tiles<norm_rotary_kernel<E, kMode, kNorm, P>>(p, cut, all, 2 * sm_count, smem, s);
 }
@@ -778,7 +789,7 @@ template <class E, int kMode>
 void bwd_mode(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
   const Cut cut = bwd_cut<E>(p, kMode, sm_count);
   using U = Units<E, kMode, 2, kBwdUnit>;
-  const size_t ring = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * cut.threads;
+  const size_t ring = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * kThreads;
   const size_t sums = p.dw_part ? size_t(cut.threads >> cut.lanes_log) * p.head_dim * sizeof(float) : 0;
   launch_tiles<norm_rotary_bwd_kernel<E, kMode>>(p, cut, p.batch * p.tokens, parts, std::max(ring, sums), s);
 }
