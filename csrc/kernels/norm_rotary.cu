@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
@@ -54,15 +55,31 @@ struct Cut {
 };
 
 Cut make_cut(int lanes, const int (&heads)[3], int64_t tokens, int sm_count) {
-  // Four heads a thread share its columns' sines and weights; where tokens are few, each has
-  // threads of its own.
-  const int batch = tokens >= 4 * sm_count ? 4 : 1;
   Cut c;
   c.lanes = lanes;
   c.lanes_log = 0;
   while (1 << c.lanes_log < lanes) ++c.lanes_log;
   const int most = kThreads >> c.lanes_log;
-  int want[3], sum = 0, total = 0;
+  // Heads a thread, which share its columns' angles: not so many that threads run out; of
+  // these the number whose groups are the least idle, a head and a half for the angles counted.
+  // (16384 tokens of 32 + 8 heads of 128: with 4, 8, 10 and 16 heads 67, 60, 61 and 66 us
+  // forward; 900 tokens of 3 times 8 heads of 64 into the cache: with 8 10.8 us, with 1 6.7 us.)
+  const int64_t all = tokens * (heads[0] + heads[1] + heads[2]) << c.lanes_log;
+  const int limit = int(std::max<int64_t>(1, std::min<int64_t>(16, all / (2 * int64_t(kThreads) * sm_count))));
+  int batch = 1, total = 0;
+  float least = INFINITY;
+  for (int i = limit; i > 0; --i) {
+    int slots = 0;
+    for (int h : heads) slots += (h + i - 1) / i;
+    int rounds = 0;
+    for (int h : heads)
+      if (h) rounds = std::max(rounds, (h + (h + i - 1) / i - 1) / ((h + i - 1) / i));
+    if (slots * (rounds + 1.5f) < least) {
+      least = slots * (rounds + 1.5f);
+      batch = i;
+    }
+  }
+  int want[3], sum = 0;
   for (int i = 0; i < 3; ++i) sum += want[i] = (heads[i] + batch - 1) / batch;
   for (int i = 0; i < 3; ++i) {
     c.slots[i] = sum <= most ? want[i] : want[i] ? std::max<int>(1, int64_t(most) * want[i] / sum) : 0;
@@ -142,15 +159,16 @@ __device__ __forceinline__ float weight_at(const NormRotaryParams& p, int kind, 
 // of a pair takes them with, each `angle_row` floats.
 __host__ __device__ inline int angle_row(int rotary_dim) { return (rotary_dim / 2 + 3) / 4 * 4; }
 
-// Those of a tile of tokens [first, first + here). turns: inv_freq / 2 pi. kFast: sine and
-// cosine of the reduced angle to 2^-21, of which 16-bit results see nothing; otherwise to two
-// steps of float32.
+// Those of a tile of tokens [first, first + here). turns: inv_freq / 2 pi, or null before these
+// are there. kFast: sine and cosine of the reduced angle to 2^-21, of which 16-bit results see
+// nothing; otherwise to two steps of float32.
+constexpr double kTurn = 0.15915494309189535;  // 1 / (2 pi)
 template <bool kFast>
 __device__ __forceinline__ void tile_angles(const RotaryParams& p, const double* turns, int64_t first, int here, float* to) {
   const int half = p.rotary_dim >> 1, row = angle_row(p.rotary_dim);
   for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
     const int tt = i / half, f = i - tt * half;
-    double t = rotary_position(p, first + tt) * turns[f];
+    double t = rotary_position(p, first + tt) * (turns ? turns[f] : p.inv_freq[f] * kTurn);
     t -= rint(t);
     float s, c;
     if constexpr (kFast) {
@@ -350,11 +368,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
         if ((threadIdx.x & 31) == 0) places[(j & 1) * cut.tile + i] = to;
       }
     }
-    tile_angles<sizeof(E) == 2>(p, turns, first, here, cs + (j & 1) * angles);
+    tile_angles<sizeof(E) == 2>(p, j ? turns : nullptr, first, here, cs + (j & 1) * angles);
   };
-  for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * 0.15915494309189535;
-  __syncthreads();
   if (units.tiles > 0) prepare(0);
+  if (units.tiles > 1)
+    for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * kTurn;
   uint64_t w0[kPairs], w1[kTwo], wo[kMode == kAny ? kPairs : 1];
   if constexpr (kNorm) {
     constexpr bool kHalfType = std::is_same_v<E, __half>;
@@ -482,11 +500,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const Norm
   auto prepare = [&](int64_t j) {
     const int64_t first = units.first(j);
     const int here = int(units.all - first < cut.tile ? units.all - first : cut.tile);
-    tile_angles<sizeof(E) == 2>(p, turns, first, here, cs + (j & 1) * angles);
+    tile_angles<sizeof(E) == 2>(p, j ? turns : nullptr, first, here, cs + (j & 1) * angles);
   };
-  for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * 0.15915494309189535;
-  __syncthreads();
   if (units.tiles > 0) prepare(0);
+  if (units.tiles > 1)
+    for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * kTurn;
   constexpr bool kHalfType = std::is_same_v<E, __half>;
   uint64_t w0[kPairs], w1[kTwo], acc0[kPairs], acc1[kTwo];
 #pragma unroll
