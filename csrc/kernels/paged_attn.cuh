@@ -85,10 +85,26 @@ struct PagedParams {
   float2* acc_ml = nullptr;  // as parts
   int2* desc = nullptr;      // of the units (paged_desc): the shares that have parts of it, first
                              // and last, or -1 where it is whole
+  // Launches that run side by side take SMs in proportion to their work, which the device
+  // knows: tiles[b] are the tiles a key head of those before sequence or group b, and the same
+  // of the others; a tile takes `cost`.
+  uint32_t* tiles = nullptr;  // [seqs + 1], or null: the launch is alone, and finds out itself
+  const uint32_t* other_tiles[2] = {nullptr, nullptr};
+  float cost = 0.f, other_cost[2] = {0.f, 0.f};  // kv_heads times a tile's time on an SM
+  int sms = 0, sm_ctas = 0;  // of the device; of this launch on an SM
   int4* join = nullptr;  // [grid] of the unit that share c began and others go on with:
                          // its first row of q, first head, rows (0: none), last share
   uint32_t* status = nullptr;
   uint64_t wait_limit_ns = 0;
+};
+
+// The launches for sequences that share prefixes: one of the sequences' own keys, others of
+// groups, by their rows.
+struct PagedSharedParams {
+  PagedParams launch[3];
+  int launches = 0;
+  int own = 0;  // which one
+  const int* member = nullptr;  // [sequences] group, or -1
 };
 
 // Entries of PagedParams::desc a key head, of `seqs` sequences or groups. Their units are
@@ -152,6 +168,11 @@ __device__ __forceinline__ PagedSeq paged_group(const PagedParams& p, int g) {
 __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
   if (p.first && b >= p.own) return paged_group(p, b - p.own);
   PagedSeq s;
+  if (p.no_own) {
+    s.q0 = s.n = s.kv = s.base = s.row = s.skip = 0;
+    s.bad = false;
+    return s;
+  }
   s.skip = 0;
   s.q0 = __ldg(p.cu_q + b);
   int end = __ldg(p.cu_q + b + 1);
@@ -178,7 +199,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
       s.skip = first / p.page;
       s.kv -= first;
     }
-    if (p.no_own) s.n = 0;
   }
   s.base = p.causal ? s.kv - s.n : s.kv;
   return s;
@@ -304,8 +324,11 @@ __device__ __forceinline__ int64_t paged_desc(const PagedParams& p, const PagedS
 }
 
 // At the end of a launch that may have begun early: it ends behind the one before it, so that
-// what waits for this one sees the results of both.
-__device__ __forceinline__ void paged_behind() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// what waits for this one sees the results of both. One CTA is enough, the last, which the others
+// have all begun before: more would keep the SMs from the launch that comes next.
+__device__ __forceinline__ void paged_behind() {
+  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 struct PagedShare {
   const PagedParams& p;
@@ -315,7 +338,8 @@ struct PagedShare {
   __device__ __forceinline__ PagedShare(const PagedParams& params, const uint32_t* pre)
       : p(params), prefix(pre) {
     total = uint64_t(prefix[p.seqs]) * uint32_t(p.kv_heads);
-    per = (total + uint32_t(p.grid) - 1) / uint32_t(p.grid);
+    const uint32_t grid = p.tiles ? prefix[p.seqs + 1] : uint32_t(p.grid);
+    per = (total + grid - 1) / grid;
     if (per < uint32_t(p.min_share)) per = uint32_t(p.min_share);
     snap = per / 2 < uint32_t(p.snap) ? uint32_t(per / 2) : uint32_t(p.snap);
   }
@@ -379,6 +403,36 @@ __device__ __forceinline__ void paged_join(const PagedShare& share, const PagedU
   p.join[blockIdx.x] = j;
 }
 
+// prefix[] from p.tiles, and behind it the CTAs among which the launch's work is divided: its
+// share of the SMs, at least one, the largest launch taking what the others' leave. False for a
+// CTA that is none of them: it should end at once.
+template <int kThreads>
+__device__ __forceinline__ bool paged_divide(const PagedParams& p, uint32_t* prefix) {
+  const uint32_t mine = p.tiles[p.seqs];
+  float work = float(mine) * p.cost, all = work;
+  float others[2];
+  bool largest = true;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    others[i] = p.other_tiles[i] ? float(p.other_tiles[i][p.seqs]) * p.other_cost[i] : 0.f;
+    all += others[i];
+    largest = largest && (others[i] < work || (others[i] == work && p.other_tiles[i] < p.tiles));
+  }
+  if (mine == 0) return false;
+  auto part = [&](float w) { return w > 0.f ? max(1, int(float(p.sms) * (w / all))) : 0; };
+  int sms = part(work);
+  if (largest) sms = max(1, p.sms - part(others[0]) - part(others[1]));
+  const int ctas = min(sms * p.sm_ctas, p.grid);
+  if (int(blockIdx.x) >= ctas) return false;
+  for (int i = threadIdx.x; i < p.seqs; i += kThreads) prefix[i] = p.tiles[i];
+  if (threadIdx.x == 0) {
+    prefix[p.seqs] = mine;
+    prefix[p.seqs + 1] = uint32_t(ctas);
+  }
+  __syncthreads();
+  return true;
+}
+
 // A CTA's way through its work, run by run: tiles [t0, t1) of unit u. Its threads walk
 // alike, each warp's or each its own copy.
 struct PagedWalk {
@@ -397,7 +451,11 @@ struct PagedWalk {
       __syncthreads();
       return any;
     }
-    paged_prefix<kThreads>(p, prefix, sums);
+    if (p.tiles) {
+      if (!paged_divide<kThreads>(p, prefix)) return false;
+    } else {
+      paged_prefix<kThreads>(p, prefix, sums);
+    }
     const PagedShare share(p, prefix);
     begin = share.begin(blockIdx.x, u);
     end = share.end(blockIdx.x);
@@ -475,13 +533,9 @@ void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
 // Sequences that share a prefix: `shared`, `first` and `member` ([own]: its group, or -1) from
 // the page table, for the groups of p. (Nothing but the arrays of the problem is read.)
 void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t stream);
+// Fills the launches' PagedParams::tiles, where they have it.
+void paged_split_launch(const PagedSharedParams& p, cudaStream_t stream);
 // Joins own and shared parts, behind the launches that left them.
-struct PagedSharedParams {
-  PagedParams own;          // of the sequences' own keys
-  PagedParams over[2];      // of the groups' prefixes, by their rows
-  int launches = 0;         // of over
-  const int* member = nullptr;  // [sequences] group, or -1
-};
 void paged_shared_launch(const PagedSharedParams& p, cudaStream_t stream);
 
 }  // namespace mgfa

@@ -557,7 +557,7 @@ void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedPara
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.grid);
   cfg.blockDim = dim3(Smem::kThreads);
-  cfg.dynamicSmemBytes = int(sizeof(Smem)) + 1024 + 4 * (p.seqs + 1);
+  cfg.dynamicSmemBytes = int(sizeof(Smem)) + 1024 + 4 * (p.seqs + 2);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -103,6 +103,19 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
 }
 
+// ---------------------------------------------------------------------- who does what
+constexpr int kSplitThreads = 1024;
+
+// CTA l: the tiles before each sequence and group of launch l (PagedParams::tiles), which its
+// CTAs then need not find out for themselves.
+__global__ void __launch_bounds__(kSplitThreads) paged_split_kernel(const __grid_constant__ PagedSharedParams p) {
+  extern __shared__ uint32_t prefix[];
+  __shared__ uint32_t sums[kSplitThreads / 32];
+  const PagedParams& l = p.launch[blockIdx.x];
+  paged_prefix<kSplitThreads>(l, prefix, sums);
+  for (int i = threadIdx.x; i <= l.seqs; i += kSplitThreads) l.tiles[i] = prefix[i];
+}
+
 // ---------------------------------------------------------------------- the join
 constexpr int kJoinWarps = 16;
 
@@ -147,7 +160,7 @@ template <int kD, bool kF16, int kSplit>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_shared_kernel(const __grid_constant__ PagedSharedParams p) {
   constexpr int kE = kD / 32, kRows = kJoinWarps / kSplit;
   __shared__ float sh[kSplit > 1 ? kJoinWarps : 1][kD];
-  const PagedParams& a = p.own;
+  const PagedParams& a = p.launch[p.own];
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
   const PagedSeq own = paged_seq(a, b);
   const int64_t rows = int64_t(own.n) * a.heads;
@@ -159,7 +172,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_shared_kernel(const __g
     g = p.member[b];
     if (g >= 0 && g < a.seqs - a.own) {
       for (; taken < p.launches; ++taken) {
-        over = paged_group(p.over[taken], g);
+        over = paged_group(p.launch[taken], g);
         if (over.n > 0) break;
       }
       const bool inside = own.q0 >= over.q0 && own.q0 + own.n <= over.q0 + over.n;
@@ -180,7 +193,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_shared_kernel(const __g
       RowParts side[2];
       side[0] = row_parts(a, own, b, i, head);
       side[1].n = 0;
-      if (over.n > 0) side[1] = row_parts(p.over[taken], over, a.own + g, own.q0 + i - over.q0, head);
+      if (over.n > 0) side[1] = row_parts(p.launch[taken], over, a.own + g, own.q0 + i - over.q0, head);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         for (int j = lane; j < side[k].n; j += 32) top = fmaxf(top, side[k].ml[side[k].at(j)].x);
@@ -251,11 +264,12 @@ void cuda_ok(cudaError_t e) {
 template <int kD, bool kF16>
 void join_launch(const PagedSharedParams& p, cudaStream_t s) {
   // Few rows may have many parts each, many rows have few.
-  const int64_t rows = int64_t(p.own.max_new) * p.own.heads;
-  const bool few = int64_t(p.own.own) * rows <= 1024;
+  const PagedParams& a = p.launch[p.own];
+  const int64_t rows = int64_t(a.max_new) * a.heads;
+  const bool few = int64_t(a.own) * rows <= 1024;
   const int per = few ? kJoinWarps / 4 : kJoinWarps;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.own.own, unsigned(std::min<int64_t>((rows + per - 1) / per, 256)));
+  cfg.gridDim = dim3(a.own, unsigned(std::min<int64_t>((rows + per - 1) / per, 256)));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -282,9 +296,15 @@ void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* membe
   cuda_ok(cudaLaunchKernelEx(&cfg, paged_plan_kernel, p, shared, first, member));
 }
 
+void paged_split_launch(const PagedSharedParams& p, cudaStream_t s) {
+  paged_split_kernel<<<p.launches, kSplitThreads, 4 * (p.launch[0].seqs + 1), s>>>(p);
+  cuda_ok(cudaGetLastError());
+}
+
 void paged_shared_launch(const PagedSharedParams& p, cudaStream_t s) {
-  if (p.own.head_dim == 64) p.own.fp16 ? join_launch<64, true>(p, s) : join_launch<64, false>(p, s);
-  else p.own.fp16 ? join_launch<128, true>(p, s) : join_launch<128, false>(p, s);
+  const PagedParams& a = p.launch[0];
+  if (a.head_dim == 64) a.fp16 ? join_launch<64, true>(p, s) : join_launch<64, false>(p, s);
+  else a.fp16 ? join_launch<128, true>(p, s) : join_launch<128, false>(p, s);
 }
 
 }  // namespace mgfa

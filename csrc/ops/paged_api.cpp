@@ -119,9 +119,13 @@ int64_t check_groups(const torch::Tensor& groups, const torch::Tensor& like, int
   return n;
 }
 
-// A group's rows a key head up to which its prefix goes to the decode kernel (32 of its rows
-// read it at once); above, to 128-row tiles.
-constexpr int64_t kGroupFewRows = 32;
+// A group's rows a key head up to which its prefix goes to the decode kernel, in units of 32
+// rows; above, to 128-row tiles. Units more than one read the prefix again (from L2), but start
+// and end much sooner: in a small call up to four of them.
+int64_t group_few_rows(const PagedParams& p) {
+  const int64_t rows = int64_t(p.tokens) * p.group;
+  return rows <= 128 && int64_t(p.width) * p.page <= 8192 ? 128 : 32;
+}
 
 // The launches for sequences that share prefixes (paged_shared.cu).
 void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q, const torch::Tensor& k,
@@ -129,82 +133,117 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
   const int64_t T = problem.tokens, D = problem.head_dim, n_groups = groups.size(0) - 1;
   const auto f32 = q.options().dtype(at::kFloat);
   PagedSharedParams j;
-  PagedParams& p = j.own;
-  p = problem;
+  PagedParams p = problem;
   p.own = p.seqs;
   p.seqs += int(n_groups);
   p.groups = groups.data_ptr<int>();
   p.shared = plan.data_ptr<int>();
   p.first = p.shared + n_groups;
   p.most_rows = -1;  // no groups
+  p.sms = sms;
   j.member = p.first + p.own;
   // rows of whole units, of what is a sequence's own and of what its group shares
   torch::Tensor acc = torch::empty({2 * T * p.heads * (D + 2)}, f32), work[3];
   p.acc_o = acc.data_ptr<float>();
   p.acc_ml = reinterpret_cast<float2*>(p.acc_o + 2 * T * p.heads * D);
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  int launched = 0;
-  auto launch = [&](PagedParams& l, bool decode, int64_t units) {
-    uint32_t heads = 1;
-    if (decode) {
-      l.tile = 64;
-      l.grid = l.form == kPagedRowsApart ? sms : 2 * sms;
-      if (l.form == kPagedHeadsApart) {
-        heads = 4;
-        l.tile = 16;
-        l.kv_heads /= 4;
-      }
+
+  // A launch of 128-row tiles, or (block_tokens set) of the decode kernel, for the groups
+  // of least_rows to most_rows rows, and the sequences' own keys unless no_own.
+  auto add = [&](PagedParams l) {
+    if (l.block_tokens) {
+      l.tile = l.form == kPagedHeadsApart ? 16 : 64;
+      l.sm_ctas = l.form == kPagedRowsApart ? 1 : 2;
+      // (a tile takes 0.9 us of an SM with 32 rows, 0.57 with 16 and two CTAs at work)
+      l.cost = l.form == kPagedRowsApart ? 0.9f : 0.57f;
+      if (l.form == kPagedHeadsApart) l.kv_heads /= 4;
     } else {
       l.block_tokens = 2 * std::max(1, 128 / l.group);
       l.tile = 128;
       l.snap = 4;
-      l.grid = sms;
+      l.sm_ctas = 1;
+      l.cost = 3.f;
     }
+    l.cost *= float(l.kv_heads);
     l.unit_rows = l.block_tokens * l.group;
     l.min_share = 2;
-    units = (units + T / l.block_tokens) * l.kv_heads;
+    const int64_t units = ((l.no_own ? 0 : T / l.block_tokens + l.own) +
+                           (l.most_rows < 0 ? 0 : T / l.block_tokens + n_groups)) * l.kv_heads;
     const int64_t tiles = std::max<int64_t>(1, (int64_t(l.width) * l.page + l.tile - 1) / l.tile);
-    l.grid = int(std::min<int64_t>(l.grid, (units * tiles + l.min_share - 1) / l.min_share));
-    const int64_t rows = 2 * int64_t(l.grid) * l.unit_rows * heads;
-    const int64_t descs = (paged_desc_rows(l, l.own) + paged_desc_rows(l, int(n_groups))) * l.kv_heads;
-    work[launched] = torch::empty({rows * (D + 2) + 2 * descs}, f32);
-    l.part_o = work[launched].data_ptr<float>();
-    l.part_ml = reinterpret_cast<float2*>(l.part_o + rows * D);
-    l.desc = reinterpret_cast<int2*>(l.part_ml + rows);
-    const uint32_t chunk = uint32_t(std::min<int64_t>(l.page, l.tile));
-    const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, heads, 1});
-    const CUtensorMap mv = map16(v, {3, 1, 2, 0}, {64, chunk, heads, 1});
-    if (decode) {
-      paged_decode_launch(mk, mv, l, stream, launched > 0);
-    } else {
-      const CUtensorMap mq = map16(q, {2, 1, 0, -1}, {64, uint32_t(l.group), uint32_t(l.block_tokens / 2), 1});
-      paged_chunk_launch(mq, mk, mv, l, stream, launched > 0);
-    }
-    ++launched;
+    l.grid = int(std::min<int64_t>(l.sm_ctas * sms, (units * tiles + l.min_share - 1) / l.min_share));
+    j.launch[j.launches++] = l;
   };
-  // The groups, by their rows, of which the host knows the bounds; the longest work, on 128-row
-  // tiles, first.
-  if (T * p.group > kGroupFewRows) {
-    PagedParams& l = j.over[j.launches++] = p;
-    l.no_own = 1;
-    l.least_rows = kGroupFewRows + 1;
-    l.most_rows = INT64_MAX;
-    launch(l, false, n_groups);
-  }
-  if (p.group <= kGroupFewRows) {
-    PagedParams& l = j.over[j.launches++] = p;
-    l.no_own = 1;
-    l.least_rows = 0;
-    l.most_rows = kGroupFewRows;
-    l.form = kPagedRowsApart;
-    l.block_tokens = int(kGroupFewRows) / l.group;
-    launch(l, true, n_groups);
-  }
+  PagedParams over = p;  // groups alone
+  over.no_own = 1;
+  const int64_t group_rows = group_few_rows(p);
   if (few) {
+    // The groups, by their rows, of which the host knows the bounds and the mean. Launches of
+    // whole SMs that have work come before the sequences' own keys, whose CTAs would otherwise
+    // take half of many; the one that probably has none comes last.
     p.block_tokens = p.max_new;
     if (p.max_new * p.group <= 16 && p.kv_heads % 4 == 0) p.form = kPagedHeadsApart;
+    const bool large_first = p.group > 32 || T * p.group > group_rows * n_groups;
+    for (int i = 0; i < 3; ++i) {
+      if (i == 1) {
+        j.own = j.launches;
+        add(p);
+      } else if (large_first == (i == 0)) {  // on 128-row tiles
+        if (T * p.group <= group_rows && p.group <= 32) continue;
+        PagedParams large = over;
+        large.least_rows = p.group > 32 ? 0 : group_rows + 1;
+        large.most_rows = INT64_MAX;
+        add(large);
+      } else if (p.group <= 32) {
+        PagedParams small = over;
+        small.least_rows = 0;
+        small.most_rows = group_rows;
+        small.form = kPagedRowsApart;
+        small.block_tokens = 32 / p.group;
+        add(small);
+      }
+    }
+  } else {
+    p.most_rows = INT64_MAX;
+    if (p.group <= 32 && T * p.group <= group_rows) {  // few rows in all: as the groups'
+      p.form = kPagedRowsApart;
+      p.block_tokens = 32 / p.group;
+    }
+    add(p);
   }
-  launch(p, few, p.own);
+
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int64_t counts = p.seqs + 1;
+  torch::Tensor tiles;
+  if (j.launches > 1) tiles = torch::empty({j.launches * counts}, plan.options());
+  for (int i = 0; i < j.launches; ++i) {
+    PagedParams& l = j.launch[i];
+    const int64_t rows = 2 * int64_t(l.grid) * l.unit_rows * (l.form == kPagedHeadsApart ? 4 : 1);
+    const int64_t descs = (paged_desc_rows(l, l.own) + paged_desc_rows(l, int(n_groups))) * l.kv_heads;
+    work[i] = torch::empty({rows * (D + 2) + 2 * descs}, f32);
+    l.part_o = work[i].data_ptr<float>();
+    l.part_ml = reinterpret_cast<float2*>(l.part_o + rows * D);
+    l.desc = reinterpret_cast<int2*>(l.part_ml + rows);
+    if (!tiles.defined()) continue;
+    uint32_t* at = reinterpret_cast<uint32_t*>(tiles.data_ptr<int>());
+    l.tiles = at + i * counts;
+    for (int k = 0, n = 0; k < j.launches; ++k)
+      if (k != i) {
+        l.other_tiles[n] = at + k * counts;
+        l.other_cost[n++] = j.launch[k].cost;
+      }
+  }
+  if (j.launches > 1) paged_split_launch(j, stream);
+  for (int i = 0; i < j.launches; ++i) {
+    const PagedParams& l = j.launch[i];
+    const uint32_t chunk = uint32_t(std::min<int64_t>(l.page, l.tile)), heads = l.form == kPagedHeadsApart ? 4 : 1;
+    const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, heads, 1});
+    const CUtensorMap mv = map16(v, {3, 1, 2, 0}, {64, chunk, heads, 1});
+    if (l.tile == 128) {
+      const CUtensorMap mq = map16(q, {2, 1, 0, -1}, {64, uint32_t(l.group), uint32_t(l.block_tokens / 2), 1});
+      paged_chunk_launch(mq, mk, mv, l, stream, i > 0);
+    } else {
+      paged_decode_launch(mk, mv, l, stream, i > 0);
+    }
+  }
   paged_shared_launch(j, stream);
 }
 
