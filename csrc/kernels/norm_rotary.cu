@@ -159,16 +159,15 @@ __device__ __forceinline__ float weight_at(const NormRotaryParams& p, int kind, 
 // of a pair takes them with, each `angle_row` floats.
 __host__ __device__ inline int angle_row(int rotary_dim) { return (rotary_dim / 2 + 3) / 4 * 4; }
 
-// Those of a tile of tokens [first, first + here). turns: inv_freq / 2 pi, or null before these
-// are there. kFast: sine and cosine of the reduced angle to 2^-21, of which 16-bit results see
-// nothing; otherwise to two steps of float32.
-constexpr double kTurn = 0.15915494309189535;  // 1 / (2 pi)
+// Those of a tile of tokens [first, first + here), formed as rotary_angle() does. inv_freq: the
+// frequencies in shared memory, or p's own before these are there. kFast: sine and cosine of the
+// reduced angle to 2^-21, of which 16-bit results see nothing; otherwise to two steps of float32.
 template <bool kFast>
-__device__ __forceinline__ void tile_angles(const RotaryParams& p, const double* turns, int64_t first, int here, float* to) {
+__device__ __forceinline__ void tile_angles(const RotaryParams& p, const double* inv_freq, int64_t first, int here, float* to) {
   const int half = p.rotary_dim >> 1, row = angle_row(p.rotary_dim);
   for (int i = threadIdx.x; i < here * half; i += blockDim.x) {
     const int tt = i / half, f = i - tt * half;
-    double t = rotary_position(p, first + tt) * (turns ? turns[f] : p.inv_freq[f] * kTurn);
+    double t = rotary_position(p, first + tt) * inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
     t -= rint(t);
     float s, c;
     if constexpr (kFast) {
@@ -346,11 +345,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
     uint4 v;
     typename Pair::Raw w[kPairs];
   };
-  // inv_freq / 2 pi; twice a tile's (append) places and angles; the ring
+  // inv_freq; twice a tile's (append) places and angles; the ring
   extern __shared__ uint4 shared[];
   const int half = p.rotary_dim >> 1, angles = 2 * cut.tile * angle_row(p.rotary_dim);
-  double* const turns = reinterpret_cast<double*>(shared);
-  AppendPlace* const places = reinterpret_cast<AppendPlace*>(turns + (half + 1) / 2 * 2);
+  double* const freqs = reinterpret_cast<double*>(shared);
+  AppendPlace* const places = reinterpret_cast<AppendPlace*>(freqs + (half + 1) / 2 * 2);
   float* const cs = reinterpret_cast<float*>(places + (kAppend ? 2 * cut.tile : 0));
   const Place<kMode, V> at(p, cut);
   RotaryTensor x[1] = {p.x[at.kind & 1]};
@@ -368,11 +367,12 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_kernel(const P p, con
         if ((threadIdx.x & 31) == 0) places[(j & 1) * cut.tile + i] = to;
       }
     }
-    tile_angles<sizeof(E) == 2>(p, j ? turns : nullptr, first, here, cs + (j & 1) * angles);
+    // (the positions alone as apply_rotary does them, to the bit)
+    tile_angles<kNorm && sizeof(E) == 2>(p, j ? freqs : p.inv_freq, first, here, cs + (j & 1) * angles);
   };
   if (units.tiles > 0) prepare(0);
   if (units.tiles > 1)
-    for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * kTurn;
+    for (int i = threadIdx.x; i < half; i += blockDim.x) freqs[i] = p.inv_freq[i];
   uint64_t w0[kPairs], w1[kTwo], wo[kMode == kAny ? kPairs : 1];
   if constexpr (kNorm) {
     constexpr bool kHalfType = std::is_same_v<E, __half>;
@@ -488,23 +488,23 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rotary_bwd_kernel(const Norm
     uint4 v;
     typename Pair::Raw w[kPairs];
   };
-  // inv_freq / 2 pi, twice a tile's angles, the ring; at the end the weights' gradients
+  // inv_freq, twice a tile's angles, the ring; at the end the weights' gradients
   extern __shared__ uint4 shared[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int half = p.rotary_dim >> 1, angles = 2 * cut.tile * angle_row(p.rotary_dim);
-  double* const turns = reinterpret_cast<double*>(shared);
-  float* const cs = reinterpret_cast<float*>(turns + (half + 1) / 2 * 2);
+  double* const freqs = reinterpret_cast<double*>(shared);
+  float* const cs = reinterpret_cast<float*>(freqs + (half + 1) / 2 * 2);
   const Place<kMode, V> at(p, cut);
   const RotaryTensor in[2] = {p.x[at.kind], p.dy[at.kind]};
   U units(p, cut, at, in, reinterpret_cast<uint4*>(cs + 2 * angles));
   auto prepare = [&](int64_t j) {
     const int64_t first = units.first(j);
     const int here = int(units.all - first < cut.tile ? units.all - first : cut.tile);
-    tile_angles<sizeof(E) == 2>(p, j ? turns : nullptr, first, here, cs + (j & 1) * angles);
+    tile_angles<sizeof(E) == 2>(p, j ? freqs : p.inv_freq, first, here, cs + (j & 1) * angles);
   };
   if (units.tiles > 0) prepare(0);
   if (units.tiles > 1)
-    for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.inv_freq[i] * kTurn;
+    for (int i = threadIdx.x; i < half; i += blockDim.x) freqs[i] = p.inv_freq[i];
   constexpr bool kHalfType = std::is_same_v<E, __half>;
   uint64_t w0[kPairs], w1[kTwo], acc0[kPairs], acc1[kTwo];
 #pragma unroll
@@ -748,7 +748,7 @@ void cuda_ok(cudaError_t e) {
 }
 
 // Bytes of the frequencies and of two tiles' angles in shared memory.
-size_t turns_and_angles(const RotaryParams& p, const Cut& cut) {
+size_t freqs_and_angles(const RotaryParams& p, const Cut& cut) {
   return size_t(p.rotary_dim / 2 + 1) / 2 * 2 * sizeof(double) + 4 * size_t(cut.tile) * angle_row(p.rotary_dim) * sizeof(float);
 }
 
@@ -770,7 +770,7 @@ void fwd_mode(const P& p, int sm_count, cudaStream_t s) {
   const int64_t all = p.batch * p.tokens;
   const Cut cut = make_cut(lanes_of(kMode, V, p.head_dim, p.rotary_dim), heads, all, sm_count);
   using U = Units<E, kMode, 1, kFwdUnit>;
-  const size_t smem = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * kThreads +
+  const size_t smem = freqs_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * kThreads +
                       (kAppend ? 2 * cut.tile * sizeof(AppendPlace) : 0);
   launch_tiles<norm_rotary_kernel<E, kMode, kNorm, P>>(p, cut, all, 2 * sm_count, smem, s);
 }
@@ -807,7 +807,7 @@ template <class E, int kMode>
 void bwd_mode(const NormRotaryParams& p, int parts, int sm_count, cudaStream_t s) {
   const Cut cut = bwd_cut<E>(p, kMode, sm_count);
   using U = Units<E, kMode, 2, kBwdUnit>;
-  const size_t ring = turns_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * kThreads;
+  const size_t ring = freqs_and_angles(p, cut) + sizeof(uint4) * U::kRing * U::kVecs * kThreads;
   const size_t sums = p.dw_part ? size_t(cut.threads >> cut.lanes_log) * p.head_dim * sizeof(float) : 0;
   launch_tiles<norm_rotary_bwd_kernel<E, kMode>>(p, cut, p.batch * p.tokens, parts, std::max(ring, sums), s);
 }

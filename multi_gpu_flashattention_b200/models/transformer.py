@@ -15,9 +15,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.logprobs import TokenLogprobs, token_logprobs
 from ..ops.norm import rms_norm
 from ..ops.paged import PagedKVCache
-from ..ops.rotary import apply_rotary, rotary_frequencies
+from ..ops.rotary import apply_norm_rotary, apply_rotary, rotary_frequencies
 from ..parallel.api import ring_attention
 from ..parallel.layouts import RingLayout
 
@@ -62,18 +63,24 @@ class RingAttentionBlock(nn.Module):
 
     fused_ops: the norms (the second with the attention's residual) and the rotary
     embeddings run on the kernels, for CUDA tensors; each rounds its result once, where
-    the plain ops round between."""
+    the plain ops round between.
+    qk_norm: each query and key head is normed (with weights of head_dim) before its rotary
+    embedding; with fused_ops in one pass with it."""
 
     fused_ops = False  # of modules that were saved whole without one
+    qk_norm = False
 
     def __init__(self, d_model: int, n_heads: int, n_kv_heads: Optional[int] = None,
                  head_dim: int = 128, mlp_mult: int = 4, causal: bool = True,
-                 fused_ops: bool = False):
+                 fused_ops: bool = False, qk_norm: bool = False):
         super().__init__()
         self.h, self.hkv = n_heads, n_kv_heads or n_heads
         self.d = head_dim
         self.causal = causal
         self.fused_ops = fused_ops
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.q_norm, self.k_norm = RMSNorm(head_dim), RMSNorm(head_dim)
         self.norm1, self.norm2 = RMSNorm(d_model), RMSNorm(d_model)
         self.wq = nn.Linear(d_model, self.h * head_dim, bias=False)
         self.wk = nn.Linear(d_model, self.hkv * head_dim, bias=False)
@@ -94,9 +101,14 @@ class RingAttentionBlock(nn.Module):
         q = self.wq(h).view(B, L, self.h, self.d)
         k = self.wk(h).view(B, L, self.hkv, self.d)
         v = self.wv(h).view(B, L, self.hkv, self.d)
-        if fused:
+        if fused and self.qk_norm:
+            q, k = apply_norm_rotary(q, k, pos.to(x.device), _frequencies(self.d, x.device),
+                                     self.q_norm.weight, self.k_norm.weight, eps=self.q_norm.eps)
+        elif fused:
             q, k = apply_rotary(q, k, pos.to(x.device), _frequencies(self.d, x.device))
         else:
+            if self.qk_norm:
+                q, k = self.q_norm(q), self.k_norm(k)
             q, k = rotary(q, pos), rotary(k, pos)
         a = ring_attention(q.contiguous(), k.contiguous(), v.contiguous(), causal=self.causal,
                            group=group, layout=layout, backend=backend)
@@ -140,19 +152,25 @@ class RingTransformerLM(nn.Module):
     the ring over `group`, everything else is per token. Parameters are
     replicated, so after `loss(...).backward()` the gradients are summed over
     the group (all-reduce, as in data parallelism) to give the unsharded
-    model's gradients."""
+    model's gradients.
+
+    fused_loss: loss() takes the tokens' log probabilities from the kernels, for CUDA
+    tensors, which keep nothing of the logits' size but their gradient."""
 
     fused_ops = False  # of modules that were saved whole without one
+    fused_loss = False
 
     def __init__(self, vocab: int, d_model: int, n_layers: int, n_heads: int,
                  n_kv_heads: Optional[int] = None, head_dim: int = 128, mlp_mult: int = 4,
-                 tie_embeddings: bool = True, fused_ops: bool = False):
+                 tie_embeddings: bool = True, fused_ops: bool = False, qk_norm: bool = False,
+                 fused_loss: bool = False):
         super().__init__()
         self.embed = nn.Embedding(vocab, d_model)
         self.fused_ops = fused_ops
+        self.fused_loss = fused_loss
         self.blocks = nn.ModuleList(
             RingAttentionBlock(d_model, n_heads, n_kv_heads, head_dim, mlp_mult, causal=True,
-                               fused_ops=fused_ops)
+                               fused_ops=fused_ops, qk_norm=qk_norm)
             for _ in range(n_layers))
         self.norm = RMSNorm(d_model)
         self.head = nn.Linear(d_model, vocab, bias=False)
@@ -191,7 +209,8 @@ class RingTransformerLM(nn.Module):
 
     @torch.no_grad()
     def serve(self, ids: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
-              cu_seqlens: torch.Tensor, max_seqlen: int) -> torch.Tensor:
+              cu_seqlens: torch.Tensor, max_seqlen: int,
+              cu_groups: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Logits [tokens, vocab] of the sequences' next tokens, on one GPU.
 
         ids [tokens] packs the new tokens of the sequences in `slots`: sequence b's are
@@ -199,18 +218,22 @@ class RingTransformerLM(nn.Module):
         a chunk of one, or single tokens. They join the cache and see all that it holds of
         their sequence (slots, cu_seqlens: int32 CUDA tensors). Rows outside every sequence
         hold nothing; those of a sequence that got no room in the cache, which stays as it
-        was, are NaN. bfloat16 or float16 parameters, head_dim 64 or 128."""
+        was, are NaN. bfloat16 or float16 parameters, head_dim 64 or 128.
+        cu_groups (int32 [groups + 1], CUDA): sequences [cu_groups[g], cu_groups[g + 1]) were
+        forked from one prompt, whose full pages the attention then reads once for all of them."""
         self._check_served(ids, cache, max_seqlen)
         pos = cache.reserve(slots, cu_seqlens, ids.numel())
+        shared = None if cu_groups is None else cache.shared_prefix(slots, cu_seqlens, cu_groups)
         inv_freq = _frequencies(self.blocks[0].d, ids.device)
         x = self.embed(ids)
         h = rms_norm(x, self.blocks[0].norm1.weight, eps=self.blocks[0].norm1.eps)
         for i, blk in enumerate(self.blocks):
             q, k, v = (w(h).view(ids.numel(), n, blk.d)
                        for w, n in ((blk.wq, blk.h), (blk.wk, blk.hkv), (blk.wv, blk.hkv)))
-            q, k = apply_rotary(q, k, pos, inv_freq)
-            cache.write(i, k, v, slots, cu_seqlens)
-            a = cache.attend(i, q, slots, cu_seqlens, max_seqlen)
+            norms = dict(q_weight=blk.q_norm.weight, k_weight=blk.k_norm.weight, eps=blk.q_norm.eps) \
+                if blk.qk_norm else {}
+            q = cache.append(i, q, k, v, pos, inv_freq, slots, cu_seqlens, **norms)
+            a = cache.attend(i, q, slots, cu_seqlens, max_seqlen, shared=shared)
             h, x = rms_norm(blk.wo(a.flatten(1)), blk.norm2.weight, residual=x, eps=blk.norm2.eps)
             after = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm
             h, x = rms_norm(blk.mlp(h), after.weight, residual=x, eps=after.eps)
@@ -223,10 +246,21 @@ class RingTransformerLM(nn.Module):
         this shard's summed loss divided by the token count of all shards."""
         import torch.distributed as dist
         logits = self(ids, layout, rank, group=group, backend=backend)
-        local = F.cross_entropy(logits.float().flatten(0, 1), targets.flatten(),
-                                ignore_index=IGNORE_INDEX, reduction="sum")
+        if self.fused_loss and logits.is_cuda:
+            local = -token_logprobs(logits, targets, ignore_index=IGNORE_INDEX).logprobs.sum()
+        else:
+            local = F.cross_entropy(logits.float().flatten(0, 1), targets.flatten(),
+                                    ignore_index=IGNORE_INDEX, reduction="sum")
         count = (targets != IGNORE_INDEX).sum().to(torch.float32)
         if dist.is_initialized() and dist.get_world_size(group) > 1:
             count = count.clone()
             dist.all_reduce(count, group=group)
         return local / count.clamp(min=1.0)
+
+    def token_logprobs(self, ids: torch.Tensor, targets: torch.Tensor, layout: RingLayout, rank: int = 0,
+                       group=None, backend: Optional[str] = None, top: int = 0) -> TokenLogprobs:
+        """Log probabilities of the shard's targets [B, L] (0 at IGNORE_INDEX) and the entropy of
+        its distributions, both differentiable, and the `top` likeliest alternatives, on a GPU:
+        for losses that weigh the tokens apart. A loss over several shards is the sum of theirs."""
+        logits = self(ids, layout, rank, group=group, backend=backend)
+        return token_logprobs(logits, targets, top=top, ignore_index=IGNORE_INDEX)
