@@ -601,6 +601,7 @@ torch::Tensor cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor table
     p.norm = 1;
   }
   if (q.size(0) == 0) return out;
+  MGFA_CHECK(p.vec, "q and new_k must have rows on 16-byte boundaries");  // (checked above)
   p.x[0].out = out.data_ptr();
   p.v = rotary_tensor(new_v);
   p.c = cache_state(k, table, lens, refs, grown, status);

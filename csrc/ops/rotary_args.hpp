@@ -18,11 +18,13 @@ inline RotaryTensor rotary_tensor(const torch::Tensor& t) {
   return r;
 }
 
-// Whether every head of t starts on a 16-byte boundary.
+// Whether every head of t starts on a 16-byte boundary. (The strides of dimensions of size 1
+// mean nothing.)
 inline bool rotary_vec(const RotaryTensor& r, const torch::Tensor& t) {
   const int64_t v = 16 / t.element_size();
-  return reinterpret_cast<uintptr_t>(r.in) % 16 == 0 && r.stride_b % v == 0 && r.stride_t % v == 0 &&
-         r.stride_h % v == 0;
+  auto fits = [&](int64_t dim, int64_t stride) { return t.size(dim) <= 1 || stride % v == 0; };
+  return reinterpret_cast<uintptr_t>(r.in) % 16 == 0 && (t.dim() < 4 || fits(0, r.stride_b)) &&
+         fits(-3, r.stride_t) && fits(-2, r.stride_h);
 }
 
 // All of p but the outputs; q and k are made contiguous where their last dimension is not.

@@ -197,3 +197,40 @@ def test_refusals():
     refused("contiguous head_dim", q=torch.zeros(2, 64, 4, device="cuda", dtype=torch.bfloat16).transpose(1, 2))
     refused("no gradient", q=q.clone().requires_grad_())
     refused("head_dim", q_weight=w[:32], k_weight=w[:32])
+
+
+def test_strides_of_single_rows_mean_nothing():
+    """One token and one head, cut from rows of an odd length."""
+    from multi_gpu_flashattention_b200 import apply_norm_rotary, apply_rotary, rotary_frequencies
+    inv, _ = rotary_frequencies(64, device="cuda")
+    w = torch.ones(64, device="cuda")
+    cache = _cache(heads=1)
+    wide = torch.randn(3, 1, 1, 67, device="cuda").bfloat16()
+    q, k, v = (wide[i, :, :, :64].as_strided((1, 1, 64), (67, 67, 1), 0) for i in range(3))
+    q, k, v = (torch.empty_strided((1, 1, 64), (67, 5, 1), dtype=torch.bfloat16, device="cuda").copy_(t) for t in (q, k, v))
+    pos = cache.reserve([0], [0, 1], 1)
+    before = cache.k.clone(), cache.v.clone()
+    out = cache.append(0, q, k, v, pos + 9, inv, _ints([0]), _ints([0, 1]))
+    _check(cache, before, 0, q, k, v, out, pos + 9, inv, _ints([0]), _ints([0, 1]), None, False, 1.0)
+    assert torch.equal(apply_rotary(q, None, pos + 9, inv), out)
+    assert torch.equal(apply_norm_rotary(q, None, pos + 9, inv, w, None), apply_norm_rotary(q.contiguous(), None, pos + 9, inv, w, None))
+
+
+def test_large_pool_offsets():
+    """Pages that begin beyond 2^31 elements of the pool."""
+    from multi_gpu_flashattention_b200 import PagedKVCache, rotary_frequencies
+    inv, _ = rotary_frequencies(128, device="cuda")
+    pages = (1 << 31) // (64 * 8 * 128) + 3
+    c = PagedKVCache.allocate(1, pages, 64, 8, 128, 2, 128)
+    c.refs[:pages - 2] = 1  # the last two are free
+    q, k, v = _batch(70, 16, 8, 128, torch.bfloat16)
+    slots, cu = _ints([1]), _ints([0, 70])
+    pos = c.reserve(slots, cu, 70)
+    out = c.append(0, q, k, v, pos, inv, slots, cu)
+    assert c.page_table[1].tolist() == [pages - 2, pages - 1]
+    one = torch.ones(128, device="cuda")
+    for x, got in ((q, out), (k, c.k[0, -2:].flatten(0, 1)[:70])):
+        r = reference(x[None], one, x[None], pos[None], inv, 1e-6, False, 1.0)
+        scale = (x.double().pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
+        close(got, r["y"][0] * scale, r["y_size"][0] * scale, 1e-6)
+    assert torch.equal(c.v[0, -2:].flatten(0, 1)[:70], v)

@@ -240,3 +240,38 @@ def test_a_captured_sampling_step():
         want = step(caches[1], ids)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(caches[0].lens, caches[1].lens)
+
+
+def test_a_forked_sequence_without_room(monkeypatch):
+    """One of a group's sequences gets no page, which is known before the first layer's append:
+    the others are served as in a step in which all had room, its logits are NaN."""
+    from multi_gpu_flashattention_b200 import KernelStatusError, PagedKVCache
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    model = _model(torch.bfloat16, fused=True)
+    prompt = torch.randint(0, VOCAB, (64,), generator=torch.Generator().manual_seed(13)).cuda()
+    append, attend = PagedKVCache.append, PagedKVCache.attend
+
+    def late(f):
+        def call(self, *a, **kw):  # what reserve() reported has arrived
+            torch.cuda.synchronize()
+            return f(self, *a, **kw)
+        return call
+
+    monkeypatch.setattr(PagedKVCache, "append", late(append))
+    monkeypatch.setattr(PagedKVCache, "attend", late(attend))
+    ids, got = torch.tensor([1, 2, 3, 4], device="cuda"), {}
+    for pages in (8, 7):  # the prompt's 4, and 4 for the sequences' new tokens
+        cache = model.make_cache(pages, 16, 4, 96)
+        model.serve(prompt, cache, _ints([0]), _ints([0, 64]), 64)
+        cache.fork([0] * 3, [1, 2, 3])
+        check_errors()
+        got[pages] = model.serve(ids, cache, _ints([0, 1, 2, 3]), _ints([0, 1, 2, 3, 4]), 1, cu_groups=_ints([0, 4]))
+    assert torch.isnan(got[7][3]).all() and torch.isfinite(got[8]).all()
+    with pytest.raises(KernelStatusError, match="too few free pages"):
+        check_errors()
+    # (the refused one's limits what is shared to the pages before its last token)
+    exact = [_exact(model, torch.cat([prompt, ids[i:i + 1]]))[0][-1] for i in range(3)]
+    plain = _model(torch.bfloat16)
+    for i in range(3):
+        far = _off(plain(torch.cat([prompt, ids[i:i + 1]])[None], _layout(65))[0, -1], exact[i])
+        assert _off(got[7][i], exact[i]) <= 1.5 * far + 1e-3
