@@ -175,7 +175,14 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
   PagedParams over = p;  // groups alone
   over.no_own = 1;
   const int64_t group_rows = group_few_rows(p);
-  if (few) {
+  const bool small = p.group <= 32 && T * p.group <= group_rows;
+  if (small) {
+    // Few rows in all: one launch of units of up to 32 rows takes everything.
+    p.most_rows = INT64_MAX;
+    p.form = kPagedRowsApart;
+    p.block_tokens = 32 / p.group;
+    add(p);
+  } else if (few) {
     // The groups, by their rows, of which the host knows the bounds and the mean. Launches of
     // whole SMs that have work come before the sequences' own keys, whose CTAs would otherwise
     // take half of many; the one that probably has none comes last.
@@ -187,7 +194,6 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
         j.own = j.launches;
         add(p);
       } else if (large_first == (i == 0)) {  // on 128-row tiles
-        if (T * p.group <= group_rows && p.group <= 32) continue;
         PagedParams large = over;
         large.least_rows = p.group > 32 ? 0 : group_rows + 1;
         large.most_rows = INT64_MAX;
@@ -201,12 +207,8 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
         add(small);
       }
     }
-  } else {
+  } else {  // one launch of 128-row tiles
     p.most_rows = INT64_MAX;
-    if (p.group <= 32 && T * p.group <= group_rows) {  // few rows in all: as the groups'
-      p.form = kPagedRowsApart;
-      p.block_tokens = 32 / p.group;
-    }
     add(p);
   }
 
