@@ -14,7 +14,12 @@
 // than shuffles; rstd is computed again from x in the backward pass, which reads x anyway.
 // The sines, cosines and weights of a thread's columns take the registers that loads under
 // way would need: so each thread has a ring in shared memory, into which it copies (cp.async)
-// what it will work on 4 or 8 heads later, and no other thread waits for it.
+// what it will work on 4 or 8 heads later, and no other thread waits for it. 16384 tokens of
+// 32 + 8 heads of 128 in bf16 take 60 us forward (336 MB, 5.6 TB/s) and 97 us back (503 MB,
+// 5.2 TB/s), the sum of the weights' parts 7 us more; the first version, which loaded into
+// registers, took 88 and 188 us. At four heads a thread the angles were 8 of 67 us forward and
+// 9 of 106 back; eight heads that share them (make_cut) gained that much. 8.4K tokens into a
+// cache, 214 MB, take 42 us; 64 single tokens 6.6 us, which is latency.
 #include "norm_rotary.cuh"
 
 #include <algorithm>

@@ -13,9 +13,16 @@
 // but the tile's; the four are added when a unit ends. 32 sequences of 8192 keys (8 key
 // heads of 128, pages of 16) take 171 us for 1.07 GB, 6.3 TB/s; one of 131072 keys 86 us,
 // and 9 us for joining 296 parts; with 4 new tokens each (16 rows) the 32 sequences take
-// 1.03 times as long, with 8 (32 rows, whose second block of 16 spills 468 bytes at head_dim
-// 128) 1.3 times. For short sequences the time is latency: one token each
+// 1.05 times as long, with 8 (32 rows, whose second block of 16 spills 528 bytes at head_dim
+// 128) 1.34 times. For short sequences the time is latency: one token each
 // over 100 to 320 keys takes 9.6 us.
+//
+// Two more forms serve sequences that share a prefix (paged_shared.cu), whose units are short or
+// have more rows. From a unit's last tile to the next one's queries, with four warps' results
+// added between them, pass 4 us. With tiles of 16 keys of four key heads each warp has rows of
+// its own and nothing to add (kHeadsApart): the own keys of 128 sequences, up to 512 each, 65 ->
+// 40 us. And eight warps read a prefix once for up to 32 rows (kRowsApart). Both together took
+// 128 answers over 32768 shared tokens from 208 to 165 us, eight groups from 133 to 92 us.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 

@@ -17,6 +17,13 @@
 // elements give is gathered in shared memory and ranked by counting, together with the
 // alternatives of the segments before. A NaN counts as the largest value; it makes its row's
 // sums NaN.
+//
+// Bound by memory: 4096 rows of 131072 in bf16 take 195 us (1.07 GB, 5.5 TB/s) and 311 us back
+// (2.15 GB, 6.9 TB/s; 517 us before a segment was loaded while the one before is worked on).
+// 1021 rows of 50001 in fp32 take 46 and 62 us (4.4 and 6.6 TB/s). 64 rows of 131072 with 20
+// alternatives, 17 MB, take 17 us, bound by the steps of a segment one behind another. The whole
+// call took 79 us when a warp inserted its alternatives one by one, and 23 us with a second
+// pass over the segment for those above the bound.
 #include "token_logprobs.cuh"
 
 #include <cooperative_groups.h>

@@ -13,6 +13,14 @@ call can be captured into a CUDA graph.
         out = cache.attend(layer, q, slots, cu_seqlens, max_seqlen_q)
     cache.fork(src, dst); cache.free(slots); cache.compact()
 
+append() does the rotary positions, head norms and the write in one pass; sequences forked
+from one prompt, a group's one behind another in the batch, read it once:
+
+    shared = cache.shared_prefix(slots, cu_seqlens, cu_groups)   # once a step
+    for layer ...:
+        q = cache.append(layer, q, k, v, pos, inv_freq, slots, cu_seqlens)
+        out = cache.attend(layer, q, slots, cu_seqlens, max_seqlen_q, shared=shared)
+
 A batch packs its sequences' new tokens: sequence b's are the rows
 [cu_seqlens[b], cu_seqlens[b + 1]). Rows outside every sequence (a batch padded for a
 graph) are left alone: outputs keep what they held there.
@@ -22,8 +30,10 @@ table that is too short, too few free pages, a page that is not in the pool) lea
 sequence concerned as it was and faults nothing; the batch's other sequences are served.
 It raises KernelStatusError at a later call on the device, of this or another cache, or
 in check_errors(): reserve() raises before it changes anything, so the call can be made
-again; free(), fork() and compact() raise after they have done their own work; write()
-and attend(), in the middle of a step, do not raise it. A slot that a batch names twice
+again; free(), fork() and compact() raise after they have done their own work; so do, before
+theirs, token_logprobs() and the functions paged_attention() and shared_prefix() without a
+status of their own; write(), append(), shared_prefix() and attend() of a cache, in the
+middle of a step, do not raise it. A slot that a batch names twice
 is the first naming's. A cache has less than 2^30 pages and 2^31 page table entries, a batch less
 than 2^30 rows.
 """
