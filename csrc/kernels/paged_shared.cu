@@ -171,11 +171,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_shared_kernel(const __g
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
   const PagedSeq own = paged_seq(a, b);
   const int64_t rows = int64_t(own.n) * a.heads;
-  // the group, and which launch took it
+  // the group, and which launch took it (none a group without new tokens)
   PagedSeq over;
   over.n = 0;
   int taken = 0, g = -1;
-  if (own.skip > 0) {
+  if (rows > 0 && own.skip > 0) {
     g = p.member[b];
     if (g >= 0 && g < a.seqs - a.own) {
       for (; taken < p.launches; ++taken) {

@@ -251,3 +251,67 @@ def test_refusals_and_errors_on_the_device():
         p.run(shared=wrong)
         with pytest.raises(KernelStatusError):
             check_errors()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(64, 1), (128, 1), (128, 2), (66, 2)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_many_heads_a_key_head(heads, kv_heads, new):
+    Forked([(300, [(20, new)] * 3), (90, [(7, new)]), (70, [(40, new)] * 2)], heads, kv_heads, 64, 16).both(least=288)
+
+
+def test_members_without_new_tokens():
+    """Also at a group's head and end, and groups of nothing else."""
+    Forked([(200, [(9, 0), (9, 1), (40, 2), (8, 0)]), (100, [(3, 0), (4, 0)]), (64, [(5, 1)] * 2)], 8, 2, 128, 16).both(least=192)
+
+
+def test_a_row_named_twice():
+    """Two sequences of a batch that read one row of the table: as without the plan."""
+    from multi_gpu_flashattention_b200 import shared_prefix
+    p = Forked([(500, [(20, 1), (31, 1)])], 8, 2, 64, 16)
+    slots, groups = _ints([1, 1]), _ints([0, 2])
+    plan = shared_prefix(p.table, p.lens, p.cu, groups, p.page, slots=slots)
+    assert plan.lens.tolist() == [(531 - 1) // 16 * 16]
+    args = (p.q, p.k, p.v, p.table, p.lens, p.cu, 1)
+    from multi_gpu_flashattention_b200 import paged_attention
+    a, la = paged_attention(*args, slots=slots, return_lse=True, shared=plan)
+    b, lb = paged_attention(*args, slots=slots, return_lse=True)
+    # each within u |out| + (u + 4e-5) max |v| of the same value
+    u, most = 2.0 ** -8, max(float(v.abs().max()) for v in p.values)
+    assert ((a.float() - b.float()).abs() <= 2 * (u * b.float().abs() + (u + 4e-5) * most)).all()
+    assert ((la - lb).abs() <= 4e-5 * (1 + lb.abs())).all()
+
+
+def test_two_streams_and_two_graphs():
+    """Calls under way side by side, and captured ones replayed in turn and side by side, have
+    workspaces of their own: the bits are those of a call alone."""
+    ps = [Forked([(3000, [(9, 1)] * 12), (2000, [(300, 1)] * 40)], 16, 4, 128, 64, seed=1),
+          Forked([(700, [(200, 1)] * 30)], 8, 2, 64, 16, seed=2)]
+    alone = [p.run(shared=p.plan()) for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for p, s in zip(ps, streams):
+            with torch.cuda.stream(s):
+                got.append(p.run(shared=p.plan()))
+        torch.cuda.synchronize()
+        for x, y in zip(alone, got):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+    graphs = []
+    for p in ps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = p.run(shared=p.plan())
+        graphs.append((g, out))
+    for side in (False, True):
+        for _ in range(5):
+            for (g, out), s in zip(graphs, streams):
+                for t in out:
+                    t.zero_()
+            torch.cuda.synchronize()
+            for (g, out), s in zip(graphs, streams):
+                with torch.cuda.stream(s if side else torch.cuda.current_stream()):
+                    g.replay()
+            torch.cuda.synchronize()
+            for x, (g, out) in zip(alone, graphs):
+                assert torch.equal(x[0], out[0]) and torch.equal(x[1], out[1])
