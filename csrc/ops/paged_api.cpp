@@ -190,17 +190,17 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
     // that probably has none comes last.
     p.block_tokens = p.max_new;
     if (p.max_new * p.group <= 16 && p.kv_heads % 4 == 0) p.form = kPagedHeadsApart;
-    const bool large_first = p.group > 32 || T * p.group > group_rows * n_groups;
+    const bool large_first = T * p.group > group_rows * n_groups;
     for (int i = 0; i < 3; ++i) {
       if (i == 1) {
         j.own = j.launches;
         add(p);
       } else if (large_first == (i == 0)) {  // on 128-row tiles
         PagedParams large = over;
-        large.least_rows = p.group > 32 ? 0 : group_rows + 1;
+        large.least_rows = group_rows + 1;
         large.most_rows = INT64_MAX;
         add(large);
-      } else if (p.group <= 32) {
+      } else {
         PagedParams small = over;
         small.least_rows = 0;
         small.most_rows = group_rows;
