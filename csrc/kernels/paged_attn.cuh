@@ -225,10 +225,11 @@ __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
 
 // prefix[b] = tiles of one key head's units of the sequences before b; prefix[seqs] the
 // total, which is 0, and an error, where it does not fit 32 bits: nothing is done then.
-// Called by all kThreads threads of the CTA; `sums` holds kThreads / 32 values.
+// Called by all kThreads threads of the CTA; `sums` holds kThreads / 32 values. report: this
+// CTA, one for each launch, tells the status word what is wrong with the sequences.
 template <int kThreads>
 __device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* prefix,
-                                             uint32_t* sums) {
+                                             uint32_t* sums, bool report) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t before = 0;
   bool bad = false;
@@ -265,7 +266,7 @@ __device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* pre
     before = 0;
   }
   if (threadIdx.x == 0) prefix[p.seqs] = before;
-  if (bad && blockIdx.x == 0 && p.status) record_error(p.status, kErrBadArgument, 60, 0);
+  if (bad && report) record_error(p.status, kErrBadArgument, 60, 0);
   __syncthreads();
 }
 
@@ -454,7 +455,7 @@ struct PagedWalk {
     if (p.tiles) {
       if (!paged_divide<kThreads>(p, prefix)) return false;
     } else {
-      paged_prefix<kThreads>(p, prefix, sums);
+      paged_prefix<kThreads>(p, prefix, sums, blockIdx.x == 0);
     }
     const PagedShare share(p, prefix);
     begin = share.begin(blockIdx.x, u);

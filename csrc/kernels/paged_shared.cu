@@ -114,12 +114,13 @@ __global__ void __launch_bounds__(kPlanThreads)
 constexpr int kSplitThreads = 1024;
 
 // CTA l: the tiles before each sequence and group of launch l (PagedParams::tiles), which its
-// CTAs then need not find out for themselves.
+// CTAs then need not find out for themselves. Each reports what its own launch's sequences and
+// groups have wrong: a launch of the groups alone looks at no sequence's own arguments.
 __global__ void __launch_bounds__(kSplitThreads) paged_split_kernel(const __grid_constant__ PagedSharedParams p) {
   extern __shared__ uint32_t prefix[];
   __shared__ uint32_t sums[kSplitThreads / 32];
   const PagedParams& l = p.launch[blockIdx.x];
-  paged_prefix<kSplitThreads>(l, prefix, sums);
+  paged_prefix<kSplitThreads>(l, prefix, sums, true);
   for (int i = threadIdx.x; i <= l.seqs; i += kSplitThreads) l.tiles[i] = prefix[i];
 }
 
