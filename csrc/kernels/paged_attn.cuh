@@ -32,6 +32,7 @@ namespace mgfa {
 
 constexpr int kPagedMaxSeqs = 4096;
 constexpr int kPagedMaxGroup = 128;
+constexpr size_t kPagedMaxSmem = 232448;  // shared memory of a CTA (227 KB)
 
 // Forms of the decode kernel that a launch may ask for; otherwise the rows of a unit decide.
 enum : int {
@@ -39,6 +40,10 @@ enum : int {
   kPagedHeadsApart = 1,  // units of four key heads, up to 16 rows each
   kPagedRowsApart = 2,   // units of up to 32 rows, which eight warps share
 };
+
+// Shared memory of a kernel that needs `used` bytes from a 1024-byte boundary on, and behind
+// them prefix[] of `seqs` sequences (with the number of CTAs, PagedShare).
+constexpr size_t paged_smem(size_t used, int seqs) { return 1024 + used + 4 * (size_t(seqs) + 2); }
 
 struct PagedParams {
   // problem
@@ -515,7 +520,7 @@ cudaError_t paged_allow_smem(Fn fn, std::atomic<uint64_t>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPagedMaxSmem));
   if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev);
   return e;
 }

@@ -542,7 +542,8 @@ int64_t chunk_local_bytes() {
 template <int kD, bool kF16>
 void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                   const PagedParams& p, cudaStream_t s, bool early) {
-  const int smem = int(sizeof(ChunkSmem<kD>)) + 1024 + 4 * (p.seqs + 2);
+  const int smem = int(paged_smem(sizeof(ChunkSmem<kD>), p.seqs));
+  static_assert(paged_smem(sizeof(ChunkSmem<kD>), kPagedMaxSeqs) <= kPagedMaxSmem, "prefix[] of the largest batch fits");
   auto fn = paged_chunk_kernel<kD, kF16>;
   static const int64_t local = chunk_local_bytes<kD, kF16>();
   if (local != 0)

@@ -26,6 +26,7 @@
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 
+#include <cstddef>
 #include <stdexcept>
 
 namespace mgfa {
@@ -64,6 +65,9 @@ struct __align__(1024) DecodeSmem {
   uint64_t full[kStages], empty[kStages];
   uint32_t abort_flag, stop;
   uint32_t sums[kThreads / 32];
+  // prefix[] begins behind the last member, not behind the struct's padding: kRowsApart has no
+  // room for both.
+  static constexpr size_t used() { return offsetof(DecodeSmem, sums) + sizeof(sums); }
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -112,7 +116,8 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
   constexpr int kTileKeys = kApart ? 16 : kKeys;
   extern __shared__ uint8_t raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint32_t* prefix = reinterpret_cast<uint32_t*>(&s + 1);
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(&s) + Smem::used());
+  static_assert(paged_smem(Smem::used(), kPagedMaxSeqs) <= kPagedMaxSmem, "prefix[] of the largest batch fits");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t warp = warp_id(), lane = lane_id();
   AbortState ab{&s.abort_flag, p.status, p.wait_limit_ns};
@@ -564,7 +569,7 @@ void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedPara
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.grid);
   cfg.blockDim = dim3(Smem::kThreads);
-  cfg.dynamicSmemBytes = int(sizeof(Smem)) + 1024 + 4 * (p.seqs + 2);
+  cfg.dynamicSmemBytes = unsigned(paged_smem(Smem::used(), p.seqs));
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

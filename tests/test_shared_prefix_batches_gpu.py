@@ -76,3 +76,18 @@ def test_a_plan_of_longer_sequences_is_reported(b):
         check_errors()
     p.new[b] = 0
     p.check(out, lse)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("groups,heads,kv_heads", [(64, 4, 2), (1, 4, 4)])
+def test_as_many_sequences_and_groups_as_a_call_takes(groups, heads, kv_heads, D):
+    """4096 in all: the kernels' tables of them take the most shared memory."""
+    per = (4096 - groups) // groups
+    sizes = [per] * (groups - 1) + [4096 - groups - per * (groups - 1)]
+    p = Forked([(16 + 16 * (g % 3), [(1 + i % 5, 1) for i in range(n)]) for g, n in enumerate(sizes)],
+               heads, kv_heads, D, 16)
+    plan = p.plan()
+    assert plan.lens.tolist() == p.expected(p.cg)
+    p.check(*p.run(shared=plan))
+    with pytest.raises(RuntimeError, match="at most 4096 sequences and groups"):
+        p.plan(groups=_ints(p.cg + [p.cg[-1]]))
