@@ -80,7 +80,9 @@ struct PagedParams {
   // sequences that share a prefix (paged_shared.cu): sequences [0, own) come without the
   // first[b] tokens that their group shares, and behind them the groups, each the new tokens
   // of its sequences over the shared[g] tokens before; `seqs` counts both
-  const int* first = nullptr;   // [own]; null: nothing is shared
+  const int* first = nullptr;   // [own]; null: nothing is shared. Behind it member, [own]: a
+                                // sequence's group, -1: none; -2 - b where a group's first one
+                                // shares nothing, b being the first that does
   const int* groups = nullptr;  // [seqs - own + 1] sequences
   const int* shared = nullptr;  // [seqs - own] tokens
   int own = 0;
@@ -109,7 +111,7 @@ struct PagedSharedParams {
   PagedParams launch[3];
   int launches = 0;
   int own = 0;  // which one
-  const int* member = nullptr;  // [sequences] group, or -1
+  const int* member = nullptr;  // [sequences], behind PagedParams::first
 };
 
 // Entries of PagedParams::desc a key head, of `seqs` sequences or groups. Their units are
@@ -159,7 +161,9 @@ __device__ __forceinline__ PagedSeq paged_group(const PagedParams& p, int g) {
   const int a = __ldg(p.groups + g), e = __ldg(p.groups + g + 1), kv = __ldg(p.shared + g);
   s.bad = a < 0 || e < a || e > p.own || kv < 0 || kv > int64_t(p.width) * p.page || kv % p.page;
   if (s.bad || kv == 0 || a == e) return s;
-  const int q0 = __ldg(p.cu_q + a), end = __ldg(p.cu_q + e), row = p.slots ? __ldg(p.slots + a) : a;
+  const int q0 = __ldg(p.cu_q + a), end = __ldg(p.cu_q + e), other = -2 - __ldg(p.first + p.own + a);
+  int row = p.slots ? __ldg(p.slots + a) : a;
+  if (other > a && other < e) row = p.slots ? __ldg(p.slots + other) : other;
   s.bad = q0 < 0 || end < q0 || end > p.tokens || row < 0 || row >= p.rows;
   const int64_t rows = int64_t(end - q0) * p.group;
   if (s.bad || rows < p.least_rows || rows > p.most_rows) return s;
@@ -536,7 +540,7 @@ void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 int64_t paged_chunk_local_bytes();
 // Joins the parts; launched behind either.
 void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
-// Sequences that share a prefix: `shared`, `first` and `member` ([own]: its group, or -1) from
+// Sequences that share a prefix: `shared`, `first` and `member` (PagedParams::first) from
 // the page table, for the groups of p. (Nothing but the arrays of the problem is read.)
 void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t stream);
 // Fills the launches' PagedParams::tiles, where they have it.

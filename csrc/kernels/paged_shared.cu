@@ -38,13 +38,21 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanCtas = 8;   // of a group, a cluster
 constexpr int kPlanLoads = 8;  // of each table that a lane has under way
 
-// shared[g]: the leading pages that all of the group's sequences name alike, as far as these
-// are full and hold none of their new tokens; 0 for a sequence alone, which reads them once
-// anyway. Invalid groups share nothing, and neither do all others of the call then.
+// shared[g]: the leading pages that all of the group's sequences with new tokens name alike, as
+// far as these are full and hold none of the new tokens; 0 for one alone, which reads them once
+// anyway. A sequence without new tokens (an answer that has ended, whose pages may be gone) or
+// without a row of the table has no say, and shares nothing; where none has new tokens, shared[g]
+// is of all. Groups whose cu_seqlens fall share nothing; invalid ones neither, nor do all others
+// of the call then.
 __global__ void __launch_bounds__(kPlanThreads)
     paged_plan_kernel(const PagedParams p, int* shared, int* first, int* member) {
   const int g = blockIdx.x / kPlanCtas, cta = blockIdx.x % kPlanCtas, n_groups = p.seqs - p.own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ int least, lead_of[2], live[2];  // of all sequences; of those with new tokens
+  if (threadIdx.x < 2) {
+    lead_of[threadIdx.x] = p.own;
+    live[threadIdx.x] = 0;
+  }
   bool bad = false;
   for (int i = threadIdx.x; i < n_groups; i += kPlanThreads) {
     const int a = __ldg(p.groups + i), e = __ldg(p.groups + i + 1);
@@ -52,37 +60,50 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
   bad = __syncthreads_or(bad);
   const int from = bad ? 0 : __ldg(p.groups + g), to = bad ? 0 : __ldg(p.groups + g + 1);
-  __shared__ int least;
-  if (threadIdx.x == 0) least = to - from > 1 ? p.width : 0;
-  __syncthreads();
   auto row_of = [&](int b) { return p.slots ? __ldg(p.slots + b) : b; };
-  if (to - from > 1) {
-    const int lead = row_of(from);
-    const bool lead_ok = lead >= 0 && lead < p.rows;
+  auto new_of = [&](int b) { return __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b); };
+  // the row of a sequence that counts: that has one (any = 1: and new tokens); else -1
+  auto counts = [&](int b, int any) {
+    const int row = row_of(b);
+    return row >= 0 && row < p.rows && new_of(b) >= any ? row : -1;
+  };
+  bool falls = false;
+  for (int b = from + int(threadIdx.x); b < to; b += kPlanThreads) {
+    falls |= new_of(b) < 0;
+    for (int any = 0; any < 2; ++any)
+      if (counts(b, any) >= 0) {
+        atomicMin(&lead_of[any], b);
+        atomicAdd(&live[any], 1);
+      }
+  }
+  falls = __syncthreads_or(falls);
+  const int any = live[1] > 0, lead = lead_of[any];
+  const bool several = live[any] > 1 && !falls;
+  if (threadIdx.x == 0) least = several ? p.width : 0;
+  __syncthreads();
+  if (several) {
+    const int* theirs = p.page_table + int64_t(row_of(lead)) * p.table_stride;
     for (int b = from + cta * (kPlanThreads / 32) + warp; b < to; b += kPlanCtas * (kPlanThreads / 32)) {
-      const int row = row_of(b), n = __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b);
-      int pages = 0;
-      if (lead_ok && row >= 0 && row < p.rows && n >= 0) {
-        const int64_t kv = std::min<int64_t>(__ldg(p.kv_lens + row), int64_t(p.width) * p.page);
-        pages = int(std::max<int64_t>(kv - n, 0) / p.page);
-        const int* mine = p.page_table + int64_t(row) * p.table_stride;
-        const int* theirs = p.page_table + int64_t(lead) * p.table_stride;
-        for (int j0 = 0; j0 < pages; j0 += 32 * kPlanLoads) {
-          bool differ[kPlanLoads];
+      const int row = counts(b, any);
+      if (row < 0) continue;
+      const int64_t kv = std::min<int64_t>(__ldg(p.kv_lens + row), int64_t(p.width) * p.page);
+      int pages = int(std::max<int64_t>(kv - new_of(b), 0) / p.page);
+      const int* mine = p.page_table + int64_t(row) * p.table_stride;
+      for (int j0 = 0; j0 < pages; j0 += 32 * kPlanLoads) {
+        bool differ[kPlanLoads];
 #pragma unroll
-          for (int k = 0; k < kPlanLoads; ++k) {
-            const int j = j0 + k * 32 + lane;
-            differ[k] = false;
-            if (j < pages) {
-              const int page = __ldg(mine + j);
-              differ[k] = page != __ldg(theirs + j) || page < 0;
-            }
+        for (int k = 0; k < kPlanLoads; ++k) {
+          const int j = j0 + k * 32 + lane;
+          differ[k] = false;
+          if (j < pages) {
+            const int page = __ldg(mine + j);
+            differ[k] = page != __ldg(theirs + j) || page < 0;
           }
+        }
 #pragma unroll
-          for (int k = 0; k < kPlanLoads; ++k) {
-            const uint32_t at = __ballot_sync(0xffffffffu, differ[k]);
-            if (at) pages = std::min(pages, j0 + k * 32 + __ffs(at) - 1);
-          }
+        for (int k = 0; k < kPlanLoads; ++k) {
+          const uint32_t at = __ballot_sync(0xffffffffu, differ[k]);
+          if (at) pages = std::min(pages, j0 + k * 32 + __ffs(at) - 1);
         }
       }
       if (lane == 0) atomicMin(&least, pages);
@@ -95,8 +116,9 @@ __global__ void __launch_bounds__(kPlanThreads)
   cluster.sync();
   const int id = cta * kPlanThreads + int(threadIdx.x), step = kPlanCtas * kPlanThreads;
   for (int b = from + id; b < to; b += step) {
-    first[b] = all * p.page;
-    member[b] = g;
+    const bool shares = counts(b, 1) >= 0;
+    first[b] = shares ? all * p.page : 0;
+    member[b] = shares ? g : b == from && all > 0 ? -2 - lead : -1;
   }
   if (id == 0) shared[g] = all * p.page;
   if (g == 0) {  // sequences of no group

@@ -253,8 +253,8 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
 
 }  // namespace
 
-// int32 [groups + 2 * sequences]: the tokens that each group shares, then for each sequence
-// those that its group shares and its group, or -1.
+// int32 [groups + 2 * sequences]: the tokens that each group shares, then those that each
+// sequence shares with its group, then each one's group, or below 0 (PagedParams::first).
 torch::Tensor shared_prefix(torch::Tensor page_table, torch::Tensor kv_lens, torch::Tensor cu_q,
                             torch::Tensor groups, int64_t page, OptTensor slots, torch::Tensor status) {
   MGFA_CHECK(page_table.is_cuda(), "page_table must be a CUDA tensor");

@@ -56,7 +56,8 @@ def _scale(head_dim: int, softmax_scale: Optional[float]) -> float:
 
 class SharedPrefix(NamedTuple):
     """What the sequences of a batch share (shared_prefix()): cu_groups, the groups; plan, int32,
-    the tokens that each group shares, then each sequence's, then its group."""
+    the tokens that each group shares, then each sequence's, then its group (below 0: it shares
+    nothing)."""
     cu_groups: torch.Tensor
     plan: torch.Tensor
 
@@ -80,9 +81,11 @@ def shared_prefix(page_table: torch.Tensor, kv_lens: torch.Tensor, cu_seqlens_q:
     """The plan with which paged_attention reads what sequences share once for all of them.
 
     cu_groups int32 [groups + 1]: group g is the batch's sequences [cu_groups[g],
-    cu_groups[g + 1]), neighbours, as forks of one prompt. They share the leading pages that
-    the page table names alike for all of them, as far as these are full and hold none of
-    their new tokens; a sequence alone, or outside every group, shares nothing. The other
+    cu_groups[g + 1]), neighbours, as forks of one prompt. Those with new tokens share the
+    leading pages that the page table names alike for all of them, as far as these are full
+    and hold none of their new tokens; one alone, or outside every group, shares nothing. A
+    group may keep sequences that have ended: without new tokens they change nothing,
+    whether they are freed or not. The other
     arguments are those of paged_attention, whose batch the plan is of: it holds until the
     lengths or the page table change, hence for all layers of a step. Up to 4096 sequences
     and groups. Everything stays on the device. cu_groups that fall or leave the batch are

@@ -91,3 +91,76 @@ def test_as_many_sequences_and_groups_as_a_call_takes(groups, heads, kv_heads, D
     p.check(*p.run(shared=plan))
     with pytest.raises(RuntimeError, match="at most 4096 sequences and groups"):
         p.plan(groups=_ints(p.cg + [p.cg[-1]]))
+
+
+@pytest.mark.parametrize("gone", [[0], [5], [0, 1, 2], [27], [3, 9, 20], list(range(27)), list(range(28))])
+def test_sequences_that_have_ended_end_no_sharing(gone):
+    """Freed members without new tokens, first ones too; one that is left alone shares nothing."""
+    p = _batch(new={b: 0 for b in gone})
+    for b in gone:
+        p.table[b] = -1
+        p.lens[b] = 0
+    plan = p.plan()
+    left = 28 - len(gone)
+    assert plan.lens.tolist() == [192 if left > 1 else 0, 112]
+    first, member = plan.plan[2:].view(2, 38).tolist()
+    for b in range(28):
+        assert first[b] == (0 if b in gone or left == 1 else 192)
+        assert (member[b] == 0) == (b not in gone)
+    for causal in (True, False):
+        p.check(*p.run(causal=causal, shared=plan), causal)
+
+
+def test_a_slot_out_of_range_ends_no_sharing():
+    """Of the first of a group, with a new token: an error, and the others share as before."""
+    from multi_gpu_flashattention_b200 import KernelStatusError
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    p = _batch()
+    slots = _ints(list(range(38)))
+    slots[0] = slots[29] = 38
+    plan = p.plan(slots=slots)
+    assert plan.lens.tolist() == [192, 112]
+    out, lse = p.run(slots=slots, shared=plan)
+    with pytest.raises(KernelStatusError):
+        check_errors()
+    p.new[0] = p.new[29] = 0
+    p.check(out, lse)
+
+
+def test_a_captured_batch_whose_answers_end_one_by_one():
+    """A padded batch of a fixed form, whose sequences are freed between replays: the rest share
+    the prompt's pages to the last pair."""
+    from multi_gpu_flashattention_b200 import PagedKVCache
+    g = torch.Generator("cuda").manual_seed(0)
+    make = lambda n, h: torch.randn(n, h, 64, device="cuda", generator=g).bfloat16()
+    cache = PagedKVCache.allocate(1, 200, 16, 2, 64, 12, 600)
+    cache.reserve([0], [0, 150], 150)
+    cache.write(0, make(150, 2), make(150, 2), [0], [0, 150])
+    cache.fork([0] * 11, list(range(1, 12)))
+    slots, cu, groups = _ints(list(range(12))), _ints(list(range(13))), _ints([0, 12])
+    k, v, q = make(12, 2), make(12, 2), make(12, 4)
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+
+    def step():
+        cache.reserve(slots, cu, 12)
+        shared = cache.shared_prefix(slots, cu, groups)
+        cache.write(0, k, v, slots, cu)
+        cache.attend(0, q, slots, cu, 1, out=a, shared=shared)
+        cache.attend(0, q, slots, cu, 1, out=b)
+        return shared.lens
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lens = step()
+    live = list(range(12))
+    for end in (0, 7, 1, 11, 4, 2, 3, 10, 5, 6):
+        live.remove(end)
+        cache.free([end])
+        # the rows stay packed, the ended sequences take none
+        cu.copy_(_ints([sum(s in live for s in range(i)) for i in range(13)]))
+        graph.replay()
+        assert lens.tolist() == [144]
+        n, u = len(live), 2.0 ** -8
+        # (as in test_cache_forks_and_streams)
+        x, y = a[:n].float(), b[:n].float()
+        assert ((x - y).abs() <= 2 * (u * y.abs() + (u + 4e-5) * 4.5)).all()
