@@ -161,10 +161,12 @@ __device__ __forceinline__ PagedSeq paged_group(const PagedParams& p, int g) {
   const int a = __ldg(p.groups + g), e = __ldg(p.groups + g + 1), kv = __ldg(p.shared + g);
   s.bad = a < 0 || e < a || e > p.own || kv < 0 || kv > int64_t(p.width) * p.page || kv % p.page;
   if (s.bad || kv == 0 || a == e) return s;
-  const int q0 = __ldg(p.cu_q + a), end = __ldg(p.cu_q + e), other = -2 - __ldg(p.first + p.own + a);
+  // (a sequence whose rows leave the batch is served by none, the others of its group are)
+  const int q0 = max(__ldg(p.cu_q + a), 0), end = min(__ldg(p.cu_q + e), p.tokens);
+  const int other = -2 - __ldg(p.first + p.own + a);
   int row = p.slots ? __ldg(p.slots + a) : a;
   if (other > a && other < e) row = p.slots ? __ldg(p.slots + other) : other;
-  s.bad = q0 < 0 || end < q0 || end > p.tokens || row < 0 || row >= p.rows;
+  s.bad = end < q0 || row < 0 || row >= p.rows;
   const int64_t rows = int64_t(end - q0) * p.group;
   if (s.bad || rows < p.least_rows || rows > p.most_rows) return s;
   s.n = end - q0;

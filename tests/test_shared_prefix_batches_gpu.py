@@ -164,3 +164,27 @@ def test_a_captured_batch_whose_answers_end_one_by_one():
         # (as in test_cache_forks_and_streams)
         x, y = a[:n].float(), b[:n].float()
         assert ((x - y).abs() <= 2 * (u * y.abs() + (u + 4e-5) * 4.5)).all()
+
+
+@pytest.mark.parametrize("small", [False, True])
+@pytest.mark.parametrize("first,last", [(-1, 0), (0, 1), (-2, 3)])
+def test_rows_that_leave_the_batch_are_reported(first, last, small):
+    """cu_seqlens that begins below 0 and ends behind the tokens: the sequences there are not
+    served, the others of their groups are, with their prefix; in three launches and in one."""
+    from multi_gpu_flashattention_b200 import KernelStatusError
+    from multi_gpu_flashattention_b200.ops.flash import check_errors
+    p = Forked([(200, [(9, 1)] * 4)] if small else [(200, [(9, 1)] * 28), (120, [(9, 1)] * 10)], 8, 2, 64, 16)
+    n = len(p.kv)
+    p.cu[0] += first
+    p.cu[n] += last
+    plan = p.plan()
+    assert plan.lens.tolist() == ([192] if small else [192, 112])
+    check_errors()
+    out, lse = p.run(max_new=4, shared=plan)
+    with pytest.raises(KernelStatusError):
+        check_errors()
+    if first:
+        p.new[0] = 0
+    if last:
+        p.new[n - 1] = 0
+    p.check(out, lse)
