@@ -109,7 +109,8 @@ class RingAttentionBlock(nn.Module):
         else:
             if self.qk_norm:
                 q, k = self.q_norm(q), self.k_norm(k)
-            q, k = rotary(q, pos), rotary(k, pos)
+            # (under autocast the norms' 32-bit weights widen q and k)
+            q, k = rotary(q, pos).to(v.dtype), rotary(k, pos).to(v.dtype)
         a = ring_attention(q.contiguous(), k.contiguous(), v.contiguous(), causal=self.causal,
                            group=group, layout=layout, backend=backend)
         a = self.wo(a.reshape(B, L, self.h * self.d).to(x.dtype))

@@ -69,3 +69,24 @@ def test_host_tensors_are_refused():
     i32 = dict(dtype=torch.int32)
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         shared_prefix(torch.zeros(2, 4, **i32), torch.ones(2, **i32), torch.arange(3, **i32), torch.tensor([0, 2], **i32), 16)
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_attention_gets_one_type_under_autocast(monkeypatch, qk_norm):
+    """32-bit norm weights widen what products in 16 bits gave; q, k and v reach the attention alike."""
+    from multi_gpu_flashattention_b200 import RingLayout
+    from multi_gpu_flashattention_b200.models import transformer
+    seen = []
+
+    def attention(q, k, v, **kw):
+        seen.append((q.dtype, k.dtype, v.dtype))
+        return q
+
+    monkeypatch.setattr(transformer, "ring_attention", attention)
+    m = _model(qk_norm=qk_norm)
+    with torch.autocast("cpu", torch.bfloat16):
+        m(torch.randint(0, 50, (1, 10)), RingLayout("contiguous", 10, 1, mask="causal"))
+    assert seen == [(torch.bfloat16,) * 3] * 2
+    seen.clear()
+    m(torch.randint(0, 50, (1, 10)), RingLayout("contiguous", 10, 1, mask="causal"))
+    assert seen == [(torch.float32,) * 3] * 2

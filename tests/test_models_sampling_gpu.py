@@ -275,3 +275,23 @@ def test_a_forked_sequence_without_room(monkeypatch):
     for i in range(3):
         far = _off(plain(torch.cat([prompt, ids[i:i + 1]])[None], _layout(65))[0, -1], exact[i])
         assert _off(got[7][i], exact[i]) <= 1.5 * far + 1e-3
+
+
+def test_training_with_normed_heads_under_autocast():
+    """A stream in 32 bits, products in 16, with and without the kernels: gradients of the fused
+    model as far from 64 bits as the plain model's."""
+    ids = torch.randint(0, VOCAB, (130,), generator=torch.Generator().manual_seed(17)).cuda()
+    lay = _layout(129)
+    offs = {}
+    for fused in (False, True):
+        model = _model(torch.float32, fused)
+        with torch.autocast("cuda", torch.bfloat16):
+            out = model(ids[None, :-1], lay)[0]
+        F.cross_entropy(out.float(), ids[1:]).backward()
+        logits, P = _exact(model, ids[:-1])
+        names = [n for n, _ in model.named_parameters()]
+        grads = torch.autograd.grad(F.cross_entropy(logits, ids[1:]), [P[n] for n in names])
+        offs[fused] = {n: _off(p.grad, g) for (n, p), g in zip(model.named_parameters(), grads)}
+    plain = sum(offs[False].values()) / len(offs[False])
+    for n, o in offs[True].items():
+        assert o <= 1.5 * max(offs[False][n], plain), (n, o, offs[False][n], plain)
