@@ -102,8 +102,7 @@ class RingAttentionBlock(nn.Module):
         k = self.wk(h).view(B, L, self.hkv, self.d)
         v = self.wv(h).view(B, L, self.hkv, self.d)
         if fused and self.qk_norm:
-            q, k = apply_norm_rotary(q, k, pos.to(x.device), _frequencies(self.d, x.device),
-                                     self.q_norm.weight, self.k_norm.weight, eps=self.q_norm.eps)
+            q, k = self._norm_rotary(q, k, pos.to(x.device))
         elif fused:
             q, k = apply_rotary(q, k, pos.to(x.device), _frequencies(self.d, x.device))
         else:
@@ -121,6 +120,14 @@ class RingAttentionBlock(nn.Module):
             x = x + a
             h = self.norm2(x)
         return x + self.mlp(h)
+
+    def _norm_rotary(self, q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor):
+        """Heads normed and rotated on the kernels; one pass takes both where their eps is one."""
+        a, b, inv_freq = self.q_norm, self.k_norm, _frequencies(self.d, q.device)
+        if a.eps == b.eps:
+            return apply_norm_rotary(q, k, pos, inv_freq, a.weight, b.weight, eps=a.eps)
+        return tuple(apply_norm_rotary(x, None, pos, inv_freq, n.weight, None, eps=n.eps)
+                     for x, n in ((q, a), (k, b)))
 
     def mlp(self, h: torch.Tensor) -> torch.Tensor:
         return self.w2(F.silu(self.w1(h)) * self.w3(h))
@@ -231,9 +238,13 @@ class RingTransformerLM(nn.Module):
         for i, blk in enumerate(self.blocks):
             q, k, v = (w(h).view(ids.numel(), n, blk.d)
                        for w, n in ((blk.wq, blk.h), (blk.wk, blk.hkv), (blk.wv, blk.hkv)))
-            norms = dict(q_weight=blk.q_norm.weight, k_weight=blk.k_norm.weight, eps=blk.q_norm.eps) \
-                if blk.qk_norm else {}
-            q = cache.append(i, q, k, v, pos, inv_freq, slots, cu_seqlens, **norms)
+            if blk.qk_norm and blk.q_norm.eps != blk.k_norm.eps:
+                q, k = blk._norm_rotary(q, k, pos)
+                cache.write(i, k, v, slots, cu_seqlens)
+            else:
+                norms = dict(q_weight=blk.q_norm.weight, k_weight=blk.k_norm.weight, eps=blk.q_norm.eps) \
+                    if blk.qk_norm else {}
+                q = cache.append(i, q, k, v, pos, inv_freq, slots, cu_seqlens, **norms)
             a = cache.attend(i, q, slots, cu_seqlens, max_seqlen, shared=shared)
             h, x = rms_norm(blk.wo(a.flatten(1)), blk.norm2.weight, residual=x, eps=blk.norm2.eps)
             after = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm

@@ -295,3 +295,46 @@ def test_training_with_normed_heads_under_autocast():
     plain = sum(offs[False].values()) / len(offs[False])
     for n, o in offs[True].items():
         assert o <= 1.5 * max(offs[False][n], plain), (n, o, offs[False][n], plain)
+
+
+def test_norms_of_queries_and_keys_have_an_eps_of_their_own():
+    """Trained on the kernels and served: as far from the formulas as the plain model, for an eps of
+    the keys that counts; each eps taken for the other's would be off by more."""
+    ids = torch.randint(0, VOCAB, (90,), generator=torch.Generator().manual_seed(19)).cuda()
+    plain, fused = _model(torch.bfloat16), _model(torch.bfloat16, fused=True)
+    for m in (plain, fused):
+        for b in m.blocks:
+            b.k_norm.eps = 0.5
+    wide = _model(torch.bfloat16).double()
+    for b in wide.blocks:
+        b.k_norm.eps = 0.5
+    want = _with_eps(wide, ids, 1e-6, 0.5)
+    far = _off(plain(ids[None], _layout(90))[0], want)
+    assert _off(_with_eps(wide, ids, 1e-6, 1e-6), want) > 4 * far and _off(_with_eps(wide, ids, 0.5, 0.5), want) > 4 * far
+    assert _off(fused(ids[None], _layout(90))[0], want) <= 1.5 * far
+    cache = fused.make_cache(8, 16, 2, 128)
+    assert _off(fused.serve(ids, cache, _ints([1]), _ints([0, 90]), 90), want) <= 1.5 * far
+
+
+def _with_eps(model, ids, q_eps, k_eps):
+    """_exact()'s logits with other eps in the heads' norms."""
+    import torch as t
+    P = {n: p.detach() for n, p in model.named_parameters()}
+    norm = lambda x, w, eps=1e-6: x * t.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w
+    S = ids.numel()
+    ang = t.arange(S, device="cuda", dtype=t.float64)[:, None] * 10000.0 ** (-t.arange(0, D, 2, device="cuda", dtype=t.float64) / D)
+    z = t.polar(t.ones_like(ang), ang)[:, None]
+    rot = lambda x: t.view_as_real(t.complex(*x.split(D // 2, -1)) * z).transpose(-1, -2).flatten(-2)
+    x = P["embed.weight"][ids]
+    hide = t.ones(S, S, dtype=t.bool, device="cuda").triu(1)
+    for i in range(LAYERS):
+        W = lambda n: P[f"blocks.{i}.{n}.weight"]
+        h = norm(x, W("norm1"))
+        q, k, v = ((h @ W(n).t()).view(S, -1, D) for n in ("wq", "wk", "wv"))
+        q, k = rot(norm(q, W("q_norm"), q_eps)), rot(norm(k, W("k_norm"), k_eps))
+        k, v = (y.repeat_interleave(HEADS // KV, 1) for y in (k, v))
+        s = t.einsum("qhd,khd->hqk", q, k) / D ** 0.5
+        x = x + t.einsum("hqk,khd->qhd", t.softmax(s.masked_fill(hide, float("-inf")), -1), v).reshape(S, -1) @ W("wo").t()
+        h = norm(x, W("norm2"))
+        x = x + (F.silu(h @ W("w1").t()) * (h @ W("w3").t())) @ W("w2").t()
+    return norm(x, P["norm.weight"]) @ P["embed.weight"].t()
