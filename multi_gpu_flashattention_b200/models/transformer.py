@@ -204,8 +204,9 @@ class RingTransformerLM(nn.Module):
         return PagedKVCache.allocate(len(self.blocks), pages, page_size, self.blocks[0].hkv,
                                      self.blocks[0].d, slots, max_tokens, dtype=w.dtype, device=w.device)
 
-    def _check_served(self, ids: torch.Tensor, cache: PagedKVCache, max_seqlen: int) -> None:
-        """What a layer would refuse, before the cache grows."""
+    def _check_served(self, ids: torch.Tensor, cache: PagedKVCache, max_seqlen: int,
+                      slots: torch.Tensor, cu_groups: Optional[torch.Tensor]) -> None:
+        """What a layer or the plan would refuse, before the cache grows."""
         w, blk, k = self.embed.weight, self.blocks[0], cache.k
         if ids.dim() != 1 or max_seqlen < 0:
             raise ValueError(f"ids must be [tokens] and max_seqlen not negative, got {list(ids.shape)} and {max_seqlen}")
@@ -214,6 +215,15 @@ class RingTransformerLM(nn.Module):
             raise ValueError("the cache does not fit the model: see make_cache()")
         if blk.h % blk.hkv or blk.h // blk.hkv > 128:
             raise ValueError("heads must be a multiple of kv heads, up to 128 times")
+        for b in self.blocks:
+            if b.qk_norm and not (b.q_norm.weight.dtype == b.k_norm.weight.dtype in (w.dtype, torch.float32)
+                                  and b.q_norm.eps >= 0 and b.k_norm.eps >= 0):
+                raise ValueError("the heads' norms need weights of one type, the model's or float32, and an eps >= 0")
+        g = cu_groups
+        if g is not None and (g.dtype != torch.int32 or g.dim() != 1 or not g.is_contiguous() or
+                              g.device != k.device or not 1 <= g.numel() <= 4097 - len(slots)):
+            raise ValueError("cu_groups must be a contiguous int32 tensor [groups + 1] on the cache's device, "
+                             "with at most 4096 sequences and groups")
 
     @torch.no_grad()
     def serve(self, ids: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
@@ -229,7 +239,9 @@ class RingTransformerLM(nn.Module):
         was, are NaN. bfloat16 or float16 parameters, head_dim 64 or 128.
         cu_groups (int32 [groups + 1], CUDA): sequences [cu_groups[g], cu_groups[g + 1]) were
         forked from one prompt, whose full pages the attention then reads once for all of them."""
-        self._check_served(ids, cache, max_seqlen)
+        if cu_groups is not None and not isinstance(cu_groups, torch.Tensor):
+            cu_groups = torch.tensor(cu_groups, dtype=torch.int32, device=cache.k.device)
+        self._check_served(ids, cache, max_seqlen, slots, cu_groups)
         pos = cache.reserve(slots, cu_seqlens, ids.numel())
         shared = None if cu_groups is None else cache.shared_prefix(slots, cu_seqlens, cu_groups)
         inv_freq = _frequencies(self.blocks[0].d, ids.device)

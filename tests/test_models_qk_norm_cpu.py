@@ -90,3 +90,50 @@ def test_attention_gets_one_type_under_autocast(monkeypatch, qk_norm):
     seen.clear()
     m(torch.randint(0, 50, (1, 10)), RingLayout("contiguous", 10, 1, mask="causal"))
     assert seen == [(torch.float32,) * 3] * 2
+
+
+class _Cache:
+    """Notes that a call has reached it."""
+
+    def __init__(self, k):
+        self.k, self.reserved = k, False
+
+    def reserve(self, *a):
+        self.reserved = True
+        raise KeyError("reserved")
+
+
+@pytest.mark.parametrize("cu_groups,fits", [
+    (torch.tensor([0, 2]), False), (torch.tensor([[0, 2]], dtype=torch.int32), False),
+    (torch.tensor([], dtype=torch.int32), False), (torch.tensor([0, 9, 2, 9], dtype=torch.int32)[::2], False),
+    (torch.zeros(4096, dtype=torch.int32), False), (torch.zeros(2, dtype=torch.int32, device="meta"), False),
+    (torch.zeros(4095, dtype=torch.int32), True), (torch.zeros(1, dtype=torch.int32), True),
+    (torch.tensor([0, 2], dtype=torch.int32), True), ([0, 1, 2], True), ([], False), (None, True)])
+def test_groups_are_refused_before_the_cache_grows(cu_groups, fits):
+    m = _model()
+    cache = _Cache(torch.zeros(2, 4, 16, 2, 16))
+    slots, cu = torch.tensor([0, 1], dtype=torch.int32), torch.tensor([0, 1, 2], dtype=torch.int32)
+    with pytest.raises(KeyError if fits else ValueError, match="reserved" if fits else "cu_groups must be"):
+        m.serve(torch.tensor([1, 2]), cache, slots, cu, 1, cu_groups=cu_groups)
+    assert cache.reserved == fits
+
+
+def test_norms_are_refused_before_the_cache_grows():
+    def double(b):
+        b.k_norm.double()
+
+    def both(b):
+        b.k_norm.double(), b.q_norm.double()
+
+    def below(b):
+        b.k_norm.eps = -1e-6
+
+    slots, cu = torch.tensor([0], dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32)
+    for change in (double, both, below, None):
+        m = _model(qk_norm=True)
+        if change:
+            change(m.blocks[1])
+        cache = _Cache(torch.zeros(2, 4, 16, 2, 16))
+        with pytest.raises(ValueError if change else KeyError, match="heads' norms" if change else "reserved"):
+            m.serve(torch.tensor([1, 2]), cache, slots, cu, 2)
+        assert cache.reserved == (change is None)
