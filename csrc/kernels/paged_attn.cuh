@@ -23,6 +23,7 @@
 
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #ifdef __CUDACC__
 #include "sm100_ptx.cuh"
@@ -71,15 +72,25 @@ struct PagedParams {
   int units = 0;         // seqs * kv_heads * max_units
   int whole = 0;         // 1: the units are dealt out whole: no shares, no parts
   int grid = 0;          // CTAs
-  int unit_rows = 0;     // rows of a part in the workspace (kPagedHeadsApart: of each of its heads)
-  int form = kPagedByRows;
+  int unit_rows = 0;     // rows of a part in the workspace
   // workspace: parts [2 * grid][unit_rows][head_dim] and their (max, sum), log2 units; the
   // parts of share c are 2 c (a unit that an earlier share began) and 2 c + 1
   float* part_o = nullptr;
   float2* part_ml = nullptr;
-  // sequences that share a prefix (paged_shared.cu): sequences [0, own) come without the
-  // first[b] tokens that their group shares, and behind them the groups, each the new tokens
-  // of its sequences over the shared[g] tokens before; `seqs` counts both
+  int4* join = nullptr;  // [grid] of the unit that share c began and others go on with:
+                         // its first row of q, first head, rows (0: none), last share
+  uint32_t* status = nullptr;
+  uint64_t wait_limit_ns = 0;
+};
+
+// A launch for sequences that share a prefix (paged_shared.cu): sequences [0, own) come without
+// the first[b] tokens that their group shares, and behind them the groups, each the new tokens
+// of its sequences over the shared[g] tokens before; `seqs` counts both. The kernels are
+// compiled for either type of parameters, so that calls without a plan pay nothing for what
+// only these need (in one kernel 64 sequences of six new tokens over up to 1024 keys took 138
+// us instead of 134, chunks of 16 tokens 100 instead of 97).
+struct PagedGroupParams : PagedParams {
+  int form = kPagedByRows;  // (kPagedHeadsApart: unit_rows are those of each of its heads)
   const int* first = nullptr;   // [own]; null: nothing is shared. Behind it member, [own]: a
                                 // sequence's group, -1: none; -2 - b where a group's first one
                                 // shares nothing, b being the first that does
@@ -99,22 +110,18 @@ struct PagedParams {
   const uint32_t* other_tiles[2] = {nullptr, nullptr};
   float cost = 0.f, other_cost[2] = {0.f, 0.f};  // kv_heads times a tile's time on an SM
   int sms = 0, sm_ctas = 0;  // of the device; of this launch on an SM
-  int4* join = nullptr;  // [grid] of the unit that share c began and others go on with:
-                         // its first row of q, first head, rows (0: none), last share
-  uint32_t* status = nullptr;
-  uint64_t wait_limit_ns = 0;
 };
 
 // The launches for sequences that share prefixes: one of the sequences' own keys, others of
 // groups, by their rows.
 struct PagedSharedParams {
-  PagedParams launch[3];
+  PagedGroupParams launch[3];
   int launches = 0;
   int own = 0;  // which one
-  const int* member = nullptr;  // [sequences], behind PagedParams::first
+  const int* member = nullptr;  // [sequences], behind PagedGroupParams::first
 };
 
-// Entries of PagedParams::desc a key head, of `seqs` sequences or groups. Their units are
+// Entries of PagedGroupParams::desc a key head, of `seqs` sequences or groups. Their units are
 // numbered by their rows (two sequences' never meet, as every sequence before adds one); the
 // groups' come behind the sequences'.
 #ifdef __CUDACC__
@@ -145,6 +152,9 @@ struct PagedBase {
   }
 };
 
+template <class P>
+constexpr bool kShares = std::is_same_v<P, PagedGroupParams>;
+
 // Sequence b as the kernels use it, whatever the arrays say: n new tokens from row q0,
 // all inside [0, tokens) and at most max_new; kv within the table's row, behind `skip` pages;
 // new token i sees keys [0, base + i], those below kv. `bad` says that something had to be
@@ -154,8 +164,8 @@ struct PagedSeq {
   bool bad;
 };
 
-// Group g (PagedParams::groups) as a sequence.
-__device__ __forceinline__ PagedSeq paged_group(const PagedParams& p, int g) {
+// Group g (PagedGroupParams::groups) as a sequence.
+__device__ __forceinline__ PagedSeq paged_group(const PagedGroupParams& p, int g) {
   PagedSeq s;
   s.n = s.kv = s.base = s.q0 = s.row = s.skip = 0;
   const int a = __ldg(p.groups + g), e = __ldg(p.groups + g + 1), kv = __ldg(p.shared + g);
@@ -176,13 +186,16 @@ __device__ __forceinline__ PagedSeq paged_group(const PagedParams& p, int g) {
   return s;
 }
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
-  if (p.first && b >= p.own) return paged_group(p, b - p.own);
+template <class P>
+__device__ __forceinline__ PagedSeq paged_seq(const P& p, int b) {
   PagedSeq s;
-  if (p.no_own) {
-    s.q0 = s.n = s.kv = s.base = s.row = s.skip = 0;
-    s.bad = false;
-    return s;
+  if constexpr (kShares<P>) {
+    if (b >= p.own) return paged_group(p, b - p.own);
+    if (p.no_own) {
+      s.q0 = s.n = s.kv = s.base = s.row = s.skip = 0;
+      s.bad = false;
+      return s;
+    }
   }
   s.skip = 0;
   s.q0 = __ldg(p.cu_q + b);
@@ -201,7 +214,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     s.bad = true;
     s.kv = s.kv < 0 ? 0 : int(most);
   }
-  if (p.first) {
+  if constexpr (kShares<P>) {
     const int first = __ldg(p.first + b);
     if (first < 0 || first > s.kv || first % p.page) {
       s.bad = true;
@@ -238,8 +251,8 @@ __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
 // total, which is 0, and an error, where it does not fit 32 bits: nothing is done then.
 // Called by all kThreads threads of the CTA; `sums` holds kThreads / 32 values. report: this
 // CTA, one for each launch, tells the status word what is wrong with the sequences.
-template <int kThreads>
-__device__ __forceinline__ void paged_prefix(const PagedParams& p, uint32_t* prefix,
+template <int kThreads, class P>
+__device__ __forceinline__ void paged_prefix(const P& p, uint32_t* prefix,
                                              uint32_t* sums, bool report) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t before = 0;
@@ -289,7 +302,8 @@ struct PagedUnit {
   uint64_t first;
 };
 
-__device__ __forceinline__ PagedUnit paged_find(const PagedParams& p, const uint32_t* prefix,
+template <class P>
+__device__ __forceinline__ PagedUnit paged_find(const P& p, const uint32_t* prefix,
                                                 uint64_t w) {
   PagedUnit u;
   int lo = 0, hi = p.seqs;  // the last b with prefix[b] * kv_heads <= w
@@ -314,7 +328,8 @@ __device__ __forceinline__ PagedUnit paged_find(const PagedParams& p, const uint
 }
 
 // The unit behind `u`, which is not the last.
-__device__ __forceinline__ void paged_next(const PagedParams& p, const uint32_t* prefix,
+template <class P>
+__device__ __forceinline__ void paged_next(const P& p, const uint32_t* prefix,
                                            PagedUnit& u) {
   u.first += uint32_t(u.tiles);
   if (++u.unit >= paged_units(p, u.s)) {
@@ -329,8 +344,8 @@ __device__ __forceinline__ void paged_next(const PagedParams& p, const uint32_t*
   u.tiles = paged_unit_tiles(p, u.s, u.unit);
 }
 
-// The place of a unit in PagedParams::desc.
-__device__ __forceinline__ int64_t paged_desc(const PagedParams& p, const PagedSeq& s, int b, int unit, int hk) {
+// The place of a unit in PagedGroupParams::desc.
+__device__ __forceinline__ int64_t paged_desc(const PagedGroupParams& p, const PagedSeq& s, int b, int unit, int hk) {
   const int64_t at = b < p.own ? b : paged_desc_rows(p, p.own) + b - p.own;
   return (at + s.q0 / p.block_tokens + unit) * p.kv_heads + hk;
 }
@@ -338,19 +353,23 @@ __device__ __forceinline__ int64_t paged_desc(const PagedParams& p, const PagedS
 // At the end of a launch that may have begun early: it ends behind the one before it, so that
 // what waits for this one sees the results of both. One CTA is enough, the last, which the others
 // have all begun before: more would keep the SMs from the launch that comes next.
+template <class P>
 __device__ __forceinline__ void paged_behind() {
-  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (kShares<P> && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+template <class P>
 struct PagedShare {
-  const PagedParams& p;
+  const P& p;
   const uint32_t* prefix;
   uint64_t total, per;
   uint32_t snap;
-  __device__ __forceinline__ PagedShare(const PagedParams& params, const uint32_t* pre)
+  __device__ __forceinline__ PagedShare(const P& params, const uint32_t* pre)
       : p(params), prefix(pre) {
     total = uint64_t(prefix[p.seqs]) * uint32_t(p.kv_heads);
-    const uint32_t grid = p.tiles ? prefix[p.seqs + 1] : uint32_t(p.grid);
+    uint32_t grid = uint32_t(p.grid);
+    if constexpr (kShares<P>)
+      if (p.tiles) grid = prefix[p.seqs + 1];
     per = (total + grid - 1) / grid;
     if (per < uint32_t(p.min_share)) per = uint32_t(p.min_share);
     snap = per / 2 < uint32_t(p.snap) ? uint32_t(per / 2) : uint32_t(p.snap);
@@ -402,7 +421,7 @@ __device__ __forceinline__ bool paged_whole(const PagedParams& p, int id, PagedU
 
 // What share c, of tiles [begin, end), leaves for others to go on with. `u` is its last
 // unit.
-__device__ __forceinline__ void paged_join(const PagedShare& share, const PagedUnit& u, bool any,
+__device__ __forceinline__ void paged_join(const PagedShare<PagedParams>& share, const PagedUnit& u, bool any,
                                            uint64_t begin, uint64_t end) {
   const PagedParams& p = share.p;
   if (!p.join) return;  // one share: nothing is left
@@ -419,7 +438,7 @@ __device__ __forceinline__ void paged_join(const PagedShare& share, const PagedU
 // share of the SMs, at least one, the largest launch taking what the others' leave. False for a
 // CTA that is none of them: it should end at once.
 template <int kThreads>
-__device__ __forceinline__ bool paged_divide(const PagedParams& p, uint32_t* prefix) {
+__device__ __forceinline__ bool paged_divide(const PagedGroupParams& p, uint32_t* prefix) {
   const uint32_t mine = p.tiles[p.seqs];
   float work = float(mine) * p.cost, all = work;
   float others[2];
@@ -445,8 +464,24 @@ __device__ __forceinline__ bool paged_divide(const PagedParams& p, uint32_t* pre
   return true;
 }
 
+// Where a row of a unit that is not written out goes, unnormalised: a whole unit's to its place in
+// acc_o and acc_ml (PagedGroupParams; of a group's unit if `group`), a part's to row `part` of
+// the workspace. It is row `at` of o and of ml.
+struct PagedRow {
+  float* o;
+  float2* ml;
+  int64_t at;
+};
+template <class P>
+__device__ __forceinline__ PagedRow paged_row(const P& p, bool whole, bool group, int64_t token, int64_t head, int64_t part) {
+  if constexpr (kShares<P>)
+    if (whole) return {p.acc_o, p.acc_ml, ((group ? int64_t(p.tokens) : 0) + token) * p.heads + head};
+  return {p.part_o, p.part_ml, part};
+}
+
 // A CTA's way through its work, run by run: tiles [t0, t1) of unit u. Its threads walk
 // alike, each warp's or each its own copy.
+template <class P>
 struct PagedWalk {
   PagedUnit u;
   int t0, t1;
@@ -456,23 +491,24 @@ struct PagedWalk {
   // The first run; false where there is none. Called by all kThreads threads, whose
   // earlier writes to shared memory all see after it.
   template <int kThreads>
-  __device__ __forceinline__ bool start(const PagedParams& p, uint32_t* prefix, uint32_t* sums) {
-    if (p.whole) {
+  __device__ __forceinline__ bool start(const P& p, uint32_t* prefix, uint32_t* sums) {
+    bool divided = false;
+    if constexpr (kShares<P>) {
+      divided = p.tiles;
+      if (divided && !paged_divide<kThreads>(p, prefix)) return false;
+    } else if (p.whole) {
       id = int(blockIdx.x) - int(gridDim.x);
       const bool any = next(p, prefix);
       __syncthreads();
       return any;
     }
-    if (p.tiles) {
-      if (!paged_divide<kThreads>(p, prefix)) return false;
-    } else {
-      paged_prefix<kThreads>(p, prefix, sums, blockIdx.x == 0);
-    }
-    const PagedShare share(p, prefix);
+    if (!divided) paged_prefix<kThreads>(p, prefix, sums, blockIdx.x == 0);
+    const PagedShare<P> share(p, prefix);
     begin = share.begin(blockIdx.x, u);
     end = share.end(blockIdx.x);
     if (begin >= end) {
-      if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
+      if constexpr (!kShares<P>)
+        if (threadIdx.x == 0) paged_join(share, u, false, begin, end);
       return false;
     }
     run(begin);
@@ -482,15 +518,17 @@ struct PagedWalk {
     t0 = int(w - u.first);
     t1 = end - u.first < uint64_t(u.tiles) ? int(end - u.first) : u.tiles;
   }
-  __device__ __forceinline__ bool next(const PagedParams& p, const uint32_t* prefix) {
-    if (p.whole) {
-      do {
-        id += int(gridDim.x);
-        if (id >= p.units) return false;
-      } while (!paged_whole(p, id, u));
-      t0 = 0;
-      t1 = u.tiles;
-      return true;
+  __device__ __forceinline__ bool next(const P& p, const uint32_t* prefix) {
+    if constexpr (!kShares<P>) {
+      if (p.whole) {
+        do {
+          id += int(gridDim.x);
+          if (id >= p.units) return false;
+        } while (!paged_whole(p, id, u));
+        t0 = 0;
+        t1 = u.tiles;
+        return true;
+      }
     }
     const uint64_t w = u.first + uint32_t(t1);
     if (w >= end) return false;
@@ -501,19 +539,17 @@ struct PagedWalk {
   __device__ __forceinline__ bool complete() const { return t0 == 0 && t1 == u.tiles; }
   // The workspace's part that takes an incomplete run.
   __device__ __forceinline__ int64_t part() const { return 2 * int64_t(blockIdx.x) + (t0 > 0 ? 0 : 1); }
-  // With desc: of each run, by one thread.
-  __device__ __forceinline__ void note(const PagedParams& p, const uint32_t* prefix) const {
-    if (!p.desc || t0 > 0) return;
-    p.desc[paged_desc(p, u.s, u.b, u.unit, u.hk)] =
-        complete() ? make_int2(-1, -1) : make_int2(int(blockIdx.x), PagedShare(p, prefix).last(u));
-  }
-  // A complete unit's row in acc_o and acc_ml.
-  __device__ __forceinline__ int64_t acc_row(const PagedParams& p, int token, int head) const {
-    return ((u.b < p.own ? 0 : int64_t(p.tokens)) + token) * p.heads + head;
+  // Of each run, by one thread (PagedGroupParams::desc).
+  __device__ __forceinline__ void note(const P& p, const uint32_t* prefix) const {
+    if constexpr (kShares<P>)
+      if (t0 == 0)
+        p.desc[paged_desc(p, u.s, u.b, u.unit, u.hk)] =
+            complete() ? make_int2(-1, -1) : make_int2(int(blockIdx.x), PagedShare<P>(p, prefix).last(u));
   }
   // After the last run, by one thread.
-  __device__ __forceinline__ void leave(const PagedParams& p, const uint32_t* prefix) const {
-    if (!p.whole) paged_join(PagedShare(p, prefix), u, true, begin, end);
+  __device__ __forceinline__ void leave(const P& p, const uint32_t* prefix) const {
+    if constexpr (!kShares<P>)
+      if (!p.whole) paged_join(PagedShare<P>(p, prefix), u, true, begin, end);
   }
 };
 
@@ -533,19 +569,22 @@ cudaError_t paged_allow_smem(Fn fn, std::atomic<uint64_t>& done) {
 
 // Few rows a key head (max_new * group <= 32).
 // early: may begin while the launch before, which it does not need, still runs.
-void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
-                         cudaStream_t stream, bool early = false);
+void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t stream);
+void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedGroupParams& p,
+                         cudaStream_t stream, bool early);
 // More rows: tcgen05 tiles.
 void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                        const PagedParams& p, cudaStream_t stream, bool early = false);
+                        const PagedParams& p, cudaStream_t stream);
+void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                        const PagedGroupParams& p, cudaStream_t stream, bool early);
 // The most local memory a thread of its forms was compiled with, which has to be none.
 int64_t paged_chunk_local_bytes();
 // Joins the parts; launched behind either.
 void paged_merge_launch(const PagedParams& p, cudaStream_t stream);
-// Sequences that share a prefix: `shared`, `first` and `member` (PagedParams::first) from
+// Sequences that share a prefix: `shared`, `first` and `member` (PagedGroupParams::first) from
 // the page table, for the groups of p. (Nothing but the arrays of the problem is read.)
-void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t stream);
-// Fills the launches' PagedParams::tiles, where they have it.
+void paged_plan_launch(const PagedGroupParams& p, int* shared, int* first, int* member, cudaStream_t stream);
+// Fills the launches' PagedGroupParams::tiles, where they have it.
 void paged_split_launch(const PagedSharedParams& p, cudaStream_t stream);
 // Joins own and shared parts, behind the launches that left them.
 void paged_shared_launch(const PagedSharedParams& p, cudaStream_t stream);

@@ -67,7 +67,7 @@ struct __align__(1024) ChunkSmem {
   // The runs, which the producer finds a few ahead: run number i in slot i & 3.
   struct Run {
     PagedSeq s;
-    int hk, unit, t0, t1, complete, part, acc;  // t1 < 0: there is none; acc: of acc_o's halves
+    int hk, unit, t0, t1, complete, part, of_group;  // t1 < 0: there is none
   } runs[4];
   uint64_t run_full[4], run_empty[4];
 };
@@ -99,11 +99,11 @@ __device__ __forceinline__ void hide(uint32_t (&sr)[64], int n) {
   }
 }
 
-template <int kD, bool kF16>
+template <int kD, bool kF16, class P>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
+                       const __grid_constant__ CUtensorMap map_v, const P p) {
   constexpr int kHalves = kD / 64;
   constexpr int kKSteps = kD / 16;  // MMA steps of S = Q K^T
   constexpr int kOChunks = kD / 32;
@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.drain, 1);
     fence_mbar_init();
   }
-  PagedWalk at;
-  if (!at.start<kThreads>(p, prefix, s.sums)) return paged_behind();  // the whole CTA
+  PagedWalk<P> at;
+  if (!at.start<kThreads>(p, prefix, s.sums)) return paged_behind<P>();  // the whole CTA
   if (warp == 0) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         r.t1 = t1;
         r.complete = at.complete();
         r.part = int(at.part());
-        r.acc = at.u.b >= p.own;
+        if constexpr (kShares<P>) r.of_group = at.u.b >= p.own;
         mbar_arrive(&s.run_full[run & 3]);
       }
       ++run;
@@ -458,13 +458,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             l = l * w0 + o.y * w1;
             m = top;
           }
-          const bool whole = u.complete, done = whole && !p.acc_o;
+          const bool whole = u.complete, done = whole && !kShares<P>;
           const int tok = tok0 + r / p.group, r_head = r % p.group;
           const bool valid = r < tile_tokens * p.group && tok < u.s.n;
           const int64_t row_tok = u.s.q0 + tok, head = int64_t(u.hk) * p.group + r_head;
-          const int64_t part = whole ? ((u.acc ? int64_t(p.tokens) : 0) + row_tok) * p.heads + head
-                                     : int64_t(u.part) * p.unit_rows +
-                                           (tok - u.unit * p.block_tokens) * p.group + r_head;
+          const int64_t part = int64_t(u.part) * p.unit_rows +
+                               (tok - u.unit * p.block_tokens) * p.group + r_head;
+          const PagedRow left = paged_row(p, whole, kShares<P> && u.of_group, row_tok, head, part);
           if (done) {
             const float scale = l == 0.f ? 0.f : 1.f / l;
             w0 *= scale;
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint8_t* to = done ? reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) +
                                                           row_tok * p.o_stride_t + head * p.o_stride_h)
-                             : reinterpret_cast<uint8_t*>((whole ? p.acc_o : p.part_o) + part * kD);
+                             : reinterpret_cast<uint8_t*>(left.o + left.at * kD);
           // one copy of the code for all columns: fetching it takes longer than running it
 #pragma unroll 1
           for (int ch = 0; ch < kOChunks; ++ch) {
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (valid) {
-            if (!done) (whole ? p.acc_ml : p.part_ml)[part] = make_float2(m, l);
+            if (!done) left.ml[left.at] = make_float2(m, l);
             else if (p.lse)
               p.lse[head * p.tokens + row_tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
@@ -528,24 +528,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc<512>(tmem);
-  paged_behind();
+  paged_behind<P>();
 }
 
-template <int kD, bool kF16>
+template <int kD, bool kF16, class P>
 int64_t chunk_local_bytes() {
   cudaFuncAttributes a;
-  const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<kD, kF16>);
+  const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<kD, kF16, P>);
   if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
   return int64_t(a.localSizeBytes);
 }
 
-template <int kD, bool kF16>
+template <int kD, bool kF16, class P>
 void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                  const PagedParams& p, cudaStream_t s, bool early) {
+                  const P& p, cudaStream_t s, bool early) {
   const int smem = int(paged_smem(sizeof(ChunkSmem<kD>), p.seqs));
   static_assert(paged_smem(sizeof(ChunkSmem<kD>), kPagedMaxSeqs) <= kPagedMaxSmem, "prefix[] of the largest batch fits");
-  auto fn = paged_chunk_kernel<kD, kF16>;
-  static const int64_t local = chunk_local_bytes<kD, kF16>();
+  auto fn = paged_chunk_kernel<kD, kF16, P>;
+  static const int64_t local = chunk_local_bytes<kD, kF16, P>();
   if (local != 0)
     throw std::runtime_error("paged attention: the chunk kernel was compiled with " + std::to_string(local) +
                              " bytes of local memory; its scores must not be spilled");
@@ -567,19 +567,34 @@ void chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
   if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
 }
 
-}  // namespace
-
-int64_t paged_chunk_local_bytes() {
-  return std::max(std::max(chunk_local_bytes<64, false>(), chunk_local_bytes<64, true>()),
-                  std::max(chunk_local_bytes<128, false>(), chunk_local_bytes<128, true>()));
+template <class P>
+int64_t any_local_bytes() {
+  return std::max(std::max(chunk_local_bytes<64, false, P>(), chunk_local_bytes<64, true, P>()),
+                  std::max(chunk_local_bytes<128, false, P>(), chunk_local_bytes<128, true, P>()));
 }
 
-void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                        const PagedParams& p, cudaStream_t s, bool early) {
+template <class P>
+void chunk_any(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const P& p, cudaStream_t s,
+               bool early) {
   if (p.head_dim == 64)
     p.fp16 ? chunk_launch<64, true>(mq, mk, mv, p, s, early) : chunk_launch<64, false>(mq, mk, mv, p, s, early);
   else
     p.fp16 ? chunk_launch<128, true>(mq, mk, mv, p, s, early) : chunk_launch<128, false>(mq, mk, mv, p, s, early);
+}
+
+}  // namespace
+
+int64_t paged_chunk_local_bytes() {
+  return std::max(any_local_bytes<PagedParams>(), any_local_bytes<PagedGroupParams>());
+}
+
+void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                        const PagedParams& p, cudaStream_t s) {
+  chunk_any(mq, mk, mv, p, s, false);
+}
+void paged_chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                        const PagedGroupParams& p, cudaStream_t s, bool early) {
+  chunk_any(mq, mk, mv, p, s, early);
 }
 
 }  // namespace mgfa

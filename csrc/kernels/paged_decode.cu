@@ -13,7 +13,7 @@
 // but the tile's; the four are added when a unit ends. 32 sequences of 8192 keys (8 key
 // heads of 128, pages of 16) take 171 us for 1.07 GB, 6.3 TB/s; one of 131072 keys 86 us,
 // and 9 us for joining 296 parts; with 4 new tokens each (16 rows) the 32 sequences take
-// 1.05 times as long, with 8 (32 rows, whose second block of 16 spills 528 bytes at head_dim
+// 1.05 times as long, with 8 (32 rows, whose second block of 16 spills 488 bytes at head_dim
 // 128) 1.34 times. For short sequences the time is latency: one token each
 // over 100 to 320 keys takes 9.6 us.
 //
@@ -105,10 +105,10 @@ __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;
 
 // kD head_dim, kF16 type. With kHeadsApart p.kv_heads counts fours of key heads, and p.tile
 // is 16.
-template <int kD, bool kF16, int kForm>
+template <int kD, bool kF16, int kForm, class P>
 __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD, kForm>::kCtas)
     paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
-                        const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
+                        const __grid_constant__ CUtensorMap map_v, const P p) {
   using Smem = DecodeSmem<kD, kForm>;
   constexpr int kStages = Smem::kStages, kHalves = kD / 64, kMT = Smem::kMT, kR = Smem::kRows;
   constexpr int kWarps = Smem::kWarps, kThreads = Smem::kThreads;
@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
     }
     fence_mbar_init();
   }
-  PagedWalk at;
-  if (!at.start<kThreads>(p, prefix, s.sums)) return paged_behind();  // the whole CTA
+  PagedWalk<P> at;
+  if (!at.start<kThreads>(p, prefix, s.sums)) return paged_behind<P>();  // the whole CTA
   uint32_t it = 0;
 
   if (warp == kWarps) {
@@ -182,12 +182,12 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
     AbortState drain{&never, nullptr, p.wait_limit_ns};
     for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
       mbar_wait(&s.full[i % kStages], (i / kStages) & 1, drain, 0);
-    return paged_behind();
+    return paged_behind<P>();
   }
 
   // -------------------------------------------------------------- consumers
   const int mi = lane >> 3, lr = lane & 7;  // matrix and row of this lane's ldmatrix address
-  const uint32_t quarter = warp % kConsumers;  // of a tile's 64 rows of K and V
+  const uint32_t quarter = Smem::kBlocks == 1 ? warp : warp % kConsumers;  // of a tile's 64 rows of K and V
   const int block = kForm == kRowsApart ? int(warp / kConsumers) * 16 : 0;  // the warp's first row of the unit's
   // K: matrices (keys 0-7, 8 columns), (keys 0-7, next 8), (keys 8-15, ..) twice
   const uint32_t k_row = quarter * 16 + (mi >> 1) * 8 + lr, k_col = (mi & 1) * 8;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
   bool ok = true;
   do {
     const PagedUnit& u = at.u;
-    // the sequence's or, of a group (PagedParams::groups, kRowsApart), the unit's
+    // the sequence's or, of a group (PagedGroupParams::groups, kRowsApart), the unit's
     const int tok0 = kForm == kRowsApart ? u.unit * p.block_tokens : 0, left = u.s.n - tok0;
     const int rows = (kForm == kRowsApart && left > p.block_tokens ? p.block_tokens : left) * p.group;
     const int q0 = u.s.q0 + tok0;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
         l = l < u.s.kv ? l : u.s.kv;
         lim[m][h] = r < rows ? l : 0;
       }
-    const int full_keys = u.s.base + tok0 + 1;  // seen by every row, those below kv
+    const int full_keys = min(u.s.base + tok0 + 1, u.s.kv);  // seen by every row
     float o[kMT][kD / 8][4], mx[kMT][2], sum[kMT][2];
 #pragma unroll
     for (int m = 0; m < kMT; ++m) {
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
         }
       }
       const int key0 = t * kTileKeys + (kApart ? 0 : int(quarter) * 16);
-      const bool whole = key0 + 16 <= full_keys && key0 + 16 <= u.s.kv;
+      const bool whole = key0 + 16 <= full_keys;
       uint32_t pf[kMT][4];
 #pragma unroll
       for (int m = 0; m < kMT; ++m) {
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
         if (r >= rows || !ok) continue;
         const int tok = q0 + r / p.group, head = hk * p.group + r % p.group, c0 = int(lane & 3) * 2;
         const float top = mx[0][h], base = top == -INFINITY ? 0.f : top;
-        if (done && !p.acc_o) {
+        if (done && !kShares<P>) {
           const float inv = total == 0.f ? 0.f : 1.f / total;  // 0: no visible key
           uint16_t* dst = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.o_stride_t + int64_t(head) * p.o_stride_h + c0;
 #pragma unroll
@@ -384,12 +384,12 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
             p.lse[int64_t(head) * p.tokens + tok] =
                 total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
         } else {
-          const int64_t to = done ? at.acc_row(p, tok, head) : (slot * kFourHeads + quarter) * p.unit_rows + r;
-          float* dst = (done ? p.acc_o : p.part_o) + to * kD + c0;
+          const PagedRow to = paged_row(p, done, at.u.b >= p.own, tok, head, (slot * kFourHeads + quarter) * p.unit_rows + r);
+          float* dst = to.o + to.at * kD + c0;
 #pragma unroll
           for (int n = 0; n < kD / 8; ++n)
             *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[0][n][2 * h], o[0][n][2 * h + 1]);
-          if (c0 == 0) (done ? p.acc_ml : p.part_ml)[to] = make_float2(top, total);
+          if (c0 == 0) to.ml[to.at] = make_float2(top, total);
         }
       }
       if (!ok) break;
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
       for (int k = 0; k < kConsumers; ++k) total += s.ml[k][r].y * ex2_approx(s.ml[k][r].x - base);
       const float* a = &s.acc[r][c];
       const int tok = q0 + r / p.group, head = u.hk * p.group + r % p.group;
-      if (done && !p.acc_o) {
+      if (done && !kShares<P>) {
         const float inv = total == 0.f ? 0.f : 1.f / total;  // 0: no visible key
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + int64_t(tok) * p.o_stride_t +
                                   int64_t(head) * p.o_stride_h + c) =
@@ -461,17 +461,19 @@ __global__ void __launch_bounds__(DecodeSmem<kD, kForm>::kThreads, DecodeSmem<kD
           p.lse[int64_t(head) * p.tokens + tok] =
               total == 0.f ? -INFINITY : (base + log2f(total)) * 0.6931471805599453f;
       } else {
-        const int64_t to = done ? at.acc_row(p, tok, head) : slot * p.unit_rows + r;
-        float* dst = (done ? p.acc_o : p.part_o) + to * kD + c;
+        bool of_group = false;
+        if constexpr (kShares<P>) of_group = u.b >= p.own;
+        const PagedRow to = paged_row(p, done, of_group, tok, head, slot * p.unit_rows + r);
+        float* dst = to.o + to.at * kD + c;
         *reinterpret_cast<float4*>(dst) = make_float4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<float4*>(dst + 4) = make_float4(a[4], a[5], a[6], a[7]);
-        if (c == 0) (done ? p.acc_ml : p.part_ml)[to] = make_float2(top, total);
+        if (c == 0) to.ml[to.at] = make_float2(top, total);
       }
     }
     if (threadIdx.x == 0) s.stop = *ab.flag;
     consumers_sync<kWarps>();  // q, acc and ml are free again
   } while (!(kApart ? *ab.flag : s.stop) && at.next(p, prefix));
-  paged_behind();
+  paged_behind<P>();
 }
 
 // ---------------------------------------------------------------------- joining the parts
@@ -560,10 +562,10 @@ void cuda_ok(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("paged attention: ") + cudaGetErrorString(e));
 }
 
-template <int kD, bool kF16, int kForm>
-void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s, bool early) {
+template <int kD, bool kF16, int kForm, class P>
+void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const P& p, cudaStream_t s, bool early) {
   using Smem = DecodeSmem<kD, kForm>;
-  auto fn = paged_decode_kernel<kD, kF16, kForm>;
+  auto fn = paged_decode_kernel<kD, kF16, kForm, P>;
   static std::atomic<uint64_t> allowed{0};
   cuda_ok(paged_allow_smem(fn, allowed));
   cudaLaunchConfig_t cfg = {};
@@ -579,25 +581,35 @@ void decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedPara
   cuda_ok(cudaLaunchKernelEx(&cfg, fn, mk, mv, p));
 }
 
-template <int kD, bool kF16>
-void decode_rows(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s, bool early) {
-  switch (p.form) {
-    case kPagedHeadsApart: return decode_launch<kD, kF16, kHeadsApart>(mk, mv, p, s, early);
-    case kPagedRowsApart: return decode_launch<kD, kF16, kRowsApart>(mk, mv, p, s, early);
-    default: break;
+template <int kD, bool kF16, class P>
+void decode_rows(const CUtensorMap& mk, const CUtensorMap& mv, const P& p, cudaStream_t s, bool early) {
+  if constexpr (kShares<P>) {
+    switch (p.form) {
+      case kPagedHeadsApart: return decode_launch<kD, kF16, kHeadsApart>(mk, mv, p, s, early);
+      case kPagedRowsApart: return decode_launch<kD, kF16, kRowsApart>(mk, mv, p, s, early);
+      default: break;
+    }
   }
   if (p.unit_rows <= 16) decode_launch<kD, kF16, kKeysOfOne>(mk, mv, p, s, early);
   else decode_launch<kD, kF16, kKeysOfTwo>(mk, mv, p, s, early);
 }
 
-}  // namespace
-
-void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
-                         cudaStream_t s, bool early) {
+template <class P>
+void decode_any(const CUtensorMap& mk, const CUtensorMap& mv, const P& p, cudaStream_t s, bool early) {
   if (p.head_dim == 64)
     p.fp16 ? decode_rows<64, true>(mk, mv, p, s, early) : decode_rows<64, false>(mk, mv, p, s, early);
   else
     p.fp16 ? decode_rows<128, true>(mk, mv, p, s, early) : decode_rows<128, false>(mk, mv, p, s, early);
+}
+
+}  // namespace
+
+void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p, cudaStream_t s) {
+  decode_any(mk, mv, p, s, false);
+}
+void paged_decode_launch(const CUtensorMap& mk, const CUtensorMap& mv, const PagedGroupParams& p,
+                         cudaStream_t s, bool early) {
+  decode_any(mk, mv, p, s, early);
 }
 
 template <int kD, bool kF16>

@@ -45,7 +45,7 @@ constexpr int kPlanLoads = 8;  // of each table that a lane has under way
 // is of all. Groups whose cu_seqlens fall share nothing; invalid ones neither, nor do all others
 // of the call then.
 __global__ void __launch_bounds__(kPlanThreads)
-    paged_plan_kernel(const PagedParams p, int* shared, int* first, int* member) {
+    paged_plan_kernel(const PagedGroupParams p, int* shared, int* first, int* member) {
   const int g = blockIdx.x / kPlanCtas, cta = blockIdx.x % kPlanCtas, n_groups = p.seqs - p.own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __shared__ int least, lead_of[2], live[2];  // of all sequences; of those with new tokens
@@ -135,13 +135,13 @@ __global__ void __launch_bounds__(kPlanThreads)
 // ---------------------------------------------------------------------- who does what
 constexpr int kSplitThreads = 1024;
 
-// CTA l: the tiles before each sequence and group of launch l (PagedParams::tiles), which its
+// CTA l: the tiles before each sequence and group of launch l (PagedGroupParams::tiles), which its
 // CTAs then need not find out for themselves. Each reports what its own launch's sequences and
 // groups have wrong: a launch of the groups alone looks at no sequence's own arguments.
 __global__ void __launch_bounds__(kSplitThreads) paged_split_kernel(const __grid_constant__ PagedSharedParams p) {
   extern __shared__ uint32_t prefix[];
   __shared__ uint32_t sums[kSplitThreads / 32];
-  const PagedParams& l = p.launch[blockIdx.x];
+  const PagedGroupParams& l = p.launch[blockIdx.x];
   paged_prefix<kSplitThreads>(l, prefix, sums, true);
   for (int i = threadIdx.x; i <= l.seqs; i += kSplitThreads) l.tiles[i] = prefix[i];
 }
@@ -159,7 +159,7 @@ struct RowParts {
 };
 
 // Of row (i, head) of sequence or group b, whose keys launch p took; heads: key heads of a unit.
-__device__ __forceinline__ RowParts row_parts(const PagedParams& p, const PagedSeq& s, int b, int i, int head) {
+__device__ __forceinline__ RowParts row_parts(const PagedGroupParams& p, const PagedSeq& s, int b, int i, int head) {
   const int heads = p.form == kPagedHeadsApart ? 4 : 1, hk = head / p.group;
   const int unit = i / p.block_tokens, tok = i - unit * p.block_tokens;
   const int2 d = p.desc[paged_desc(p, s, b, unit, hk / heads)];
@@ -190,7 +190,7 @@ template <int kD, bool kF16, int kSplit>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_shared_kernel(const __grid_constant__ PagedSharedParams p) {
   constexpr int kE = kD / 32, kRows = kJoinWarps / kSplit;
   __shared__ float sh[kSplit > 1 ? kJoinWarps : 1][kD];
-  const PagedParams& a = p.launch[p.own];
+  const PagedGroupParams& a = p.launch[p.own];
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
   const PagedSeq own = paged_seq(a, b);
   const int64_t rows = int64_t(own.n) * a.heads;
@@ -294,7 +294,7 @@ void cuda_ok(cudaError_t e) {
 template <int kD, bool kF16>
 void join_launch(const PagedSharedParams& p, cudaStream_t s) {
   // Few rows may have many parts each, many rows have few.
-  const PagedParams& a = p.launch[p.own];
+  const PagedGroupParams& a = p.launch[p.own];
   const int64_t rows = int64_t(a.max_new) * a.heads;
   const bool few = int64_t(a.own) * rows <= 1024;
   const int per = few ? kJoinWarps / 4 : kJoinWarps;
@@ -312,7 +312,7 @@ void join_launch(const PagedSharedParams& p, cudaStream_t s) {
 
 }  // namespace
 
-void paged_plan_launch(const PagedParams& p, int* shared, int* first, int* member, cudaStream_t s) {
+void paged_plan_launch(const PagedGroupParams& p, int* shared, int* first, int* member, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.seqs - p.own) * kPlanCtas);
   cfg.blockDim = dim3(kPlanThreads);
@@ -332,7 +332,7 @@ void paged_split_launch(const PagedSharedParams& p, cudaStream_t s) {
 }
 
 void paged_shared_launch(const PagedSharedParams& p, cudaStream_t s) {
-  const PagedParams& a = p.launch[0];
+  const PagedGroupParams& a = p.launch[0];
   if (a.head_dim == 64) a.fp16 ? join_launch<64, true>(p, s) : join_launch<64, false>(p, s);
   else a.fp16 ? join_launch<128, true>(p, s) : join_launch<128, false>(p, s);
 }

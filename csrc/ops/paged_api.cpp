@@ -133,7 +133,8 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
   const int64_t T = problem.tokens, D = problem.head_dim, n_groups = groups.size(0) - 1;
   const auto f32 = q.options().dtype(at::kFloat);
   PagedSharedParams j;
-  PagedParams p = problem;
+  PagedGroupParams p;
+  static_cast<PagedParams&>(p) = problem;
   p.own = p.seqs;
   p.seqs += int(n_groups);
   p.groups = groups.data_ptr<int>();
@@ -149,7 +150,7 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
 
   // A launch of 128-row tiles, or (block_tokens set) of the decode kernel, for the groups
   // of least_rows to most_rows rows, and the sequences' own keys unless no_own.
-  auto add = [&](PagedParams l) {
+  auto add = [&](PagedGroupParams l) {
     if (l.block_tokens) {
       l.tile = l.form == kPagedHeadsApart ? 16 : 64;
       l.sm_ctas = l.form == kPagedRowsApart ? 1 : 2;
@@ -172,7 +173,7 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
     l.grid = int(std::min<int64_t>(l.sm_ctas * sms, (units * tiles + l.min_share - 1) / l.min_share));
     j.launch[j.launches++] = l;
   };
-  PagedParams over = p;  // groups alone
+  PagedGroupParams over = p;  // groups alone
   over.no_own = 1;
   const int64_t group_rows = group_few_rows(p);
   const bool small = p.group <= 32 && T * p.group <= group_rows;
@@ -196,12 +197,12 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
         j.own = j.launches;
         add(p);
       } else if (large_first == (i == 0)) {  // on 128-row tiles
-        PagedParams large = over;
+        PagedGroupParams large = over;
         large.least_rows = group_rows + 1;
         large.most_rows = INT64_MAX;
         add(large);
       } else {
-        PagedParams small = over;
+        PagedGroupParams small = over;
         small.least_rows = 0;
         small.most_rows = group_rows;
         small.form = kPagedRowsApart;
@@ -219,7 +220,7 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
   torch::Tensor tiles;
   if (j.launches > 1) tiles = torch::empty({j.launches * counts}, plan.options());
   for (int i = 0; i < j.launches; ++i) {
-    PagedParams& l = j.launch[i];
+    PagedGroupParams& l = j.launch[i];
     const int64_t rows = 2 * int64_t(l.grid) * l.unit_rows * (l.form == kPagedHeadsApart ? 4 : 1);
     const int64_t descs = (paged_desc_rows(l, l.own) + paged_desc_rows(l, int(n_groups))) * l.kv_heads;
     work[i] = torch::empty({rows * (D + 2) + 2 * descs}, f32);
@@ -237,7 +238,7 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
   }
   if (j.launches > 1) paged_split_launch(j, stream);
   for (int i = 0; i < j.launches; ++i) {
-    const PagedParams& l = j.launch[i];
+    const PagedGroupParams& l = j.launch[i];
     const uint32_t chunk = uint32_t(std::min<int64_t>(l.page, l.tile)), heads = l.form == kPagedHeadsApart ? 4 : 1;
     const CUtensorMap mk = map16(k, {3, 1, 2, 0}, {64, chunk, heads, 1});
     const CUtensorMap mv = map16(v, {3, 1, 2, 0}, {64, chunk, heads, 1});
@@ -254,7 +255,7 @@ void attend_shared(const PagedParams& problem, bool few, const torch::Tensor& q,
 }  // namespace
 
 // int32 [groups + 2 * sequences]: the tokens that each group shares, then those that each
-// sequence shares with its group, then each one's group, or below 0 (PagedParams::first).
+// sequence shares with its group, then each one's group, or below 0 (PagedGroupParams::first).
 torch::Tensor shared_prefix(torch::Tensor page_table, torch::Tensor kv_lens, torch::Tensor cu_q,
                             torch::Tensor groups, int64_t page, OptTensor slots, torch::Tensor status) {
   MGFA_CHECK(page_table.is_cuda(), "page_table must be a CUDA tensor");
@@ -276,7 +277,7 @@ torch::Tensor shared_prefix(torch::Tensor page_table, torch::Tensor kv_lens, tor
   const int64_t n = check_groups(groups, page_table, seqs);
   c10::cuda::CUDAGuard guard(page_table.device());
   torch::Tensor plan = torch::empty({n + 2 * seqs}, page_table.options());
-  PagedParams p;
+  PagedGroupParams p;
   p.status = status_ptr(status, page_table);
   if (n == 0) return plan;
   p.page_table = page_table.data_ptr<int>();
