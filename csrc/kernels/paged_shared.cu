@@ -48,11 +48,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     paged_plan_kernel(const PagedGroupParams p, int* shared, int* first, int* member) {
   const int g = blockIdx.x / kPlanCtas, cta = blockIdx.x % kPlanCtas, n_groups = p.seqs - p.own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __shared__ int least, lead_of[2], live[2];  // of all sequences; of those with new tokens
-  if (threadIdx.x < 2) {
-    lead_of[threadIdx.x] = p.own;
-    live[threadIdx.x] = 0;
-  }
+  __shared__ int least;
+  if (threadIdx.x == 0) least = p.width;
   bool bad = false;
   for (int i = threadIdx.x; i < n_groups; i += kPlanThreads) {
     const int a = __ldg(p.groups + i), e = __ldg(p.groups + i + 1);
@@ -62,32 +59,41 @@ __global__ void __launch_bounds__(kPlanThreads)
   const int from = bad ? 0 : __ldg(p.groups + g), to = bad ? 0 : __ldg(p.groups + g + 1);
   auto row_of = [&](int b) { return p.slots ? __ldg(p.slots + b) : b; };
   auto new_of = [&](int b) { return __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b); };
-  // the row of a sequence that counts: that has one (any = 1: and new tokens); else -1
-  auto counts = [&](int b, int any) {
-    const int row = row_of(b);
-    return row >= 0 && row < p.rows && new_of(b) >= any ? row : -1;
-  };
-  bool falls = false;
-  for (int b = from + int(threadIdx.x); b < to; b += kPlanThreads) {
-    falls |= new_of(b) < 0;
-    for (int any = 0; any < 2; ++any)
-      if (counts(b, any) >= 0) {
-        atomicMin(&lead_of[any], b);
-        atomicAdd(&live[any], 1);
-      }
+  auto counts = [&](int row, int n, int any) { return row >= 0 && row < p.rows && n >= any; };
+  const int mine_first = from + cta * (kPlanThreads / 32) + warp;  // of this warp's sequences
+  int row = 0, n = 0;
+  if (mine_first < to) {
+    row = row_of(mine_first);
+    n = new_of(mine_first);
   }
-  falls = __syncthreads_or(falls);
-  const int any = live[1] > 0, lead = lead_of[any];
-  const bool several = live[any] > 1 && !falls;
-  if (threadIdx.x == 0) least = several ? p.width : 0;
-  __syncthreads();
+  // Each warp finds the first that counts, and whether there is a second, for itself: mostly
+  // among the first 32, and nothing has to wait for other warps. [1]: with new tokens.
+  int lead_of[2] = {to, to}, lead_row[2] = {0, 0}, live[2] = {0, 0};
+  for (int b0 = from; b0 < to && live[1] < 2; b0 += 32) {
+    const int b = b0 + lane, r = b < to ? row_of(b) : -1, m = b < to ? new_of(b) : 0;
+#pragma unroll
+    for (int any = 0; any < 2; ++any) {
+      const uint32_t mask = __ballot_sync(0xffffffffu, counts(r, m, any));
+      if (mask && live[any] == 0) {
+        lead_of[any] = b0 + __ffs(mask) - 1;
+        lead_row[any] = __shfl_sync(0xffffffffu, r, __ffs(mask) - 1);
+      }
+      live[any] += __popc(mask);
+    }
+  }
+  const int any = live[1] > 0, lead = any ? lead_of[1] : lead_of[0];
+  const bool several = (any ? live[1] : live[0]) > 1;
   if (several) {
-    const int* theirs = p.page_table + int64_t(row_of(lead)) * p.table_stride;
-    for (int b = from + cta * (kPlanThreads / 32) + warp; b < to; b += kPlanCtas * (kPlanThreads / 32)) {
-      const int row = counts(b, any);
-      if (row < 0) continue;
+    const int* theirs = p.page_table + int64_t(any ? lead_row[1] : lead_row[0]) * p.table_stride;
+    for (int b = mine_first; b < to; b += kPlanCtas * (kPlanThreads / 32)) {
+      if (b > mine_first) {
+        row = row_of(b);
+        n = new_of(b);
+      }
+      if (n < 0 && lane == 0) atomicMin(&least, 0);
+      if (!counts(row, n, any)) continue;
       const int64_t kv = std::min<int64_t>(__ldg(p.kv_lens + row), int64_t(p.width) * p.page);
-      int pages = int(std::max<int64_t>(kv - new_of(b), 0) / p.page);
+      int pages = int(std::max<int64_t>(kv - n, 0) / p.page);
       const int* mine = p.page_table + int64_t(row) * p.table_stride;
       for (int j0 = 0; j0 < pages; j0 += 32 * kPlanLoads) {
         bool differ[kPlanLoads];
@@ -109,14 +115,16 @@ __global__ void __launch_bounds__(kPlanThreads)
       if (lane == 0) atomicMin(&least, pages);
     }
   }
+  const int id = cta * kPlanThreads + int(threadIdx.x), step = kPlanCtas * kPlanThreads;
+  auto shares_of = [&](int b) { return counts(row_of(b), new_of(b), 1); };
+  bool shares = from + id < to && shares_of(from + id);
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  int all = least;
+  int all = several ? least : 0;
   for (int i = 0; i < kPlanCtas; ++i) all = std::min(all, *cluster.map_shared_rank(&least, i));
   cluster.sync();
-  const int id = cta * kPlanThreads + int(threadIdx.x), step = kPlanCtas * kPlanThreads;
   for (int b = from + id; b < to; b += step) {
-    const bool shares = counts(b, 1) >= 0;
+    if (b > from + id) shares = shares_of(b);
     first[b] = shares ? all * p.page : 0;
     member[b] = shares ? g : b == from && all > 0 ? -2 - lead : -1;
   }
