@@ -333,6 +333,7 @@ std::tuple<torch::Tensor, OptTensor> paged_attention(
   }
   MGFA_CHECK(page_table.size(1) * page < (int64_t(1) << 30), "page_table is too wide");
   MGFA_CHECK(max_new >= 0, "max_seqlen_q must not be negative");
+  MGFA_CHECK(groups.has_value() == plan.has_value(), "cu_groups and the plan of the shared prefixes come together");
   const int64_t n_groups = groups.has_value() ? check_groups(*groups, k, seqs) : 0;
   if (n_groups) {
     check_ints(*plan, k, 1, "the plan");

@@ -188,3 +188,12 @@ def test_rows_that_leave_the_batch_are_reported(first, last, small):
     if last:
         p.new[n - 1] = 0
     p.check(out, lse)
+
+
+def test_half_a_plan_is_refused():
+    from multi_gpu_flashattention_b200 import SharedPrefix
+    p = Forked([(100, [(5, 1), (6, 1)])], 4, 2, 64, 16)
+    for half in (SharedPrefix(p.groups, None), SharedPrefix(None, p.plan().plan)):
+        with pytest.raises(RuntimeError, match="come together"):
+            p.run(shared=half)
+    p.check(*p.run(shared=p.plan()))
