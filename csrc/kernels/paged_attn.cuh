@@ -87,8 +87,8 @@ struct PagedParams {
 // the first[b] tokens that their group shares, and behind them the groups, each the new tokens
 // of its sequences over the shared[g] tokens before; `seqs` counts both. The kernels are
 // compiled for either type of parameters, so that calls without a plan pay nothing for what
-// only these need (in one kernel 64 sequences of six new tokens over up to 1024 keys took 138
-// us instead of 134, chunks of 16 tokens 100 instead of 97).
+// only these need (in one kernel 64 sequences of six new tokens over up to 1024 keys took 139
+// us instead of 133, chunks of 16 tokens 98 instead of 94).
 struct PagedGroupParams : PagedParams {
   int form = kPagedByRows;  // (kPagedHeadsApart: unit_rows are those of each of its heads)
   const int* first = nullptr;   // [own]; null: nothing is shared. Behind it member, [own]: a

@@ -13,8 +13,8 @@
 // but the tile's; the four are added when a unit ends. 32 sequences of 8192 keys (8 key
 // heads of 128, pages of 16) take 171 us for 1.07 GB, 6.3 TB/s; one of 131072 keys 86 us,
 // and 9 us for joining 296 parts; with 4 new tokens each (16 rows) the 32 sequences take
-// 1.05 times as long, with 8 (32 rows, whose second block of 16 spills 488 bytes at head_dim
-// 128) 1.34 times. For short sequences the time is latency: one token each
+// 1.03 times as long, with 8 (32 rows, whose second block of 16 spills 488 bytes at head_dim
+// 128, with a plan 820) 1.33 times. For short sequences the time is latency: one token each
 // over 100 to 320 keys takes 9.6 us.
 //
 // Two more forms serve sequences that share a prefix (paged_shared.cu), whose units are short or

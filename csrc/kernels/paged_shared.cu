@@ -15,9 +15,9 @@
 // The prefix of many rows is work for the tensor cores (paged_chunk.cu), own keys and the prefix
 // of few rows are bound by reading them (paged_decode.cu). The launches run side by side, on SMs
 // in proportion to their work: one token each of 128 sequences over 32768 shared and up to 512
-// own keys (32/8 heads of 128) takes 113 us that way, 139 us one behind another. The plan takes
-// 12 us of that call (once a step, not once a layer), the tiles before each sequence 4 us, the
-// join 9 us. Eight groups of up to eight sequences over up to 8192 keys: 60 of 80 us.
+// own keys (32/8 heads of 128) takes 113 to 118 us that way, 139 us one behind another. The plan
+// takes 11 us of that call (once a step, not once a layer), the tiles before each sequence 4 us,
+// the join 9 us. Eight groups of up to eight sequences over up to 8192 keys: 59 of 79 us.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 

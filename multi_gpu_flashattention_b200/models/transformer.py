@@ -238,7 +238,9 @@ class RingTransformerLM(nn.Module):
         hold nothing; those of a sequence that got no room in the cache, which stays as it
         was, are NaN. bfloat16 or float16 parameters, head_dim 64 or 128.
         cu_groups (int32 [groups + 1], CUDA): sequences [cu_groups[g], cu_groups[g + 1]) were
-        forked from one prompt, whose full pages the attention then reads once for all of them."""
+        forked from one prompt, whose full pages the attention then reads once for all of them
+        (shared_prefix() says when that pays). Sequences that have ended may stay in their group
+        without tokens, freed or not."""
         if cu_groups is not None and not isinstance(cu_groups, torch.Tensor):
             cu_groups = torch.tensor(cu_groups, dtype=torch.int32, device=cache.k.device)
         self._check_served(ids, cache, max_seqlen, slots, cu_groups)
