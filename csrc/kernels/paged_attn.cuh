@@ -91,7 +91,7 @@ struct PagedParams {
 // us instead of 133, chunks of 16 tokens 98 instead of 94).
 struct PagedGroupParams : PagedParams {
   int form = kPagedByRows;  // (kPagedHeadsApart: unit_rows are those of each of its heads)
-  const int* first = nullptr;   // [own]; null: nothing is shared. Behind it member, [own]: a
+  const int* first = nullptr;   // [own] tokens that sequence b shares; behind it member, [own]: a
                                 // sequence's group, -1: none; -2 - b where a group's first one
                                 // shares nothing, b being the first that does
   const int* groups = nullptr;  // [seqs - own + 1] sequences
